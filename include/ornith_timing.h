@@ -27,6 +27,8 @@
  *                    transform_bf16, transform_bf16_frag, dequantize
  *   heads            head_encode, head_w8_mfma, act, head_mfma, argmax,
  *                    logits_argmax, logits_argmax_finish (long rows), fill
+ *   sampling         sample_parts, sample_select, sample_gather, sample_finish,
+ *                    sample_empty (no columns)
  *   shared expert    fixed8_act, fixed8_gate
  *   other            repack_codes, repack_meta, silu_selfcheck */
 #ifndef ORNITH_TIMING_H

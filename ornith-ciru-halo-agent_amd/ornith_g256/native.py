@@ -108,6 +108,9 @@ _PROTOTYPES = {
     # storage conversion (include/ornith_storage.h)
     'ornith_repack_n16_to_n32': ([_VP] * 4 + [_INT] * 3 + [_VP], _INT),
     'ornith_logits_argmax_launch': ([_VP, _INT, _INT, _I64, _VP, _VP], _INT),
+    # sampling (include/ornith_sample.h)
+    'ornith_logits_sample_get_layout': ([_INT, _INT, C.POINTER(_SZ)], _INT),
+    'ornith_logits_sample_launch': ([_VP] + [_INT] * 3 + [_I64] + [_VP] * 6 + [_SZ] + [_VP] * 4, _INT),
     # measurement (include/ornith_timing.h)
     'ornith_mi355x_timing_arm': ([C.c_char_p, _INT], _INT),
     'ornith_mi355x_timing_read': ([C.c_char_p, C.POINTER(_INT), C.POINTER(C.c_double)], _INT),
@@ -563,6 +566,53 @@ def logits_argmax(logits, out):
         raise ValueError('logits must be bf16 [M, N] with unit column stride; out int64 [M]')
     check(lib().ornith_logits_argmax_launch(ptr(logits), logits.shape[0], logits.shape[1], logits.stride(0),
                                             ptr(out), stream(logits)), 'logits argmax')
+
+
+LOGITS_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def logits_sample_bytes(capacity, n):
+    """Workspace bytes of logits_sample for up to `capacity` rows of n columns."""
+    size = _SZ(0)
+    check(lib().ornith_logits_sample_get_layout(capacity, n, C.byref(size)), f'sampling layout for {capacity} x {n}')
+    return size.value
+
+
+def logits_sample(logits, uniform, workspace, out, flags, temperature=None, top_k=None, top_p=None, min_p=None,
+                  logprob=None):
+    """Stochastic hand-off: out int64 [M] = one token per row of bf16, fp16 or
+    fp32 logits [M, N], by the row's temperature, top_p and min_p (fp32 [M]),
+    top_k (int32 [M]) and uniform number in [0, 1) (fp32 [M]); None is off.
+    temperature 0 is greedy.  logprob fp32 [M] (optional): the log of the
+    probability the token was drawn with.  What each setting keeps, and the
+    sticky flags (1 NaN logit, 2 setting out of range, 4 empty row; the last
+    two give token -1): include/ornith_sample.h."""
+    rows = logits.shape[0] if logits.ndim == 2 else -1
+    if rows < 0 or logits.dtype not in LOGITS_TYPES or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError('logits must be bf16, fp16 or fp32 [M, N] with unit column stride')
+    if rows > 1 and logits.stride(0) < logits.shape[1]:
+        raise ValueError(f'logits rows overlap: row stride {logits.stride(0)} of {logits.shape[1]} columns')
+    for name, t, dtype in (('uniform', uniform, torch.float32), ('temperature', temperature, torch.float32),
+                           ('top_k', top_k, torch.int32), ('top_p', top_p, torch.float32),
+                           ('min_p', min_p, torch.float32), ('logprob', logprob, torch.float32),
+                           ('out', out, torch.int64)):
+        if t is None:
+            if name in ('uniform', 'out'):
+                raise ValueError(f'{name} is required')
+            continue
+        if t.dtype != dtype or tuple(t.shape) != (rows,) or not t.is_contiguous():
+            raise ValueError(f'{name} must be a contiguous {dtype} [{rows}] tensor, got {tuple(t.shape)} {t.dtype}')
+    if flags.dtype != torch.int32 or flags.numel() != 1 or workspace.element_size() != 1:
+        raise ValueError('flags must be one int32 word, workspace bytes')
+    tensors = [t for t in (logits, uniform, temperature, top_k, top_p, min_p, logprob, out, flags, workspace)
+               if t is not None]
+    if logits.device.type != 'cuda' or any(t.device != logits.device for t in tensors):
+        raise ValueError('logits, settings, outputs, flags and workspace must be on one GPU')
+    with torch.cuda.device(logits.device):
+        check(lib().ornith_logits_sample_launch(
+            ptr(logits), LOGITS_TYPES[logits.dtype], rows, logits.shape[1], max(logits.stride(0), logits.shape[1]),
+            ptr(uniform), ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), ptr(workspace), workspace.numel(),
+            ptr(out), ptr(logprob), ptr(flags), stream(logits)), 'logits sample')
 
 
 def dense_head(x, codes, meta, workspace, logits, logits_bf16, argmax, flags, capacity):
