@@ -29,6 +29,7 @@
  *                    logits_argmax, logits_argmax_finish (long rows), fill
  *   sampling         sample_parts, sample_select, sample_gather, sample_finish,
  *                    sample_empty (no columns)
+ *   plain 4-bit      w4, w4_pack_codes, w4_pack_meta
  *   shared expert    fixed8_act, fixed8_gate
  *   other            repack_codes, repack_meta, silu_selfcheck */
 #ifndef ORNITH_TIMING_H

@@ -111,6 +111,10 @@ _PROTOTYPES = {
     # sampling (include/ornith_sample.h)
     'ornith_logits_sample_get_layout': ([_INT, _INT, C.POINTER(_SZ)], _INT),
     'ornith_logits_sample_launch': ([_VP] + [_INT] * 3 + [_I64] + [_VP] * 6 + [_SZ] + [_VP] * 4, _INT),
+    # plain 4-bit linears (include/ornith_w4.h)
+    'ornith_w4_get_layout': ([_INT] * 3 + [C.POINTER(_SZ)] * 2, _INT),
+    'ornith_w4_pack': ([_VP] * 2 + [_INT] + [_VP] * 3 + [_INT] * 3 + [_VP], _INT),
+    'ornith_w4_launch': ([_VP, _INT, _I64] + [_VP] * 3 + [_INT, _I64, _VP] + [_INT] * 4 + [_VP], _INT),
     # measurement (include/ornith_timing.h)
     'ornith_mi355x_timing_arm': ([C.c_char_p, _INT], _INT),
     'ornith_mi355x_timing_read': ([C.c_char_p, C.POINTER(_INT), C.POINTER(C.c_double)], _INT),
@@ -613,6 +617,45 @@ def logits_sample(logits, uniform, workspace, out, flags, temperature=None, top_
             ptr(logits), LOGITS_TYPES[logits.dtype], rows, logits.shape[1], max(logits.stride(0), logits.shape[1]),
             ptr(uniform), ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), ptr(workspace), workspace.numel(),
             ptr(out), ptr(logprob), ptr(flags), stream(logits)), 'logits sample')
+
+
+W4_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def w4_layout(n, k, group):
+    """Shapes of the packed codes and metadata of a plain 4-bit linear."""
+    codes, meta = _SZ(0), _SZ(0)
+    check(lib().ornith_w4_get_layout(n, k, group, C.byref(codes), C.byref(meta)), f'w4 layout N{n} K{k} G{group}')
+    return (-(-n // 16), -(-k // 128), 64, 4), (-(-n // 16), -(-k // group), 16)
+
+
+def w4_out(x, codes, metadata, out, flags, n, k, group):
+    """Plain 4-bit linear: out [rows, n] (bf16, fp16 or fp32) = x [rows, k]
+    (bf16 or fp16, as it is) times the banks of storage.pack_w4.  Any number of
+    rows; the weights are read once per 64."""
+    if x.ndim != 2 or x.shape[1] != k or x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f'input must be a bf16 or fp16 [rows, {k}] tensor, got {tuple(x.shape)} {x.dtype}')
+    rows = x.shape[0]
+    if tuple(out.shape) != (rows, n) or out.dtype not in W4_TYPES:
+        raise ValueError(f'output must be a bf16, fp16 or fp32 [{rows}, {n}] tensor, got {tuple(out.shape)} {out.dtype}')
+    for name, t, cols in (('input', x, k), ('output', out, n)):
+        if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+            raise ValueError(f'{name} rows must have unit column stride and not overlap')
+    ldx, ldo = x.stride(0) if rows > 1 and k else k, out.stride(0) if rows > 1 and n else n
+    if ldx % 8 or x.data_ptr() % 16:
+        raise ValueError('input rows must start on the 16-byte grid')
+    want = w4_layout(n, k, group)
+    for name, t, shape in (('codes', codes, want[0]), ('metadata', metadata, want[1])):
+        if t.element_size() != 4 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f'{name} must be the contiguous 32-bit {shape} bank of storage.pack_w4, '
+                             f'got {tuple(t.shape)} {t.dtype}')
+    if flags.dtype != torch.int32 or flags.numel() != 1:
+        raise ValueError('flags must be one int32 word')
+    if x.device.type != 'cuda' or any(t.device != x.device for t in (codes, metadata, out, flags)):
+        raise ValueError('input, banks, output and flags must be on one GPU')
+    with torch.cuda.device(x.device):
+        check(lib().ornith_w4_launch(ptr(x), W4_TYPES[x.dtype], ldx, ptr(codes), ptr(metadata), ptr(out),
+                                     W4_TYPES[out.dtype], ldo, ptr(flags), rows, n, k, group, stream(x)), 'w4 linear')
 
 
 def dense_head(x, codes, meta, workspace, logits, logits_bf16, argmax, flags, capacity):

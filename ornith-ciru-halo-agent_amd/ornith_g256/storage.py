@@ -116,3 +116,37 @@ def repack_n32(codes16: torch.Tensor, meta16: torch.Tensor, n: int, k: int):
                                                        native.ptr(meta32), banks, n, k,
                                                        native.stream(codes16)), 'N16 -> N32 repack')
     return codes32, meta32
+
+
+def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, group: int):
+    """A plain 4-bit linear's checkpoint rows (on the GPU) -> the banks that
+    native.w4_out reads, once, through the library's pack kernel:
+    codes 32-bit words [n, k/8] of eight low-first codes, scales bf16 or fp16
+    [n, ceil(k/group)], zeros uint8 of that shape, 0..15, or None (8
+    everywhere).  Returns int32 codes and metadata (include/ornith_w4.h)."""
+    if codes.device.type != 'cuda' or scales.device != codes.device or (zeros is not None and
+                                                                         zeros.device != codes.device):
+        raise ValueError('the pack runs on GPU-resident banks')
+    if codes.ndim != 2 or codes.dtype not in (torch.int32, torch.uint32):
+        raise ValueError(f'codes must be 32-bit words [n, k/8], got {tuple(codes.shape)} {codes.dtype}')
+    if scales.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f'scales must be bf16 or fp16, got {scales.dtype}')
+    if group not in (32, 64, 128, 256):
+        raise ValueError(f'group {group} is not 32, 64, 128 or 256')
+    n, k = codes.shape[0], codes.shape[1] * 8
+    shape = (n, -(-k // group))
+    if tuple(scales.shape) != shape or (zeros is not None and (tuple(zeros.shape) != shape
+                                                               or zeros.dtype != torch.uint8)):
+        raise ValueError(f'scales and uint8 zeros must be {shape}')
+    if not bool(torch.isfinite(scales).all()):
+        raise AdmissionError('non-finite scale')
+    if zeros is not None and zeros.numel() and int(zeros.max()) > 15:
+        raise AdmissionError('zero point above 15')
+    codes, scales = codes.contiguous(), scales.contiguous()
+    zeros = None if zeros is None else zeros.contiguous()
+    packed = [torch.empty(s, dtype=torch.int32, device=codes.device) for s in native.w4_layout(n, k, group)]
+    with torch.cuda.device(codes.device):
+        native.check(native.lib().ornith_w4_pack(native.ptr(codes), native.ptr(scales), native.W4_TYPES[scales.dtype],
+                                                 native.ptr(zeros), native.ptr(packed[0]), native.ptr(packed[1]), n, k,
+                                                 group, native.stream(codes)), 'w4 pack')
+    return tuple(packed)
