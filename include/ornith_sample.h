@@ -39,8 +39,9 @@ extern "C" {
 /* logits_type of the launch */
 enum { ORNITH_LOGITS_BF16 = 0, ORNITH_LOGITS_F16 = 1, ORNITH_LOGITS_F32 = 2 };
 
-/* Workspace for calls of up to Mcap rows of N columns (more than 64 rows need
- * no more than 64 do).  Mcap >= 0, 0 <= N <= 2^20. */
+/* Workspace for calls of up to Mcap rows of N columns: 0 bytes (a NULL
+ * workspace) up to 8192 columns, and no more for many rows than for the 64 or,
+ * of shorter rows, up to 512 that share it.  Mcap >= 0, 0 <= N <= 2^20. */
 ORNITH_EXPORT hipError_t ornith_logits_sample_get_layout(int Mcap, int N, size_t* workspace_bytes);
 
 /* logits of logits_type [M, N], row stride ld >= N elements, aligned to their

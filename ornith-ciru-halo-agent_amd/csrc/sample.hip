@@ -2,27 +2,31 @@
 // (definitions: include/ornith_sample.h).
 //
 // Every cut keeps a prefix of the order (value descending, column ascending),
-// so a row's kept set is { i : comp(i) >= threshold } with
-// comp = (ordered value bits << 32) | ~column.  The threshold is found through
-// a histogram and a short list, without a sort:
+// so a row's kept set is { i : comp(i) >= threshold } with comp = (ordered value
+// bits << 20) | complement of the column.  The threshold is found through a
+// histogram and a short list, without a sort:
 //   parts   one block per 8192 columns: counts and masses of the part in bins
 //           an eighth of a power of two of mass wide, 37 powers of two deep;
 //   select  one block per row: the parts' histograms added up, the bins that
 //           hold the borders; rows with no cut, and greedy ones, end here;
-//   gather  one block per part: (value, column) of the logits in those bins;
+//   gather  one block per part: (value, column) of the logits in those bins, or,
+//           where no more than 256 logits lie in or above them, of all those;
 //   finish  one block per row: the threshold inside its bin, the kept mass per
-//           part, and the walk through the one part that holds the token.
+//           part, and the walk through the one part that holds the token (of the
+//           256: threshold and token from the list alone).
+// Rows of one part do all of it in one block and one launch (sample_row).
 //
 // Masses.  With c = log2(e) / T and t = l c in fp64, e = 2^(t - j) for the
-// whole number j = ceil(max t) of its part: a degree-8 polynomial in the
-// fraction of t (relative error 2^-39.7), rounded to a whole number of units
-// 2^-36.  One 64-bit LDS add carries count (14 bits) and mass (50 bits: 8192
-// entries of at most 2^36).  Whole numbers make the sums independent of the
-// order of the atomics.  A row adds parts in units of 2^-42 of 2^J, J the
-// largest j: (mass << 6) >> (J - j), below 2^63 for 2^20 columns.  Row units
-// truncate per (part, bin) where J - j > 6, a relative 2^-42 each.
-// The bin, floor(8 t), comes from t alone, so equal values share a bin in every
-// part and bins are ordered as values are.
+// whole number j = ceil(max t) of its part: a degree-8 polynomial in t - rint(t)
+// (relative error 2^-39.7), rounded to a whole number of units 2^-36.  One
+// 64-bit LDS add carries count (14 bits) and mass (50 bits: 8192 entries of at
+// most 2^36).  Whole numbers make the sums independent of the order of the
+// atomics.  A row adds parts in units of 2^-42 of 2^J, J the largest j:
+// (mass << 6) >> (J - j), below 2^63 for 2^20 columns.  Row units truncate per
+// (part, bin) where J - j > 6, a relative 2^-42 each.  The bin, rint(8 t), comes
+// from t alone, so equal values share a bin in every part and bins are ordered
+// as values are.
+#include <algorithm>
 #include "kernels.hpp"
 #include "timing.hpp"
 #include "validate.hpp"
@@ -32,45 +36,62 @@ namespace ornith {
 namespace {
 
 constexpr int kPart = 8192, kPartsMax = 128;         // columns of a part; parts of 2^20 columns
+constexpr int kColBits = 20;
 constexpr int kOctaves = 37, kSub = 8;
 constexpr int kTopBin = kOctaves * kSub;             // bin of t == j; bins 0 .. kTopBin
 constexpr int kBins = 304;                           // padded
-constexpr int kMaskWords = 10;
 constexpr int kMassBits = 50;
 constexpr uint64_t kMassMask = (uint64_t(1) << kMassBits) - 1;
+constexpr uint64_t kPartOne = uint64_t(1) << 36;     // mass 1 in part units
 constexpr int kRowShift = 6;                         // part units -> row units at j == J
-constexpr int kListMax = 32768, kListLds = 4096;     // border entries kept per row, and in LDS
-constexpr int kChunkRows = 64;                       // rows that share the workspace at once
-constexpr int kPartThreads = 256, kRowThreads = 512;
+constexpr int kListMax = 16384, kListLds = 4096;     // border entries kept per row, and in LDS
+constexpr int kSmall = 256;                          // rows decided by a list of all their candidates
+constexpr int kMaximaK = 256;                        // top_k up to which a part drops what cannot be among it
+constexpr int kQueue = 512;                          // a wave's surviving values, compacted up to here
+constexpr int kRowThreads = 1024, kRowWaves = kRowThreads / 64, kPer = kPart / kRowThreads;
+constexpr uint32_t kMinusInf = 0x007fffffu;          // ordered(-inf)
+constexpr uint32_t kKeyEnd = 0xffffffffu;            // above every key
 
 enum : uint32_t { kSampleNan = 1, kSampleSetting = 2, kSampleEmpty = 4 };
+enum : int { kDone = 0, kModeSmall = 1, kModeList = 2, kModeWalk = 3 };
 
-struct PartMeta { double j; uint32_t key; int32_t arg; };     // key 0: nothing takes part
+// key: the largest value (0: nothing takes part); arg: its first column (greedy rows); mass: of rows
+// without a cut; least: values below it are not in the histogram
+struct PartMeta { double j; uint64_t mass; uint32_t key; int32_t arg; float least; };
 
-struct RowState {
+// What select leaves for gather and finish.
+struct Plan {
     double J;
+    float mx;                                        // the row's largest value
     uint64_t threshold_q;                            // min-p's threshold (0: none)
-    int32_t done, walk;                              // ended in select; border bins too full for the list
-    int32_t bin_k, use_k, use_p;
+    uint64_t total, above_mass;                      // row mass; mass of the bins above bin_k
+    int32_t mode, use_k, use_p, bin_k, bin_q, above_count;
+    uint32_t lo[3], hi[3];                           // key ranges [lo, hi) to gather (the first: bin_k's; unused: empty)
+};
+struct RowState {
+    Plan plan;
     uint32_t count;                                  // list entries
-    uint32_t mask[kMaskWords];                       // border bins
     uint64_t cum_mass[kBins];                        // of bins >= i
-    uint32_t cum_count[kBins];
 };
 
 struct SampleArgs {
-    const void* logits; int64_t ld; int N, parts;
+    const void* logits; int64_t ld; int N, parts, list_max;
     const float *uniform, *temperature; const int32_t* top_k; const float *top_p, *min_p;
     uint64_t* hist;                                  // [rows, parts, kBins] count << 50 | mass
     PartMeta* meta;                                  // [rows, parts]
     RowState* state;                                 // [rows]
-    uint2* list;                                     // [rows, kListMax] value bits (ordered), column
+    uint2* list;                                     // [rows, list_max] ordered value bits, column
     int64_t* token; float* logprob; uint32_t* flags;
 };
 
 // ---- values -------------------------------------------------------------------
 template <int TYPE> constexpr int kBytes = TYPE == ORNITH_LOGITS_F32 ? 4 : 2;
+// low bits of the ordered value that no logit of the type has
+template <int TYPE> constexpr int kDrop = TYPE == ORNITH_LOGITS_F32 ? 0 : TYPE == ORNITH_LOGITS_BF16 ? 16 : 13;
 
+template <int TYPE> __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row) {
+    return static_cast<const uint8_t*>(a.logits) + size_t(row) * size_t(a.ld) * kBytes<TYPE>;
+}
 template <int TYPE> __device__ __forceinline__ float load1(const void* row, int col) {
     if constexpr (TYPE == ORNITH_LOGITS_F32) return static_cast<const float*>(row)[col];
     const uint32_t b = static_cast<const uint16_t*>(row)[col];
@@ -111,49 +132,78 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 __device__ __forceinline__ float unordered(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
-constexpr uint32_t kMinusInf = 0x007fffffu;          // ordered(-inf)
-__device__ __forceinline__ uint64_t comp_of(uint32_t key, int col) { return (uint64_t(key) << 32) | uint32_t(~col); }
+constexpr uint32_t kColMask = (1u << kColBits) - 1;
+template <int TYPE> __device__ __forceinline__ uint64_t comp_of(uint32_t key, int col) {
+    return (uint64_t(key >> kDrop<TYPE>) << kColBits) | (kColMask - uint32_t(col));
+}
+// (a negative value's dropped bits are ones)
+template <int TYPE> __device__ __forceinline__ uint32_t comp_key(uint64_t comp) {
+    const uint32_t k = uint32_t(comp >> kColBits) << kDrop<TYPE>;
+    return k & 0x80000000u ? k : k | ((1u << kDrop<TYPE>) - 1);
+}
+__device__ __forceinline__ int comp_col(uint64_t comp) { return int(kColMask - (uint32_t(comp) & kColMask)); }
 
-// 2^(x + 1/2) for |x| <= 1/2, degree 8 (Chebyshev interpolation; relative error 2^-39.7)
-__device__ __forceinline__ double exp2_half(double x) {
-    double p = 0x1.f7318d7c8c8f4p-20;
-    p = __builtin_fma(p, x, 0x1.6b416dbad124ep-16);
-    p = __builtin_fma(p, x, 0x1.c8d6c3ed5deadp-13);
-    p = __builtin_fma(p, x, 0x1.ee4eccd91f352p-10);
-    p = __builtin_fma(p, x, 0x1.bdb6970fc2c99p-7);
-    p = __builtin_fma(p, x, 0x1.41839f011e158p-4);
-    p = __builtin_fma(p, x, 0x1.5be298adea926p-2);
-    p = __builtin_fma(p, x, 0x1.f5e465377fff3p-1);
-    return __builtin_fma(p, x, 0x1.6a09e667f3bccp+0);
+// 2^x for |x| <= 1/2, degree 8 (Chebyshev interpolation; relative error 2^-39.7, 1 at 0)
+__device__ __forceinline__ double exp2_poly(double x) {
+    double p = 0x1.63cf7dec51603p-20;
+    p = __builtin_fma(p, x, 0x1.00dc48dc4d96cp-16);
+    p = __builtin_fma(p, x, 0x1.4308ae274a207p-13);
+    p = __builtin_fma(p, x, 0x1.5d8745a95d2d4p-10);
+    p = __builtin_fma(p, x, 0x1.3b2ab71725c04p-7);
+    p = __builtin_fma(p, x, 0x1.c6b08dd6fb6b1p-5);
+    p = __builtin_fma(p, x, 0x1.ebfbdff824847p-3);
+    p = __builtin_fma(p, x, 0x1.62e42fef84cf7p-1);
+    return __builtin_fma(p, x, 0x1p+0);
 }
 
-// Bin and mass of a value in a part with the given j; bin < 0: below the bins
-// (NaN and -inf too).  The high word of `packed` lacks the count.
-__device__ __forceinline__ int bin_mass(float v, double c, double j, uint64_t& mass) {
-    const double t = double(v) * c;
-    if (j == __builtin_huge_val()) {                  // uniform: +inf in the part, its mass all there is
-        mass = uint64_t(1) << (kMassBits - 14);
-        return v == __builtin_huge_valf() ? kTopBin : -1;
-    }
-    const double n = __builtin_floor(t), r = t - n;
-    const int up = int(fmax(n - j, -64.0));           // <= 0 (fmax takes the number of a NaN difference)
-    const int bin = up * kSub + int(r * double(kSub)) + kTopBin;
-    double e = exp2_half(r - 0.5);
-    e = __longlong_as_double(__double_as_longlong(e) + (int64_t(up + 36) << 52));
+// From |j| = 2^40 on, the neighbours of the largest value lie 2^16 powers of two below it: it has
+// all the mass (+inf among such).  The scale (0, 0) gives it one.
+constexpr double kFar = 0x1p40, kWhole = 0x1.8p52;
+__device__ __forceinline__ bool is_far(double j) { return !(__builtin_fabs(j) < kFar); }
+struct Scale { double c, j; };
+__device__ __forceinline__ Scale scale_of(double c, double j) { return is_far(j) ? Scale{0.0, 0.0} : Scale{c, j}; }
+
+// Bin and mass of a value at or above its part's `least` (of others, anything) with the part's
+// scale.  Whole numbers come from the low word of a sum with 1.5 * 2^52: o = rint(l c) - j there,
+// with one rounding of the exact product, so o + j and its eighths are the same in every part.
+__device__ __forceinline__ int bin_mass(float v, const Scale& k, uint64_t& mass) {
+    const double l = double(fminf(v, 0x1.fffffep127f)), m = kWhole - k.j;
+    const double q = __builtin_fma(l, k.c, m);
+    const double x = __builtin_fma(l, k.c, m - q);                            // l c - rint(l c)
+    const int o = int(uint32_t(__double_as_longlong(q)));                     // <= 0
+    const int f = int(uint32_t(__double_as_longlong(__builtin_fma(x, double(kSub), kWhole))));
+    const double e = __longlong_as_double(__double_as_longlong(exp2_poly(x)) + (int64_t(o + 36) << 52));
     mass = uint64_t(__double_as_longlong(e + 0x1p52)) & ((uint64_t(1) << 52) - 1);
-    return v > -__builtin_huge_valf() ? bin : -1;
+    return o * kSub + f + kTopBin;
+}
+// The bin, for the row or part with the largest value mx, of any value up to a little above it (NaN
+// and -inf among them); -1: below the bins.
+__device__ __forceinline__ int bin_of(float v, float mx, double c, double j) {
+    if (is_far(j)) return v >= mx ? kTopBin : -1;
+    uint64_t unused;
+    const int bin = bin_mass(v, Scale{c, j}, unused);
+    return double(v) * c > j - 64.0 ? max(bin, -1) : -1;
+}
+// A value a little below the lower edge of `bin`; never -inf.
+__device__ __forceinline__ float below_bin(int bin, float mx, double c, double j) {
+    if (is_far(j)) return mx;
+    const float at = float((j + (double(bin - kTopBin) - 0.5) * (1.0 / kSub)) / c);
+    return fmaxf(at - __builtin_fabsf(at) * 0x1p-20f - 0x1p-126f, -0x1.fffffep127f);
 }
 
-__device__ __forceinline__ int part_shift(double J, double j) {
-    return J == j ? 0 : int(fmin(J - j, 64.0));
-}
+__device__ __forceinline__ int part_shift(double J, double j) { return J == j ? 0 : int(fmin(J - j, 64.0)); }
 __device__ __forceinline__ uint64_t row_mass(uint64_t m, int shift) {
     return shift < 64 ? (m << kRowShift) >> shift : 0;
 }
 // u in [0, 1) as a 64-bit fraction (below 2^-40 its last bits are cut)
 __device__ __forceinline__ uint64_t fraction(float u) { return uint64_t(double(u) * 0x1p64); }
+// the least whole number at or above p of `mass` (p < 1), at least 1
+__device__ __forceinline__ uint64_t share(float p, uint64_t mass) {
+    const uint64_t f = fraction(p);
+    return max(__umul64hi(f, mass) + (f * mass != 0), uint64_t(1));
+}
 
-struct Setting { float T, p, q, u; int k; bool valid; double c; };
+struct Setting { float T, p, q, u; int k; bool valid, cut; double c; };
 __device__ __forceinline__ Setting setting(const SampleArgs& a, int row) {
     Setting s;
     s.T = a.temperature ? a.temperature[row] : 1.f;
@@ -163,573 +213,968 @@ __device__ __forceinline__ Setting setting(const SampleArgs& a, int row) {
     s.u = a.uniform[row];
     s.valid = s.T >= 0.f && s.T < __builtin_huge_valf() && s.p > 0.f && s.p <= 1.f && s.q >= 0.f && s.q <= 1.f &&
               s.u >= 0.f && s.u < 1.f;
+    s.cut = (s.k > 0 && s.k < a.N) || s.p < 1.f || s.q > 0.f;
     s.c = s.T > 0.f ? 0x1.71547652b82fep+0 / double(s.T) : 0.0;
     return s;
 }
 
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
+// ---- waves ----------------------------------------------------------------------
+template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(v)), CTRL, ROWS, 0xF, false));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(v >> 32)), CTRL, ROWS, 0xF, false));
+    return (uint64_t(hi) << 32) | lo;
+}
+// inclusive prefix sum over the 64 lanes (wave_prefix_sum in 64 bits)
+__device__ __forceinline__ uint64_t wave_prefix_u64(uint64_t v) {
+    v += dpp_u64<0x111, 0xF>(v);
+    v += dpp_u64<0x112, 0xF>(v);
+    v += dpp_u64<0x114, 0xF>(v);
+    v += dpp_u64<0x118, 0xF>(v);
+    v += dpp_u64<0x142, 0xA>(v);
+    v += dpp_u64<0x143, 0xC>(v);
     return v;
 }
+__device__ __forceinline__ uint64_t readlane_u64(uint64_t v, int lane) {
+    return (uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), lane))) << 32) |
+           uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), lane));
+}
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) { return readlane_u64(wave_prefix_u64(v), 63); }
 
-// ---- parts ----------------------------------------------------------------------
-template <int TYPE>
-__global__ __launch_bounds__(kPartThreads) void sample_parts_kernel(SampleArgs a, int row0) {
-    const int part = blockIdx.x, slot = blockIdx.y, row = row0 + slot, tid = threadIdx.x;
-    __shared__ uint64_t s_hist[kBins];
-    __shared__ uint32_t s_key[kPartThreads / 64];
-    __shared__ int s_arg[kPartThreads / 64];
-    const auto* src = static_cast<const uint8_t*>(a.logits) + size_t(row) * size_t(a.ld) * kBytes<TYPE>;
-    const Setting s = setting(a, row);
-    constexpr int kPieces = kPart / 8 / kPartThreads;
-    float v[kPieces][8];
-#pragma unroll
-    for (int u = 0; u < kPieces; ++u) load8<TYPE>(src, part * kPart + (u * kPartThreads + tid) * 8, a.N, v[u]);
-    for (int i = tid; i < kBins; i += kPartThreads) s_hist[i] = 0;
+// The least key whose bin is at least `bin`, by the whole wave: the estimate of the bin's lower edge
+// is off by less than a step of fp32, so the 64 keys around it hold it.
+__device__ __forceinline__ uint32_t bin_edge(int bin, float mx, double c, double j) {
+    if (is_far(j)) return ordered(mx);
+    const double at = (j + (double(bin - kTopBin) - 0.5) * (1.0 / kSub)) / c;
+    const uint32_t first = max(ordered(float(at)), kMinusInf + 33) - 32, k0 = first + (threadIdx.x & 63);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(k0 >= ordered(__builtin_huge_valf()) ||
+                                                    bin_of(unordered(k0), mx, c, j) >= bin);
+    return first + (in ? uint32_t(__builtin_ctzll(in)) : 64u);
+}
+
+// ---- one part --------------------------------------------------------------------
+template <int THREADS> struct PartShared {
+    uint64_t hist[kBins];
+    uint32_t count[kBins];                            // of thread maxima
+    uint32_t key[THREADS / 64];
+    int arg[THREADS / 64];
+    uint64_t mass[THREADS / 64];
+    float queue[THREADS / 64][kQueue];
+};
+
+// Histogram (cut rows), whole mass (others) or first maximum (greedy) of the values that the
+// block's threads hold, eight consecutive columns a piece.  The histogram is complete after the
+// caller's next barrier; of a cut row, it lacks values that no cut can keep.
+template <int THREADS, int PIECES>
+__device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting& s, const float (&v)[PIECES][8],
+                                              int col0, PartShared<THREADS>& sh) {
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    constexpr int W = THREADS / 64;
+    for (int i = tid; i < kBins; i += THREADS) {
+        sh.hist[i] = 0;
+        sh.count[i] = 0;
+    }
     float mx = -__builtin_huge_valf();
     bool nan = false;
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
+    for (int u = 0; u < PIECES; ++u)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             nan |= v[u][e] != v[u][e];
             mx = fmaxf(mx, v[u][e]);
         }
-    if (__builtin_amdgcn_ballot_w64(nan) && (tid & 63) == 0) flag_or(a.flags, kSampleNan);
+    if (__builtin_amdgcn_ballot_w64(nan) && lane == 0) flag_or(a.flags, kSampleNan);
     const uint32_t wkey = wave_max_u(ordered(mx));
-    if ((tid & 63) == 0) s_key[tid >> 6] = wkey;
+    if (lane == 0) sh.key[wv] = wkey;
     __syncthreads();
-    uint32_t key = s_key[0];
+    uint32_t key = sh.key[0];
 #pragma unroll
-    for (int w = 1; w < kPartThreads / 64; ++w) key = max(key, s_key[w]);
-    PartMeta* meta = a.meta + size_t(slot) * a.parts + part;
-    uint64_t* hist = a.hist + (size_t(slot) * a.parts + part) * kBins;
-    if (key <= kMinusInf) {
-        if (tid == 0) *meta = PartMeta{-__builtin_huge_val(), 0, 0};
-        return;
-    }
+    for (int w = 1; w < W; ++w) key = max(key, sh.key[w]);
+    if (key <= kMinusInf || !s.valid) return PartMeta{-__builtin_huge_val(), 0, 0, 0, 0.f};
     if (s.T == 0.f) {                                 // greedy: the first column of the largest value
         int arg = 0x7fffffff;
 #pragma unroll
-        for (int u = kPieces - 1; u >= 0; --u)
+        for (int u = PIECES - 1; u >= 0; --u)
 #pragma unroll
             for (int e = 7; e >= 0; --e)
-                if (ordered(v[u][e]) == key && v[u][e] == v[u][e]) arg = part * kPart + (u * kPartThreads + tid) * 8 + e;
+                if (v[u][e] == v[u][e] && ordered(v[u][e]) == key) arg = col0 + 8 * THREADS * u + e;
         arg = wave_min_i(arg);
-        if ((tid & 63) == 0) s_arg[tid >> 6] = arg;
+        if (lane == 0) sh.arg[wv] = arg;
         __syncthreads();
-        if (tid == 0) {
+        arg = sh.arg[0];
 #pragma unroll
-            for (int w = 1; w < kPartThreads / 64; ++w) arg = min(arg, s_arg[w]);
-            *meta = PartMeta{0.0, key, arg};
-        }
-        return;
+        for (int w = 1; w < W; ++w) arg = min(arg, sh.arg[w]);
+        return PartMeta{0.0, 0, key, arg, 0.f};
     }
-    const double j = __builtin_ceil(double(unordered(key)) * s.c);
+    const float part_mx = unordered(key);
+    const double j = __builtin_ceil(double(part_mx) * s.c);
+    const Scale k = scale_of(s.c, j);
+    float least = below_bin(0, part_mx, s.c, j);
+    if (!s.cut) {
+        uint64_t sum = 0;
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            uint64_t mass;
-            const int bin = bin_mass(v[u][e], s.c, j, mass);
-            if (bin >= 0) atomicAdd(reinterpret_cast<unsigned long long*>(&s_hist[bin]),
-                                    (unsigned long long)(mass + (uint64_t(1) << kMassBits)));
-        }
-    __syncthreads();
-    for (int i = tid; i < kBins; i += kPartThreads) hist[i] = s_hist[i];
-    if (tid == 0) *meta = PartMeta{j, key, 0};
-}
-
-// ---- the end of a row --------------------------------------------------------------
-struct RowShared {
-    double j[kPartsMax];
-    int shift[kPartsMax];
-    uint64_t part_mass[kPartsMax];
-    uint64_t wave[kRowThreads / 64];
-    uint64_t rest, total;
-    int part;
-};
-
-// Loads the parts' j and the shifts to the row's J.
-__device__ __forceinline__ void load_parts(const SampleArgs& a, int slot, double J, RowShared& sh) {
-    const PartMeta* meta = a.meta + size_t(slot) * a.parts;
-    for (int p = threadIdx.x; p < a.parts; p += kRowThreads) {
-        const double j = meta[p].key ? meta[p].j : -__builtin_huge_val();
-        sh.j[p] = j;
-        sh.shift[p] = meta[p].key ? part_shift(J, j) : 64;
-    }
-}
-
-// part_mass[p] = the row mass of the part's bins above `bin`.
-__device__ __forceinline__ void sum_parts(const SampleArgs& a, int slot, int bin, RowShared& sh) {
-    const int lane = threadIdx.x & 63;
-    for (int p = threadIdx.x >> 6; p < a.parts; p += kRowThreads / 64) {
-        uint64_t m = 0;
-        if (sh.shift[p] < 64) {
-            const uint64_t* hist = a.hist + (size_t(slot) * a.parts + p) * kBins;
-            for (int i = bin + 1 + lane + kSub * sh.shift[p]; i <= kTopBin; i += 64)
-                m += row_mass(hist[i] & kMassMask, sh.shift[p]);
-        }
-        m = wave_sum_u64(m);
-        if (lane == 0) sh.part_mass[p] = m;
-    }
-}
-
-// part_mass holds the kept mass of every part: the part that holds the token,
-// then the token inside it.  Kept: comp >= threshold.
-template <int TYPE>
-__device__ void draw(const SampleArgs& a, int row, const Setting& s, double J, uint64_t threshold, RowShared& sh) {
-    const int tid = threadIdx.x, lane = tid & 63;
-    if (tid < 64) {
-        uint64_t m[kPartsMax / 64], before = 0;
-#pragma unroll
-        for (int h = 0; h < kPartsMax / 64; ++h) {
-            const int p = h * 64 + lane;
-            m[h] = p < a.parts ? sh.part_mass[p] : 0;
-        }
-        uint64_t total = 0;
-#pragma unroll
-        for (int h = 0; h < kPartsMax / 64; ++h) total += wave_sum_u64(m[h]);
-        const uint64_t target = __umul64hi(fraction(s.u), total);      // token: the first column past it
-#pragma unroll
-        for (int h = 0; h < kPartsMax / 64; ++h) {
-            uint64_t run = m[h];
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint64_t o = __shfl_up(run, d, 64);
-                if (lane >= d) run += o;
-            }
-            if (before + run > target && before + run - m[h] <= target) {
-                sh.part = h * 64 + lane;
-                sh.rest = target - (before + run - m[h]);
-            }
-            before += __shfl(run, 63, 64);
-        }
-        if (lane == 0) sh.total = total;
-    }
-    __syncthreads();
-    const int part = sh.part, shift = sh.shift[part];
-    const uint64_t rest = sh.rest;
-    const double j = sh.j[part];
-    const auto* src = static_cast<const uint8_t*>(a.logits) + size_t(row) * size_t(a.ld) * kBytes<TYPE>;
-    constexpr int kPer = kPart / kRowThreads;           // consecutive columns of a thread
-    const int col0 = part * kPart + tid * kPer;
-    float v[kPer / 8][8];
-    uint64_t sum = 0;
-    auto mass_at = [&](float x, int col) -> uint64_t {
-        uint64_t m;
-        const int bin = bin_mass(x, s.c, j, m);
-        return bin >= 0 && comp_of(ordered(x), col) >= threshold ? m : 0;
-    };
-#pragma unroll
-    for (int u = 0; u < kPer / 8; ++u) load8<TYPE>(src, col0 + 8 * u, a.N, v[u]);
-#pragma unroll
-    for (int u = 0; u < kPer / 8; ++u)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum += mass_at(v[u][e], col0 + 8 * u + e);
-    uint64_t run = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up(run, d, 64);
-        if (lane >= d) run += o;
-    }
-    if (lane == 63) sh.wave[tid >> 6] = run;
-    __syncthreads();
-    for (int w = 0; w < (tid >> 6); ++w) run += sh.wave[w];
-    if (row_mass(run, shift) > rest && row_mass(run - sum, shift) <= rest) {
-        uint64_t at = run - sum;
-        bool found = false;
-#pragma unroll
-        for (int u = 0; u < kPer / 8; ++u)
+        for (int u = 0; u < PIECES; ++u)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint64_t m = mass_at(v[u][e], col0 + 8 * u + e);
-                at += m;
-                if (!found && row_mass(at, shift) > rest) {
-                    found = true;
-                    a.token[row] = col0 + 8 * u + e;
-                    if (a.logprob) {
-                        const double t = double(v[u][e]) * s.c;
-                        const double up = J == __builtin_huge_val() ? 0.0 : t - J;
-                        const double ln = up * 0x1.62e42fefa39efp-1 - log(double(sh.total) * 0x1p-42);
-                        a.logprob[row] = row_mass(m, shift) == sh.total ? 0.f : float(ln);   // alone
-                    }
-                }
+                uint64_t m;
+                if (bin_mass(v[u][e], k, m) >= 0 && v[u][e] >= least) sum += m;
             }
+        sum = wave_sum_u64(sum);
+        if (lane == 0) sh.mass[wv] = sum;
+        __syncthreads();
+        sum = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) sum += sh.mass[w];
+        return PartMeta{j, sum, key, 0, least};
+    }
+    // Values that take part in no cut are left out: those below the bins, and with a small top_k
+    // those below the bin that holds the k-th largest of the threads' maxima (k values of this
+    // part alone lie in or above it).
+    if (s.k > 0 && s.k <= kMaximaK && THREADS >= kMaximaK) {
+        uint64_t unused;
+        const int b = bin_mass(mx, k, unused);
+        if (b >= 0 && mx >= least) atomicAdd(&sh.count[b], 1u);
+        __syncthreads();
+        constexpr int per = (kTopBin + 64) / 64;
+        uint32_t c[per], sum = 0;
+#pragma unroll
+        for (int e = 0; e < per; ++e) {
+            const int i = kTopBin - (per * lane + e);
+            c[e] = i >= 0 ? sh.count[i] : 0;
+            sum += c[e];
+        }
+        uint32_t run = uint32_t(wave_prefix_sum(int(sum))) - sum;
+        int found = 0;
+#pragma unroll
+        for (int e = 0; e < per; ++e) {
+            if (run < uint32_t(s.k) && run + c[e] >= uint32_t(s.k)) found = kTopBin - (per * lane + e);
+            run += c[e];
+        }
+        least = below_bin(int(wave_max_u(uint32_t(found))), part_mx, s.c, j);
+    }
+    auto add = [&](float x) {
+        uint64_t m;
+        const int bin = bin_mass(x, k, m);
+        if (bin >= 0) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[bin]),
+                                (unsigned long long)(m + (uint64_t(1) << kMassBits)));
+    };
+    int left = 0;
+#pragma unroll
+    for (int u = 0; u < PIECES; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) left += __popcll(__builtin_amdgcn_ballot_w64(v[u][e] >= least));
+    if (left <= min(kQueue, PIECES * 8 * 64 / 2)) {   // few: side by side first
+        float* queue = sh.queue[wv];
+        int at = 0;
+#pragma unroll
+        for (int u = 0; u < PIECES; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint64_t b = __builtin_amdgcn_ballot_w64(v[u][e] >= least);
+                if (v[u][e] >= least) queue[at + __builtin_amdgcn_mbcnt_hi(uint32_t(b >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo(uint32_t(b), 0))] = v[u][e];
+                at += __popcll(b);
+            }
+        for (int i = lane; i < left; i += 64) add(queue[i]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < PIECES; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (v[u][e] >= least) add(v[u][e]);
+    }
+    return PartMeta{j, 0, key, 0, least};
+}
+
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_parts_kernel(SampleArgs a, int row0) {
+    const int part = blockIdx.x, slot = blockIdx.y, row = row0 + slot, tid = threadIdx.x;
+    __shared__ PartShared<THREADS> sh;
+    constexpr int kPieces = kPart / 8 / THREADS;
+    const void* src = row_of<TYPE>(a, row);
+    const int col0 = part * kPart + tid * 8;
+    float v[kPieces][8];
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u) load8<TYPE>(src, col0 + 8 * THREADS * u, a.N, v[u]);
+    const Setting s = setting(a, row);
+    const PartMeta m = part_pass<THREADS, kPieces>(a, s, v, col0, sh);
+    __syncthreads();
+    const size_t at = size_t(slot) * a.parts + part;
+    if (tid == 0) a.meta[at] = m;
+    if (m.key && s.cut && s.T != 0.f)
+        for (int i = tid; i < kBins; i += THREADS) a.hist[at * kBins + i] = sh.hist[i];
+}
+
+// ---- the row ------------------------------------------------------------------------
+struct RowShared {
+    uint64_t cm[kBins];                               // mass and
+    uint32_t cc[kBins];                               // count of bins >= i
+    uint64_t part_mass[kPartsMax];
+    Scale scale[kPartsMax];
+    int shift[kPartsMax];
+    float least[kPartsMax];
+    uint64_t wave_mass[kRowWaves];
+    uint32_t wave_count[kRowWaves];
+    uint64_t lo, hi, rest, total;
+    int bin[3], part;                                 // bin_k; top-p's highest and lowest
+    uint32_t qkey, edge[6];
+    Plan plan;
+};
+
+// What the parts of a row with the given J add to it: scale, shift, least.  (Where J is far, every
+// part that adds anything has that j.)
+__device__ __forceinline__ PartMeta load_part(const SampleArgs& a, int slot, int p, double c, double J, RowShared& sh) {
+    const PartMeta m = a.meta[size_t(slot) * a.parts + p];
+    sh.scale[p] = scale_of(c, m.j);
+    sh.shift[p] = m.key ? part_shift(J, m.j) : 64;
+    sh.least[p] = m.least;
+    return m;
+}
+// Thread i <= kTopBin holds bin kTopBin - i's mass and count: cm and cc (after the barriers in it).
+__device__ __forceinline__ void cumulate(uint64_t mass, uint32_t count, RowShared& sh) {
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    constexpr int W = (kTopBin + 64) / 64;
+    if (wv < W) {
+        mass = wave_prefix_u64(mass);
+        count = uint32_t(wave_prefix_sum(int(count)));
+        if (lane == 63) {
+            sh.wave_mass[wv] = mass;
+            sh.wave_count[wv] = count;
+        }
+    }
+    if (tid == 0) {
+        sh.bin[0] = sh.bin[1] = sh.bin[2] = -1;
+        sh.qkey = kMinusInf + 1;
+        sh.part = -1;
+    }
+    __syncthreads();
+    if (tid <= kTopBin) {
+        for (int w = 0; w < wv; ++w) {
+            mass += sh.wave_mass[w];
+            count += sh.wave_count[w];
+        }
+        sh.cm[kTopBin - tid] = mass;
+        sh.cc[kTopBin - tid] = count;
+    }
+    __syncthreads();
+}
+
+// The borders of a cut row from cm and cc: sh.plan (after its last barrier).
+__device__ __forceinline__ void borders(const SampleArgs& a, const Setting& s, float mx, double J, int list_max,
+                                        RowShared& sh) {
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const uint64_t* cm = sh.cm;
+    const uint32_t* cc = sh.cc;
+    const bool use_k = s.k > 0 && s.k < a.N && cc[0] >= uint32_t(s.k), use_p = s.p < 1.f, use_q = s.q > 0.f;
+    // the bin that holds the k-th value, and the range of the mass of the first k
+    if (tid <= kTopBin) {
+        const uint64_t next = tid == kTopBin ? 0 : cm[tid + 1];
+        const uint32_t before = tid == kTopBin ? 0 : cc[tid + 1];
+        if (use_k) {
+            if (cc[tid] >= uint32_t(s.k) && before < uint32_t(s.k)) {
+                sh.bin[0] = tid;
+                sh.hi = cm[tid];
+                sh.lo = cc[tid] == uint32_t(s.k) ? cm[tid] : next;
+            }
+        } else if (tid == 0) sh.hi = sh.lo = cm[0];
+    }
+    // min-p's least value: the estimate mx + T ln q is off by less than a step of fp32 there, so the
+    // 64 values around it hold the border
+    if (use_q && wv == kRowWaves - 1) {
+        const uint32_t top = ordered(mx);
+        const float at = float(double(mx) + double(s.T) * log(double(s.q)));
+        const uint32_t mid = at == at ? ordered(at) : kMinusInf + 1;
+        const uint32_t k0 = max(min(mid, top), kMinusInf + 33) - 32 + lane;
+        const float v = unordered(k0);
+        const bool in = k0 <= top && (v == mx || (double(v) - double(mx)) * s.c >= log2(double(s.q)));
+        const uint64_t b = __builtin_amdgcn_ballot_w64(in);
+        if (lane == 0) sh.qkey = b ? k0 + uint32_t(__builtin_ctzll(b)) : top;
+    }
+    __syncthreads();
+    // the bins that top-p's border can lie in
+    if (use_p && tid <= kTopBin) {
+        const uint64_t f = fraction(s.p);
+        const uint64_t lo = max(__umul64hi(f, sh.lo), uint64_t(1)), hi = __umul64hi(f, sh.hi) + 1;
+        const uint64_t next = tid == kTopBin ? 0 : cm[tid + 1];
+        if (cm[tid] >= lo && next < lo) sh.bin[1] = tid;
+        if ((cm[tid] >= hi || tid == 0) && next < hi) sh.bin[2] = tid;
+    }
+    __syncthreads();
+    const int bk = sh.bin[0], p_hi = use_p ? sh.bin[1] : -1, p_lo = use_p ? sh.bin[2] : -1;
+    const int bq = use_q ? bin_of(unordered(sh.qkey), mx, s.c, J) : -1;
+    const bool q_alone = bq > max(bk, p_hi);          // min-p's border lies above the others' bins
+    const bool q_in = bq >= 0 && bq >= max(bk, p_lo);
+    int lo[3] = {q_alone ? -1 : bk, q_alone ? -1 : p_lo, q_in ? bq : -1}, hi[3] = {lo[0], q_alone ? -1 : p_hi, lo[2]};
+    int least = kTopBin + 1;
+    uint32_t entries = 0;
+#pragma unroll
+    for (int r = 0; r < 3; ++r)
+        if (lo[r] >= 0) {
+            least = min(least, lo[r]);
+            entries += cc[lo[r]] - (hi[r] == kTopBin ? 0 : cc[hi[r] + 1]);
+        }
+    const bool none = least > kTopBin;                // every border lies below the bins
+    const bool small = !none && cc[least] <= uint32_t(kSmall);
+    if (small) {
+        lo[0] = least;
+        hi[0] = kTopBin;
+        lo[1] = lo[2] = -1;
+    }
+    if (wv < 6) {
+        const int r = wv >> 1, b = wv & 1 ? hi[r] + 1 : lo[r];
+        const uint32_t edge = lo[r] < 0 || b > kTopBin ? kKeyEnd : bin_edge(b, mx, s.c, J);
+        if (lane == 0) sh.edge[wv] = edge;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        Plan& p = sh.plan;
+        p.J = J;
+        p.mx = mx;
+        p.threshold_q = 0;
+        p.total = cm[0];
+        p.mode = small ? kModeSmall : entries <= uint32_t(list_max) ? kModeList : kModeWalk;
+        p.use_k = use_k && !q_alone;
+        p.use_p = use_p && !q_alone;
+        p.bin_k = bk;
+        p.bin_q = bq;
+        p.above_count = bk < 0 || bk == kTopBin ? 0 : int(cc[bk + 1]);
+        p.above_mass = bk < 0 || bk == kTopBin ? 0 : cm[bk + 1];
+#pragma unroll
+        for (int r = 0; r < 3; ++r) {
+            p.lo[r] = sh.edge[2 * r];
+            p.hi[r] = sh.edge[2 * r + 1];
+        }
+    }
+    __syncthreads();
+}
+template <int TYPE> __device__ __forceinline__ uint64_t q_threshold(uint32_t qkey) {
+    const uint32_t up = qkey & 0x80000000u ? (1u << kDrop<TYPE>) - 1 : 0;     // to a value of the type
+    return uint64_t((qkey + up) >> kDrop<TYPE>) << kColBits;
+}
+__device__ __forceinline__ bool in_ranges(const Plan& p, uint32_t key) {
+    return key - p.lo[0] < p.hi[0] - p.lo[0] || key - p.lo[1] < p.hi[1] - p.lo[1] || key - p.lo[2] < p.hi[2] - p.lo[2];
+}
+
+__device__ __forceinline__ void give(const SampleArgs& a, int row, int token, float logprob) {
+    a.token[row] = token;
+    if (a.logprob) a.logprob[row] = logprob;
+}
+// ln of mass(v) / total; 0 where the token is all there is
+__device__ __forceinline__ float log_share(float v, const Setting& s, double J, uint64_t mass, uint64_t total) {
+    if (mass == total) return 0.f;
+    const double up = is_far(J) ? 0.0 : __builtin_fma(double(v), s.c, -J);
+    return float(up * 0x1.62e42fefa39efp-1 - log(double(total) * 0x1p-42));
+}
+
+// part_mass holds the kept mass of every part (after a barrier): sh.part, sh.rest (what is left of
+// u S there) and sh.total.
+__device__ __forceinline__ void draw_part(int parts, const Setting& s, RowShared& sh) {
+    const int tid = threadIdx.x;
+    if (tid < 64) {
+        uint64_t m[kPartsMax / 64], run[kPartsMax / 64], total = 0;
+#pragma unroll
+        for (int h = 0; h < kPartsMax / 64; ++h) {
+            const int p = h * 64 + tid;
+            m[h] = p < parts ? sh.part_mass[p] : 0;
+            run[h] = wave_prefix_u64(m[h]) + total;
+            total = readlane_u64(run[h], 63);
+        }
+        const uint64_t target = __umul64hi(fraction(s.u), total);      // token: the first column past it
+        if (tid == 0) {
+            sh.total = total;
+            sh.part = -1;
+        }
+#pragma unroll
+        for (int h = 0; h < kPartsMax / 64; ++h)
+            if (run[h] > target && run[h] - m[h] <= target) {
+                sh.part = h * 64 + tid;
+                sh.rest = target - (run[h] - m[h]);
+            }
+    }
+    __syncthreads();
+}
+// The token inside the part: thread i holds its columns col0 .. col0 + 7, ascending over the block.
+template <int TYPE>
+__device__ __forceinline__ void draw_column(const SampleArgs& a, int row, const Setting& s, double J, const Scale& k,
+                                            float least, int shift, uint64_t threshold, const float (&v)[kPer], int col0, RowShared& sh) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    uint64_t m[kPer], sum = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        const int bin = bin_mass(v[e], k, m[e]);
+        if (bin < 0 || !(v[e] >= least) || comp_of<TYPE>(ordered(v[e]), col0 + e) < threshold) m[e] = 0;
+        sum += m[e];
+    }
+    uint64_t run = wave_prefix_u64(sum);
+    if (lane == 63) sh.wave_mass[wv] = run;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) run += w < wv ? sh.wave_mass[w] : 0;
+    const uint64_t rest = sh.rest;
+    if (row_mass(run, shift) > rest && row_mass(run - sum, shift) <= rest) {
+        uint64_t at = run - sum;
+        int col = 0;
+        float val = 0.f;
+        uint64_t mass = 0;
+#pragma unroll
+        for (int e = kPer - 1; e >= 0; --e) {
+            uint64_t upto = at;
+#pragma unroll
+            for (int f = 0; f <= e; ++f) upto += m[f];
+            if (row_mass(upto, shift) > rest) {
+                col = col0 + e;
+                val = v[e];
+                mass = m[e];
+            }
+        }
+        give(a, row, col, log_share(val, s, J, row_mass(mass, shift), sh.total));
     }
 }
 
-// ---- select -----------------------------------------------------------------------
+// A list of every candidate (n <= kSmall): cuts and draw by ranks, four threads an entry.
+struct SmallList { uint64_t comp[kSmall], mass[kSmall]; float val[kSmall]; unsigned long long k, k_mass, p; };
+__device__ __forceinline__ void finish_small(const SampleArgs& a, int row, const Setting& s, const Plan& plan, int n,
+                                             uint64_t threshold, SmallList& sl) {
+    const int tid = threadIdx.x, e = tid >> 2;
+    if (tid == 0) {
+        sl.k = 0;
+        sl.p = 0;
+        sl.k_mass = plan.total;
+    }
+    __syncthreads();
+    auto quad = [](uint64_t v) {
+        v += dpp_u64<kDppXor1, 0xF>(v);
+        return v + dpp_u64<kDppXor2, 0xF>(v);
+    };
+    const bool live = e < n;
+    const uint64_t comp = live ? sl.comp[e] : 0, mass = live ? sl.mass[e] : 0;
+    uint64_t count = 0, before = 0;
+    for (int i = tid & 3; i < n; i += 4) {
+        const bool b = sl.comp[i] > comp;
+        count += b;
+        before += b ? sl.mass[i] : 0;
+    }
+    count = quad(count);
+    before = quad(before);
+    if (plan.use_k && live && count == uint64_t(s.k) - 1) {
+        sl.k = comp;
+        sl.k_mass = before + mass;
+    }
+    __syncthreads();
+    if (plan.use_p) {
+        // (entries can sum to a few units less than their bins, whose sums are cut once per part: then all are kept)
+        const uint64_t target = share(s.p, sl.k_mass);
+        if (live && before < target && before + mass >= target) sl.p = comp;
+        __syncthreads();
+    }
+    threshold = max(threshold, max(uint64_t(sl.k), uint64_t(sl.p)));
+    uint64_t total = 0, run = 0;
+    for (int i = tid & 3; i < n; i += 4) {
+        const uint64_t m = sl.comp[i] >= threshold ? sl.mass[i] : 0;
+        total += m;
+        run += (sl.comp[i] & kColMask) >= (comp & kColMask) ? m : 0;      // columns up to this one
+    }
+    total = quad(total);
+    run = quad(run);
+    const uint64_t target = __umul64hi(fraction(s.u), total);
+    if (live && comp >= threshold && (tid & 3) == 0 && run > target && run - mass <= target)
+        give(a, row, comp_col(comp), log_share(sl.val[e], s, plan.J, mass, total));
+}
+
+// Descent to a border inside one bin's key range: the entry at which, from the largest down, `need`
+// is reached - a count, or a mass.  each(f) runs f(comp, row mass) over the entries of the range
+// [lo, hi) of keys, spread over the block.  A round counts the entries by the next ten bits of
+// comp - base; 64 or fewer are ranked by one wave.
+struct Descent {
+    uint32_t count[1024];
+    unsigned long long mass[1024];
+    uint64_t comp[64], m[64];
+    uint64_t wave_mass[kRowWaves];
+    uint32_t wave_count[kRowWaves];
+    uint64_t need, above, found;
+    uint32_t digit, group, n;
+};
+template <int TYPE, class Each>
+__device__ __forceinline__ void descend(uint32_t lo, uint32_t hi, bool by_mass, uint64_t need, Each&& each, Descent& d) {
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    static_assert(kRowThreads == 1024, "a thread per digit");
+    uint64_t base = uint64_t(lo >> kDrop<TYPE>) << kColBits;
+    uint64_t span = (uint64_t(((hi - 1) >> kDrop<TYPE>) + 1) << kColBits) - base;   // comps lie in [base, base + span)
+    uint64_t above = 0;
+    uint32_t group = 65;
+    while (true) {
+        const int bits = 64 - __builtin_clzll(span - 1 | 1);
+        const int sft = bits > 10 ? bits - 10 : 0;
+        __syncthreads();
+        d.count[tid] = 0;
+        d.mass[tid] = 0;
+        if (tid == 0) {
+            d.n = 0;
+            d.group = 0;
+        }
+        __syncthreads();
+        if (group <= 64) break;
+        each([&](uint64_t comp, uint64_t m) {
+            if (comp - base >= span) return;
+            const uint32_t i = uint32_t((comp - base) >> sft);
+            atomicAdd(&d.count[i], 1u);
+            atomicAdd(&d.mass[i], (unsigned long long)m);
+        });
+        __syncthreads();
+        // thread i: digit 1023 - i
+        const uint32_t c = d.count[1023 - tid];
+        const uint64_t m = d.mass[1023 - tid];
+        uint32_t cr = uint32_t(wave_prefix_sum(int(c)));
+        uint64_t mr = wave_prefix_u64(m);
+        if (lane == 63) {
+            d.wave_count[wv] = cr;
+            d.wave_mass[wv] = mr;
+        }
+        __syncthreads();
+        uint32_t call = 0;
+        uint64_t mall = 0;
+#pragma unroll
+        for (int w = 0; w < kRowWaves; ++w) {
+            cr += w < wv ? d.wave_count[w] : 0;
+            mr += w < wv ? d.wave_mass[w] : 0;
+            call += d.wave_count[w];
+            mall += d.wave_mass[w];
+        }
+        // the entries can sum to a few units less than their bin (cut once per part): then the last is the border
+        const bool short_of = by_mass ? mall < need : call < need;
+        const uint64_t b0 = by_mass ? mr - m : cr - c, b1 = by_mass ? mr : cr;
+        if (c && (short_of ? cr == call : b0 < need && b1 >= need)) {
+            d.digit = uint32_t(1023 - tid);
+            d.group = c;
+            d.need = short_of ? ~uint64_t(0) : need - b0;
+            d.above = above + (mr - m);
+        }
+        __syncthreads();
+        group = d.group;
+        if (group == 0) {                             // nothing in the range
+            if (tid == 0) {
+                d.found = 0;
+                d.above = 0;
+            }
+            __syncthreads();
+            return;
+        }
+        need = d.need;
+        above = d.above;
+        base += uint64_t(d.digit) << sft;
+        span = uint64_t(1) << sft;
+    }
+    each([&](uint64_t comp, uint64_t m) {
+        if (comp - base >= span) return;
+        const uint32_t i = atomicAdd(&d.n, 1u);
+        if (i < 64) {
+            d.comp[i] = comp;
+            d.m[i] = m;
+        }
+    });
+    __syncthreads();
+    const int n = min(int(d.n), 64);
+    if (tid < 64) {
+        const uint64_t comp = tid < n ? d.comp[tid] : 0, m = tid < n ? d.m[tid] : 0;
+        uint64_t count = 0, before = 0;
+        for (int i = 0; i < n; ++i) {
+            const bool b = d.comp[i] > comp;
+            count += b;
+            before += b ? d.m[i] : 0;
+        }
+        const bool at = by_mass ? before < need && before + m >= need : count + 1 == need;
+        const bool any = __builtin_amdgcn_ballot_w64(tid < n && at);
+        if (tid < n && (any ? at : count + 1 == uint64_t(n))) {
+            d.found = comp;
+            d.above = above + before + m;
+        }
+    }
+    __syncthreads();
+}
+
+// Threshold of a row in list (or walk) mode.  bf: the bin it lies in (-1: below the bins).
+template <int TYPE, class Each>
+__device__ __forceinline__ uint64_t threshold_of(const Setting& s, const Plan& plan, const uint64_t* cm, uint64_t threshold,
+                                                 Each&& each, Descent& d, RowShared& sh, int& bf) {
+    const int tid = threadIdx.x, wv = tid >> 6;
+    bf = threshold ? plan.bin_q : -1;
+    uint64_t of = plan.total;
+    if (plan.use_k) {
+        descend<TYPE>(plan.lo[0], plan.hi[0], false, uint64_t(s.k) - uint64_t(plan.above_count),
+                      [&](auto&& f) { each(plan.lo[0], plan.hi[0], f); }, d);
+        if (d.found > threshold) {
+            threshold = d.found;
+            bf = plan.bin_k;
+        }
+        of = plan.above_mass + d.above;
+    }
+    if (plan.use_p) {
+        const uint64_t target = share(s.p, of);
+        __syncthreads();
+        if (tid == 0) sh.bin[0] = 0;
+        __syncthreads();
+        if (tid <= kTopBin) {
+            const uint64_t next = tid == kTopBin ? 0 : cm[tid + 1];
+            if (cm[tid] >= target && next < target) {
+                sh.bin[0] = tid;
+                sh.lo = target - next;
+            }
+        }
+        __syncthreads();
+        const int b = sh.bin[0];
+        if (wv < 2) {
+            const uint32_t edge = b + wv > kTopBin ? kKeyEnd : bin_edge(b + wv, plan.mx, s.c, plan.J);
+            if ((tid & 63) == 0) sh.edge[wv] = edge;
+        }
+        __syncthreads();
+        const uint32_t lo = sh.edge[0], hi = sh.edge[1];
+        descend<TYPE>(lo, hi, true, sh.lo, [&](auto&& f) { each(lo, hi, f); }, d);
+        if (d.found > threshold) {
+            threshold = d.found;
+            bf = b;
+        }
+    }
+    __syncthreads();
+    return threshold;
+}
+
 template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(SampleArgs a, int row0) {
-    const int slot = blockIdx.x, row = row0 + slot, tid = threadIdx.x;
+    const int slot = blockIdx.x, row = row0 + slot, tid = threadIdx.x, lane = tid & 63;
     __shared__ RowShared sh;
-    __shared__ uint64_t s_mass[2][kRowThreads];
-    __shared__ uint32_t s_count[2][kRowThreads];
-    __shared__ uint32_t s_mask[kMaskWords];
-    __shared__ uint64_t s_lo, s_hi;
-    __shared__ int s_bin[3];
-    __shared__ unsigned long long s_best;
-    __shared__ uint32_t s_qkey, s_entries;
+    __shared__ uint64_t s_mass[2][kTopBin + 24];
+    __shared__ uint32_t s_count[2][kTopBin + 24];
     RowState* st = a.state + slot;
     const Setting s = setting(a, row);
     const PartMeta* meta = a.meta + size_t(slot) * a.parts;
 
-    if (tid == 0) s_best = 0;
-    if (tid < kMaskWords) s_mask[tid] = 0;
-    if (tid < 3) s_bin[tid] = -1;
-    __syncthreads();
-    // the row's largest value, and (greedy) its first column: parts ascend, so the first part wins
-    for (int p = tid; p < a.parts; p += kRowThreads)
-        if (meta[p].key) atomicMax(&s_best, (unsigned long long)((uint64_t(meta[p].key) << 32) | uint32_t(~p)));
-    __syncthreads();
-    const uint32_t top = uint32_t(s_best >> 32);
+    // the row's largest value (every wave for itself) and its first part
+    uint32_t key[kPartsMax / 64], top = 0;
+#pragma unroll
+    for (int h = 0; h < kPartsMax / 64; ++h) {
+        key[h] = h * 64 + lane < a.parts ? meta[h * 64 + lane].key : 0;
+        top = max(top, wave_max_u(key[h]));
+    }
     if (!s.valid || top == 0 || s.T == 0.f) {
         if (tid == 0) {
-            st->done = 1;
+            int first = 0;
+            while (first + 1 < a.parts && meta[first].key != top) ++first;
             const bool fine = s.valid && top != 0;
-            a.token[row] = fine ? meta[~uint32_t(s_best)].arg : -1;
-            if (a.logprob) a.logprob[row] = fine ? 0.f : __builtin_nanf("");
+            st->plan.mode = kDone;
+            give(a, row, fine ? meta[first].arg : -1, fine ? 0.f : __builtin_nanf(""));
             flag_or(a.flags, !s.valid ? kSampleSetting : top == 0 ? kSampleEmpty : 0u);
         }
         return;
     }
     const float mx = unordered(top);
     const double J = __builtin_ceil(double(mx) * s.c);
-    load_parts(a, slot, J, sh);
-    __syncthreads();
-    uint64_t mass = 0;
-    uint32_t count = 0;
-    if (tid <= kTopBin) {
-        const uint64_t* hist = a.hist + size_t(slot) * a.parts * kBins;
-        for (int p = 0; p < a.parts; ++p) {
-            const int i = tid + kSub * sh.shift[p];
-            if (i > kTopBin) continue;
-            const uint64_t w = hist[size_t(p) * kBins + i];
-            count += uint32_t(w >> kMassBits);
-            mass += row_mass(w & kMassMask, sh.shift[p]);
-        }
-    }
-    // sums over bins >= tid
-    s_mass[0][tid] = mass;
-    s_count[0][tid] = count;
-    int from = 0;
-    for (int d = 1; d < kRowThreads; d <<= 1, from ^= 1) {
-        __syncthreads();
-        if (tid + d < kRowThreads) {
-            mass += s_mass[from][tid + d];
-            count += s_count[from][tid + d];
-        }
-        s_mass[from ^ 1][tid] = mass;
-        s_count[from ^ 1][tid] = count;
+    if (tid < a.parts) {
+        const PartMeta m = load_part(a, slot, tid, s.c, J, sh);
+        sh.part_mass[tid] = row_mass(m.mass, sh.shift[tid]);
     }
     __syncthreads();
-    const uint64_t* cm = s_mass[from];
-    const uint32_t* cc = s_count[from];
-    const bool use_k = s.k > 0 && uint32_t(s.k) < cc[0], use_p = s.p < 1.f, use_q = s.q > 0.f;
-    if (!use_k && !use_p && !use_q) {
-        sum_parts(a, slot, -1, sh);
-        if (tid == 0) st->done = 1;
-        __syncthreads();
-        draw<TYPE>(a, row, s, J, 0, sh);
+    if (!s.cut) {
+        if (tid == 0) st->plan.mode = kDone;
+        draw_part(a.parts, s, sh);
+        const int part = sh.part;
+        if (part < 0) {                               // (logits that changed under the call)
+            if (tid == 0) give(a, row, -1, __builtin_nanf(""));
+            return;
+        }
+        float v[kPer];
+        const int col0 = part * kPart + tid * kPer;
+        load8<TYPE>(row_of<TYPE>(a, row), col0, a.N, v);
+        draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], 0, v, col0, sh);
         return;
     }
-    // the bin that holds the k-th value, and the range of the mass of the first k
-    if (tid == 0) { s_lo = cm[0]; s_hi = cm[0]; s_qkey = kMinusInf + 1; }
-    __syncthreads();
-    if (use_k && tid <= kTopBin && cc[tid] >= uint32_t(s.k) && (tid == kTopBin || cc[tid + 1] < uint32_t(s.k))) {
-        s_bin[0] = tid;
-        s_hi = cm[tid];
-        s_lo = cc[tid] == uint32_t(s.k) ? cm[tid] : tid == kTopBin ? 0 : cm[tid + 1];
+    // the parts' bins: three groups of threads, a third of the parts each
+    const int g = tid / (kTopBin + 24), i = tid % (kTopBin + 24), bin = kTopBin - i;
+    uint64_t mass = 0;
+    uint32_t count = 0;
+    if (g < 3 && bin >= 0) {
+        const uint64_t* hist = a.hist + size_t(slot) * a.parts * kBins;
+        constexpr int U = 6;
+        for (int p0 = g; p0 < a.parts; p0 += 3 * U) {
+            uint64_t w[U];
+            int sf[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int p = p0 + 3 * u;
+                sf[u] = p < a.parts ? sh.shift[p] : 64;
+                const int at = bin + kSub * sf[u];
+                w[u] = at <= kTopBin ? hist[size_t(p) * kBins + at] : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                count += uint32_t(w[u] >> kMassBits);
+                mass += row_mass(w[u] & kMassMask, sf[u]);
+            }
+        }
+        if (g) {
+            s_mass[g - 1][i] = mass;
+            s_count[g - 1][i] = count;
+        }
     }
     __syncthreads();
-    // the bins that top-p's border can lie in
-    if (use_p && tid <= kTopBin) {
-        const uint64_t f = fraction(s.p);
-        const uint64_t lo = max(__umul64hi(f, s_lo), uint64_t(1)), hi = __umul64hi(f, s_hi) + 1;
-        const uint64_t next = tid == kTopBin ? 0 : cm[tid + 1];
-        if (cm[tid] >= lo && next < lo) s_bin[1] = tid;                      // upper end
-        if ((cm[tid] >= hi || tid == 0) && next < hi) s_bin[2] = tid;        // lower end
+    if (tid <= kTopBin) {
+        mass += s_mass[0][tid] + s_mass[1][tid];
+        count += s_count[0][tid] + s_count[1][tid];
     }
-    // min-p's least value: the estimate mx + T ln q is off by less than a step of fp32 there, so
-    // the 64 values around it hold the border
-    if (use_q && tid < 64) {
-        const float at = float(double(mx) + double(s.T) * log(double(s.q)));
-        const uint32_t mid = at == at ? ordered(at) : kMinusInf + 1;
-        const uint32_t k0 = max(min(mid, top), kMinusInf + 33) - 32 + tid;
-        const float v = unordered(k0);
-        const bool in = k0 <= top && (v == mx || (double(v) - double(mx)) * s.c >= log2(double(s.q)));
-        const uint64_t b = __builtin_amdgcn_ballot_w64(in);
-        if (tid == 0) s_qkey = b ? k0 + uint32_t(__builtin_ctzll(b)) : top;
-    }
-    __syncthreads();
+    cumulate(mass, count, sh);
+    borders(a, s, mx, J, a.list_max, sh);
     if (tid == 0) {
-        uint64_t tq = 0;
-        auto mark = [&](int lo, int hi) {
-            for (int i = max(lo, 0); i <= hi; ++i) s_mask[i >> 5] |= 1u << (i & 31);
-        };
-        // the strictest bin the other cuts can end in, and the least strict
-        const int kp_hi = max(use_k ? s_bin[0] : -1, use_p ? s_bin[1] : -1);
-        const int kp_lo = max(use_k ? s_bin[0] : -1, use_p ? s_bin[2] : -1);
-        int bq = -1;
-        if (use_q) {
-            tq = uint64_t(s_qkey) << 32;
-            uint64_t unused;
-            bq = bin_mass(unordered(s_qkey), s.c, J, unused);
-        }
-        int32_t k = use_k, p = use_p;
-        if (bq > kp_hi) {                                  // min-p alone decides
-            k = 0;
-            p = 0;
-            mark(bq, bq);
-        } else {
-            if (use_k) mark(s_bin[0], s_bin[0]);
-            if (use_p) mark(s_bin[2], s_bin[1]);
-            if (bq >= 0 && bq >= kp_lo) mark(bq, bq);
-        }
-        st->J = J;
-        st->threshold_q = tq;
-        st->done = 0;
-        st->use_k = k;
-        st->use_p = p;
-        st->bin_k = s_bin[0];
+        sh.plan.threshold_q = s.q > 0.f ? q_threshold<TYPE>(sh.qkey) : 0;
+        st->plan = sh.plan;
         st->count = 0;
-        s_entries = 0;
     }
-    __syncthreads();
-    if (tid <= kTopBin && (s_mask[tid >> 5] >> (tid & 31) & 1))
-        atomicAdd(&s_entries, cc[tid] - (tid == kTopBin ? 0 : cc[tid + 1]));
-    __syncthreads();
-    if (tid == 0) st->walk = s_entries > kListMax;
-    if (tid < kMaskWords) st->mask[tid] = s_mask[tid];
-    if (tid < kBins) {
-        st->cum_mass[tid] = cm[tid];
-        st->cum_count[tid] = cc[tid];
-    }
+    if (tid < kBins) st->cum_mass[tid] = sh.cm[tid];
 }
 
-// ---- gather -----------------------------------------------------------------------
-template <int TYPE>
-__global__ __launch_bounds__(kPartThreads) void sample_gather_kernel(SampleArgs a, int row0) {
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_gather_kernel(SampleArgs a, int row0) {
     const int part = blockIdx.x, slot = blockIdx.y, row = row0 + slot, tid = threadIdx.x;
     RowState* st = a.state + slot;
-    if (st->done || st->walk) return;
+    const Plan& plan = st->plan;
+    if (plan.mode != kModeSmall && plan.mode != kModeList) return;
     const PartMeta meta = a.meta[size_t(slot) * a.parts + part];
-    if (!meta.key) return;
-    const double J = st->J;
-    const int shift = part_shift(J, meta.j);
-    if (shift >= 64) return;
-    __shared__ uint32_t s_mask[kMaskWords];
-    __shared__ int s_any;
-    if (tid < kMaskWords) s_mask[tid] = st->mask[tid];
-    if (tid == 0) s_any = 0;
-    __syncthreads();
-    const uint64_t* hist = a.hist + (size_t(slot) * a.parts + part) * kBins;
-    bool any = false;
-    for (int i = tid + kSub * shift; i <= kTopBin; i += kPartThreads) {
-        const int b = i - kSub * shift;
-        any |= (s_mask[b >> 5] >> (b & 31) & 1) && (hist[i] >> kMassBits);
-    }
-    if (any) s_any = 1;
-    __syncthreads();
-    if (!s_any) return;
-    const Setting s = setting(a, row);
-    const auto* src = static_cast<const uint8_t*>(a.logits) + size_t(row) * size_t(a.ld) * kBytes<TYPE>;
-    uint2* list = a.list + size_t(slot) * kListMax;
-    constexpr int kPieces = kPart / 8 / kPartThreads;
+    const uint32_t key = meta.key;
+    __shared__ int s_n[THREADS / 64];
+    __shared__ uint32_t s_at;
+    if (key < plan.lo[0] && key < plan.lo[1] && key < plan.lo[2]) return;
+    const void* src = row_of<TYPE>(a, row);
+    uint2* list = a.list + size_t(slot) * a.list_max;
+    constexpr int kPieces = kPart / 8 / THREADS;
+    const int col0 = part * kPart + tid * 8;
     float v[kPieces][8];
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) load8<TYPE>(src, part * kPart + (u * kPartThreads + tid) * 8, a.N, v[u]);
+    for (int u = 0; u < kPieces; ++u) load8<TYPE>(src, col0 + 8 * THREADS * u, a.N, v[u]);
+    // the block takes its place in the list with one addition
+    uint32_t in = 0;
 #pragma unroll
     for (int u = 0; u < kPieces; ++u)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            uint64_t mass;
-            const int b = bin_mass(v[u][e], s.c, meta.j, mass) - kSub * shift;
-            if (b >= 0 && (s_mask[b >> 5] >> (b & 31) & 1)) {
-                const uint32_t at = atomicAdd(&st->count, 1u);
-                if (at < kListMax)
-                    list[at] = make_uint2(ordered(v[u][e]), uint32_t(part * kPart + (u * kPartThreads + tid) * 8 + e));
+        for (int e = 0; e < 8; ++e)                   // (v >= least is false for NaN)
+            in |= uint32_t(v[u][e] >= meta.least && in_ranges(plan, ordered(v[u][e]))) << (8 * u + e);
+    const int lane = tid & 63, wv = tid >> 6, own = __popc(in), run = wave_prefix_sum(own);
+    if (lane == 63) s_n[wv] = run;
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        before += w < wv ? s_n[w] : 0;
+        total += s_n[w];
+    }
+    if (!total) return;
+    if (tid == 0) s_at = atomicAdd(&st->count, uint32_t(total));
+    __syncthreads();
+    uint32_t at = s_at + uint32_t(before + run - own);
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (in >> (8 * u + e) & 1) {
+                if (at < uint32_t(a.list_max)) list[at] = make_uint2(ordered(v[u][e]), uint32_t(col0 + 8 * THREADS * u + e));
+                ++at;
             }
-        }
 }
 
-// ---- finish -----------------------------------------------------------------------
-struct Entries {
-    uint64_t comp[kListLds], mass[kListLds];
-    uint16_t bin[kListLds];
-};
+// part_mass[p] = the row mass of the part's bins above `bin`
+__device__ __forceinline__ void sum_parts(const SampleArgs& a, int slot, int bin, RowShared& sh) {
+    const int lane = threadIdx.x & 63;
+    for (int p = threadIdx.x >> 6; p < a.parts; p += kRowWaves) {
+        const int shift = sh.shift[p];
+        uint64_t m = 0;
+        if (shift < 64) {
+            const uint64_t* hist = a.hist + (size_t(slot) * a.parts + p) * kBins;
+            for (int i = bin + 1 + lane + kSub * shift; i <= kTopBin; i += 64) m += row_mass(hist[i] & kMassMask, shift);
+        }
+        m = wave_sum_u64(m);
+        if (lane == 0) sh.part_mass[p] = m;
+    }
+}
+
+struct EntryList { uint64_t comp[kListLds], mass[kListLds]; };
 
 template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a, int row0) {
     const int slot = blockIdx.x, row = row0 + slot, tid = threadIdx.x;
-    RowState* st = a.state + slot;
-    if (st->done) return;
+    const RowState* st = a.state + slot;
+    const int mode = st->plan.mode;
+    if (mode == kDone) return;
     __shared__ RowShared sh;
-    __shared__ Entries en;
-    __shared__ uint32_t s_cnt[256];
-    __shared__ unsigned long long s_mass[256], s_found;
-    __shared__ uint32_t s_digit, s_group;
-    __shared__ uint64_t s_need;
-    __shared__ unsigned long long s_sum;
-    __shared__ int s_bin;
+    __shared__ union { SmallList small; struct { EntryList list; Descent descent; } border; } un;
     const Setting s = setting(a, row);
-    const double J = st->J;
-    load_parts(a, slot, J, sh);
+    const double J = st->plan.J;
+    if (tid < a.parts) load_part(a, slot, tid, s.c, J, sh);
+    if (tid == 0) sh.plan = st->plan;
+    if (tid < kBins) sh.cm[tid] = st->cum_mass[tid];
+    const int n = mode == kModeWalk ? 0 : int(min(st->count, uint32_t(a.list_max)));
+    const uint2* list = a.list + size_t(slot) * a.list_max;
+    const void* src = row_of<TYPE>(a, row);
     __syncthreads();
-    const bool walk = st->walk;
-    const int n = walk ? 0 : int(min(st->count, uint32_t(kListMax)));
-    const uint2* list = a.list + size_t(slot) * kListMax;
-    const auto* src = static_cast<const uint8_t*>(a.logits) + size_t(row) * size_t(a.ld) * kBytes<TYPE>;
-
-    // f(comp, row mass, row bin, part) of a border entry
-    auto entry = [&](float v, int col, auto&& f) {
-        const int part = col / kPart, shift = sh.shift[part];
-        if (shift >= 64) return;
+    const Plan& plan = sh.plan;
+    const uint64_t tq = plan.threshold_q;
+    auto entry_mass = [&](uint32_t key, int col) -> uint64_t {
+        const int part = col / kPart;
         uint64_t m;
-        const int b = bin_mass(v, s.c, sh.j[part], m) - kSub * shift;
-        if (b >= 0) f(comp_of(ordered(v), col), row_mass(m, shift), b, part);
+        return bin_mass(unordered(key), sh.scale[part], m) >= 0 ? row_mass(m, sh.shift[part]) : 0;
     };
-    const bool lds = !walk && n <= kListLds;
+    if (mode == kModeSmall) {
+        const int e = min(n, kSmall);
+        if (tid < e) {
+            const uint2 w = list[tid];
+            un.small.comp[tid] = comp_of<TYPE>(w.x, int(w.y));
+            un.small.mass[tid] = entry_mass(w.x, int(w.y));
+            un.small.val[tid] = unordered(w.x);
+        }
+        finish_small(a, row, s, plan, e, tq, un.small);
+        return;
+    }
+    const bool lds = mode == kModeList && n <= kListLds;
+    EntryList& en = un.border.list;
     if (lds) {
-        for (int i = tid; i < n; i += kRowThreads)
-            entry(unordered(list[i].x), int(list[i].y), [&](uint64_t comp, uint64_t m, int b, int) {
-                en.comp[i] = comp;
-                en.mass[i] = m;
-                en.bin[i] = uint16_t(b);
-            });
+        for (int i = tid; i < n; i += kRowThreads) {
+            const uint2 w = list[i];
+            en.comp[i] = comp_of<TYPE>(w.x, int(w.y));
+            en.mass[i] = entry_mass(w.x, int(w.y));
+        }
         __syncthreads();
     }
-    // every border entry (and, walking the row, every other one) once over the block
-    auto each = [&](auto&& f) {
+    // f(comp, row mass) of the entries with a key in [lo, hi)
+    auto each = [&](uint32_t lo, uint32_t hi, auto&& f) {
         if (lds) {
-            for (int i = tid; i < n; i += kRowThreads)
-                f(en.comp[i], en.mass[i], int(en.bin[i]), int(~uint32_t(en.comp[i])) / kPart);
-        } else if (!walk) {
-            for (int i = tid; i < n; i += kRowThreads) entry(unordered(list[i].x), int(list[i].y), f);
+            for (int i = tid; i < n; i += kRowThreads) {
+                const uint32_t k = comp_key<TYPE>(en.comp[i]);
+                if (k >= lo && k < hi) f(en.comp[i], en.mass[i]);
+            }
+        } else if (mode == kModeList) {
+            for (int i = tid; i < n; i += kRowThreads) {
+                const uint2 w = list[i];
+                if (w.x >= lo && w.x < hi) f(comp_of<TYPE>(w.x, int(w.y)), entry_mass(w.x, int(w.y)));
+            }
         } else {
-            for (int i = tid; i < a.N; i += kRowThreads) entry(load1<TYPE>(src, i), i, f);
+            for (int c0 = tid * 8; c0 < a.N; c0 += kRowThreads * 8) {
+                float v[8];
+                load8<TYPE>(src, c0, a.N, v);
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t k = ordered(v[e]);
+                    if (k >= lo && k < hi && v[e] >= sh.least[(c0 + e) / kPart]) f(comp_of<TYPE>(k, c0 + e), entry_mass(k, c0 + e));
+                }
+            }
         }
     };
-    // The entry of bin `bin` at which, from the largest down, `need` is reached: a count, or a mass.  Byte by byte, the entries that share the prefix counted per next byte
-    // (columns stay below 2^20, so byte 3 of comp is 0xff).  Ends with s_found the comp and s_sum
-    // the mass from the bin's largest entry down to it.
-    auto descend = [&](int bin, bool by_mass, uint64_t need) {
-        uint64_t prefix = 0, known = 0, above = 0;
-        const int shifts[7] = {56, 48, 40, 32, 16, 8, 0};
-        for (int d = 0; d < 7; ++d) {
-            const int sft = shifts[d];
-            if (sft == 16) {
-                prefix |= uint64_t(0xff) << 24;
-                known |= uint64_t(0xff) << 24;
-            }
-            __syncthreads();
-            if (tid < 256) {
-                s_cnt[tid] = 0;
-                s_mass[tid] = 0;
-            }
-            __syncthreads();
-            each([&](uint64_t comp, uint64_t m, int b, int) {
-                if (b != bin || (comp & known) != prefix) return;
-                const int i = int(comp >> sft) & 255;
-                atomicAdd(&s_cnt[i], 1u);
-                atomicAdd(&s_mass[i], (unsigned long long)m);
-            });
-            __syncthreads();
-            if (tid < 64) {
-                // lane l: the digits 255 - 4 l .. 252 - 4 l
-                uint32_t c[4];
-                uint64_t m[4], cs = 0, ms = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = 255 - (4 * tid + e);
-                    c[e] = s_cnt[i];
-                    m[e] = s_mass[i];
-                    cs += c[e];
-                    ms += m[e];
-                }
-                uint64_t cr = cs, mr = ms;
-#pragma unroll
-                for (int k = 1; k < 64; k <<= 1) {
-                    const uint64_t oc = __shfl_up(cr, k, 64), om = __shfl_up(mr, k, 64);
-                    if (tid >= k) { cr += oc; mr += om; }
-                }
-                uint64_t cb = cr - cs, mb = mr - ms;
-                // the bin's entries can sum to a few units less than its parts' sums (which are cut
-                // once per part): then the last entry is the border
-                const uint64_t of = by_mass ? mr : cr;
-                const bool short_of = uint64_t(__shfl(of, 63, 64)) < need;
-                const int last = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(cs != 0) | 1);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint64_t b0 = by_mass ? mb : cb, b1 = by_mass ? mb + m[e] : cb + c[e];
-                    if (short_of ? tid == last && c[e] : b0 < need && b1 >= need) {
-                        s_digit = 255 - (4 * tid + e);
-                        s_group = c[e];
-                        s_need = short_of ? ~uint64_t(0) : need - b0;
-                        s_sum = above + mb;
-                    }
-                    cb += c[e];
-                    mb += m[e];
-                }
-            }
-            __syncthreads();
-            prefix |= uint64_t(s_digit) << sft;
-            known |= uint64_t(0xff) << sft;
-            need = s_need;
-            above = s_sum;
-            if (s_group == 1) break;
-        }
-        __syncthreads();
-        each([&](uint64_t comp, uint64_t m, int b, int) {      // one entry is left
-            if (b == bin && (comp & known) == prefix) {
-                s_found = comp;
-                s_sum = above + m;
-            }
-        });
-        __syncthreads();
-    };
-
-    uint64_t threshold = st->threshold_q;
-    uint64_t kept_k = 0;                                  // mass of the first k
-    if (st->use_k) {
-        const int b = st->bin_k;
-        const uint32_t count_above = b == kTopBin ? 0 : st->cum_count[b + 1];
-        const uint64_t mass_above = b == kTopBin ? 0 : st->cum_mass[b + 1];
-        descend(b, false, uint64_t(s.k) - count_above);
-        threshold = max(threshold, uint64_t(s_found));
-        kept_k = mass_above + s_sum;
+    int bf;
+    const uint64_t threshold = threshold_of<TYPE>(s, plan, sh.cm, tq, each, un.border.descent, sh, bf);
+    sum_parts(a, slot, bf, sh);
+    if (tid < 2 * 64) {
+        const int wv = tid >> 6;
+        const uint32_t edge = bf < 0 || bf + wv > kTopBin ? kKeyEnd : bin_edge(bf + wv, plan.mx, s.c, J);
+        if ((tid & 63) == 0) sh.edge[wv] = edge;
     }
-    if (st->use_p) {
-        const uint64_t of = st->use_k ? kept_k : st->cum_mass[0];
-        const uint64_t f = fraction(s.p);
-        const uint64_t target = max(__umul64hi(f, of) + (f * of != 0), uint64_t(1));
-        if (tid <= kTopBin) {
-            const uint64_t next = tid == kTopBin ? 0 : st->cum_mass[tid + 1];
-            if (st->cum_mass[tid] >= target && next < target) s_bin = tid;
-        }
-        __syncthreads();
-        const int b = s_bin;
-        descend(b, true, target - (b == kTopBin ? 0 : st->cum_mass[b + 1]));
-        threshold = max(threshold, uint64_t(s_found));
-    }
-    __syncthreads();
-    if (tid == 0) {
-        uint64_t unused;
-        s_bin = bin_mass(unordered(uint32_t(threshold >> 32)), s.c, J, unused);
-    }
-    __syncthreads();
-    const int bf = s_bin;
-    sum_parts(a, slot, bf < 0 ? -1 : bf, sh);
     __syncthreads();
     if (bf >= 0)
-        each([&](uint64_t comp, uint64_t m, int b, int part) {
-            if (b == bf && comp >= threshold)
-                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.part_mass[part]), (unsigned long long)m);
+        each(sh.edge[0], sh.edge[1], [&](uint64_t comp, uint64_t m) {
+            if (comp >= threshold)
+                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.part_mass[comp_col(comp) / kPart]), (unsigned long long)m);
         });
     __syncthreads();
-    draw<TYPE>(a, row, s, J, threshold, sh);
+    draw_part(a.parts, s, sh);
+    const int part = sh.part;
+    if (part < 0) {                                   // (logits that changed under the call)
+        if (tid == 0) give(a, row, -1, __builtin_nanf(""));
+        return;
+    }
+    float v[kPer];
+    const int col0 = part * kPart + tid * kPer;
+    load8<TYPE>(src, col0, a.N, v);
+    draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], threshold, v, col0, sh);
+}
+
+// Rows of one part: all of it by one block, the logits in LDS after the histogram.
+template <int TYPE>
+__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
+    const int row = blockIdx.x, tid = threadIdx.x;
+    __shared__ RowShared sh;
+    __shared__ union { PartShared<kRowThreads> part; SmallList small; Descent descent; } un;
+    __shared__ __attribute__((aligned(16))) float s_v[kPart];
+    __shared__ uint32_t s_count;
+    const int col0 = tid * kPer;
+    float v[1][kPer];
+    load8<TYPE>(row_of<TYPE>(a, row), col0, a.N, v[0]);
+    const Setting s = setting(a, row);
+    const PartMeta m = part_pass<kRowThreads, 1>(a, s, v, col0, un.part);
+    if (!s.valid || !m.key || s.T == 0.f) {
+        if (tid == 0) {
+            const bool fine = s.valid && m.key;
+            give(a, row, fine ? m.arg : -1, fine ? 0.f : __builtin_nanf(""));
+            flag_or(a.flags, !s.valid ? kSampleSetting : !m.key ? kSampleEmpty : 0u);
+        }
+        return;
+    }
+    const double J = m.j;
+    const Scale k = scale_of(s.c, J);
+    uint64_t threshold = 0;
+    if (s.cut) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) s_v[col0 + e] = v[0][e];
+        if (tid == 0) s_count = 0;
+        __syncthreads();
+        const uint64_t w = tid <= kTopBin ? un.part.hist[kTopBin - tid] : 0;
+        cumulate(row_mass(w & kMassMask, 0), uint32_t(w >> kMassBits), sh);
+        borders(a, s, unordered(m.key), J, kPart, sh);
+        const Plan& plan = sh.plan;
+        threshold = s.q > 0.f ? q_threshold<TYPE>(sh.qkey) : 0;
+        auto mass_of = [&](float x) -> uint64_t {
+            uint64_t e;
+            return bin_mass(x, k, e) >= 0 ? row_mass(e, 0) : 0;
+        };
+        if (plan.mode == kModeSmall) {
+            for (int c = tid; c < a.N; c += kRowThreads) {
+                const float x = s_v[c];
+                const uint32_t key = ordered(x);
+                if (x >= m.least && in_ranges(plan, key)) {
+                    const uint32_t at = atomicAdd(&s_count, 1u);
+                    if (at < uint32_t(kSmall)) {
+                        un.small.comp[at] = comp_of<TYPE>(key, c);
+                        un.small.mass[at] = mass_of(x);
+                        un.small.val[at] = x;
+                    }
+                }
+            }
+            __syncthreads();
+            finish_small(a, row, s, plan, min(int(s_count), kSmall), threshold, un.small);
+            return;
+        }
+        auto each = [&](uint32_t lo, uint32_t hi, auto&& f) {
+            for (int c = tid; c < a.N; c += kRowThreads) {
+                const float x = s_v[c];
+                const uint32_t key = ordered(x);
+                if (key >= lo && key < hi && x >= m.least) f(comp_of<TYPE>(key, c), mass_of(x));
+            }
+        };
+        int bf;
+        threshold = threshold_of<TYPE>(s, plan, sh.cm, threshold, each, un.descent, sh, bf);
+    }
+    // the kept mass, and the token
+    uint64_t sum = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        uint64_t x;
+        const int bin = bin_mass(v[0][e], k, x);
+        if (bin >= 0 && v[0][e] >= m.least && comp_of<TYPE>(ordered(v[0][e]), col0 + e) >= threshold) sum += x;
+    }
+    sum = wave_sum_u64(sum);
+    __syncthreads();
+    if ((tid & 63) == 0) sh.wave_mass[tid >> 6] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        uint64_t total = 0;
+#pragma unroll
+        for (int w = 0; w < kRowWaves; ++w) total += sh.wave_mass[w];
+        sh.total = row_mass(total, 0);
+        sh.rest = __umul64hi(fraction(s.u), sh.total);
+    }
+    __syncthreads();
+    draw_column<TYPE>(a, row, s, J, k, m.least, 0, threshold, v[0], col0, sh);
 }
 
 // rows of an empty vocabulary
@@ -741,30 +1186,53 @@ __global__ __launch_bounds__(64) void sample_empty_kernel(int M, int64_t* token,
     if (threadIdx.x == 0) flag_or(flags, kSampleEmpty);
 }
 
-struct SampleLayout { size_t hist, meta, state, list, bytes; };
+int sample_parts_of(int N) { return (N + kPart - 1) / kPart; }
+// rows that share the workspace at once: at least 64, and 1024 parts
+int sample_chunk(int N) { return std::max(64, 1024 / std::max(sample_parts_of(N), 1)); }
+
+struct SampleLayout { size_t hist, meta, state, list, bytes; int list_max; };
 SampleLayout sample_layout(int Mcap, int N) {
     SampleLayout l{};
-    const size_t rows = size_t(Mcap < kChunkRows ? Mcap : kChunkRows), parts = (size_t(N) + kPart - 1) / kPart;
+    const int parts = sample_parts_of(N);
+    if (parts <= 1) return l;                        // one launch, nothing between blocks
+    const size_t rows = size_t(std::min(Mcap, sample_chunk(N)));
     size_t cursor = 0;
     auto add = [&](size_t& field, size_t bytes) { field = cursor; cursor = align256(cursor + bytes); };
+    l.list_max = std::min(N, kListMax);
     add(l.hist, rows * parts * kBins * 8);
     add(l.meta, rows * parts * sizeof(PartMeta));
     add(l.state, rows * sizeof(RowState));
-    add(l.list, rows * size_t(kListMax) * 8);
+    add(l.list, rows * size_t(l.list_max) * 8);
     l.bytes = cursor;
     return l;
 }
 
 template <int TYPE> hipError_t sample_rows(const SampleArgs& a, int row0, int rows, hipStream_t s) {
     const dim3 parts(a.parts, rows);
-    timed_launch("sample_parts", sample_parts_kernel<TYPE>, parts, dim3(kPartThreads), 0, s, a, row0);
+    const bool few = a.parts * rows <= 2 * device_cu_count();
+    if (few) timed_launch("sample_parts", sample_parts_kernel<TYPE, 1024>, parts, dim3(1024), 0, s, a, row0);
+    else timed_launch("sample_parts", sample_parts_kernel<TYPE, 256>, parts, dim3(256), 0, s, a, row0);
     timed_launch("sample_select", sample_select_kernel<TYPE>, dim3(rows), dim3(kRowThreads), 0, s, a, row0);
     hipError_t st = hipGetLastError();
     // with no cut at all, select has drawn every row
     if (st != hipSuccess || (!a.top_k && !a.top_p && !a.min_p)) return st;
-    timed_launch("sample_gather", sample_gather_kernel<TYPE>, parts, dim3(kPartThreads), 0, s, a, row0);
+    if (few) timed_launch("sample_gather", sample_gather_kernel<TYPE, 1024>, parts, dim3(1024), 0, s, a, row0);
+    else timed_launch("sample_gather", sample_gather_kernel<TYPE, 256>, parts, dim3(256), 0, s, a, row0);
     timed_launch("sample_finish", sample_finish_kernel<TYPE>, dim3(rows), dim3(kRowThreads), 0, s, a, row0);
     return hipGetLastError();
+}
+
+template <int TYPE> hipError_t sample_all(const SampleArgs& a, int M, hipStream_t s) {
+    if (a.parts == 1) {
+        timed_launch("sample_row", sample_row_kernel<TYPE>, dim3(M), dim3(kRowThreads), 0, s, a);
+        return hipGetLastError();
+    }
+    const int chunk = sample_chunk(a.N);
+    for (int r = 0; r < M; r += chunk) {
+        const hipError_t st = sample_rows<TYPE>(a, r, std::min(M - r, chunk), s);
+        if (st != hipSuccess) return st;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
@@ -806,18 +1274,13 @@ extern "C" hipError_t ornith_logits_sample_launch(const void* logits, int logits
                      static_cast<int64_t*>(token), static_cast<float*>(logprob), static_cast<uint32_t*>(flags));
         return hipGetLastError();
     }
-    const SampleArgs a{logits, ld, N, (N + kPart - 1) / kPart, static_cast<const float*>(uniform),
+    const SampleArgs a{logits, ld, N, sample_parts_of(N), l.list_max, static_cast<const float*>(uniform),
                        static_cast<const float*>(temperature), static_cast<const int32_t*>(top_k),
                        static_cast<const float*>(top_p), static_cast<const float*>(min_p),
                        at<uint64_t>(workspace, l.hist), at<PartMeta>(workspace, l.meta),
                        at<RowState>(workspace, l.state), at<uint2>(workspace, l.list),
                        static_cast<int64_t*>(token), static_cast<float*>(logprob), static_cast<uint32_t*>(flags)};
-    for (int r = 0; r < M; r += kChunkRows) {
-        const int rows = M - r < kChunkRows ? M - r : kChunkRows;
-        const hipError_t st = logits_type == ORNITH_LOGITS_BF16  ? sample_rows<ORNITH_LOGITS_BF16>(a, r, rows, stream)
-                              : logits_type == ORNITH_LOGITS_F16 ? sample_rows<ORNITH_LOGITS_F16>(a, r, rows, stream)
-                                                                 : sample_rows<ORNITH_LOGITS_F32>(a, r, rows, stream);
-        if (st != hipSuccess) return st;
-    }
-    return hipSuccess;
+    if (logits_type == ORNITH_LOGITS_BF16) return sample_all<ORNITH_LOGITS_BF16>(a, M, stream);
+    if (logits_type == ORNITH_LOGITS_F16) return sample_all<ORNITH_LOGITS_F16>(a, M, stream);
+    return sample_all<ORNITH_LOGITS_F32>(a, M, stream);
 }

@@ -21,19 +21,21 @@ def test_layout(lib):
     size = C.c_size_t(0)
     q = lib.ornith_logits_sample_get_layout
     assert q(64, 248320, C.byref(size)) == 0 and size.value > 0
-    assert q(0, 100, C.byref(size)) == 0 and size.value == 0
+    assert q(0, 10000, C.byref(size)) == 0 and size.value == 0
     assert q(1, 1 << 20, C.byref(size)) == 0
     for bad in ((-1, 10), (1, -1), (1, (1 << 20) + 1)):
         assert q(*bad, C.byref(size)) == INVALID
     assert q(1, 10, None) == INVALID
-    # rows past 64 share what 64 use
-    assert native.logits_sample_bytes(64, 5000) == native.logits_sample_bytes(4000, 5000)
-    assert native.logits_sample_bytes(2, 5000) < native.logits_sample_bytes(3, 5000)
+    # rows of up to 8192 columns need none; many rows share what some use
+    assert native.logits_sample_bytes(64, 8192) == 0 < native.logits_sample_bytes(1, 8193)
+    assert native.logits_sample_bytes(1024, 10000) == native.logits_sample_bytes(4000, 10000)
+    assert native.logits_sample_bytes(64, 248320) == native.logits_sample_bytes(65, 248320)
+    assert native.logits_sample_bytes(2, 10000) < native.logits_sample_bytes(3, 10000)
 
 
 def _args(**kw):
     p = C.c_void_p
-    a = dict(logits=p(0x10000), type=0, M=2, N=100, ld=100, uniform=p(0x20000), T=p(0x21000), k=p(0x22000),
+    a = dict(logits=p(0x10000), type=0, M=2, N=10000, ld=10000, uniform=p(0x20000), T=p(0x21000), k=p(0x22000),
              p=p(0x23000), q=p(0x24000), ws=p(0x1000000), bytes=1 << 22, token=p(0x30000), logprob=p(0x31000),
              flags=p(0x32000), stream=None)
     assert set(kw) <= set(a)
@@ -42,7 +44,7 @@ def _args(**kw):
 
 
 @pytest.mark.parametrize('bad', [dict(type=3), dict(type=-1), dict(M=-1), dict(N=-1), dict(N=(1 << 20) + 1, ld=1 << 21),
-                                 dict(ld=99), dict(bytes=1000), dict(logits=None), dict(uniform=None),
+                                 dict(ld=9999), dict(bytes=1000), dict(logits=None), dict(uniform=None),
                                  dict(token=None), dict(flags=None), dict(ws=None), dict(logits=C.c_void_p(0x10001)),
                                  dict(type=2, logits=C.c_void_p(0x10002)), dict(uniform=C.c_void_p(0x20002)),
                                  dict(token=C.c_void_p(0x30004)), dict(ws=C.c_void_p(0x1000080)),
