@@ -92,37 +92,42 @@ template <int TYPE> constexpr int kDrop = TYPE == ORNITH_LOGITS_F32 ? 0 : TYPE =
 template <int TYPE> __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row) {
     return static_cast<const uint8_t*>(a.logits) + size_t(row) * size_t(a.ld) * kBytes<TYPE>;
 }
-template <int TYPE> __device__ __forceinline__ float load1(const void* row, int col) {
-    if constexpr (TYPE == ORNITH_LOGITS_F32) return static_cast<const float*>(row)[col];
-    const uint32_t b = static_cast<const uint16_t*>(row)[col];
-    return TYPE == ORNITH_LOGITS_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
-}
+// Eight consecutive columns in the type's own bits (half the registers for the 16-bit types).
 // Rows start at any element: 16-byte loads of element-aligned memory.
 struct __attribute__((packed, aligned(2))) Raw16 { uint32_t w[4]; };
-// Eight columns from col; columns at or past N read as -inf.
-template <int TYPE> __device__ __forceinline__ void load8(const void* row, int col, int N, float (&v)[8]) {
-    if (col + 8 <= N) {
-        const auto* p = reinterpret_cast<const Raw16*>(static_cast<const uint8_t*>(row) + size_t(col) * kBytes<TYPE>);
-        if constexpr (TYPE == ORNITH_LOGITS_F32) {
-            const Raw16 a = p[0], b = p[1];
+template <int TYPE> struct Piece {
+    static constexpr int kWords = TYPE == ORNITH_LOGITS_F32 ? 8 : 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ float operator[](int e) const {
+        if constexpr (TYPE == ORNITH_LOGITS_F32) return __uint_as_float(w[e]);
+        if constexpr (TYPE == ORNITH_LOGITS_BF16)
+            return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        return f16_bits_to_f32((w[e >> 1] >> (16 * (e & 1))) & 0xffffu);
+    }
+    // columns at or past N read as -inf
+    __device__ __forceinline__ void load(const void* row, int col, int N) {
+        if (col + 8 <= N) {
+            const auto* p = reinterpret_cast<const Raw16*>(static_cast<const uint8_t*>(row) + size_t(col) * kBytes<TYPE>);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = __uint_as_float(a.w[e]);
-                v[4 + e] = __uint_as_float(b.w[e]);
+            for (int h = 0; h < kWords / 4; ++h) {
+                const Raw16 r = p[h];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[4 * h + i] = r.w[i];
             }
         } else {
-            const Raw16 a = p[0];
+            constexpr uint32_t none = TYPE == ORNITH_LOGITS_F32 ? 0xff800000u : TYPE == ORNITH_LOGITS_BF16 ? 0xff80u : 0xfc00u;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t b = (a.w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
-                v[e] = TYPE == ORNITH_LOGITS_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+            for (int i = 0; i < kWords; ++i) {
+                if constexpr (TYPE == ORNITH_LOGITS_F32) w[i] = col + i < N ? static_cast<const uint32_t*>(row)[col + i] : none;
+                else {
+                    const auto* h = static_cast<const uint16_t*>(row);
+                    const uint32_t lo = col + 2 * i < N ? h[col + 2 * i] : none, hi = col + 2 * i + 1 < N ? h[col + 2 * i + 1] : none;
+                    w[i] = lo | (hi << 16);
+                }
             }
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = col + e < N ? load1<TYPE>(row, col + e) : -__builtin_huge_valf();
     }
-}
+};
 
 // Bits ordered as the values are (-0 as +0; never 0 for a value above -inf).
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -264,8 +269,8 @@ template <int THREADS> struct PartShared {
 // Histogram (cut rows), whole mass (others) or first maximum (greedy) of the values that the
 // block's threads hold, eight consecutive columns a piece.  The histogram is complete after the
 // caller's next barrier; of a cut row, it lacks values that no cut can keep.
-template <int THREADS, int PIECES>
-__device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting& s, const float (&v)[PIECES][8],
+template <int TYPE, int THREADS, int PIECES>
+__device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting& s, const Piece<TYPE> (&v)[PIECES],
                                               int col0, PartShared<THREADS>& sh) {
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     constexpr int W = THREADS / 64;
@@ -392,11 +397,11 @@ __global__ __launch_bounds__(THREADS) void sample_parts_kernel(SampleArgs a, int
     constexpr int kPieces = kPart / 8 / THREADS;
     const void* src = row_of<TYPE>(a, row);
     const int col0 = part * kPart + tid * 8;
-    float v[kPieces][8];
+    Piece<TYPE> v[kPieces];
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) load8<TYPE>(src, col0 + 8 * THREADS * u, a.N, v[u]);
+    for (int u = 0; u < kPieces; ++u) v[u].load(src, col0 + 8 * THREADS * u, a.N);
     const Setting s = setting(a, row);
-    const PartMeta m = part_pass<THREADS, kPieces>(a, s, v, col0, sh);
+    const PartMeta m = part_pass<TYPE, THREADS, kPieces>(a, s, v, col0, sh);
     __syncthreads();
     const size_t at = size_t(slot) * a.parts + part;
     if (tid == 0) a.meta[at] = m;
@@ -429,6 +434,19 @@ __device__ __forceinline__ PartMeta load_part(const SampleArgs& a, int slot, int
     sh.least[p] = m.least;
     return m;
 }
+// Sums of the waves before this one, and of all, from every wave's own (in LDS, after a barrier).
+__device__ __forceinline__ uint64_t waves_before(const uint64_t (&w)[kRowWaves], uint64_t& all) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t own = lane < kRowWaves ? w[lane] : 0, run = wave_prefix_u64(own);
+    all = readlane_u64(run, kRowWaves - 1);
+    return readlane_u64(run - own, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+}
+__device__ __forceinline__ uint32_t waves_before(const uint32_t (&w)[kRowWaves], uint32_t& all) {
+    const int lane = threadIdx.x & 63;
+    const int own = lane < kRowWaves ? int(w[lane]) : 0, run = wave_prefix_sum(own);
+    all = uint32_t(__builtin_amdgcn_readlane(run, kRowWaves - 1));
+    return uint32_t(__builtin_amdgcn_readlane(run - own, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)));
+}
 // Thread i <= kTopBin holds bin kTopBin - i's mass and count: cm and cc (after the barriers in it).
 __device__ __forceinline__ void cumulate(uint64_t mass, uint32_t count, RowShared& sh) {
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -447,13 +465,15 @@ __device__ __forceinline__ void cumulate(uint64_t mass, uint32_t count, RowShare
         sh.part = -1;
     }
     __syncthreads();
-    if (tid <= kTopBin) {
-        for (int w = 0; w < wv; ++w) {
-            mass += sh.wave_mass[w];
-            count += sh.wave_count[w];
+    if (wv < W) {
+        uint64_t mass_all;
+        uint32_t count_all;
+        mass += waves_before(sh.wave_mass, mass_all);
+        count += waves_before(sh.wave_count, count_all);
+        if (tid <= kTopBin) {
+            sh.cm[kTopBin - tid] = mass;
+            sh.cc[kTopBin - tid] = count;
         }
-        sh.cm[kTopBin - tid] = mass;
-        sh.cc[kTopBin - tid] = count;
     }
     __syncthreads();
 }
@@ -593,91 +613,166 @@ __device__ __forceinline__ void draw_part(int parts, const Setting& s, RowShared
     __syncthreads();
 }
 // The token inside the part: thread i holds its columns col0 .. col0 + 7, ascending over the block.
+// Where at most an eighth of the part is kept, those values are set side by side in LDS first: one
+// mass a thread, not eight.
+struct DrawShared { float val[kRowThreads]; uint16_t col[kRowThreads]; };
 template <int TYPE>
 __device__ __forceinline__ void draw_column(const SampleArgs& a, int row, const Setting& s, double J, const Scale& k,
-                                            float least, int shift, uint64_t threshold, const float (&v)[kPer], int col0, RowShared& sh) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+                                            float least, int shift, uint64_t threshold, const Piece<TYPE>& v, int col0,
+                                            RowShared& sh, DrawShared& ds) {
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const uint64_t rest = sh.rest, total = sh.total;
+    uint32_t keep = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+        keep |= uint32_t(v[e] >= least && comp_of<TYPE>(ordered(v[e]), col0 + e) >= threshold) << e;
+    const uint32_t own = uint32_t(__popc(keep));
+    uint32_t at = uint32_t(wave_prefix_sum(int(own))), kept;
+    if (lane == 63) sh.wave_count[wv] = at;
+    __syncthreads();
+    at += waves_before(sh.wave_count, kept) - own;
+    auto mass_of = [&](float x) -> uint64_t {
+        uint64_t m;
+        return bin_mass(x, k, m) >= 0 ? m : 0;
+    };
+    // sums up to and including a thread's
+    auto upto = [&](uint64_t sum) -> uint64_t {
+        const uint64_t run = wave_prefix_u64(sum);
+        if (lane == 63) sh.wave_mass[wv] = run;
+        __syncthreads();
+        uint64_t all;
+        return run + waves_before(sh.wave_mass, all);
+    };
+    if (kept <= uint32_t(kRowThreads)) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+            if (keep >> e & 1) {
+                ds.val[at] = v[e];
+                ds.col[at] = uint16_t(tid * kPer + e);
+                ++at;
+            }
+        __syncthreads();
+        const bool live = uint32_t(tid) < kept;
+        const float x = live ? ds.val[tid] : 0.f;
+        const uint64_t m = live ? mass_of(x) : 0, run = upto(m);
+        if (row_mass(run, shift) > rest && row_mass(run - m, shift) <= rest)
+            give(a, row, col0 - tid * kPer + ds.col[tid], log_share(x, s, J, row_mass(m, shift), total));
+        return;
+    }
     uint64_t m[kPer], sum = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-        const int bin = bin_mass(v[e], k, m[e]);
-        if (bin < 0 || !(v[e] >= least) || comp_of<TYPE>(ordered(v[e]), col0 + e) < threshold) m[e] = 0;
+        m[e] = keep >> e & 1 ? mass_of(v[e]) : 0;
         sum += m[e];
     }
-    uint64_t run = wave_prefix_u64(sum);
-    if (lane == 63) sh.wave_mass[wv] = run;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kRowWaves; ++w) run += w < wv ? sh.wave_mass[w] : 0;
-    const uint64_t rest = sh.rest;
+    const uint64_t run = upto(sum);
     if (row_mass(run, shift) > rest && row_mass(run - sum, shift) <= rest) {
-        uint64_t at = run - sum;
-        int col = 0;
+        uint64_t before = run - sum, mass = 0;
+        int col = -1;
         float val = 0.f;
-        uint64_t mass = 0;
 #pragma unroll
-        for (int e = kPer - 1; e >= 0; --e) {
-            uint64_t upto = at;
-#pragma unroll
-            for (int f = 0; f <= e; ++f) upto += m[f];
-            if (row_mass(upto, shift) > rest) {
+        for (int e = 0; e < kPer; ++e) {
+            before += m[e];
+            if (col < 0 && row_mass(before, shift) > rest) {
                 col = col0 + e;
                 val = v[e];
                 mass = m[e];
             }
         }
-        give(a, row, col, log_share(val, s, J, row_mass(mass, shift), sh.total));
+        give(a, row, col, log_share(val, s, J, row_mass(mass, shift), total));
     }
 }
 
-// A list of every candidate (n <= kSmall): cuts and draw by ranks, four threads an entry.
-struct SmallList { uint64_t comp[kSmall], mass[kSmall]; float val[kSmall]; unsigned long long k, k_mass, p; };
+// A list of every candidate (n <= kSmall, zeros past n): each entry's rank by value and by column
+// (four threads an entry), then one wave walks both orders, four entries a lane.
+struct SmallList {
+    uint64_t comp[kSmall], mass[kSmall], by_value[kSmall], by_column[kSmall];
+    uint8_t at[kSmall];                               // the entry of a column rank
+    float val[kSmall];
+    uint32_t rank[kSmall];
+};
 __device__ __forceinline__ void finish_small(const SampleArgs& a, int row, const Setting& s, const Plan& plan, int n,
                                              uint64_t threshold, SmallList& sl) {
     const int tid = threadIdx.x, e = tid >> 2;
-    if (tid == 0) {
-        sl.k = 0;
-        sl.p = 0;
-        sl.k_mass = plan.total;
+    __syncthreads();
+    const int end = (n + 31) & ~31;
+    if ((tid & ~63) < 4 * end) {                      // (whole waves)
+        const uint64_t comp = sl.comp[e];
+        const uint32_t col = uint32_t(comp) & kColMask;
+        uint32_t by_value = 0, by_column = 0;
+#pragma unroll 8
+        for (int i = tid & 3; i < end; i += 4) {
+            const uint64_t c = sl.comp[i];
+            by_value += c > comp;
+            by_column += (uint32_t(c) & kColMask) > col;      // (complements: lower columns)
+        }
+        by_value += uint32_t(dpp_i<kDppXor1>(int(by_value)));
+        by_value += uint32_t(dpp_i<kDppXor2>(int(by_value)));
+        by_column += uint32_t(dpp_i<kDppXor1>(int(by_column)));
+        by_column += uint32_t(dpp_i<kDppXor2>(int(by_column)));
+        if (e < n && (tid & 3) == 0) {
+            sl.by_value[by_value] = sl.mass[e];
+            sl.rank[e] = by_value;
+            sl.at[by_column] = uint8_t(e);
+        }
     }
     __syncthreads();
-    auto quad = [](uint64_t v) {
-        v += dpp_u64<kDppXor1, 0xF>(v);
-        return v + dpp_u64<kDppXor2, 0xF>(v);
+    if (tid >= 64) return;
+    constexpr int per = kSmall / 64;
+    static_assert(kSmall == 256, "four entries a lane, a byte an entry");
+    uint64_t m[per], sum = 0;
+    auto walk = [&](auto&& mass_of) {                 // m[i]: sums up to entry per * tid + i
+        sum = 0;
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+            const int r = per * tid + i;
+            sum += r < n ? mass_of(r) : 0;
+            m[i] = sum;
+        }
+        const uint64_t before = wave_prefix_u64(sum) - sum;
+#pragma unroll
+        for (int i = 0; i < per; ++i) m[i] += before;
     };
-    const bool live = e < n;
-    const uint64_t comp = live ? sl.comp[e] : 0, mass = live ? sl.mass[e] : 0;
-    uint64_t count = 0, before = 0;
-    for (int i = tid & 3; i < n; i += 4) {
-        const bool b = sl.comp[i] > comp;
-        count += b;
-        before += b ? sl.mass[i] : 0;
+    walk([&](int r) { return sl.by_value[r]; });
+    // how many the cuts keep
+    int keep = n;
+    uint64_t of = plan.total;
+    if (plan.use_k) {
+        keep = min(keep, s.k);
+        const int lane = (keep - 1) / per, i = (keep - 1) % per;
+        const uint64_t at = i == 0 ? m[0] : i == 1 ? m[1] : i == 2 ? m[2] : m[3];
+        of = readlane_u64(at, __builtin_amdgcn_readfirstlane(lane));
     }
-    count = quad(count);
-    before = quad(before);
-    if (plan.use_k && live && count == uint64_t(s.k) - 1) {
-        sl.k = comp;
-        sl.k_mass = before + mass;
-    }
-    __syncthreads();
     if (plan.use_p) {
-        // (entries can sum to a few units less than their bins, whose sums are cut once per part: then all are kept)
-        const uint64_t target = share(s.p, sl.k_mass);
-        if (live && before < target && before + mass >= target) sl.p = comp;
-        __syncthreads();
+        // (the entries can sum to a few units less than their bins, which are cut once per part: then all stay)
+        const uint64_t target = share(s.p, of);
+        int below = 0;
+#pragma unroll
+        for (int i = 0; i < per; ++i) below += __popcll(__builtin_amdgcn_ballot_w64(per * tid + i < n && m[i] < target));
+        keep = min(keep, below + 1);
     }
-    threshold = max(threshold, max(uint64_t(sl.k), uint64_t(sl.p)));
-    uint64_t total = 0, run = 0;
-    for (int i = tid & 3; i < n; i += 4) {
-        const uint64_t m = sl.comp[i] >= threshold ? sl.mass[i] : 0;
-        total += m;
-        run += (sl.comp[i] & kColMask) >= (comp & kColMask) ? m : 0;      // columns up to this one
+    if (threshold) {
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < per; ++i)
+            above += __popcll(__builtin_amdgcn_ballot_w64(per * tid + i < n && sl.comp[per * tid + i] >= threshold));
+        keep = min(keep, above);
     }
-    total = quad(total);
-    run = quad(run);
-    const uint64_t target = __umul64hi(fraction(s.u), total);
-    if (live && comp >= threshold && (tid & 3) == 0 && run > target && run - mass <= target)
-        give(a, row, comp_col(comp), log_share(sl.val[e], s, plan.J, mass, total));
+    walk([&](int r) {
+        const int x = sl.at[r];
+        return sl.rank[x] < uint32_t(keep) ? sl.mass[x] : 0;
+    });
+    const uint64_t total = readlane_u64(m[per - 1], 63), target = __umul64hi(fraction(s.u), total);
+#pragma unroll
+    for (int i = 0; i < per; ++i) {
+        const int r = per * tid + i;
+        if (r < n) {
+            const int x = sl.at[r];
+            const uint64_t mass = sl.rank[x] < uint32_t(keep) ? sl.mass[x] : 0;
+            if (m[i] > target && m[i] - mass <= target)
+                give(a, row, comp_col(sl.comp[x]), log_share(sl.val[x], s, plan.J, mass, total));
+        }
+    }
 }
 
 // Descent to a border inside one bin's key range: the entry at which, from the largest down, `need`
@@ -707,6 +802,10 @@ __device__ __forceinline__ void descend(uint32_t lo, uint32_t hi, bool by_mass, 
         __syncthreads();
         d.count[tid] = 0;
         d.mass[tid] = 0;
+        if (tid < 64) {
+            d.comp[tid] = 0;
+            d.m[tid] = 0;
+        }
         if (tid == 0) {
             d.n = 0;
             d.group = 0;
@@ -730,15 +829,10 @@ __device__ __forceinline__ void descend(uint32_t lo, uint32_t hi, bool by_mass, 
             d.wave_mass[wv] = mr;
         }
         __syncthreads();
-        uint32_t call = 0;
-        uint64_t mall = 0;
-#pragma unroll
-        for (int w = 0; w < kRowWaves; ++w) {
-            cr += w < wv ? d.wave_count[w] : 0;
-            mr += w < wv ? d.wave_mass[w] : 0;
-            call += d.wave_count[w];
-            mall += d.wave_mass[w];
-        }
+        uint32_t call;
+        uint64_t mall;
+        cr += waves_before(d.wave_count, call);
+        mr += waves_before(d.wave_mass, mall);
         // the entries can sum to a few units less than their bin (cut once per part): then the last is the border
         const bool short_of = by_mass ? mall < need : call < need;
         const uint64_t b0 = by_mass ? mr - m : cr - c, b1 = by_mass ? mr : cr;
@@ -776,10 +870,13 @@ __device__ __forceinline__ void descend(uint32_t lo, uint32_t hi, bool by_mass, 
     if (tid < 64) {
         const uint64_t comp = tid < n ? d.comp[tid] : 0, m = tid < n ? d.m[tid] : 0;
         uint64_t count = 0, before = 0;
-        for (int i = 0; i < n; ++i) {
+        // (zeros past n: the loads of eight steps in flight at once)
+#pragma unroll 8
+        for (int i = 0; i < 64; ++i) {
+            const uint64_t mi = d.m[i];
             const bool b = d.comp[i] > comp;
             count += b;
-            before += b ? d.m[i] : 0;
+            before += b ? mi : 0;
         }
         const bool at = by_mass ? before < need && before + m >= need : count + 1 == need;
         const bool any = __builtin_amdgcn_ballot_w64(tid < n && at);
@@ -843,6 +940,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(SampleArgs a
     __shared__ RowShared sh;
     __shared__ uint64_t s_mass[2][kTopBin + 24];
     __shared__ uint32_t s_count[2][kTopBin + 24];
+    __shared__ DrawShared s_draw;
     RowState* st = a.state + slot;
     const Setting s = setting(a, row);
     const PartMeta* meta = a.meta + size_t(slot) * a.parts;
@@ -880,10 +978,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(SampleArgs a
             if (tid == 0) give(a, row, -1, __builtin_nanf(""));
             return;
         }
-        float v[kPer];
+        Piece<TYPE> v;
         const int col0 = part * kPart + tid * kPer;
-        load8<TYPE>(row_of<TYPE>(a, row), col0, a.N, v);
-        draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], 0, v, col0, sh);
+        v.load(row_of<TYPE>(a, row), col0, a.N);
+        draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], 0, v, col0, sh, s_draw);
         return;
     }
     // the parts' bins: three groups of threads, a third of the parts each
@@ -944,9 +1042,9 @@ __global__ __launch_bounds__(THREADS) void sample_gather_kernel(SampleArgs a, in
     uint2* list = a.list + size_t(slot) * a.list_max;
     constexpr int kPieces = kPart / 8 / THREADS;
     const int col0 = part * kPart + tid * 8;
-    float v[kPieces][8];
+    Piece<TYPE> v[kPieces];
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) load8<TYPE>(src, col0 + 8 * THREADS * u, a.N, v[u]);
+    for (int u = 0; u < kPieces; ++u) v[u].load(src, col0 + 8 * THREADS * u, a.N);
     // the block takes its place in the list with one addition
     uint32_t in = 0;
 #pragma unroll
@@ -977,18 +1075,37 @@ __global__ __launch_bounds__(THREADS) void sample_gather_kernel(SampleArgs a, in
             }
 }
 
-// part_mass[p] = the row mass of the part's bins above `bin`
-__device__ __forceinline__ void sum_parts(const SampleArgs& a, int slot, int bin, RowShared& sh) {
-    const int lane = threadIdx.x & 63;
-    for (int p = threadIdx.x >> 6; p < a.parts; p += kRowWaves) {
+// The parts' histograms, in registers ahead of the border they are cut at: lane l of a wave holds
+// bins l, l + 64, .. of parts wave, wave + 16 (rows of more parts load the others when they sum).
+constexpr int kAhead = 2, kBinSteps = (kTopBin + 64) / 64;
+__device__ __forceinline__ void load_bins(const SampleArgs& a, int slot, int p, uint64_t (&w)[kBinSteps]) {
+    const uint64_t* hist = a.hist + (size_t(slot) * a.parts + p) * kBins;
+#pragma unroll
+    for (int i = 0; i < kBinSteps; ++i) {
+        const int b = 64 * i + int(threadIdx.x & 63);
+        w[i] = p < a.parts && b <= kTopBin ? hist[b] : 0;
+    }
+}
+// part_mass[p] = the row mass of the part's bins above `bin` of the row
+__device__ __forceinline__ void sum_parts(const SampleArgs& a, int slot, int bin, uint64_t (&ahead)[kAhead][kBinSteps],
+                                          RowShared& sh) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    auto sum = [&](int p, const uint64_t (&w)[kBinSteps]) {
         const int shift = sh.shift[p];
         uint64_t m = 0;
-        if (shift < 64) {
-            const uint64_t* hist = a.hist + (size_t(slot) * a.parts + p) * kBins;
-            for (int i = bin + 1 + lane + kSub * shift; i <= kTopBin; i += 64) m += row_mass(hist[i] & kMassMask, shift);
-        }
+#pragma unroll
+        for (int i = 0; i < kBinSteps; ++i)
+            m += 64 * i + lane > bin + kSub * shift ? row_mass(w[i] & kMassMask, shift) : 0;
         m = wave_sum_u64(m);
         if (lane == 0) sh.part_mass[p] = m;
+    };
+#pragma unroll
+    for (int h = 0; h < kAhead; ++h)
+        if (wv + h * kRowWaves < a.parts) sum(wv + h * kRowWaves, ahead[h]);
+    for (int p = wv + kAhead * kRowWaves; p < a.parts; p += kRowWaves) {
+        uint64_t w[kBinSteps];
+        load_bins(a, slot, p, w);
+        sum(p, w);
     }
 }
 
@@ -998,42 +1115,48 @@ template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a, int row0) {
     const int slot = blockIdx.x, row = row0 + slot, tid = threadIdx.x;
     const RowState* st = a.state + slot;
-    const int mode = st->plan.mode;
-    if (mode == kDone) return;
     __shared__ RowShared sh;
-    __shared__ union { SmallList small; struct { EntryList list; Descent descent; } border; } un;
-    const Setting s = setting(a, row);
-    const double J = st->plan.J;
-    if (tid < a.parts) load_part(a, slot, tid, s.c, J, sh);
-    if (tid == 0) sh.plan = st->plan;
-    if (tid < kBins) sh.cm[tid] = st->cum_mass[tid];
-    const int n = mode == kModeWalk ? 0 : int(min(st->count, uint32_t(a.list_max)));
+    __shared__ union { SmallList small; struct { EntryList list; Descent descent; } border; DrawShared draw; } un;
+    // all that the row needs is loaded at once (the list has at least 8193 entries' room)
     const uint2* list = a.list + size_t(slot) * a.list_max;
     const void* src = row_of<TYPE>(a, row);
+    const uint2 ahead0 = list[tid];
+    const uint64_t cum = tid < kBins ? st->cum_mass[tid] : 0;
+    const int mode = st->plan.mode;
+    const double J = st->plan.J;
+    const uint32_t listed = st->count;
+    const Setting s = setting(a, row);
+    if (mode == kDone) return;
+    if (tid < a.parts) load_part(a, slot, tid, s.c, J, sh);
+    if (tid == 0) sh.plan = st->plan;
+    if (tid < kBins) sh.cm[tid] = cum;
+    const int n = mode == kModeWalk ? 0 : int(min(listed, uint32_t(a.list_max)));
     __syncthreads();
     const Plan& plan = sh.plan;
     const uint64_t tq = plan.threshold_q;
     auto entry_mass = [&](uint32_t key, int col) -> uint64_t {
-        const int part = col / kPart;
+        const int part = (col / kPart) & (kPartsMax - 1);
         uint64_t m;
         return bin_mass(unordered(key), sh.scale[part], m) >= 0 ? row_mass(m, sh.shift[part]) : 0;
     };
     if (mode == kModeSmall) {
         const int e = min(n, kSmall);
-        if (tid < e) {
-            const uint2 w = list[tid];
-            un.small.comp[tid] = comp_of<TYPE>(w.x, int(w.y));
-            un.small.mass[tid] = entry_mass(w.x, int(w.y));
-            un.small.val[tid] = unordered(w.x);
+        if (tid < kSmall) {
+            un.small.comp[tid] = tid < e ? comp_of<TYPE>(ahead0.x, int(ahead0.y)) : 0;
+            un.small.mass[tid] = tid < e ? entry_mass(ahead0.x, int(ahead0.y)) : 0;
+            un.small.val[tid] = unordered(ahead0.x);
         }
         finish_small(a, row, s, plan, e, tq, un.small);
         return;
     }
+    uint64_t ahead[kAhead][kBinSteps];
+#pragma unroll
+    for (int h = 0; h < kAhead; ++h) load_bins(a, slot, (tid >> 6) + h * kRowWaves, ahead[h]);
     const bool lds = mode == kModeList && n <= kListLds;
     EntryList& en = un.border.list;
     if (lds) {
         for (int i = tid; i < n; i += kRowThreads) {
-            const uint2 w = list[i];
+            const uint2 w = i == tid ? ahead0 : list[i];
             en.comp[i] = comp_of<TYPE>(w.x, int(w.y));
             en.mass[i] = entry_mass(w.x, int(w.y));
         }
@@ -1053,8 +1176,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
             }
         } else {
             for (int c0 = tid * 8; c0 < a.N; c0 += kRowThreads * 8) {
-                float v[8];
-                load8<TYPE>(src, c0, a.N, v);
+                Piece<TYPE> v;
+                v.load(src, c0, a.N);
+#pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const uint32_t k = ordered(v[e]);
                     if (k >= lo && k < hi && v[e] >= sh.least[(c0 + e) / kPart]) f(comp_of<TYPE>(k, c0 + e), entry_mass(k, c0 + e));
@@ -1064,7 +1188,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     };
     int bf;
     const uint64_t threshold = threshold_of<TYPE>(s, plan, sh.cm, tq, each, un.border.descent, sh, bf);
-    sum_parts(a, slot, bf, sh);
+    sum_parts(a, slot, bf, ahead, sh);
     if (tid < 2 * 64) {
         const int wv = tid >> 6;
         const uint32_t edge = bf < 0 || bf + wv > kTopBin ? kKeyEnd : bin_edge(bf + wv, plan.mx, s.c, J);
@@ -1083,10 +1207,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
         if (tid == 0) give(a, row, -1, __builtin_nanf(""));
         return;
     }
-    float v[kPer];
+    Piece<TYPE> v;
     const int col0 = part * kPart + tid * kPer;
-    load8<TYPE>(src, col0, a.N, v);
-    draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], threshold, v, col0, sh);
+    v.load(src, col0, a.N);
+    draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], threshold, v, col0, sh, un.draw);
 }
 
 // Rows of one part: all of it by one block, the logits in LDS after the histogram.
@@ -1094,14 +1218,14 @@ template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
     const int row = blockIdx.x, tid = threadIdx.x;
     __shared__ RowShared sh;
-    __shared__ union { PartShared<kRowThreads> part; SmallList small; Descent descent; } un;
+    __shared__ union { PartShared<kRowThreads> part; SmallList small; Descent descent; DrawShared draw; } un;
     __shared__ __attribute__((aligned(16))) float s_v[kPart];
     __shared__ uint32_t s_count;
     const int col0 = tid * kPer;
-    float v[1][kPer];
-    load8<TYPE>(row_of<TYPE>(a, row), col0, a.N, v[0]);
+    Piece<TYPE> v[1];
+    v[0].load(row_of<TYPE>(a, row), col0, a.N);
     const Setting s = setting(a, row);
-    const PartMeta m = part_pass<kRowThreads, 1>(a, s, v, col0, un.part);
+    const PartMeta m = part_pass<TYPE, kRowThreads, 1>(a, s, v, col0, un.part);
     if (!s.valid || !m.key || s.T == 0.f) {
         if (tid == 0) {
             const bool fine = s.valid && m.key;
@@ -1128,6 +1252,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
             return bin_mass(x, k, e) >= 0 ? row_mass(e, 0) : 0;
         };
         if (plan.mode == kModeSmall) {
+            if (tid < kSmall) {
+                un.small.comp[tid] = 0;
+                un.small.mass[tid] = 0;
+            }
+            __syncthreads();
             for (int c = tid; c < a.N; c += kRowThreads) {
                 const float x = s_v[c];
                 const uint32_t key = ordered(x);
@@ -1174,7 +1303,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
         sh.rest = __umul64hi(fraction(s.u), sh.total);
     }
     __syncthreads();
-    draw_column<TYPE>(a, row, s, J, k, m.least, 0, threshold, v[0], col0, sh);
+    draw_column<TYPE>(a, row, s, J, k, m.least, 0, threshold, v[0], col0, sh, un.draw);
 }
 
 // rows of an empty vocabulary

@@ -27,7 +27,7 @@ from __future__ import annotations
 
 import contextvars
 import ctypes as C
-from contextlib import contextmanager
+from contextlib import contextmanager, nullcontext
 from dataclasses import dataclass, field
 from pathlib import Path
 
@@ -572,6 +572,21 @@ def logits_argmax(logits, out):
                                             ptr(out), stream(logits)), 'logits argmax')
 
 
+def on_device(device):
+    """The device guard of a launch (nothing to do on the current device)."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _row_ptr(t, name, dtype, shape, device):
+    """Address of an optional per-row tensor, checked."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f'{name} must be a contiguous {dtype} {list(shape)} tensor on {device}, '
+                         f'got {tuple(t.shape)} {t.dtype} on {t.device}')
+    return t.data_ptr()
+
+
 LOGITS_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -591,32 +606,31 @@ def logits_sample(logits, uniform, workspace, out, flags, temperature=None, top_
     probability the token was drawn with.  What each setting keeps, and the
     sticky flags (1 NaN logit, 2 setting out of range, 4 empty row; the last
     two give token -1): include/ornith_sample.h."""
-    rows = logits.shape[0] if logits.ndim == 2 else -1
-    if rows < 0 or logits.dtype not in LOGITS_TYPES or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    kind = LOGITS_TYPES.get(logits.dtype)
+    if kind is None or logits.ndim != 2:
         raise ValueError('logits must be bf16, fp16 or fp32 [M, N] with unit column stride')
-    if rows > 1 and logits.stride(0) < logits.shape[1]:
-        raise ValueError(f'logits rows overlap: row stride {logits.stride(0)} of {logits.shape[1]} columns')
-    for name, t, dtype in (('uniform', uniform, torch.float32), ('temperature', temperature, torch.float32),
-                           ('top_k', top_k, torch.int32), ('top_p', top_p, torch.float32),
-                           ('min_p', min_p, torch.float32), ('logprob', logprob, torch.float32),
-                           ('out', out, torch.int64)):
-        if t is None:
-            if name in ('uniform', 'out'):
-                raise ValueError(f'{name} is required')
-            continue
-        if t.dtype != dtype or tuple(t.shape) != (rows,) or not t.is_contiguous():
-            raise ValueError(f'{name} must be a contiguous {dtype} [{rows}] tensor, got {tuple(t.shape)} {t.dtype}')
+    (rows, n), (ld, step), dev = logits.shape, logits.stride(), logits.device
+    if step != 1 and n > 1:
+        raise ValueError('logits must be bf16, fp16 or fp32 [M, N] with unit column stride')
+    if rows <= 1:
+        ld = n
+    elif ld < n:
+        raise ValueError(f'logits rows overlap: row stride {ld} of {n} columns')
+    row = (rows,)
+    args = [_row_ptr(t, name, dtype, row, dev) for t, name, dtype in
+            ((uniform, 'uniform', torch.float32), (temperature, 'temperature', torch.float32),
+             (top_k, 'top_k', torch.int32), (top_p, 'top_p', torch.float32), (min_p, 'min_p', torch.float32),
+             (out, 'out', torch.int64), (logprob, 'logprob', torch.float32))]
+    if args[0] is None or args[5] is None:
+        raise ValueError('uniform and out are required')
     if flags.dtype != torch.int32 or flags.numel() != 1 or workspace.element_size() != 1:
         raise ValueError('flags must be one int32 word, workspace bytes')
-    tensors = [t for t in (logits, uniform, temperature, top_k, top_p, min_p, logprob, out, flags, workspace)
-               if t is not None]
-    if logits.device.type != 'cuda' or any(t.device != logits.device for t in tensors):
+    if dev.type != 'cuda' or flags.device != dev or workspace.device != dev:
         raise ValueError('logits, settings, outputs, flags and workspace must be on one GPU')
-    with torch.cuda.device(logits.device):
+    with on_device(dev):
         check(lib().ornith_logits_sample_launch(
-            ptr(logits), LOGITS_TYPES[logits.dtype], rows, logits.shape[1], max(logits.stride(0), logits.shape[1]),
-            ptr(uniform), ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), ptr(workspace), workspace.numel(),
-            ptr(out), ptr(logprob), ptr(flags), stream(logits)), 'logits sample')
+            logits.data_ptr(), kind, rows, n, ld, *args[:5], workspace.data_ptr() or None, workspace.numel(), *args[5:],
+            flags.data_ptr(), torch.cuda.current_stream(dev).cuda_stream), 'logits sample')
 
 
 W4_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -633,29 +647,38 @@ def w4_out(x, codes, metadata, out, flags, n, k, group):
     """Plain 4-bit linear: out [rows, n] (bf16, fp16 or fp32) = x [rows, k]
     (bf16 or fp16, as it is) times the banks of storage.pack_w4.  Any number of
     rows; the weights are read once per 64."""
-    if x.ndim != 2 or x.shape[1] != k or x.dtype not in (torch.bfloat16, torch.float16):
+    x_type, out_type = W4_TYPES.get(x.dtype, 2), W4_TYPES.get(out.dtype)
+    if x_type > 1 or x.ndim != 2 or x.shape[1] != k:
         raise ValueError(f'input must be a bf16 or fp16 [rows, {k}] tensor, got {tuple(x.shape)} {x.dtype}')
-    rows = x.shape[0]
-    if tuple(out.shape) != (rows, n) or out.dtype not in W4_TYPES:
+    rows, dev = x.shape[0], x.device
+    if out_type is None or out.shape != (rows, n):
         raise ValueError(f'output must be a bf16, fp16 or fp32 [{rows}, {n}] tensor, got {tuple(out.shape)} {out.dtype}')
-    for name, t, cols in (('input', x, k), ('output', out, n)):
-        if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
-            raise ValueError(f'{name} rows must have unit column stride and not overlap')
-    ldx, ldo = x.stride(0) if rows > 1 and k else k, out.stride(0) if rows > 1 and n else n
-    if ldx % 8 or x.data_ptr() % 16:
+    (ldx, sx), (ldo, so) = x.stride(), out.stride()
+    if rows <= 1 or not k:
+        ldx = k
+    if rows <= 1 or not n:
+        ldo = n
+    if (sx != 1 and k > 1) or (so != 1 and n > 1) or ldx < k or ldo < n:
+        raise ValueError('input and output rows must have unit column stride and not overlap')
+    x_ptr = x.data_ptr()
+    if ldx % 8 or x_ptr % 16:
         raise ValueError('input rows must start on the 16-byte grid')
-    want = w4_layout(n, k, group)
-    for name, t, shape in (('codes', codes, want[0]), ('metadata', metadata, want[1])):
-        if t.element_size() != 4 or tuple(t.shape) != shape or not t.is_contiguous():
-            raise ValueError(f'{name} must be the contiguous 32-bit {shape} bank of storage.pack_w4, '
-                             f'got {tuple(t.shape)} {t.dtype}')
+    if group not in (32, 64, 128, 256) or k % 8:
+        raise ValueError(f'group {group} is not 32, 64, 128 or 256, or K{k} not a multiple of 8')
+    tiles = (n + 15) // 16
+    if (codes.shape != (tiles, (k + 127) // 128, 64, 4) or metadata.shape != (tiles, -(-k // group), 16)
+            or codes.element_size() != 4 or metadata.element_size() != 4 or not codes.is_contiguous()
+            or not metadata.is_contiguous()):
+        raise ValueError(f'codes and metadata must be the contiguous 32-bit banks of storage.pack_w4 for N{n} K{k} '
+                         f'G{group}, got {tuple(codes.shape)} and {tuple(metadata.shape)}')
     if flags.dtype != torch.int32 or flags.numel() != 1:
         raise ValueError('flags must be one int32 word')
-    if x.device.type != 'cuda' or any(t.device != x.device for t in (codes, metadata, out, flags)):
+    if dev.type != 'cuda' or codes.device != dev or metadata.device != dev or out.device != dev or flags.device != dev:
         raise ValueError('input, banks, output and flags must be on one GPU')
-    with torch.cuda.device(x.device):
-        check(lib().ornith_w4_launch(ptr(x), W4_TYPES[x.dtype], ldx, ptr(codes), ptr(metadata), ptr(out),
-                                     W4_TYPES[out.dtype], ldo, ptr(flags), rows, n, k, group, stream(x)), 'w4 linear')
+    with on_device(dev):
+        check(lib().ornith_w4_launch(x_ptr, x_type, ldx, codes.data_ptr(), metadata.data_ptr(), out.data_ptr(), out_type,
+                                     ldo, flags.data_ptr(), rows, n, k, group,
+                                     torch.cuda.current_stream(dev).cuda_stream), 'w4 linear')
 
 
 def dense_head(x, codes, meta, workspace, logits, logits_bf16, argmax, flags, capacity):

@@ -145,7 +145,7 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     codes, scales = codes.contiguous(), scales.contiguous()
     zeros = None if zeros is None else zeros.contiguous()
     packed = [torch.empty(s, dtype=torch.int32, device=codes.device) for s in native.w4_layout(n, k, group)]
-    with torch.cuda.device(codes.device):
+    with native.on_device(codes.device):
         native.check(native.lib().ornith_w4_pack(native.ptr(codes), native.ptr(scales), native.W4_TYPES[scales.dtype],
                                                  native.ptr(zeros), native.ptr(packed[0]), native.ptr(packed[1]), n, k,
                                                  group, native.stream(codes)), 'w4 pack')
