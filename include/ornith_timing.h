@@ -30,7 +30,8 @@
  *   sampling         sample_row (up to 8192 columns); sample_parts, sample_select,
  *                    and with a cut sample_gather, sample_finish; sample_empty
  *                    (no columns)
- *   plain 4-bit      w4, w4_pack_codes, w4_pack_meta
+ *   plain 4-bit      w4_tile, w4_run (more than 16 rows of many columns),
+ *                    w4_zero (no inputs), w4_pack_codes, w4_pack_meta
  *   shared expert    fixed8_act, fixed8_gate
  *   other            repack_codes, repack_meta, silu_selfcheck */
 #ifndef ORNITH_TIMING_H

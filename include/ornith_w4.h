@@ -28,9 +28,10 @@ enum { ORNITH_W4_BF16 = 0, ORNITH_W4_F16 = 1, ORNITH_W4_F32 = 2 };
  *   codes [ceil(N/16), ceil(K/128), 64, 4]: word j of lane 16 q + c holds column
  *         c's k = 128 b + 32 j + 8 q .. + 7, k + 2 i at bits 4 i and k + 2 i + 1
  *         at bits 16 + 4 i; codes past N or K are 8;
- *   meta  [ceil(N/16), ceil(K/G), 16]: the scale as fp32 (bf16 and fp16 scales
+ *   meta  [ceil(N/16), ceil(K/128), 16, 128/G], for G = 256 [ceil(N/16),
+ *         ceil(ceil(K/128)/2), 16, 1]: the scale as fp32 (bf16 and fp16 scales
  *         leave its low bits clear) with the zero point in bits 0..3; scales
- *         past N are 0.
+ *         past N or K are 0.
  * 0 <= N <= 2^20, 0 <= K <= 65536, K % 8 == 0. */
 ORNITH_EXPORT hipError_t ornith_w4_get_layout(int N, int K, int G, size_t* code_words, size_t* meta_words);
 

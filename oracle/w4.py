@@ -17,7 +17,8 @@ def weights(words, scales, zeros, group):
 
 
 def packed(words, scales_bits32, zeros, group):
-    """The banks of ornith_w4_pack: codes [n/16, k/128, 64, 4], meta [n/16, groups, 16]."""
+    """The banks of ornith_w4_pack: codes [n/16, k/128, 64, 4], meta [n/16, k/128, 16, 128/group]
+    (group 256: [n/16, k/256, 16, 1])."""
     c = codes_of(words)
     n, k = c.shape
     tiles, blocks, groups = -(-n // 16), -(-k // 128), -(-k // group)
@@ -26,7 +27,9 @@ def packed(words, scales_bits32, zeros, group):
     v = full.reshape(tiles, 16, blocks, 4, 4, 4, 2)                # tile, column, block, j, q, i, parity
     word = sum(v[..., i, e] << np.uint32(4 * i + 16 * e) for i in range(4) for e in range(2))
     codes = word.transpose(0, 2, 4, 1, 3).reshape(tiles, blocks, 64, 4)
-    meta = np.full((tiles * 16, groups), 8, np.uint32)
+    per = max(128 // group, 1)
+    chunks = -(-blocks // 2) if group == 256 else blocks
+    meta = np.full((tiles * 16, chunks * per), 8, np.uint32)
     z = np.uint32(8) if zeros is None else np.asarray(zeros, np.uint32)
-    meta[:n] = (scales_bits32 & ~np.uint32(15)) | z
-    return codes, meta.reshape(tiles, 16, groups).transpose(0, 2, 1)
+    meta[:n, :groups] = (scales_bits32 & ~np.uint32(15)) | z
+    return codes, meta.reshape(tiles, 16, chunks, per).transpose(0, 2, 1, 3)

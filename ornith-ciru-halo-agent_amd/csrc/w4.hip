@@ -8,6 +8,7 @@
 // each product is exact, and the first sum is at most 31 / |c - z| times the
 // wanted one, so its roundings cost two to three bits of fp32, not of the
 // result's type.  acc += s * (that), groups in ascending order within a wave.
+#include <algorithm>
 #include "kernels.hpp"
 #include "timing.hpp"
 #include "validate.hpp"
@@ -16,7 +17,7 @@
 namespace ornith {
 namespace {
 
-constexpr int kW4MaxN = 1 << 20, kW4MaxK = 65536, kW4Rows = 64, kW4Block = 128;
+constexpr int kW4MaxN = 1 << 20, kW4MaxK = 65536, kW4Block = 128;
 
 typedef __bf16 w4_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 w4_f16x8 __attribute__((ext_vector_type(8)));
@@ -61,13 +62,14 @@ __global__ __launch_bounds__(256) void w4_pack_codes_kernel(const uint32_t* __re
 
 __global__ __launch_bounds__(256) void w4_pack_meta_kernel(const uint16_t* __restrict__ scales, int scale_type,
                                                            const uint8_t* __restrict__ zeros, uint32_t* __restrict__ out,
-                                                           int N, int groups, size_t words) {
+                                                           int N, int groups, int chunks, int per, size_t words) {
     const size_t i = size_t(blockIdx.x) * 256 + threadIdx.x;
     if (i >= words) return;
-    const size_t tg = i >> 4;
-    const int n = int(tg / size_t(groups)) * 16 + int(i & 15), g = int(tg % size_t(groups));
+    const size_t tc = i / size_t(16 * per);
+    const int in = int(i % size_t(16 * per)), n = int(tc / size_t(chunks)) * 16 + in / per;
+    const int g = int(tc % size_t(chunks)) * per + in % per;
     uint32_t w = 8;
-    if (n < N) {
+    if (n < N && g < groups) {
         const size_t at = size_t(n) * groups + g;
         const float s = scale_type == ORNITH_W4_BF16 ? bf16_bits_to_f32(scales[at]) : f16_bits_to_f32(scales[at]);
         w = (__float_as_uint(s) & ~15u) | (zeros ? zeros[at] & 15u : 8u);
@@ -83,77 +85,290 @@ struct W4Args {
     uint32_t* flags;
     int M, N, K, log2g;
 };
+// One result in the output's type; the flag of a non-finite 16-bit one.
+__device__ __forceinline__ uint32_t w4_store(const W4Args& a, size_t at, float v) {
+    if (a.out_type == ORNITH_W4_F32) {
+        static_cast<float*>(a.out)[at] = v;
+        return 0;
+    }
+    const uint16_t b = a.out_type == ORNITH_W4_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+    const uint32_t top = a.out_type == ORNITH_W4_BF16 ? 0x7f80u : 0x7c00u;
+    static_cast<uint16_t*>(a.out)[at] = b;
+    return (b & top) == top ? kDenseNonfiniteBf16 : 0;
+}
+__host__ __device__ inline int w4_blocks(int K) { return (K + kW4Block - 1) / kW4Block; }
 
-// One block per 16 columns and 64 rows: its waves take the 128-k blocks in
-// turn and add their sums in LDS, in wave order.
-template <int TYPE, int MT, int W>
-__global__ __launch_bounds__(64 * W) void w4_kernel(W4Args a) {
-    __shared__ float s_acc[W][MT * 4][64];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, li = lane & 15, q = lane >> 4;
-    const int tile = blockIdx.x, row0 = int(blockIdx.y) * kW4Rows, rows = min(a.M - row0, MT * 16);
-    const int blocks = (a.K + kW4Block - 1) / kW4Block, groups = (a.K + (1 << a.log2g) - 1) >> a.log2g;
-    const uint32_t* codes = a.codes + size_t(tile) * blocks * 256 + 4 * lane;
-    const uint32_t* meta = a.meta + size_t(tile) * groups * 16 + li;
-    const uint16_t* x = a.x + size_t(row0) * size_t(a.ldx);
-    const int per = min(a.log2g, 7) - 5;                       // 32-k steps of a group in a block: 1, 2, 4
-    const uint32_t one = TYPE == ORNITH_W4_BF16 ? 0x3f803f80u : 0x3c003c00u;
-    const u32x4 ones = {one, one, one, one};
-    f32x4 acc[MT];
+// More than 16 rows of many tiles.  A block takes a run of pairs of 16-column tiles and all its rows' x
+// (16 MT of them) into LDS once.  Its waves share the run's units (pair, 128 k) evenly, in order: a wave
+// ends the pair that an earlier one began, takes whole pairs, and begins one that later waves end; the
+// parts of a pair meet in LDS, in wave order.  PER: groups in 128 k (1 for groups of 128 and 256).
+// x lies in pieces of 8 k: piece (k / 8) * 16 MT + row; behind it its sums over groups (of 256: over their
+// halves, as the products are added per 128 k), [group, 16 MT].
+// W waves of a block, D units' codes of a wave in flight.
+constexpr size_t w4_x_bytes(int MT, int K) { return size_t(16 * MT) * ((K + kW4Block - 1) / kW4Block) * (2 * kW4Block); }
+
+template <int TYPE, int MT, int PER, int W, int D>
+__global__ __launch_bounds__(64 * W) void w4_run_kernel(W4Args a) {
+    extern __shared__ __attribute__((aligned(16))) u32x4 s_x[];
+    __shared__ int s_pair[W];                   // the pair whose end or middle a wave holds
+    typedef uint32_t meta_t __attribute__((ext_vector_type(PER)));
+    constexpr int RP = 16 * MT;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
+    const int row0 = int(blockIdx.y) * RP, R = min(a.M - row0, RP);
+    const int blocks = w4_blocks(a.K), last_tile = (a.N - 1) >> 4, pairs = (last_tile >> 1) + 1;
+    const int half = a.log2g == 8, chunks = half ? (blocks + 1) >> 1 : blocks;
+    // this block's pairs, this wave's units
+    const int base = pairs / int(gridDim.x), extra = pairs % int(gridDim.x), bx = blockIdx.x;
+    const int p0 = bx * base + min(bx, extra), np = base + (bx < extra);
+    const int units = np * blocks, ubase = units / W, uextra = units % W;
+    const int u0 = wv * ubase + min(wv, uextra), u1 = u0 + ubase + (wv < uextra);
+
+    u32x4 cw[D][2];
+    meta_t mw[D][2];
+    int np_ = u0 / blocks, nk = u0 % blocks;           // pair and block to load next
+    auto load = [&](int slot) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wv; kb < blocks; kb += W) {
-        const u32x4 w4 = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(codes + size_t(kb) * 256));
-        f32x4 c[MT], sx[MT];
+        for (int t = 0; t < 2; ++t) {                  // (past the last tile: that one again)
+            const size_t tile = size_t(min(2 * (p0 + np_) + t, last_tile));
+            cw[slot][t] = __builtin_nontemporal_load(
+                reinterpret_cast<const u32x4*>(a.codes + (tile * blocks + nk) * 256 + 4 * lane));
+            mw[slot][t] = *reinterpret_cast<const meta_t*>(a.meta + (tile * chunks + (nk >> half)) * (16 * PER) + PER * li);
+        }
+        if (++nk == blocks) {
+            nk = 0;
+            ++np_;
+        }
+    };
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = kb * kW4Block + 32 * j + 8 * q;
-            if ((j & ((1 << per) - 1)) == 0)
+    for (int d = 0; d < D; ++d)
+        if (u0 + d < u1) load(d);
+
+    float* s_sum = reinterpret_cast<float*>(s_x + size_t(RP) * blocks * 16);
+    {
+        // four lanes read 64 bytes of a row (rows past R: the last again), eight loads of a thread in flight
+        const uint16_t* x = a.x + size_t(row0) * size_t(a.ldx);
+        constexpr int kBatch = 8;
+        for (int i0 = tid; i0 < RP * blocks * 16; i0 += 64 * W * kBatch) {
+            u32x4 v[kBatch];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) c[mt] = sx[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-            const u32x4 b = w4_unpack<TYPE>(w4[j]);
+            for (int b = 0; b < kBatch; ++b) {
+                const int i = i0 + 64 * W * b, r = min((i >> 2) % RP, R - 1), piece = ((i >> 2) / RP) * 4 + (i & 3);
+                v[b] = u32x4{0, 0, 0, 0};
+                if (8 * piece < a.K) v[b] = *reinterpret_cast<const u32x4*>(x + size_t(r) * size_t(a.ldx) + 8 * piece);
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int i = i0 + 64 * W * b;
+                if (i < RP * blocks * 16) s_x[(((i >> 2) / RP) * 4 + (i & 3)) * RP + (i >> 2) % RP] = v[b];
+            }
+        }
+    }
+    __syncthreads();
+    const u32x4* mine = s_x + q * RP + li;             // this lane's pieces: step * 4 RP + 16 mt
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    {
+        const uint32_t one = TYPE == ORNITH_W4_BF16 ? 0x3f803f80u : 0x3c003c00u;
+        const u32x4 ones = {one, one, one, one};
+        constexpr int steps = 4 / PER;
+        for (int g = wv; g < blocks * PER; g += W) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const int r = min(16 * mt + li, rows - 1);
-                u32x4 av = {0, 0, 0, 0};
-                if (k < a.K) av = *reinterpret_cast<const u32x4*>(x + size_t(r) * size_t(a.ldx) + k);
-                c[mt] = w4_mfma<TYPE>(av, b, c[mt]);
-                sx[mt] = w4_mfma<TYPE>(av, ones, sx[mt]);
+                f32x4 sum = zero;
+#pragma unroll
+                for (int j = 0; j < steps; ++j) sum = w4_mfma<TYPE>(mine[(g * steps + j) * (4 * RP) + 16 * mt], ones, sum);
+                if (li == 0) *reinterpret_cast<f32x4*>(&s_sum[g * RP + 16 * mt + 4 * q]) = sum;
             }
-            if (((j + 1) & ((1 << per) - 1)) == 0) {
-                const int g = min((kb * kW4Block + 32 * j) >> a.log2g, groups - 1);
-                const uint32_t m = meta[size_t(g) * 16];
-                const float s = __uint_as_float(m & ~15u), z = -16.f - float(m & 15u);
+        }
+    }
+    __syncthreads();
+
+    f32x4 acc[2][MT], head[2][MT];                     // head: the end of a pair that an earlier wave began
+    auto clear = [&] {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) acc[t][mt] = zero;
+    };
+    clear();
+    uint32_t flags = 0;
+    auto store = [&](int pair) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int n = (2 * (p0 + pair) + t) * 16 + li;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = 16 * mt + 4 * q + i;
+                    if (row >= R || n >= a.N) continue;
+                    const float v = acc[t][mt][i];
+                    if (!isfinite(v)) flags |= kDenseNonfiniteProjection;
+                    flags |= w4_store(a, size_t(row0 + row) * size_t(a.ldo) + n, v);
+                }
+        }
+    };
+    int head_pair = -1, pair = u0 / blocks, kb = u0 % blocks;
+    bool began = kb == 0;
+    for (int u = u0; u < u1; u += D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (u + d >= u1) break;
+            u32x4 w4[2];
+            meta_t mm[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                w4[t] = cw[d][t];
+                mm[t] = mw[d][t];
+            }
+            if (u + d + D < u1) load(d);
+            const u32x4* xk = mine + kb * (16 * RP);
+            const float* sk = s_sum + kb * (PER * RP) + 4 * q;
+            f32x4 c[2][MT];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool first = j % (4 / PER) == 0, last = j % (4 / PER) == 4 / PER - 1;
+                u32x4 av[MT];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) av[mt] = xk[j * (4 * RP) + 16 * mt];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const u32x4 b = w4_unpack<TYPE>(w4[t][j]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) c[t][mt] = w4_mfma<TYPE>(av[mt], b, first ? zero : c[t][mt]);
+                }
+                if (!last) continue;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const f32x4 sx = *reinterpret_cast<const f32x4*>(sk + (j / (4 / PER)) * RP + 16 * mt);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const uint32_t m = mm[t][j / (4 / PER)];
+                        const float sc = __uint_as_float(m & ~15u), z = -16.f - float(m & 15u);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            acc[t][mt][i] = __builtin_fmaf(sc, __builtin_fmaf(z, sx[i], c[t][mt][i]), acc[t][mt][i]);
+                    }
+                }
+            }
+            if (++kb == blocks) {
+                if (began) store(pair);
+                else {
+                    head_pair = pair;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) head[t][mt] = acc[t][mt];
+                }
+                clear();
+                kb = 0;
+                ++pair;
+                began = true;
+            }
+        }
+    }
+    // pairs that several waves share
+    __syncthreads();
+    float* s_part = reinterpret_cast<float*>(s_x);
+    const bool middle = kb != 0 && !began;             // began by an earlier wave, ended by a later one
+    if (middle) head_pair = pair;
+    if (lane == 0) s_pair[wv] = head_pair;
+    if (head_pair >= 0) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s_part[((wv * 2 + t) * MT * 4 + 4 * mt + i) * 64 + lane] = middle ? acc[t][mt][i] : head[t][mt][i];
+    }
+    __syncthreads();
+    if (began && kb != 0) {
+        for (int w = wv + 1; w < W && s_pair[w] == pair; ++w)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[mt][i] = __builtin_fmaf(s, __builtin_fmaf(z, sx[mt][i], c[mt][i]), acc[mt][i]);
+                    for (int i = 0; i < 4; ++i) acc[t][mt][i] += s_part[((w * 2 + t) * MT * 4 + 4 * mt + i) * 64 + lane];
+        store(pair);
+    }
+    flag_or(a.flags, flags);
+}
+
+// A block per NT tiles and 16 rows, whose waves take 128-k blocks in turn, x straight from memory, and
+// meet in LDS in wave order.
+template <int TYPE, int PER, int NT, int W>
+__global__ __launch_bounds__(64 * W) void w4_tile_kernel(W4Args a) {
+    typedef uint32_t meta_t __attribute__((ext_vector_type(PER)));
+    __shared__ float s_acc[W][NT * 4][64];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
+    const int tile0 = int(blockIdx.x) * NT, last_tile = (a.N - 1) >> 4, row0 = int(blockIdx.y) * 16, R = min(a.M - row0, 16);
+    const int blocks = w4_blocks(a.K), half = a.log2g == 8, chunks = half ? (blocks + 1) >> 1 : blocks;
+    const uint16_t* x = a.x + size_t(row0 + min(li, R - 1)) * size_t(a.ldx) + 8 * q;
+    const uint32_t one = TYPE == ORNITH_W4_BF16 ? 0x3f803f80u : 0x3c003c00u;
+    const u32x4 ones = {one, one, one, one};
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    f32x4 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = zero;
+    for (int kb = wv; kb < blocks; kb += W) {
+        u32x4 cw[NT], xa[4];
+        meta_t mw[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {                 // (past the last tile: that one again)
+            const size_t tile = size_t(min(tile0 + t, last_tile));
+            cw[t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.codes + (tile * blocks + kb) * 256 + 4 * lane));
+            mw[t] = *reinterpret_cast<const meta_t*>(a.meta + (tile * chunks + (kb >> half)) * (16 * PER) + PER * li);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = kb * kW4Block + 32 * j;
+            xa[j] = u32x4{0, 0, 0, 0};
+            if (k + 8 * q < a.K) xa[j] = *reinterpret_cast<const u32x4*>(x + k);
+        }
+        f32x4 c[NT], sx;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool first = j % (4 / PER) == 0, last = j % (4 / PER) == 4 / PER - 1;
+            sx = w4_mfma<TYPE>(xa[j], ones, first ? zero : sx);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                c[t] = w4_mfma<TYPE>(xa[j], w4_unpack<TYPE>(cw[t][j]), first ? zero : c[t]);
+                if (!last) continue;
+                const uint32_t m = mw[t][j / (4 / PER)];
+                const float sc = __uint_as_float(m & ~15u), z = -16.f - float(m & 15u);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(sc, __builtin_fmaf(z, sx[i], c[t][i]), acc[t][i]);
             }
         }
     }
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_acc[wv][4 * mt + i][lane] = acc[mt][i];
+        for (int i = 0; i < 4; ++i) s_acc[wv][4 * t + i][lane] = acc[t][i];
     __syncthreads();
     uint32_t flags = 0;
-    for (int o = tid; o < MT * 4 * 64; o += 64 * W) {
-        const int e = o >> 6, l = o & 63, row = 16 * (e >> 2) + 4 * (l >> 4) + (e & 3), n = tile * 16 + (l & 15);
+    for (int e = wv; e < NT * 4; e += W) {             // a wave per register of a fragment
+        const int row = 4 * q + (e & 3), n = (tile0 + (e >> 2)) * 16 + li;
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) v += s_acc[w][e][l];
-        if (row >= rows || n >= a.N) continue;
+        for (int w = 0; w < W; ++w) v += s_acc[w][e][lane];
+        if (row >= R || n >= a.N) continue;
         if (!isfinite(v)) flags |= kDenseNonfiniteProjection;
-        const size_t at = size_t(row0 + row) * size_t(a.ldo) + n;
-        if (a.out_type == ORNITH_W4_F32) static_cast<float*>(a.out)[at] = v;
-        else {
-            const uint16_t b = a.out_type == ORNITH_W4_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
-            const uint32_t top = a.out_type == ORNITH_W4_BF16 ? 0x7f80u : 0x7c00u;
-            if ((b & top) == top) flags |= kDenseNonfiniteBf16;
-            static_cast<uint16_t*>(a.out)[at] = b;
-        }
+        flags |= w4_store(a, size_t(row0 + row) * size_t(a.ldo) + n, v);
     }
     flag_or(a.flags, flags);
+}
+
+// K == 0: zeros
+__global__ __launch_bounds__(256) void w4_zero_kernel(W4Args a) {
+    const int n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= a.N) return;
+    for (int row = blockIdx.y; row < a.M; row += gridDim.y) {
+        const size_t at = size_t(row) * size_t(a.ldo) + n;
+        if (a.out_type == ORNITH_W4_F32) static_cast<float*>(a.out)[at] = 0.f;
+        else static_cast<uint16_t*>(a.out)[at] = 0;
+    }
 }
 
 int w4_log2g(int G) { return G == 32 ? 5 : G == 64 ? 6 : G == 128 ? 7 : G == 256 ? 8 : -1; }
@@ -162,19 +377,43 @@ bool w4_words(int N, int K, int G, size_t& codes, size_t& meta) {
     if (N < 0 || N > kW4MaxN || K < 0 || K > kW4MaxK || K % 8 || w4_log2g(G) < 0) return false;
     const size_t tiles = (size_t(N) + 15) / 16;
     codes = tiles * ((size_t(K) + kW4Block - 1) / kW4Block) * 256;
-    meta = tiles * ((size_t(K) + G - 1) / G) * 16;
+    const size_t blocks = (size_t(K) + kW4Block - 1) / kW4Block;
+    meta = tiles * (G == 256 ? (blocks + 1) / 2 : blocks * (kW4Block / G)) * 16;
     return true;
 }
 
-template <int TYPE> void w4_rows(const W4Args& a, hipStream_t s) {
-    constexpr int W = 8;
-    const dim3 grid((a.N + 15) / 16, (a.M + kW4Rows - 1) / kW4Rows);
-    const int mt = a.M > 48 ? 4 : (a.M + 15) / 16;
-    auto go = [&](auto kernel) { timed_launch("w4", kernel, grid, dim3(64 * W), 0, s, a); };
-    if (mt == 1) go(w4_kernel<TYPE, 1, W>);
-    else if (mt == 2) go(w4_kernel<TYPE, 2, W>);
-    else if (mt == 3) go(w4_kernel<TYPE, 3, W>);
-    else go(w4_kernel<TYPE, 4, W>);
+constexpr size_t kW4XBytes = 128 * 1024;               // x of a block in LDS
+
+template <int TYPE, int MT, int W, int D> hipError_t w4_run(const W4Args& a, hipStream_t s) {
+    constexpr size_t part = size_t(W) * 2 * MT * 1024;
+    const int groups = a.log2g < 7 ? w4_blocks(a.K) * (kW4Block >> a.log2g) : w4_blocks(a.K);
+    const size_t lds = std::max(w4_x_bytes(MT, a.K), part) + size_t(groups) * 16 * MT * 4;
+    const int pairs = (a.N + 31) / 32, rows = (a.M + 16 * MT - 1) / (16 * MT);
+    const dim3 grid(std::min(pairs, std::max(device_cu_count() / rows, 1)), rows);
+    auto go = [&](auto kernel) { timed_launch("w4_run", kernel, grid, dim3(64 * W), uint32_t(lds), s, a); };
+    if (a.log2g == 5) go(w4_run_kernel<TYPE, MT, 4, W, D>);
+    else if (a.log2g == 6) go(w4_run_kernel<TYPE, MT, 2, W, D>);
+    else go(w4_run_kernel<TYPE, MT, 1, W, D>);
+    return hipGetLastError();
+}
+template <int TYPE, int NT, int W> hipError_t w4_tiles(const W4Args& a, hipStream_t s) {
+    const dim3 grid(((a.N + 15) / 16 + NT - 1) / NT, (a.M + 15) / 16);
+    auto go = [&](auto kernel) { timed_launch("w4_tile", kernel, grid, dim3(64 * W), 0, s, a); };
+    if (a.log2g == 5) go(w4_tile_kernel<TYPE, 4, NT, W>);
+    else if (a.log2g == 6) go(w4_tile_kernel<TYPE, 2, NT, W>);
+    else go(w4_tile_kernel<TYPE, 1, NT, W>);
+    return hipGetLastError();
+}
+template <int TYPE> hipError_t w4_rows(const W4Args& a, hipStream_t s) {
+    const int64_t tiles = (a.N + 15) / 16, cells = tiles * ((a.M + 15) / 16);
+    if (a.M > 16 && cells > 3072) {
+        if (a.M > 48 && w4_x_bytes(4, a.K) <= kW4XBytes) return w4_run<TYPE, 4, 8, 4>(a, s);
+        if (a.M > 32 && w4_x_bytes(3, a.K) <= kW4XBytes) return w4_run<TYPE, 3, 8, 4>(a, s);
+        if (w4_x_bytes(2, a.K) <= kW4XBytes) return w4_run<TYPE, 2, 16, 2>(a, s);
+    }
+    if (a.M > 8 ? cells >= 768 : tiles >= 4096) return w4_tiles<TYPE, 4, 8>(a, s);
+    if (a.M > 8 ? cells >= 384 : tiles >= 1536) return w4_tiles<TYPE, 2, 8>(a, s);
+    return w4_blocks(a.K) >= 24 ? w4_tiles<TYPE, 1, 16>(a, s) : w4_tiles<TYPE, 1, 8>(a, s);
 }
 
 }  // namespace
@@ -210,7 +449,8 @@ extern "C" hipError_t ornith_w4_pack(const void* codes, const void* scales, int 
     if (st != hipSuccess) return st;
     timed_launch("w4_pack_meta", w4_pack_meta_kernel, dim3(unsigned((m + 255) / 256)), dim3(256), 0, stream,
                  static_cast<const uint16_t*>(scales), scale_type, static_cast<const uint8_t*>(zeros),
-                 static_cast<uint32_t*>(packed_meta), N, groups, m);
+                 static_cast<uint32_t*>(packed_meta), N, groups,
+                 G == 256 ? (w4_blocks(K) + 1) / 2 : w4_blocks(K), G == 256 ? 1 : kW4Block / G, m);
     return hipGetLastError();
 }
 
@@ -229,16 +469,18 @@ extern "C" hipError_t ornith_w4_launch(const void* x, int x_type, int64_t ldx, c
                               {out, (size_t(M - 1) * size_t(ldo) + size_t(N)) * size, size, true, false},
                               {flags, 4, 4, true, false}};
     if (!check_buffers(buffers)) return hipErrorInvalidValue;
-    // rows ride on the grid's y axis (65535 blocks of 64 rows at most)
-    constexpr int kMost = 65535 * kW4Rows;
+    // rows ride on the grid's y axis (65535 blocks of 16 rows at least)
+    constexpr int kMost = 65535 * 16;
     for (int r = 0; r < M; r += kMost) {
         const W4Args a{static_cast<const uint16_t*>(x) + size_t(r) * size_t(ldx), ldx,
                        static_cast<const uint32_t*>(codes), static_cast<const uint32_t*>(meta),
                        static_cast<uint8_t*>(out) + size_t(r) * size_t(ldo) * size, out_type, ldo,
                        static_cast<uint32_t*>(flags), M - r < kMost ? M - r : kMost, N, K, w4_log2g(G)};
-        if (x_type == ORNITH_W4_BF16) w4_rows<ORNITH_W4_BF16>(a, stream);
-        else w4_rows<ORNITH_W4_F16>(a, stream);
-        const hipError_t st = hipGetLastError();
+        hipError_t st;
+        if (!K) {
+            timed_launch("w4_zero", w4_zero_kernel, dim3((N + 255) / 256, std::min(a.M, 1024)), dim3(256), 0, stream, a);
+            st = hipGetLastError();
+        } else st = x_type == ORNITH_W4_BF16 ? w4_rows<ORNITH_W4_BF16>(a, stream) : w4_rows<ORNITH_W4_F16>(a, stream);
         if (st != hipSuccess) return st;
     }
     return hipSuccess;

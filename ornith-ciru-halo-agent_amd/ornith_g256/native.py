@@ -640,7 +640,12 @@ def w4_layout(n, k, group):
     """Shapes of the packed codes and metadata of a plain 4-bit linear."""
     codes, meta = _SZ(0), _SZ(0)
     check(lib().ornith_w4_get_layout(n, k, group, C.byref(codes), C.byref(meta)), f'w4 layout N{n} K{k} G{group}')
-    return (-(-n // 16), -(-k // 128), 64, 4), (-(-n // 16), -(-k // group), 16)
+    return _w4_shapes(n, k, group)
+
+
+def _w4_shapes(n, k, group):
+    tiles, blocks = (n + 15) // 16, (k + 127) // 128
+    return (tiles, blocks, 64, 4), (tiles, (blocks + 1) // 2 if group == 256 else blocks, 16, max(128 // group, 1))
 
 
 def w4_out(x, codes, metadata, out, flags, n, k, group):
@@ -665,9 +670,8 @@ def w4_out(x, codes, metadata, out, flags, n, k, group):
         raise ValueError('input rows must start on the 16-byte grid')
     if group not in (32, 64, 128, 256) or k % 8:
         raise ValueError(f'group {group} is not 32, 64, 128 or 256, or K{k} not a multiple of 8')
-    tiles = (n + 15) // 16
-    if (codes.shape != (tiles, (k + 127) // 128, 64, 4) or metadata.shape != (tiles, -(-k // group), 16)
-            or codes.element_size() != 4 or metadata.element_size() != 4 or not codes.is_contiguous()
+    shapes = _w4_shapes(n, k, group)
+    if (codes.shape != shapes[0] or metadata.shape != shapes[1] or codes.element_size() != 4 or metadata.element_size() != 4 or not codes.is_contiguous()
             or not metadata.is_contiguous()):
         raise ValueError(f'codes and metadata must be the contiguous 32-bit banks of storage.pack_w4 for N{n} K{k} '
                          f'G{group}, got {tuple(codes.shape)} and {tuple(metadata.shape)}')

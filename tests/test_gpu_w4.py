@@ -82,7 +82,7 @@ def _check(c, got, out_type):
 
 SHAPES = [(1, 1, 8), (1, 16, 32), (2, 15, 40), (1, 17, 128), (5, 100, 136), (16, 33, 256), (17, 64, 264),
           (33, 48, 520), (48, 30, 1024), (49, 257, 384), (64, 96, 2048), (65, 31, 640), (130, 40, 2120), (1, 2048, 512),
-          (3, 1000, 4096), (8, 640, 8192), (1, 70000, 128), (7, 5003, 264), (2, 16, 65536)]
+          (3, 1000, 4096), (8, 640, 8192), (1, 70000, 128), (7, 5003, 264), (3, 16, 32768), (2, 40, 65536)]
 
 
 @pytest.mark.parametrize('dtype', ['bf16', 'fp16'])

@@ -92,7 +92,7 @@ def test_packed_layout_by_hand():
     words[3, 0] = 9 << 20
     bits = np.full((4, 1), 0x3f800000, np.uint32)
     codes, meta = O.packed(words, bits, None, 128)
-    assert codes.shape == (1, 1, 64, 4) and meta.shape == (1, 1, 16)
+    assert codes.shape == (1, 1, 64, 4) and meta.shape == (1, 1, 16, 1)
     assert codes[0, 0, 3, 0] == 9 << 24 and codes[0, 0, 3, 1] == 0
     assert codes[0, 0, 4, 0] == 0x88888888               # past N
-    assert meta[0, 0, 3] == 0x3f800008 and meta[0, 0, 4] == 8
+    assert meta[0, 0, 3, 0] == 0x3f800008 and meta[0, 0, 4, 0] == 8
