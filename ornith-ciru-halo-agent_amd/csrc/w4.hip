@@ -9,6 +9,7 @@
 // wanted one, so its roundings cost two to three bits of fp32, not of the
 // result's type.  acc += s * (that), groups in ascending order within a wave.
 #include <algorithm>
+#include <type_traits>
 #include "kernels.hpp"
 #include "timing.hpp"
 #include "validate.hpp"
@@ -85,16 +86,32 @@ struct W4Args {
     uint32_t* flags;
     int M, N, K, log2g;
 };
-// One result in the output's type; the flag of a non-finite 16-bit one.
-__device__ __forceinline__ uint32_t w4_store(const W4Args& a, size_t at, float v) {
-    if (a.out_type == ORNITH_W4_F32) {
-        static_cast<float*>(a.out)[at] = v;
-        return 0;
+// Results in the output's type, and what they raise: a lane keeps the largest magnitude it stored and
+// a sum of zero times each (NaN once one was not finite).
+template <int OUT> __device__ __forceinline__ void w4_put(void* out, size_t at, float v) {
+    if constexpr (OUT == ORNITH_W4_F32) static_cast<float*>(out)[at] = v;
+    else if constexpr (OUT == ORNITH_W4_BF16) static_cast<__bf16*>(out)[at] = static_cast<__bf16>(v);
+    else static_cast<_Float16*>(out)[at] = static_cast<_Float16>(v);
+}
+struct W4Seen {
+    float most = 0.f, zero = 0.f;
+    __device__ __forceinline__ void see(float v) {
+        most = fmaxf(most, __builtin_fabsf(v));
+        zero = __builtin_fmaf(v, 0.f, zero);
     }
-    const uint16_t b = a.out_type == ORNITH_W4_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
-    const uint32_t top = a.out_type == ORNITH_W4_BF16 ? 0x7f80u : 0x7c00u;
-    static_cast<uint16_t*>(a.out)[at] = b;
-    return (b & top) == top ? kDenseNonfiniteBf16 : 0;
+    // 16-bit results round to infinity from half a step above the type's largest value
+    __device__ __forceinline__ uint32_t flags(int out_type) const {
+        const bool bad = zero != zero;
+        const float end = out_type == ORNITH_W4_BF16 ? 0x1.ffp127f : 65520.f;
+        return (bad ? kDenseNonfiniteProjection : 0u) |
+               (out_type != ORNITH_W4_F32 && (bad || most >= end) ? kDenseNonfiniteBf16 : 0u);
+    }
+};
+// f with the output's type as a constant.
+template <class F> __device__ __forceinline__ void w4_by_type(int out_type, F&& f) {
+    if (out_type == ORNITH_W4_F32) f(std::integral_constant<int, ORNITH_W4_F32>{});
+    else if (out_type == ORNITH_W4_BF16) f(std::integral_constant<int, ORNITH_W4_BF16>{});
+    else f(std::integral_constant<int, ORNITH_W4_F16>{});
 }
 __host__ __device__ inline int w4_blocks(int K) { return (K + kW4Block - 1) / kW4Block; }
 
@@ -105,6 +122,7 @@ __host__ __device__ inline int w4_blocks(int K) { return (K + kW4Block - 1) / kW
 // x lies in pieces of 8 k: piece (k / 8) * 16 MT + row; behind it its sums over groups (of 256: over their
 // halves, as the products are added per 128 k), [group, 16 MT].
 // W waves of a block, D units' codes of a wave in flight.
+constexpr size_t kW4XBytes = 128 * 1024;               // x of a block, at most
 constexpr size_t w4_x_bytes(int MT, int K) { return size_t(16 * MT) * ((K + kW4Block - 1) / kW4Block) * (2 * kW4Block); }
 
 template <int TYPE, int MT, int PER, int W, int D>
@@ -139,28 +157,26 @@ __global__ __launch_bounds__(64 * W) void w4_run_kernel(W4Args a) {
             ++np_;
         }
     };
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-        if (u0 + d < u1) load(d);
-
     float* s_sum = reinterpret_cast<float*>(s_x + size_t(RP) * blocks * 16);
     {
-        // four lanes read 64 bytes of a row (rows past R: the last again), eight loads of a thread in flight
+        // all of a thread's pieces of x, then its first codes, in flight at once; four lanes read 64 bytes
+        // of a row (rows past R: the last again)
         const uint16_t* x = a.x + size_t(row0) * size_t(a.ldx);
-        constexpr int kBatch = 8;
-        for (int i0 = tid; i0 < RP * blocks * 16; i0 += 64 * W * kBatch) {
-            u32x4 v[kBatch];
+        constexpr int kBatch = (int(kW4XBytes / 16) + 64 * W - 1) / (64 * W);
+        u32x4 v[kBatch];
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int i = i0 + 64 * W * b, r = min((i >> 2) % RP, R - 1), piece = ((i >> 2) / RP) * 4 + (i & 3);
-                v[b] = u32x4{0, 0, 0, 0};
-                if (8 * piece < a.K) v[b] = *reinterpret_cast<const u32x4*>(x + size_t(r) * size_t(a.ldx) + 8 * piece);
-            }
+        for (int b = 0; b < kBatch; ++b) {
+            const int i = tid + 64 * W * b, r = min((i >> 2) % RP, R - 1), piece = ((i >> 2) / RP) * 4 + (i & 3);
+            v[b] = u32x4{0, 0, 0, 0};
+            if (8 * piece < a.K) v[b] = *reinterpret_cast<const u32x4*>(x + size_t(r) * size_t(a.ldx) + 8 * piece);
+        }
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int i = i0 + 64 * W * b;
-                if (i < RP * blocks * 16) s_x[(((i >> 2) / RP) * 4 + (i & 3)) * RP + (i >> 2) % RP] = v[b];
-            }
+        for (int d = 0; d < D; ++d)
+            if (u0 + d < u1) load(d);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int i = tid + 64 * W * b;
+            if (i < RP * blocks * 16) s_x[(((i >> 2) / RP) * 4 + (i & 3)) * RP + (i >> 2) % RP] = v[b];
         }
     }
     __syncthreads();
@@ -190,22 +206,24 @@ __global__ __launch_bounds__(64 * W) void w4_run_kernel(W4Args a) {
             for (int mt = 0; mt < MT; ++mt) acc[t][mt] = zero;
     };
     clear();
-    uint32_t flags = 0;
+    W4Seen seen;
     auto store = [&](int pair) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int n = (2 * (p0 + pair) + t) * 16 + li;
+        w4_by_type(a.out_type, [&](auto out) {
+            constexpr int OUT = decltype(out)::value;
+            const int n0 = (p0 + pair) * 32;
+            const size_t at = size_t(row0 + 4 * q) * size_t(a.ldo) + size_t(n0 + li);
+            const bool whole = R == RP && n0 + 32 <= a.N;       // (wave-uniform)
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = 16 * mt + 4 * q + i;
-                    if (row >= R || n >= a.N) continue;
-                    const float v = acc[t][mt][i];
-                    if (!isfinite(v)) flags |= kDenseNonfiniteProjection;
-                    flags |= w4_store(a, size_t(row0 + row) * size_t(a.ldo) + n, v);
-                }
-        }
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (!whole && (16 * mt + 4 * q + i >= R || n0 + 16 * t + li >= a.N)) continue;
+                        seen.see(acc[t][mt][i]);
+                        w4_put<OUT>(a.out, at + size_t(16 * mt + i) * size_t(a.ldo) + 16 * t, acc[t][mt][i]);
+                    }
+        });
     };
     int head_pair = -1, pair = u0 / blocks, kb = u0 % blocks;
     bool began = kb == 0;
@@ -292,7 +310,7 @@ __global__ __launch_bounds__(64 * W) void w4_run_kernel(W4Args a) {
                     for (int i = 0; i < 4; ++i) acc[t][mt][i] += s_part[((w * 2 + t) * MT * 4 + 4 * mt + i) * 64 + lane];
         store(pair);
     }
-    flag_or(a.flags, flags);
+    flag_or(a.flags, seen.flags(a.out_type));
 }
 
 // A block per NT tiles and 16 rows, whose waves take 128-k blocks in turn, x straight from memory, and
@@ -347,17 +365,18 @@ __global__ __launch_bounds__(64 * W) void w4_tile_kernel(W4Args a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) s_acc[wv][4 * t + i][lane] = acc[t][i];
     __syncthreads();
-    uint32_t flags = 0;
+    W4Seen seen;
     for (int e = wv; e < NT * 4; e += W) {             // a wave per register of a fragment
         const int row = 4 * q + (e & 3), n = (tile0 + (e >> 2)) * 16 + li;
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) v += s_acc[w][e][lane];
         if (row >= R || n >= a.N) continue;
-        if (!isfinite(v)) flags |= kDenseNonfiniteProjection;
-        flags |= w4_store(a, size_t(row0 + row) * size_t(a.ldo) + n, v);
+        seen.see(v);
+        const size_t at = size_t(row0 + row) * size_t(a.ldo) + n;
+        w4_by_type(a.out_type, [&](auto out) { w4_put<decltype(out)::value>(a.out, at, v); });
     }
-    flag_or(a.flags, flags);
+    flag_or(a.flags, seen.flags(a.out_type));
 }
 
 // K == 0: zeros
@@ -381,8 +400,6 @@ bool w4_words(int N, int K, int G, size_t& codes, size_t& meta) {
     meta = tiles * (G == 256 ? (blocks + 1) / 2 : blocks * (kW4Block / G)) * 16;
     return true;
 }
-
-constexpr size_t kW4XBytes = 128 * 1024;               // x of a block in LDS
 
 template <int TYPE, int MT, int W, int D> hipError_t w4_run(const W4Args& a, hipStream_t s) {
     constexpr size_t part = size_t(W) * 2 * MT * 1024;
@@ -409,7 +426,7 @@ template <int TYPE> hipError_t w4_rows(const W4Args& a, hipStream_t s) {
     if (a.M > 16 && cells > 3072) {
         if (a.M > 48 && w4_x_bytes(4, a.K) <= kW4XBytes) return w4_run<TYPE, 4, 8, 4>(a, s);
         if (a.M > 32 && w4_x_bytes(3, a.K) <= kW4XBytes) return w4_run<TYPE, 3, 8, 4>(a, s);
-        if (w4_x_bytes(2, a.K) <= kW4XBytes) return w4_run<TYPE, 2, 16, 2>(a, s);
+        if (w4_x_bytes(2, a.K) <= kW4XBytes) return w4_run<TYPE, 2, 12, 3>(a, s);
     }
     if (a.M > 8 ? cells >= 768 : tiles >= 4096) return w4_tiles<TYPE, 4, 8>(a, s);
     if (a.M > 8 ? cells >= 384 : tiles >= 1536) return w4_tiles<TYPE, 2, 8>(a, s);

@@ -577,6 +577,12 @@ def on_device(device):
     return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def raw_stream(device):
+    """The handle of torch's current stream on `device` (an int; stream() without building a Stream object,
+    which costs 2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _row_ptr(t, name, dtype, shape, device):
     """Address of an optional per-row tensor, checked."""
     if t is None:
@@ -630,7 +636,7 @@ def logits_sample(logits, uniform, workspace, out, flags, temperature=None, top_
     with on_device(dev):
         check(lib().ornith_logits_sample_launch(
             logits.data_ptr(), kind, rows, n, ld, *args[:5], workspace.data_ptr() or None, workspace.numel(), *args[5:],
-            flags.data_ptr(), torch.cuda.current_stream(dev).cuda_stream), 'logits sample')
+            flags.data_ptr(), raw_stream(dev)), 'logits sample')
 
 
 W4_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -681,8 +687,7 @@ def w4_out(x, codes, metadata, out, flags, n, k, group):
         raise ValueError('input, banks, output and flags must be on one GPU')
     with on_device(dev):
         check(lib().ornith_w4_launch(x_ptr, x_type, ldx, codes.data_ptr(), metadata.data_ptr(), out.data_ptr(), out_type,
-                                     ldo, flags.data_ptr(), rows, n, k, group,
-                                     torch.cuda.current_stream(dev).cuda_stream), 'w4 linear')
+                                     ldo, flags.data_ptr(), rows, n, k, group, raw_stream(dev)), 'w4 linear')
 
 
 def dense_head(x, codes, meta, workspace, logits, logits_bf16, argmax, flags, capacity):
