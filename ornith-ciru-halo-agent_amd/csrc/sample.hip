@@ -148,17 +148,21 @@ template <int TYPE> __device__ __forceinline__ uint32_t comp_key(uint64_t comp) 
 }
 __device__ __forceinline__ int comp_col(uint64_t comp) { return int(kColMask - (uint32_t(comp) & kColMask)); }
 
-// 2^x for |x| <= 1/2, degree 8 (Chebyshev interpolation; relative error 2^-39.7, 1 at 0)
+// 2^x for |x| <= 1/2, degree 8 (Chebyshev interpolation; relative error 2^-39.7, 1 at 0).  The
+// coefficients are kept in scalar registers: as literals, each fma is preceded by two moves.
+__device__ __forceinline__ double in_sgpr(double v) {
+    asm("" : "+s"(v));
+    return v;
+}
 __device__ __forceinline__ double exp2_poly(double x) {
-    double p = 0x1.63cf7dec51603p-20;
-    p = __builtin_fma(p, x, 0x1.00dc48dc4d96cp-16);
-    p = __builtin_fma(p, x, 0x1.4308ae274a207p-13);
-    p = __builtin_fma(p, x, 0x1.5d8745a95d2d4p-10);
-    p = __builtin_fma(p, x, 0x1.3b2ab71725c04p-7);
-    p = __builtin_fma(p, x, 0x1.c6b08dd6fb6b1p-5);
-    p = __builtin_fma(p, x, 0x1.ebfbdff824847p-3);
-    p = __builtin_fma(p, x, 0x1.62e42fef84cf7p-1);
-    return __builtin_fma(p, x, 0x1p+0);
+    double p = __builtin_fma(x, in_sgpr(0x1.63cf7dec51603p-20), in_sgpr(0x1.00dc48dc4d96cp-16));
+    p = __builtin_fma(p, x, in_sgpr(0x1.4308ae274a207p-13));
+    p = __builtin_fma(p, x, in_sgpr(0x1.5d8745a95d2d4p-10));
+    p = __builtin_fma(p, x, in_sgpr(0x1.3b2ab71725c04p-7));
+    p = __builtin_fma(p, x, in_sgpr(0x1.c6b08dd6fb6b1p-5));
+    p = __builtin_fma(p, x, in_sgpr(0x1.ebfbdff824847p-3));
+    p = __builtin_fma(p, x, in_sgpr(0x1.62e42fef84cf7p-1));
+    return __builtin_fma(p, x, 1.0);
 }
 
 // From |j| = 2^40 on, the neighbours of the largest value lie 2^16 powers of two below it: it has
@@ -178,7 +182,10 @@ __device__ __forceinline__ int bin_mass(float v, const Scale& k, uint64_t& mass)
     const int o = int(uint32_t(__double_as_longlong(q)));                     // <= 0
     const int f = int(uint32_t(__double_as_longlong(__builtin_fma(x, double(kSub), kWhole))));
     const double e = __longlong_as_double(__double_as_longlong(exp2_poly(x)) + (int64_t(o + 36) << 52));
-    mass = uint64_t(__double_as_longlong(e + 0x1p52)) & ((uint64_t(1) << 52) - 1);
+    const uint64_t w = uint64_t(__double_as_longlong(e + 0x1p52));
+    uint32_t lo = uint32_t(w), hi = uint32_t(w >> 32) & 0xfffffu;
+    asm volatile("" : "+v"(lo), "+v"(hi));             // (computed for every lane: no branch per value)
+    mass = (uint64_t(hi) << 32) | lo;
     return o * kSub + f + kTopBin;
 }
 // The bin, for the row or part with the largest value mx, of any value up to a little above it (NaN
