@@ -27,9 +27,9 @@
  *                    transform_bf16, transform_bf16_frag, dequantize
  *   heads            head_encode, head_w8_mfma, act, head_mfma, argmax,
  *                    logits_argmax, logits_argmax_finish (long rows), fill
- *   sampling         sample_row (up to 8192 columns); sample_parts, sample_select,
- *                    and with a cut sample_gather, sample_finish; sample_empty
- *                    (no columns)
+ *   sampling         sample_row (up to 8192 columns); sample_parts, then of few
+ *                    rows sample_rest, of more sample_select and with a cut
+ *                    sample_gather, sample_finish; sample_empty (no columns)
  *   plain 4-bit      w4_tile, w4_run (more than 16 rows of many columns),
  *                    w4_zero (no inputs), w4_pack_codes, w4_pack_meta
  *   shared expert    fixed8_act, fixed8_gate

@@ -48,6 +48,7 @@ constexpr int kListMax = 16384, kListLds = 4096;     // border entries kept per 
 constexpr int kSmall = 256;                          // rows decided by a list of all their candidates
 constexpr int kMaximaK = 256;                        // top_k up to which a part drops what cannot be among it
 constexpr int kQueue = 512;                          // a wave's surviving values, compacted up to here
+constexpr int kFewParts = 256;                       // parts of a call up to which two launches do it
 constexpr int kRowThreads = 1024, kRowWaves = kRowThreads / 64, kPer = kPart / kRowThreads;
 constexpr uint32_t kMinusInf = 0x007fffffu;          // ordered(-inf)
 constexpr uint32_t kKeyEnd = 0xffffffffu;            // above every key
@@ -70,7 +71,7 @@ struct Plan {
 };
 struct RowState {
     Plan plan;
-    uint32_t count;                                  // list entries
+    uint32_t count, arrived;                         // list entries; blocks that have listed theirs (few rows)
     uint64_t cum_mass[kBins];                        // of bins >= i
 };
 
@@ -411,7 +412,10 @@ __global__ __launch_bounds__(THREADS) void sample_parts_kernel(SampleArgs a, int
     const PartMeta m = part_pass<TYPE, THREADS, kPieces>(a, s, v, col0, sh);
     __syncthreads();
     const size_t at = size_t(slot) * a.parts + part;
-    if (tid == 0) a.meta[at] = m;
+    if (tid == 0) {
+        a.meta[at] = m;
+        if (part == 0) a.state[slot].count = a.state[slot].arrived = 0;
+    }
     if (m.key && s.cut && s.T != 0.f)
         for (int i = tid; i < kBins; i += THREADS) a.hist[at * kBins + i] = sh.hist[i];
 }
@@ -941,18 +945,15 @@ __device__ __forceinline__ uint64_t threshold_of(const Setting& s, const Plan& p
     return threshold;
 }
 
+// The row's plan in sh.plan, with sh.cm, scale, shift and least; or, of a row that needs none (greedy,
+// empty, refused, without a cut), its token (given by the block with `lead`) and false.
+struct PlanShared { uint64_t mass[2][kTopBin + 24]; uint32_t count[2][kTopBin + 24]; };
 template <int TYPE>
-__global__ __launch_bounds__(kRowThreads) void sample_select_kernel(SampleArgs a, int row0) {
-    const int slot = blockIdx.x, row = row0 + slot, tid = threadIdx.x, lane = tid & 63;
-    __shared__ RowShared sh;
-    __shared__ uint64_t s_mass[2][kTopBin + 24];
-    __shared__ uint32_t s_count[2][kTopBin + 24];
-    __shared__ DrawShared s_draw;
-    RowState* st = a.state + slot;
-    const Setting s = setting(a, row);
+__device__ __forceinline__ bool plan_row(const SampleArgs& a, int slot, int row, const Setting& s, bool lead, RowShared& sh,
+                                         PlanShared& ps, DrawShared& ds) {
+    const int tid = threadIdx.x, lane = tid & 63;
     const PartMeta* meta = a.meta + size_t(slot) * a.parts;
-
-    // the row's largest value (every wave for itself) and its first part
+    // the row's largest value and its first part (every wave for itself)
     uint32_t key[kPartsMax / 64], top = 0;
 #pragma unroll
     for (int h = 0; h < kPartsMax / 64; ++h) {
@@ -960,16 +961,20 @@ __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(SampleArgs a
         top = max(top, wave_max_u(key[h]));
     }
     if (!s.valid || top == 0 || s.T == 0.f) {
-        if (tid == 0) {
-            int first = 0;
-            while (first + 1 < a.parts && meta[first].key != top) ++first;
+        int first = 0;
+#pragma unroll
+        for (int h = kPartsMax / 64 - 1; h >= 0; --h) {
+            const uint64_t at = __builtin_amdgcn_ballot_w64(key[h] == top);
+            if (at) first = h * 64 + __builtin_ctzll(at);
+        }
+        if (lead && tid == 0) {
             const bool fine = s.valid && top != 0;
-            st->plan.mode = kDone;
             give(a, row, fine ? meta[first].arg : -1, fine ? 0.f : __builtin_nanf(""));
             flag_or(a.flags, !s.valid ? kSampleSetting : top == 0 ? kSampleEmpty : 0u);
         }
-        return;
+        return false;
     }
+    if (!s.cut && !lead) return false;
     const float mx = unordered(top);
     const double J = __builtin_ceil(double(mx) * s.c);
     if (tid < a.parts) {
@@ -978,18 +983,17 @@ __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(SampleArgs a
     }
     __syncthreads();
     if (!s.cut) {
-        if (tid == 0) st->plan.mode = kDone;
         draw_part(a.parts, s, sh);
         const int part = sh.part;
         if (part < 0) {                               // (logits that changed under the call)
             if (tid == 0) give(a, row, -1, __builtin_nanf(""));
-            return;
+            return false;
         }
         Piece<TYPE> v;
         const int col0 = part * kPart + tid * kPer;
         v.load(row_of<TYPE>(a, row), col0, a.N);
-        draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], 0, v, col0, sh, s_draw);
-        return;
+        draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], 0, v, col0, sh, ds);
+        return false;
     }
     // the parts' bins: three groups of threads, a third of the parts each
     const int g = tid / (kTopBin + 24), i = tid % (kTopBin + 24), bin = kTopBin - i;
@@ -1015,71 +1019,105 @@ __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(SampleArgs a
             }
         }
         if (g) {
-            s_mass[g - 1][i] = mass;
-            s_count[g - 1][i] = count;
+            ps.mass[g - 1][i] = mass;
+            ps.count[g - 1][i] = count;
         }
     }
     __syncthreads();
     if (tid <= kTopBin) {
-        mass += s_mass[0][tid] + s_mass[1][tid];
-        count += s_count[0][tid] + s_count[1][tid];
+        mass += ps.mass[0][tid] + ps.mass[1][tid];
+        count += ps.count[0][tid] + ps.count[1][tid];
     }
     cumulate(mass, count, sh);
     borders(a, s, mx, J, a.list_max, sh);
+    if (tid == 0) sh.plan.threshold_q = s.q > 0.f ? q_threshold<TYPE>(sh.qkey) : 0;
+    return true;
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(kRowThreads) void sample_select_kernel(SampleArgs a, int row0) {
+    const int slot = blockIdx.x, row = row0 + slot, tid = threadIdx.x;
+    __shared__ RowShared sh;
+    __shared__ PlanShared s_plan;
+    __shared__ DrawShared s_draw;
+    RowState* st = a.state + slot;
+    const Setting s = setting(a, row);
+    if (!plan_row<TYPE>(a, slot, row, s, true, sh, s_plan, s_draw)) {
+        if (tid == 0) st->plan.mode = kDone;
+        return;
+    }
     if (tid == 0) {
-        sh.plan.threshold_q = s.q > 0.f ? q_threshold<TYPE>(sh.qkey) : 0;
         st->plan = sh.plan;
         st->count = 0;
     }
     if (tid < kBins) st->cum_mass[tid] = sh.cm[tid];
 }
 
-template <int TYPE, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_gather_kernel(SampleArgs a, int row0) {
-    const int part = blockIdx.x, slot = blockIdx.y, row = row0 + slot, tid = threadIdx.x;
-    RowState* st = a.state + slot;
-    const Plan& plan = st->plan;
-    if (plan.mode != kModeSmall && plan.mode != kModeList) return;
-    const PartMeta meta = a.meta[size_t(slot) * a.parts + part];
-    const uint32_t key = meta.key;
-    __shared__ int s_n[THREADS / 64];
-    __shared__ uint32_t s_at;
-    if (key < plan.lo[0] && key < plan.lo[1] && key < plan.lo[2]) return;
-    const void* src = row_of<TYPE>(a, row);
+// Lists the entries of the plan's ranges among the values that the block's threads hold.  The block takes
+// its place in the list with one addition.
+// Inside one launch (HERE) the entries pass between blocks: relaxed accesses of device scope, past the
+// caches that are not coherent between the chip's parts.
+template <bool HERE> __device__ __forceinline__ void put_entry(uint2* list, uint32_t at, uint32_t key, uint32_t col) {
+    if constexpr (HERE)
+        __hip_atomic_store(reinterpret_cast<uint64_t*>(list) + at, (uint64_t(col) << 32) | key, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+    else list[at] = make_uint2(key, col);
+}
+template <bool HERE> __device__ __forceinline__ uint2 get_entry(const uint2* list, int at) {
+    if constexpr (!HERE) return list[at];
+    const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(list) + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_uint2(uint32_t(w), uint32_t(w >> 32));
+}
+template <int THREADS> struct GatherShared { int n[THREADS / 64]; uint32_t at; };
+template <int TYPE, int THREADS, int PIECES, bool HERE>
+__device__ __forceinline__ void gather_part(const SampleArgs& a, int slot, const Plan& plan, float least,
+                                            const Piece<TYPE> (&v)[PIECES], int col0, GatherShared<THREADS>& gs) {
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     uint2* list = a.list + size_t(slot) * a.list_max;
-    constexpr int kPieces = kPart / 8 / THREADS;
-    const int col0 = part * kPart + tid * 8;
-    Piece<TYPE> v[kPieces];
-#pragma unroll
-    for (int u = 0; u < kPieces; ++u) v[u].load(src, col0 + 8 * THREADS * u, a.N);
-    // the block takes its place in the list with one addition
     uint32_t in = 0;
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
+    for (int u = 0; u < PIECES; ++u)
 #pragma unroll
         for (int e = 0; e < 8; ++e)                   // (v >= least is false for NaN)
-            in |= uint32_t(v[u][e] >= meta.least && in_ranges(plan, ordered(v[u][e]))) << (8 * u + e);
-    const int lane = tid & 63, wv = tid >> 6, own = __popc(in), run = wave_prefix_sum(own);
-    if (lane == 63) s_n[wv] = run;
+            in |= uint32_t(v[u][e] >= least && in_ranges(plan, ordered(v[u][e]))) << (8 * u + e);
+    const int own = __popc(in), run = wave_prefix_sum(own);
+    if (lane == 63) gs.n[wv] = run;
     __syncthreads();
     int before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w) {
-        before += w < wv ? s_n[w] : 0;
-        total += s_n[w];
+        before += w < wv ? gs.n[w] : 0;
+        total += gs.n[w];
     }
     if (!total) return;
-    if (tid == 0) s_at = atomicAdd(&st->count, uint32_t(total));
+    if (tid == 0) gs.at = atomicAdd(&a.state[slot].count, uint32_t(total));
     __syncthreads();
-    uint32_t at = s_at + uint32_t(before + run - own);
+    uint32_t at = gs.at + uint32_t(before + run - own);
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
+    for (int u = 0; u < PIECES; ++u)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (in >> (8 * u + e) & 1) {
-                if (at < uint32_t(a.list_max)) list[at] = make_uint2(ordered(v[u][e]), uint32_t(col0 + 8 * THREADS * u + e));
+                if (at < uint32_t(a.list_max)) put_entry<HERE>(list, at, ordered(v[u][e]), uint32_t(col0 + 8 * THREADS * u + e));
                 ++at;
             }
+}
+
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_gather_kernel(SampleArgs a, int row0) {
+    const int part = blockIdx.x, slot = blockIdx.y, row = row0 + slot;
+    const Plan& plan = a.state[slot].plan;
+    __shared__ GatherShared<THREADS> gs;
+    if (plan.mode != kModeSmall && plan.mode != kModeList) return;
+    const PartMeta meta = a.meta[size_t(slot) * a.parts + part];
+    if (meta.key < plan.lo[0] && meta.key < plan.lo[1] && meta.key < plan.lo[2]) return;
+    const void* src = row_of<TYPE>(a, row);
+    constexpr int kPieces = kPart / 8 / THREADS;
+    const int col0 = part * kPart + int(threadIdx.x) * 8;
+    Piece<TYPE> v[kPieces];
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u) v[u].load(src, col0 + 8 * THREADS * u, a.N);
+    gather_part<TYPE, THREADS, kPieces, false>(a, slot, plan, meta.least, v, col0, gs);
 }
 
 // The parts' histograms, in registers ahead of the border they are cut at: lane l of a wave holds
@@ -1118,27 +1156,17 @@ __device__ __forceinline__ void sum_parts(const SampleArgs& a, int slot, int bin
 
 struct EntryList { uint64_t comp[kListLds], mass[kListLds]; };
 
-template <int TYPE>
-__global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a, int row0) {
-    const int slot = blockIdx.x, row = row0 + slot, tid = threadIdx.x;
-    const RowState* st = a.state + slot;
-    __shared__ RowShared sh;
-    __shared__ union { SmallList small; struct { EntryList list; Descent descent; } border; DrawShared draw; } un;
-    // all that the row needs is loaded at once (the list has at least 8193 entries' room)
+union FinishShared { PlanShared plan; SmallList small; struct { EntryList list; Descent descent; } border; DrawShared draw; };
+
+// The token of a row with a plan and its entries listed (n of them; ahead0: entry `tid`, of which
+// there is room for 1024 at least).
+template <int TYPE, bool HERE>
+__device__ __forceinline__ void finish_row(const SampleArgs& a, int slot, int row, const Setting& s, int n, uint2 ahead0,
+                                           RowShared& sh, FinishShared& un) {
+    const int tid = threadIdx.x, mode = sh.plan.mode;
+    const double J = sh.plan.J;
     const uint2* list = a.list + size_t(slot) * a.list_max;
     const void* src = row_of<TYPE>(a, row);
-    const uint2 ahead0 = list[tid];
-    const uint64_t cum = tid < kBins ? st->cum_mass[tid] : 0;
-    const int mode = st->plan.mode;
-    const double J = st->plan.J;
-    const uint32_t listed = st->count;
-    const Setting s = setting(a, row);
-    if (mode == kDone) return;
-    if (tid < a.parts) load_part(a, slot, tid, s.c, J, sh);
-    if (tid == 0) sh.plan = st->plan;
-    if (tid < kBins) sh.cm[tid] = cum;
-    const int n = mode == kModeWalk ? 0 : int(min(listed, uint32_t(a.list_max)));
-    __syncthreads();
     const Plan& plan = sh.plan;
     const uint64_t tq = plan.threshold_q;
     auto entry_mass = [&](uint32_t key, int col) -> uint64_t {
@@ -1163,7 +1191,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     EntryList& en = un.border.list;
     if (lds) {
         for (int i = tid; i < n; i += kRowThreads) {
-            const uint2 w = i == tid ? ahead0 : list[i];
+            const uint2 w = i == tid ? ahead0 : get_entry<HERE>(list, i);
             en.comp[i] = comp_of<TYPE>(w.x, int(w.y));
             en.mass[i] = entry_mass(w.x, int(w.y));
         }
@@ -1178,7 +1206,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
             }
         } else if (mode == kModeList) {
             for (int i = tid; i < n; i += kRowThreads) {
-                const uint2 w = list[i];
+                const uint2 w = get_entry<HERE>(list, i);
                 if (w.x >= lo && w.x < hi) f(comp_of<TYPE>(w.x, int(w.y)), entry_mass(w.x, int(w.y)));
             }
         } else {
@@ -1218,6 +1246,57 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     const int col0 = part * kPart + tid * kPer;
     v.load(src, col0, a.N);
     draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], threshold, v, col0, sh, un.draw);
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a, int row0) {
+    const int slot = blockIdx.x, row = row0 + slot, tid = threadIdx.x;
+    const RowState* st = a.state + slot;
+    __shared__ RowShared sh;
+    __shared__ FinishShared un;
+    // all that the row needs is loaded at once
+    const uint2 ahead0 = a.list[size_t(slot) * a.list_max + tid];
+    const uint64_t cum = tid < kBins ? st->cum_mass[tid] : 0;
+    const int mode = st->plan.mode;
+    const double J = st->plan.J;
+    const uint32_t listed = st->count;
+    const Setting s = setting(a, row);
+    if (mode == kDone) return;
+    if (tid < a.parts) load_part(a, slot, tid, s.c, J, sh);
+    if (tid == 0) sh.plan = st->plan;
+    if (tid < kBins) sh.cm[tid] = cum;
+    __syncthreads();
+    finish_row<TYPE, false>(a, slot, row, s, mode == kModeWalk ? 0 : int(min(listed, uint32_t(a.list_max))), ahead0, sh, un);
+}
+
+// Select, gather and finish of few rows in one launch: every block of a row makes its plan, lists its
+// part's entries, and the last one to have done so ends the row.
+template <int TYPE>
+__global__ __launch_bounds__(kRowThreads) void sample_rest_kernel(SampleArgs a, int row0) {
+    const int part = blockIdx.x, slot = blockIdx.y, row = row0 + slot, tid = threadIdx.x;
+    RowState* st = a.state + slot;
+    __shared__ RowShared sh;
+    __shared__ FinishShared un;
+    __shared__ GatherShared<kRowThreads> gs;
+    __shared__ uint32_t s_arrived;
+    Piece<TYPE> v[1];
+    const int col0 = part * kPart + tid * kPer;
+    v[0].load(row_of<TYPE>(a, row), col0, a.N);
+    const Setting s = setting(a, row);
+    // (a draw's scratch lies over the plan's: rows without a cut do not use that)
+    if (!plan_row<TYPE>(a, slot, row, s, part == 0, sh, un.plan, un.draw)) return;
+    __syncthreads();
+    if (sh.plan.mode != kModeWalk && sh.shift[part] < 64)
+        gather_part<TYPE, kRowThreads, 1, true>(a, slot, sh.plan, sh.least[part], v, col0, gs);
+    // every wave's entries have reached the device's memory before the block counts as done
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) s_arrived = __hip_atomic_fetch_add(&st->arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (s_arrived != uint32_t(a.parts) - 1) return;
+    const uint32_t listed = __hip_atomic_load(&st->count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint2 ahead0 = get_entry<true>(a.list + size_t(slot) * a.list_max, tid);
+    finish_row<TYPE, true>(a, slot, row, s, sh.plan.mode == kModeWalk ? 0 : int(min(listed, uint32_t(a.list_max))), ahead0, sh, un);
 }
 
 // Rows of one part: all of it by one block, the logits in LDS after the histogram.
@@ -1345,15 +1424,17 @@ SampleLayout sample_layout(int Mcap, int N) {
 
 template <int TYPE> hipError_t sample_rows(const SampleArgs& a, int row0, int rows, hipStream_t s) {
     const dim3 parts(a.parts, rows);
-    const bool few = a.parts * rows <= 2 * device_cu_count();
-    if (few) timed_launch("sample_parts", sample_parts_kernel<TYPE, 1024>, parts, dim3(1024), 0, s, a, row0);
-    else timed_launch("sample_parts", sample_parts_kernel<TYPE, 256>, parts, dim3(256), 0, s, a, row0);
+    if (a.parts * rows <= kFewParts) {
+        timed_launch("sample_parts", sample_parts_kernel<TYPE, 1024>, parts, dim3(1024), 0, s, a, row0);
+        timed_launch("sample_rest", sample_rest_kernel<TYPE>, parts, dim3(kRowThreads), 0, s, a, row0);
+        return hipGetLastError();
+    }
+    timed_launch("sample_parts", sample_parts_kernel<TYPE, 256>, parts, dim3(256), 0, s, a, row0);
     timed_launch("sample_select", sample_select_kernel<TYPE>, dim3(rows), dim3(kRowThreads), 0, s, a, row0);
-    hipError_t st = hipGetLastError();
+    const hipError_t st = hipGetLastError();
     // with no cut at all, select has drawn every row
     if (st != hipSuccess || (!a.top_k && !a.top_p && !a.min_p)) return st;
-    if (few) timed_launch("sample_gather", sample_gather_kernel<TYPE, 1024>, parts, dim3(1024), 0, s, a, row0);
-    else timed_launch("sample_gather", sample_gather_kernel<TYPE, 256>, parts, dim3(256), 0, s, a, row0);
+    timed_launch("sample_gather", sample_gather_kernel<TYPE, 256>, parts, dim3(256), 0, s, a, row0);
     timed_launch("sample_finish", sample_finish_kernel<TYPE>, dim3(rows), dim3(kRowThreads), 0, s, a, row0);
     return hipGetLastError();
 }
