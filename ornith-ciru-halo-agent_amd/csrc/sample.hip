@@ -67,6 +67,7 @@ struct Plan {
     uint64_t threshold_q;                            // min-p's threshold (0: none)
     uint64_t total, above_mass;                      // row mass; mass of the bins above bin_k
     int32_t mode, use_k, use_p, bin_k, bin_q, above_count;
+    int32_t bin_lo[3], bin_hi[3];                    // the ranges' bins
     uint32_t lo[3], hi[3];                           // key ranges [lo, hi) to gather (the first: bin_k's; unused: empty)
 };
 struct RowState {
@@ -198,9 +199,9 @@ __device__ __forceinline__ int bin_of(float v, float mx, double c, double j) {
     return double(v) * c > j - 64.0 ? max(bin, -1) : -1;
 }
 // A value a little below the lower edge of `bin`; never -inf.
-__device__ __forceinline__ float below_bin(int bin, float mx, double c, double j) {
+__device__ __forceinline__ float below_bin(int bin, float mx, double inv, double j) {
     if (is_far(j)) return mx;
-    const float at = float((j + (double(bin - kTopBin) - 0.5) * (1.0 / kSub)) / c);
+    const float at = float((j + (double(bin - kTopBin) - 0.5) * (1.0 / kSub)) * inv);
     return fmaxf(at - __builtin_fabsf(at) * 0x1p-20f - 0x1p-126f, -0x1.fffffep127f);
 }
 
@@ -216,7 +217,7 @@ __device__ __forceinline__ uint64_t share(float p, uint64_t mass) {
     return max(__umul64hi(f, mass) + (f * mass != 0), uint64_t(1));
 }
 
-struct Setting { float T, p, q, u; int k; bool valid, cut; double c; };
+struct Setting { float T, p, q, u; int k; bool valid, cut; double c, inv; };      // c = log2(e) / T, inv = 1 / c
 __device__ __forceinline__ Setting setting(const SampleArgs& a, int row) {
     Setting s;
     s.T = a.temperature ? a.temperature[row] : 1.f;
@@ -228,6 +229,7 @@ __device__ __forceinline__ Setting setting(const SampleArgs& a, int row) {
               s.u >= 0.f && s.u < 1.f;
     s.cut = (s.k > 0 && s.k < a.N) || s.p < 1.f || s.q > 0.f;
     s.c = s.T > 0.f ? 0x1.71547652b82fep+0 / double(s.T) : 0.0;
+    s.inv = double(s.T) * 0x1.62e42fefa39efp-1;
     return s;
 }
 
@@ -255,9 +257,9 @@ __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) { return readlane_u
 
 // The least key whose bin is at least `bin`, by the whole wave: the estimate of the bin's lower edge
 // is off by less than a step of fp32, so the 64 keys around it hold it.
-__device__ __forceinline__ uint32_t bin_edge(int bin, float mx, double c, double j) {
+__device__ __forceinline__ uint32_t bin_edge(int bin, float mx, double c, double inv, double j) {
     if (is_far(j)) return ordered(mx);
-    const double at = (j + (double(bin - kTopBin) - 0.5) * (1.0 / kSub)) / c;
+    const double at = (j + (double(bin - kTopBin) - 0.5) * (1.0 / kSub)) * inv;
     const uint32_t first = max(ordered(float(at)), kMinusInf + 33) - 32, k0 = first + (threadIdx.x & 63);
     const uint64_t in = __builtin_amdgcn_ballot_w64(k0 >= ordered(__builtin_huge_valf()) ||
                                                     bin_of(unordered(k0), mx, c, j) >= bin);
@@ -321,7 +323,7 @@ __device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting
     const float part_mx = unordered(key);
     const double j = __builtin_ceil(double(part_mx) * s.c);
     const Scale k = scale_of(s.c, j);
-    float least = below_bin(0, part_mx, s.c, j);
+    float least = below_bin(0, part_mx, s.inv, j);
     if (!s.cut) {
         uint64_t sum = 0;
 #pragma unroll
@@ -362,7 +364,7 @@ __device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting
             if (run < uint32_t(s.k) && run + c[e] >= uint32_t(s.k)) found = kTopBin - (per * lane + e);
             run += c[e];
         }
-        least = below_bin(int(wave_max_u(uint32_t(found))), part_mx, s.c, j);
+        least = below_bin(int(wave_max_u(uint32_t(found))), part_mx, s.inv, j);
     }
     auto add = [&](float x) {
         uint64_t m;
@@ -552,7 +554,7 @@ __device__ __forceinline__ void borders(const SampleArgs& a, const Setting& s, f
     }
     if (wv < 6) {
         const int r = wv >> 1, b = wv & 1 ? hi[r] + 1 : lo[r];
-        const uint32_t edge = lo[r] < 0 || b > kTopBin ? kKeyEnd : bin_edge(b, mx, s.c, J);
+        const uint32_t edge = lo[r] < 0 || b > kTopBin ? kKeyEnd : bin_edge(b, mx, s.c, s.inv, J);
         if (lane == 0) sh.edge[wv] = edge;
     }
     __syncthreads();
@@ -571,9 +573,29 @@ __device__ __forceinline__ void borders(const SampleArgs& a, const Setting& s, f
         p.above_mass = bk < 0 || bk == kTopBin ? 0 : cm[bk + 1];
 #pragma unroll
         for (int r = 0; r < 3; ++r) {
+            p.bin_lo[r] = lo[r];
+            p.bin_hi[r] = hi[r];
             p.lo[r] = sh.edge[2 * r];
             p.hi[r] = sh.edge[2 * r + 1];
         }
+    }
+    __syncthreads();
+}
+// The key range of one bin into sh.edge[0 .. 1] (after the barrier in it); mostly a range of the plan.
+__device__ __forceinline__ void bin_range(int bin, const Setting& s, const Plan& plan, RowShared& sh) {
+    const int tid = threadIdx.x, wv = tid >> 6;
+    int at = -1;
+#pragma unroll
+    for (int r = 0; r < 3; ++r)
+        if (plan.bin_lo[r] == bin && plan.bin_hi[r] == bin) at = r;
+    if (at >= 0) {
+        if (tid == 0) {
+            sh.edge[0] = plan.lo[at];
+            sh.edge[1] = plan.hi[at];
+        }
+    } else if (wv < 2) {
+        const uint32_t edge = bin < 0 || bin + wv > kTopBin ? kKeyEnd : bin_edge(bin + wv, plan.mx, s.c, s.inv, plan.J);
+        if ((tid & 63) == 0) sh.edge[wv] = edge;
     }
     __syncthreads();
 }
@@ -788,11 +810,11 @@ __device__ __forceinline__ void finish_small(const SampleArgs& a, int row, const
 
 // Descent to a border inside one bin's key range: the entry at which, from the largest down, `need`
 // is reached - a count, or a mass.  each(f) runs f(comp, row mass) over the entries of the range
-// [lo, hi) of keys, spread over the block.  A round counts the entries by the next ten bits of
-// comp - base; 64 or fewer are ranked by one wave.
+// [lo, hi) of keys, spread over the block.  A round counts the entries by the next eight bits of
+// comp - base; 64 or fewer are ranked, four threads an entry.
 struct Descent {
-    uint32_t count[1024];
-    unsigned long long mass[1024];
+    uint32_t count[256];
+    unsigned long long mass[256];
     uint64_t comp[64], m[64];
     uint64_t wave_mass[kRowWaves];
     uint32_t wave_count[kRowWaves];
@@ -800,26 +822,27 @@ struct Descent {
     uint32_t digit, group, n;
 };
 template <int TYPE, class Each>
-__device__ __forceinline__ void descend(uint32_t lo, uint32_t hi, bool by_mass, uint64_t need, Each&& each, Descent& d) {
+__device__ __forceinline__ void descend(uint32_t lo, uint32_t hi, bool by_mass, uint64_t need, uint32_t group, Each&& each, Descent& d) {
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    static_assert(kRowThreads == 1024, "a thread per digit");
     uint64_t base = uint64_t(lo >> kDrop<TYPE>) << kColBits;
     uint64_t span = (uint64_t(((hi - 1) >> kDrop<TYPE>) + 1) << kColBits) - base;   // comps lie in [base, base + span)
     uint64_t above = 0;
-    uint32_t group = 65;
-    while (true) {
+    while (true) {                                    // group: entries left, or more
         const int bits = 64 - __builtin_clzll(span - 1 | 1);
-        const int sft = bits > 10 ? bits - 10 : 0;
+        const int sft = bits > 8 ? bits - 8 : 0;
         __syncthreads();
-        d.count[tid] = 0;
-        d.mass[tid] = 0;
-        if (tid < 64) {
-            d.comp[tid] = 0;
-            d.m[tid] = 0;
+        if (tid < 256) {
+            d.count[tid] = 0;
+            d.mass[tid] = 0;
+            if (tid < 64) {
+                d.comp[tid] = 0;
+                d.m[tid] = 0;
+            }
         }
         if (tid == 0) {
             d.n = 0;
             d.group = 0;
+            d.found = 0;
         }
         __syncthreads();
         if (group <= 64) break;
@@ -830,43 +853,54 @@ __device__ __forceinline__ void descend(uint32_t lo, uint32_t hi, bool by_mass, 
             atomicAdd(&d.mass[i], (unsigned long long)m);
         });
         __syncthreads();
-        // thread i: digit 1023 - i
-        const uint32_t c = d.count[1023 - tid];
-        const uint64_t m = d.mass[1023 - tid];
-        uint32_t cr = uint32_t(wave_prefix_sum(int(c)));
-        uint64_t mr = wave_prefix_u64(m);
-        if (lane == 63) {
-            d.wave_count[wv] = cr;
-            d.wave_mass[wv] = mr;
+        // thread i < 256: digit 255 - i
+        uint32_t c = 0, cr = 0;
+        uint64_t m = 0, mr = 0;
+        if (wv < 4) {
+            c = d.count[255 - tid];
+            m = d.mass[255 - tid];
+            cr = uint32_t(wave_prefix_sum(int(c)));
+            mr = wave_prefix_u64(m);
+            if (lane == 63) {
+                d.wave_count[wv] = cr;
+                d.wave_mass[wv] = mr;
+            }
         }
         __syncthreads();
-        uint32_t call;
-        uint64_t mall;
-        cr += waves_before(d.wave_count, call);
-        mr += waves_before(d.wave_mass, mall);
-        // the entries can sum to a few units less than their bin (cut once per part): then the last is the border
-        const bool short_of = by_mass ? mall < need : call < need;
-        const uint64_t b0 = by_mass ? mr - m : cr - c, b1 = by_mass ? mr : cr;
-        if (c && (short_of ? cr == call : b0 < need && b1 >= need)) {
-            d.digit = uint32_t(1023 - tid);
-            d.group = c;
-            d.need = short_of ? ~uint64_t(0) : need - b0;
-            d.above = above + (mr - m);
+        if (wv < 4) {
+            uint32_t call = 0;
+            uint64_t mall = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t cw = d.wave_count[w];
+                const uint64_t mw = d.wave_mass[w];
+                cr += w < wv ? cw : 0;
+                mr += w < wv ? mw : 0;
+                call += cw;
+                mall += mw;
+            }
+            // the entries can sum to a few units less than their bin (cut once per part): then the last is the border
+            const bool short_of = by_mass ? mall < need : call < need;
+            const uint64_t b0 = by_mass ? mr - m : cr - c, b1 = by_mass ? mr : cr;
+            if (c && (short_of ? cr == call : b0 < need && b1 >= need)) {
+                d.digit = uint32_t(255 - tid);
+                d.group = c;
+                d.need = short_of ? ~uint64_t(0) : need - b0;
+                d.above = above + (mr - m);
+            }
         }
         __syncthreads();
         group = d.group;
-        if (group == 0) {                             // nothing in the range
-            if (tid == 0) {
-                d.found = 0;
-                d.above = 0;
-            }
-            __syncthreads();
-            return;
-        }
+        if (group == 0) break;                        // nothing in the range
         need = d.need;
         above = d.above;
         base += uint64_t(d.digit) << sft;
         span = uint64_t(1) << sft;
+    }
+    if (group == 0) {
+        if (tid == 0) d.above = 0;
+        __syncthreads();
+        return;
     }
     each([&](uint64_t comp, uint64_t m) {
         if (comp - base >= span) return;
@@ -878,20 +912,24 @@ __device__ __forceinline__ void descend(uint32_t lo, uint32_t hi, bool by_mass, 
     });
     __syncthreads();
     const int n = min(int(d.n), 64);
-    if (tid < 64) {
-        const uint64_t comp = tid < n ? d.comp[tid] : 0, m = tid < n ? d.m[tid] : 0;
-        uint64_t count = 0, before = 0;
-        // (zeros past n: the loads of eight steps in flight at once)
-#pragma unroll 8
-        for (int i = 0; i < 64; ++i) {
-            const uint64_t mi = d.m[i];
-            const bool b = d.comp[i] > comp;
-            count += b;
-            before += b ? mi : 0;
+    if (tid < 256) {                                  // (zeros past n)
+        const int e = tid >> 2;
+        const uint64_t comp = d.comp[e], m = d.m[e];
+        uint32_t count = 0;
+        uint64_t before = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint64_t ci = d.comp[4 * i + (tid & 3)], mi = d.m[4 * i + (tid & 3)];
+            count += ci > comp;
+            before += ci > comp ? mi : 0;
         }
-        const bool at = by_mass ? before < need && before + m >= need : count + 1 == need;
-        const bool any = __builtin_amdgcn_ballot_w64(tid < n && at);
-        if (tid < n && (any ? at : count + 1 == uint64_t(n))) {
+        count += uint32_t(dpp_i<kDppXor1>(int(count)));
+        count += uint32_t(dpp_i<kDppXor2>(int(count)));
+        before += dpp_u64<kDppXor1, 0xF>(before);
+        before += dpp_u64<kDppXor2, 0xF>(before);
+        // (short of `need` again: the last)
+        const bool at = by_mass ? before < need && (before + m >= need || count + 1 == uint32_t(n)) : count + 1 == min(need, uint64_t(n));
+        if (e < n && at) {
             d.found = comp;
             d.above = above + before + m;
         }
@@ -899,15 +937,16 @@ __device__ __forceinline__ void descend(uint32_t lo, uint32_t hi, bool by_mass, 
     __syncthreads();
 }
 
-// Threshold of a row in list (or walk) mode.  bf: the bin it lies in (-1: below the bins).
+// Threshold of a row in list (or walk) mode.  group: the entries of all ranges, or more; bf: the bin it
+// lies in (-1: below the bins).
 template <int TYPE, class Each>
 __device__ __forceinline__ uint64_t threshold_of(const Setting& s, const Plan& plan, const uint64_t* cm, uint64_t threshold,
-                                                 Each&& each, Descent& d, RowShared& sh, int& bf) {
-    const int tid = threadIdx.x, wv = tid >> 6;
+                                                 uint32_t group, Each&& each, Descent& d, RowShared& sh, int& bf) {
+    const int tid = threadIdx.x;
     bf = threshold ? plan.bin_q : -1;
     uint64_t of = plan.total;
     if (plan.use_k) {
-        descend<TYPE>(plan.lo[0], plan.hi[0], false, uint64_t(s.k) - uint64_t(plan.above_count),
+        descend<TYPE>(plan.lo[0], plan.hi[0], false, uint64_t(s.k) - uint64_t(plan.above_count), group,
                       [&](auto&& f) { each(plan.lo[0], plan.hi[0], f); }, d);
         if (d.found > threshold) {
             threshold = d.found;
@@ -929,13 +968,9 @@ __device__ __forceinline__ uint64_t threshold_of(const Setting& s, const Plan& p
         }
         __syncthreads();
         const int b = sh.bin[0];
-        if (wv < 2) {
-            const uint32_t edge = b + wv > kTopBin ? kKeyEnd : bin_edge(b + wv, plan.mx, s.c, plan.J);
-            if ((tid & 63) == 0) sh.edge[wv] = edge;
-        }
-        __syncthreads();
+        bin_range(b, s, plan, sh);
         const uint32_t lo = sh.edge[0], hi = sh.edge[1];
-        descend<TYPE>(lo, hi, true, sh.lo, [&](auto&& f) { each(lo, hi, f); }, d);
+        descend<TYPE>(lo, hi, true, sh.lo, group, [&](auto&& f) { each(lo, hi, f); }, d);
         if (d.found > threshold) {
             threshold = d.found;
             bf = b;
@@ -1001,7 +1036,7 @@ __device__ __forceinline__ bool plan_row(const SampleArgs& a, int slot, int row,
     uint32_t count = 0;
     if (g < 3 && bin >= 0) {
         const uint64_t* hist = a.hist + size_t(slot) * a.parts * kBins;
-        constexpr int U = 6;
+        constexpr int U = 11;                         // (33 parts' loads in flight at once)
         for (int p0 = g; p0 < a.parts; p0 += 3 * U) {
             uint64_t w[U];
             int sf[U];
@@ -1222,14 +1257,9 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, int slot, int ro
         }
     };
     int bf;
-    const uint64_t threshold = threshold_of<TYPE>(s, plan, sh.cm, tq, each, un.border.descent, sh, bf);
+    const uint64_t threshold = threshold_of<TYPE>(s, plan, sh.cm, tq, mode == kModeWalk ? ~0u : uint32_t(n), each, un.border.descent, sh, bf);
     sum_parts(a, slot, bf, ahead, sh);
-    if (tid < 2 * 64) {
-        const int wv = tid >> 6;
-        const uint32_t edge = bf < 0 || bf + wv > kTopBin ? kKeyEnd : bin_edge(bf + wv, plan.mx, s.c, J);
-        if ((tid & 63) == 0) sh.edge[wv] = edge;
-    }
-    __syncthreads();
+    bin_range(bf, s, plan, sh);
     if (bf >= 0)
         each(sh.edge[0], sh.edge[1], [&](uint64_t comp, uint64_t m) {
             if (comp >= threshold)
@@ -1367,7 +1397,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
             }
         };
         int bf;
-        threshold = threshold_of<TYPE>(s, plan, sh.cm, threshold, each, un.descent, sh, bf);
+        threshold = threshold_of<TYPE>(s, plan, sh.cm, threshold, ~0u, each, un.descent, sh, bf);
     }
     // the kept mass, and the token
     uint64_t sum = 0;
