@@ -37,11 +37,12 @@ ORNITH_EXPORT hipError_t ornith_w4_get_layout(int N, int K, int G, size_t* code_
 
 /* Banks from a checkpoint's rows: codes uint32 [N, K/8], eight low-first 4-bit
  * values per word; scales [N, ceil(K/G)] bf16 or fp16 (scale_type); zeros uint8
- * [N, ceil(K/G)] (only bits 0..3 are read) or NULL: 8 everywhere.  Code buffers
- * 4- and 16-byte aligned, meta 4; the outputs must not overlap anything. */
+ * [N, ceil(K/G)] or NULL: 8 everywhere.  Code buffers 4- and 16-byte aligned,
+ * meta 4; the outputs must not overlap anything.  Flags (sticky): 1 a scale that
+ * is not finite, 2 a zero point above 15 (its low four bits are taken). */
 ORNITH_EXPORT hipError_t ornith_w4_pack(const void* codes_u32, const void* scales, int scale_type,
-                                        const void* zeros_u8, void* packed_codes, void* packed_meta, int N, int K,
-                                        int G, hipStream_t stream);
+                                        const void* zeros_u8, void* packed_codes, void* packed_meta,
+                                        void* flags_u32, int N, int K, int G, hipStream_t stream);
 
 /* out [M, N] of out_type (stride ldo >= N) from x [M, K] of x_type (bf16 or
  * fp16; stride ldx >= K).  x and ldx on the 16-byte grid; out aligned to its

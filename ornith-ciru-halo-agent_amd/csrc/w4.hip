@@ -63,7 +63,8 @@ __global__ __launch_bounds__(256) void w4_pack_codes_kernel(const uint32_t* __re
 
 __global__ __launch_bounds__(256) void w4_pack_meta_kernel(const uint16_t* __restrict__ scales, int scale_type,
                                                            const uint8_t* __restrict__ zeros, uint32_t* __restrict__ out,
-                                                           int N, int groups, int chunks, int per, size_t words) {
+                                                           int N, int groups, int chunks, int per, size_t words,
+                                                           uint32_t* flags) {
     const size_t i = size_t(blockIdx.x) * 256 + threadIdx.x;
     if (i >= words) return;
     const size_t tc = i / size_t(16 * per);
@@ -73,7 +74,9 @@ __global__ __launch_bounds__(256) void w4_pack_meta_kernel(const uint16_t* __res
     if (n < N && g < groups) {
         const size_t at = size_t(n) * groups + g;
         const float s = scale_type == ORNITH_W4_BF16 ? bf16_bits_to_f32(scales[at]) : f16_bits_to_f32(scales[at]);
-        w = (__float_as_uint(s) & ~15u) | (zeros ? zeros[at] & 15u : 8u);
+        const uint32_t z = zeros ? zeros[at] : 8u;
+        flag_or(flags, (isfinite(s) ? 0u : 1u) | (z > 15u ? 2u : 0u));
+        w = (__float_as_uint(s) & ~15u) | (z & 15u);
     }
     out[i] = w;
 }
@@ -447,7 +450,8 @@ extern "C" hipError_t ornith_w4_get_layout(int N, int K, int G, size_t* code_wor
 }
 
 extern "C" hipError_t ornith_w4_pack(const void* codes, const void* scales, int scale_type, const void* zeros,
-                                     void* packed_codes, void* packed_meta, int N, int K, int G, hipStream_t stream) {
+                                     void* packed_codes, void* packed_meta, void* flags, int N, int K, int G,
+                                     hipStream_t stream) {
     size_t c = 0, m = 0;
     if (!w4_words(N, K, G, c, m) || (scale_type != ORNITH_W4_BF16 && scale_type != ORNITH_W4_F16))
         return hipErrorInvalidValue;
@@ -458,7 +462,8 @@ extern "C" hipError_t ornith_w4_pack(const void* codes, const void* scales, int 
                               {scales, pairs * 2, 2, false, false},
                               {zeros, pairs, 1, false, true},
                               {packed_codes, c * 4, 16, true, false},
-                              {packed_meta, m * 4, 4, true, false}};
+                              {packed_meta, m * 4, 4, true, false},
+                              {flags, 4, 4, true, false}};
     if (!check_buffers(buffers)) return hipErrorInvalidValue;
     timed_launch("w4_pack_codes", w4_pack_codes_kernel, dim3(unsigned((c + 255) / 256)), dim3(256), 0, stream,
                  static_cast<const uint32_t*>(codes), static_cast<uint32_t*>(packed_codes), N, K, c);
@@ -467,7 +472,7 @@ extern "C" hipError_t ornith_w4_pack(const void* codes, const void* scales, int 
     timed_launch("w4_pack_meta", w4_pack_meta_kernel, dim3(unsigned((m + 255) / 256)), dim3(256), 0, stream,
                  static_cast<const uint16_t*>(scales), scale_type, static_cast<const uint8_t*>(zeros),
                  static_cast<uint32_t*>(packed_meta), N, groups,
-                 G == 256 ? (w4_blocks(K) + 1) / 2 : w4_blocks(K), G == 256 ? 1 : kW4Block / G, m);
+                 G == 256 ? (w4_blocks(K) + 1) / 2 : w4_blocks(K), G == 256 ? 1 : kW4Block / G, m, static_cast<uint32_t*>(flags));
     return hipGetLastError();
 }
 

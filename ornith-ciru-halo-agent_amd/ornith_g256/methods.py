@@ -9,6 +9,9 @@ registration that routes vLLM's layers to them is in vllm_plugin.py.
   [N/16, K/256, 32, 16] / [N/16, K/256, 16] (method.py:35-62).
 * ``W8HeadMethod`` - the W8 G128 LM head: [15520, 128, 4, 16] words and
   fp16 scales [248320, 16], applied in chunks of 64 rows (method.py:65-88).
+* ``W4LinearMethod`` - a linear of plain 4-bit weights with group scales and
+  perhaps zero points, on unrotated bf16 or fp16 rows (no reference
+  counterpart); the banks are packed once on the GPU.
 * ``G256MoEMethod`` - the routed experts: four N16 banks
   (method.py:100-122), optionally repacked to N32 once on the GPU
   (method.py:124-158), and ``apply`` (method.py:165-183).
@@ -92,6 +95,51 @@ class W8HeadMethod(G256LinearMethod):
             native.head_out(x[start:end], layer.head_tilebank_codes, layer.head_scales, rt.workspace,
                             out[start:end], rt.slots[self.slot], rt.head_geometry)
         return out
+
+
+    def sample(self, layer, x, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
+        """One token per row of the head's logits (native.logits_sample): int64
+        tokens and the logs of the probabilities they were drawn with."""
+        logits = self.apply(layer, x)
+        token = torch.empty(logits.shape[0], dtype=torch.int64, device=logits.device)
+        logprob = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+        native.logits_sample(logits, uniform, self.runtime.workspace, token, self.runtime.slots[self.slot],
+                             temperature, top_k, top_p, min_p, logprob)
+        return token, logprob
+
+
+class W4LinearMethod:
+    """out_dtype: the rows' dtype if None (fp32 for a head whose logits are
+    sampled from)."""
+
+    def __init__(self, prefix, n, k, group=128, zeros=False, scale_dtype=torch.bfloat16, out_dtype=None):
+        self.prefix, self.n, self.k, self.group = prefix, int(n), int(k), int(group)
+        self.zeros, self.scale_dtype, self.out_dtype = bool(zeros), scale_dtype, out_dtype
+        self.runtime, self.slot = None, None
+
+    def create_weights(self, layer):
+        _register(layer, storage.w4_shapes(self.n, self.k, self.group, self.zeros), storage.w4_dtypes(self.scale_dtype))
+
+    def process_weights_after_loading(self, layer):
+        """Packs the loaded fields on the layer's GPU, in their place."""
+        layer._ornith_loader.seal()
+        packed = storage.pack_w4(layer.w4_codes.data, layer.w4_scales.data,
+                                 layer.w4_zeros.data if self.zeros else None, self.group)
+        for name in storage.w4_shapes(self.n, self.k, self.group, self.zeros):
+            delattr(layer, name)
+        for name, bank in zip(('w4_bank', 'w4_metadata'), packed):
+            layer.register_buffer(name, bank, persistent=False)
+
+    def apply(self, layer, x, bias=None):
+        if self.runtime is None or not hasattr(layer, 'w4_bank') or bias is not None:
+            raise RuntimeError(f'{self.prefix}: needs packed weights, no bias and a bound runtime')
+        shape = x.shape[:-1]
+        x = x.reshape(-1, self.k)
+        if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+            x = x.contiguous()
+        out = torch.empty((x.shape[0], self.n), dtype=self.out_dtype or x.dtype, device=x.device)
+        native.w4_out(x, layer.w4_bank, layer.w4_metadata, out, self.runtime.slots[self.slot], self.n, self.k, self.group)
+        return out.view(*shape, self.n)
 
 
 class G256MoEMethod:
@@ -291,7 +339,7 @@ class Runtime:
             raise ValueError('dense_a8_max_rows must be 32 or 64')
         if self.dense_geometry not in (0, 1, 2) or self.head_geometry not in (0, 1, 2):
             raise ValueError('geometry settings must be 0, 1 or 2')
-        kinds = (G256LinearMethod, G256MoEMethod, RouterGateMethod)
+        kinds = (G256LinearMethod, W4LinearMethod, G256MoEMethod, RouterGateMethod)
         self.layers = [(name, m) for name, m in model.named_modules() if isinstance(getattr(m, 'quant_method', None), kinds)]
         modules = dict(model.named_modules())
         # shared experts: '<block>.shared_expert' MLPs whose projections are G256

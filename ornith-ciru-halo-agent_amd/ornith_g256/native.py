@@ -113,7 +113,7 @@ _PROTOTYPES = {
     'ornith_logits_sample_launch': ([_VP] + [_INT] * 3 + [_I64] + [_VP] * 6 + [_SZ] + [_VP] * 4, _INT),
     # plain 4-bit linears (include/ornith_w4.h)
     'ornith_w4_get_layout': ([_INT] * 3 + [C.POINTER(_SZ)] * 2, _INT),
-    'ornith_w4_pack': ([_VP] * 2 + [_INT] + [_VP] * 3 + [_INT] * 3 + [_VP], _INT),
+    'ornith_w4_pack': ([_VP] * 2 + [_INT] + [_VP] * 4 + [_INT] * 3 + [_VP], _INT),
     'ornith_w4_launch': ([_VP, _INT, _I64] + [_VP] * 3 + [_INT, _I64, _VP] + [_INT] * 4 + [_VP], _INT),
     # measurement (include/ornith_timing.h)
     'ornith_mi355x_timing_arm': ([C.c_char_p, _INT], _INT),
@@ -200,7 +200,7 @@ def configure(settings, capacity, shapes, shared_expert=False):
     """Resolve the library roles, bind the launch entries and return the
     workspace size the caller allocates once (the max over the routed
     layout, the dense layouts plus the GEMM's transformed rows, the W8 head
-    layout and, with `shared_expert`, the fused shared slot and fixed8)."""
+    layout, sampling from its logits and, with `shared_expert`, the fused shared slot and fixed8)."""
     global _binding
     a8 = settings.get('routed_activation_bits', 8)
     a8_prefill = settings.get('routed_prefill_activation_bits', 8)
@@ -256,6 +256,7 @@ def configure(settings, capacity, shapes, shared_expert=False):
         # the GEMM's bf16(H128 x), rows padded to 16, then its split-K slice sums
         sizes.append((int(capacity) + 15) // 16 * 16 * k * 2 + DENSE_SLICE_BYTES)
     sizes.append(head_layout(HEAD_MAX_ROWS, HEAD_VOCAB, tile=roles['head']).workspace_bytes)
+    sizes.append(logits_sample_bytes(HEAD_MAX_ROWS, HEAD_VOCAB))
     if shared_expert:
         # the fused ninth slot (at most 16 rows, any routed build) and fixed8
         for tile in {roles['routed'], 32}:

@@ -34,6 +34,18 @@ def routed_shapes(experts=256, hidden=2048, inter=512, tile=16):
     return out
 
 
+def w4_shapes(n, k, group, zeros):
+    """Shapes of a plain 4-bit linear's checkpoint fields (dtypes: w4_dtypes)."""
+    if not 0 < n <= 1 << 20 or not 0 < k <= 65536 or k % 8 or group not in (32, 64, 128, 256):
+        raise AdmissionError(f'unsupported 4-bit linear geometry N{n}/K{k}/G{group}')
+    groups = (n, -(-k // group))
+    return {'w4_codes': (n, k // 8), 'w4_scales': groups} | ({'w4_zeros': groups} if zeros else {})
+
+
+def w4_dtypes(scale_dtype):
+    return {'w4_codes': torch.uint32, 'w4_scales': scale_dtype, 'w4_zeros': torch.uint8}
+
+
 def dense_shapes(n, k, tile=16):
     """Shapes of a dense G256 linear's codes and metadata (method.py:44-45)."""
     if not 0 < n <= 12288 or n % 16 or not 0 < k <= 8192 or k % 256:
@@ -123,7 +135,8 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     native.w4_out reads, once, through the library's pack kernel:
     codes 32-bit words [n, k/8] of eight low-first codes, scales bf16 or fp16
     [n, ceil(k/group)], zeros uint8 of that shape, 0..15, or None (8
-    everywhere).  Returns int32 codes and metadata (include/ornith_w4.h)."""
+    everywhere).  Returns int32 codes and metadata (include/ornith_w4.h);
+    scales must be finite.  Waits for the device."""
     if codes.device.type != 'cuda' or scales.device != codes.device or (zeros is not None and
                                                                          zeros.device != codes.device):
         raise ValueError('the pack runs on GPU-resident banks')
@@ -138,15 +151,15 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     if tuple(scales.shape) != shape or (zeros is not None and (tuple(zeros.shape) != shape
                                                                or zeros.dtype != torch.uint8)):
         raise ValueError(f'scales and uint8 zeros must be {shape}')
-    if not bool(torch.isfinite(scales).all()):
-        raise AdmissionError('non-finite scale')
-    if zeros is not None and zeros.numel() and int(zeros.max()) > 15:
-        raise AdmissionError('zero point above 15')
     codes, scales = codes.contiguous(), scales.contiguous()
     zeros = None if zeros is None else zeros.contiguous()
     packed = [torch.empty(s, dtype=torch.int32, device=codes.device) for s in native.w4_layout(n, k, group)]
+    flags = torch.zeros(1, dtype=torch.int32, device=codes.device)
     with native.on_device(codes.device):
         native.check(native.lib().ornith_w4_pack(native.ptr(codes), native.ptr(scales), native.W4_TYPES[scales.dtype],
-                                                 native.ptr(zeros), native.ptr(packed[0]), native.ptr(packed[1]), n, k,
-                                                 group, native.stream(codes)), 'w4 pack')
+                                                 native.ptr(zeros), native.ptr(packed[0]), native.ptr(packed[1]),
+                                                 native.ptr(flags), n, k, group, native.stream(codes)), 'w4 pack')
+    bad = int(flags.item())
+    if bad:
+        raise AdmissionError('non-finite scale' if bad & 1 else 'zero point above 15')
     return tuple(packed)

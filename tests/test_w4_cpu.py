@@ -54,15 +54,16 @@ def test_launch_refusals(lib, bad):
 def test_nothing_to_do(lib):
     assert lib.ornith_w4_launch(*_args(M=0)) == 0
     assert lib.ornith_w4_launch(None, 0, 8, None, None, None, 0, 0, None, 0, 0, 8, 32, None) == 0
-    assert lib.ornith_w4_pack(None, None, 0, None, None, None, 0, 8, 32, None) == 0
+    assert lib.ornith_w4_pack(None, None, 0, None, None, None, None, 0, 8, 32, None) == 0
 
 
 @pytest.mark.parametrize('bad', [dict(t=2), dict(N=-1), dict(K=12), dict(G=16), dict(codes=None), dict(scales=None),
                                  dict(pc=None), dict(pm=None), dict(pc=C.c_void_p(0x40008)),
-                                 dict(pm=C.c_void_p(0x40100)), dict(pc=C.c_void_p(0x10100))])
+                                 dict(pm=C.c_void_p(0x40100)), dict(pc=C.c_void_p(0x10100)), dict(flags=None),
+                                 dict(flags=C.c_void_p(0x80000))])
 def test_pack_refusals(lib, bad):
     p = C.c_void_p
-    a = dict(codes=p(0x10000), scales=p(0x20000), t=0, z=p(0x30000), pc=p(0x40000), pm=p(0x80000), N=40, K=256, G=64,
+    a = dict(codes=p(0x10000), scales=p(0x20000), t=0, z=p(0x30000), pc=p(0x40000), pm=p(0x80000), flags=p(0x90000), N=40, K=256, G=64,
              stream=None) | bad
     assert lib.ornith_w4_pack(*a.values()) == INVALID
 
