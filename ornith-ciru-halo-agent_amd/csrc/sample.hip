@@ -44,7 +44,7 @@ constexpr int kMassBits = 50;
 constexpr uint64_t kMassMask = (uint64_t(1) << kMassBits) - 1;
 constexpr uint64_t kPartOne = uint64_t(1) << 36;     // mass 1 in part units
 constexpr int kRowShift = 6;                         // part units -> row units at j == J
-constexpr int kListMax = 16384, kListLds = 4096;     // border entries kept per row, and in LDS
+constexpr int kListMax = 16384, kListLds = 8192;     // border entries kept per row, and in LDS
 constexpr int kSmall = 256;                          // rows decided by a list of all their candidates
 constexpr int kMaximaK = 256;                        // top_k up to which a part drops what cannot be among it
 constexpr int kQueue = 512;                          // a wave's surviving values, compacted up to here
@@ -646,9 +646,8 @@ __device__ __forceinline__ void draw_part(int parts, const Setting& s, RowShared
     __syncthreads();
 }
 // The token inside the part: thread i holds its columns col0 .. col0 + 7, ascending over the block.
-// Where at most an eighth of the part is kept, those values are set side by side in LDS first: one
-// mass a thread, not eight.
-struct DrawShared { float val[kRowThreads]; uint16_t col[kRowThreads]; };
+// Unless most of the part is kept, the kept values are set side by side in LDS first: fewer masses a thread.
+struct DrawShared { float val[kPart]; uint16_t col[kPart]; };
 template <int TYPE>
 __device__ __forceinline__ void draw_column(const SampleArgs& a, int row, const Setting& s, double J, const Scale& k,
                                             float least, int shift, uint64_t threshold, const Piece<TYPE>& v, int col0,
@@ -676,7 +675,8 @@ __device__ __forceinline__ void draw_column(const SampleArgs& a, int row, const 
         uint64_t all;
         return run + waves_before(sh.wave_mass, all);
     };
-    if (kept <= uint32_t(kRowThreads)) {
+    const int per = int(kept + kRowThreads - 1) / kRowThreads;
+    if (per <= kPer / 2) {
 #pragma unroll
         for (int e = 0; e < kPer; ++e)
             if (keep >> e & 1) {
@@ -685,11 +685,21 @@ __device__ __forceinline__ void draw_column(const SampleArgs& a, int row, const 
                 ++at;
             }
         __syncthreads();
-        const bool live = uint32_t(tid) < kept;
-        const float x = live ? ds.val[tid] : 0.f;
-        const uint64_t m = live ? mass_of(x) : 0, run = upto(m);
-        if (row_mass(run, shift) > rest && row_mass(run - m, shift) <= rest)
-            give(a, row, col0 - tid * kPer + ds.col[tid], log_share(x, s, J, row_mass(m, shift), total));
+        const int i0 = tid * per, i1 = min(i0 + per, int(kept));
+        uint64_t sum = 0;
+        for (int i = i0; i < i1; ++i) sum += mass_of(ds.val[i]);
+        const uint64_t run = upto(sum);
+        if (row_mass(run, shift) > rest && row_mass(run - sum, shift) <= rest) {
+            uint64_t before = run - sum;
+            for (int i = i0; i < i1; ++i) {
+                const uint64_t m = mass_of(ds.val[i]);
+                before += m;
+                if (row_mass(before, shift) > rest) {
+                    give(a, row, col0 - tid * kPer + ds.col[i], log_share(ds.val[i], s, J, row_mass(m, shift), total));
+                    break;
+                }
+            }
+        }
         return;
     }
     uint64_t m[kPer], sum = 0;
@@ -1225,17 +1235,33 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, int slot, int ro
     const bool lds = mode == kModeList && n <= kListLds;
     EntryList& en = un.border.list;
     if (lds) {
-        for (int i = tid; i < n; i += kRowThreads) {
-            const uint2 w = i == tid ? ahead0 : get_entry<HERE>(list, i);
-            en.comp[i] = comp_of<TYPE>(w.x, int(w.y));
-            en.mass[i] = entry_mass(w.x, int(w.y));
+        constexpr int kBatch = 4;                     // loads of a thread in flight
+        uint2 w[kBatch] = {ahead0};
+        for (int i0 = tid; i0 < n; i0 += kBatch * kRowThreads) {
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int i = i0 + b * kRowThreads;
+                if (i != tid && i < n) w[b] = get_entry<HERE>(list, i);
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int i = i0 + b * kRowThreads;
+                if (i >= n) break;
+                en.comp[i] = comp_of<TYPE>(w[b].x, int(w[b].y));
+                en.mass[i] = entry_mass(w[b].x, int(w[b].y));
+            }
         }
         __syncthreads();
     }
-    // f(comp, row mass) of the entries with a key in [lo, hi)
+    // f(comp, row mass) of the entries with a key in [lo, hi).  The list holds a part's entries side by
+    // side: a wave's lanes take entries n / 64 apart, or its LDS additions would mostly meet at one address
+    // (2800 entries of a few bf16 values: 7200 clocks a round, 64 columns of one part a wave).
+    const int apart = ((n + 63) >> 6) | 1;            // (odd: no bank conflicts)
     auto each = [&](uint32_t lo, uint32_t hi, auto&& f) {
         if (lds) {
-            for (int i = tid; i < n; i += kRowThreads) {
+            for (int t = tid >> 6; t < apart; t += kRowWaves) {
+                const int i = (tid & 63) * apart + t;
+                if (i >= n) continue;
                 const uint32_t k = comp_key<TYPE>(en.comp[i]);
                 if (k >= lo && k < hi) f(en.comp[i], en.mass[i]);
             }
@@ -1334,8 +1360,11 @@ template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
     const int row = blockIdx.x, tid = threadIdx.x;
     __shared__ RowShared sh;
-    __shared__ union { PartShared<kRowThreads> part; SmallList small; Descent descent; DrawShared draw; } un;
-    __shared__ __attribute__((aligned(16))) float s_v[kPart];
+    __shared__ union {
+        struct { union { PartShared<kRowThreads> part; SmallList small; Descent descent; }; float v[kPart]; };
+        DrawShared draw;
+    } un;
+    float* s_v = un.v;
     __shared__ uint32_t s_count;
     const int col0 = tid * kPer;
     Piece<TYPE> v[1];

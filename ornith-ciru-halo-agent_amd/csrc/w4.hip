@@ -7,7 +7,15 @@
 // both sums in fp32 on the matrix cores (sum x against a fragment of ones);
 // each product is exact, and the first sum is at most 31 / |c - z| times the
 // wanted one, so its roundings cost two to three bits of fp32, not of the
-// result's type.  acc += s * (that), groups in ascending order within a wave.
+// result's type.  acc += s * (that), groups in ascending order within a wave,
+// waves in ascending order.
+//
+// Bound by the codes' stream where it is long (151936 x 2048, 32 rows, fp32
+// results: 41.7 us, 180 MB, 4.3 TB/s; the steady part streams 7 TB/s, the rest
+// is x to LDS, 5 us, and the last wave's end), and by launch and the round trips
+// of one wave where it is short (6144 x 2048, 1 row: 4.3 us against 1.2 at
+// 5.5 TB/s).  Codes lie so that a lane's 16 bytes are its column's share of four
+// matrix steps: 1 KB contiguous a wave and load.
 #include <algorithm>
 #include <type_traits>
 #include "kernels.hpp"
@@ -424,16 +432,31 @@ template <int TYPE, int NT, int W> hipError_t w4_tiles(const W4Args& a, hipStrea
     else go(w4_tile_kernel<TYPE, 1, NT, W>);
     return hipGetLastError();
 }
+// Which kernel (us a call, bf16, group 128, calls in a graph over banks of 600 MB in turn or 24, K = 2048
+// but where another is given):
+//  - Tiles of a block.  One keeps more blocks than CUs where tiles are few; more read x, which comes from
+//    L2 for every block, less often.  1 / 2 / 4 tiles: 6144 columns, 1 row 4.3 / 4.5 / 5.6, 8 rows 5.1 /
+//    4.9 / 5.9, 16 rows 6.9 / 5.2 / 6.3, 64 rows 14.8 / 10.1 / 9.4; 24576 columns, 1 row 9.6 / 8.3 / 8.8,
+//    8 rows 10.4 / 8.3 / 9.5, 16 rows 14.9 / 10.6 / 10.5; 151936 columns, 1 row 42.8 / 32.3 / 32.5,
+//    8 rows 52.0 / 37.9 / 34.6.  2048 columns, K = 4096, 32 rows 6.7 / 7.0 / 9.3, 64 rows 10.7 / 7.1 / 9.2.
+//  - 16 waves where a wave of 8 would take three 128-k blocks or more in turn, or tiles are few: 8 / 16
+//    waves, 1 row, 2048 columns, K = 4096 5.1 / 4.2, K = 8192 8.6 / 6.4; 1024 columns 3.5 / 3.2; but 12288
+//    columns 6.4 / 6.7 and 16 rows of K = 8192 10.3 / 10.7.
+//  - x in LDS for more than 16 rows of many columns (4 tiles / in LDS): 24576 columns, 32 rows 14.2 / 14.2,
+//    64 rows 25.2 / 17.9; 12288 columns of groups of 32, 64 rows 15.9 / 16.5; 151936 columns, 32 rows
+//    70.6 / 41.9, 64 rows 137 / 68.5 (two passes over the weights: 32 rows are what LDS holds).
 template <int TYPE> hipError_t w4_rows(const W4Args& a, hipStream_t s) {
-    const int64_t tiles = (a.N + 15) / 16, cells = tiles * ((a.M + 15) / 16);
+    const int64_t cells = int64_t((a.N + 15) / 16) * ((a.M + 15) / 16);      // tiles of 16 x 16 results
+    const int blocks = w4_blocks(a.K);
     if (a.M > 16 && cells > 3072) {
         if (a.M > 48 && w4_x_bytes(4, a.K) <= kW4XBytes) return w4_run<TYPE, 4, 8, 4>(a, s);
         if (a.M > 32 && w4_x_bytes(3, a.K) <= kW4XBytes) return w4_run<TYPE, 3, 8, 4>(a, s);
         if (w4_x_bytes(2, a.K) <= kW4XBytes) return w4_run<TYPE, 2, 12, 3>(a, s);
     }
-    if (a.M > 8 ? cells >= 768 : tiles >= 4096) return w4_tiles<TYPE, 4, 8>(a, s);
-    if (a.M > 8 ? cells >= 384 : tiles >= 1536) return w4_tiles<TYPE, 2, 8>(a, s);
-    return w4_blocks(a.K) >= 24 ? w4_tiles<TYPE, 1, 16>(a, s) : w4_tiles<TYPE, 1, 8>(a, s);
+    if (cells >= (a.M <= 8 ? 4096 : 768)) return w4_tiles<TYPE, 4, 8>(a, s);
+    if (cells >= (a.M <= 4 ? 1536 : 384)) return w4_tiles<TYPE, 2, 8>(a, s);
+    if (a.M <= 8 && (blocks >= 24 || (blocks > 8 && cells <= 128))) return w4_tiles<TYPE, 1, 16>(a, s);
+    return w4_tiles<TYPE, 1, 8>(a, s);
 }
 
 }  // namespace

@@ -27,7 +27,7 @@ from __future__ import annotations
 
 import contextvars
 import ctypes as C
-from contextlib import contextmanager, nullcontext
+from contextlib import contextmanager
 from dataclasses import dataclass, field
 from pathlib import Path
 
@@ -573,15 +573,14 @@ def logits_argmax(logits, out):
                                             ptr(out), stream(logits)), 'logits argmax')
 
 
-def on_device(device):
-    """The device guard of a launch (nothing to do on the current device)."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def raw_stream(device):
-    """The handle of torch's current stream on `device` (an int; stream() without building a Stream object,
-    which costs 2 us a call)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def call_on(device, entry, operation, *args):
+    """A launch entry on `device` (made current if it is not) and torch's current stream there.  The stream's
+    handle comes without a Stream object, which costs 2 us a call."""
+    if device.index == torch.cuda.current_device():
+        check(entry(*args, torch._C._cuda_getCurrentRawStream(device.index)), operation)
+    else:
+        with torch.cuda.device(device):
+            check(entry(*args, torch._C._cuda_getCurrentRawStream(device.index)), operation)
 
 
 def _row_ptr(t, name, dtype, shape, device):
@@ -630,14 +629,13 @@ def logits_sample(logits, uniform, workspace, out, flags, temperature=None, top_
              (out, 'out', torch.int64), (logprob, 'logprob', torch.float32))]
     if args[0] is None or args[5] is None:
         raise ValueError('uniform and out are required')
-    if flags.dtype != torch.int32 or flags.numel() != 1 or workspace.element_size() != 1:
-        raise ValueError('flags must be one int32 word, workspace bytes')
+    if flags.dtype != torch.int32 or flags.numel() != 1 or workspace.element_size() != 1 or not workspace.is_contiguous():
+        raise ValueError('flags must be one int32 word, workspace contiguous bytes')
     if dev.type != 'cuda' or flags.device != dev or workspace.device != dev:
         raise ValueError('logits, settings, outputs, flags and workspace must be on one GPU')
-    with on_device(dev):
-        check(lib().ornith_logits_sample_launch(
+    call_on(dev, lib().ornith_logits_sample_launch, 'logits sample',
             logits.data_ptr(), kind, rows, n, ld, *args[:5], workspace.data_ptr() or None, workspace.numel(), *args[5:],
-            flags.data_ptr(), raw_stream(dev)), 'logits sample')
+            flags.data_ptr())
 
 
 W4_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -658,7 +656,8 @@ def _w4_shapes(n, k, group):
 def w4_out(x, codes, metadata, out, flags, n, k, group):
     """Plain 4-bit linear: out [rows, n] (bf16, fp16 or fp32) = x [rows, k]
     (bf16 or fp16, as it is) times the banks of storage.pack_w4.  Any number of
-    rows; the weights are read once per 64."""
+    rows (made for the few of a decode step).  Flags: 4 a non-finite sum, 8 a
+    non-finite 16-bit result."""
     x_type, out_type = W4_TYPES.get(x.dtype, 2), W4_TYPES.get(out.dtype)
     if x_type > 1 or x.ndim != 2 or x.shape[1] != k:
         raise ValueError(f'input must be a bf16 or fp16 [rows, {k}] tensor, got {tuple(x.shape)} {x.dtype}')
@@ -678,17 +677,16 @@ def w4_out(x, codes, metadata, out, flags, n, k, group):
     if group not in (32, 64, 128, 256) or k % 8:
         raise ValueError(f'group {group} is not 32, 64, 128 or 256, or K{k} not a multiple of 8')
     shapes = _w4_shapes(n, k, group)
-    if (codes.shape != shapes[0] or metadata.shape != shapes[1] or codes.element_size() != 4 or metadata.element_size() != 4 or not codes.is_contiguous()
-            or not metadata.is_contiguous()):
+    if (codes.shape != shapes[0] or metadata.shape != shapes[1] or codes.element_size() != 4
+            or metadata.element_size() != 4 or not codes.is_contiguous() or not metadata.is_contiguous()):
         raise ValueError(f'codes and metadata must be the contiguous 32-bit banks of storage.pack_w4 for N{n} K{k} '
                          f'G{group}, got {tuple(codes.shape)} and {tuple(metadata.shape)}')
     if flags.dtype != torch.int32 or flags.numel() != 1:
         raise ValueError('flags must be one int32 word')
     if dev.type != 'cuda' or codes.device != dev or metadata.device != dev or out.device != dev or flags.device != dev:
         raise ValueError('input, banks, output and flags must be on one GPU')
-    with on_device(dev):
-        check(lib().ornith_w4_launch(x_ptr, x_type, ldx, codes.data_ptr(), metadata.data_ptr(), out.data_ptr(), out_type,
-                                     ldo, flags.data_ptr(), rows, n, k, group, raw_stream(dev)), 'w4 linear')
+    call_on(dev, lib().ornith_w4_launch, 'w4 linear', x_ptr, x_type, ldx, codes.data_ptr(), metadata.data_ptr(),
+            out.data_ptr(), out_type, ldo, flags.data_ptr(), rows, n, k, group)
 
 
 def dense_head(x, codes, meta, workspace, logits, logits_bf16, argmax, flags, capacity):
