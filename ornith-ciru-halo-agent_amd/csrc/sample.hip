@@ -150,21 +150,21 @@ template <int TYPE> __device__ __forceinline__ uint32_t comp_key(uint64_t comp) 
 }
 __device__ __forceinline__ int comp_col(uint64_t comp) { return int(kColMask - (uint32_t(comp) & kColMask)); }
 
-// 2^x for |x| <= 1/2, degree 8 (Chebyshev interpolation; relative error 2^-39.7, 1 at 0).  The
-// coefficients are kept in scalar registers: as literals, each fma is preceded by two moves.
+// 2^(36 + x) for |x| <= 1/2, degree 8 (Chebyshev interpolation; relative error 2^-39.7, 2^36 at 0).
+// The coefficients are kept in scalar registers: as literals, each fma is preceded by two moves.
 __device__ __forceinline__ double in_sgpr(double v) {
     asm("" : "+s"(v));
     return v;
 }
-__device__ __forceinline__ double exp2_poly(double x) {
-    double p = __builtin_fma(x, in_sgpr(0x1.63cf7dec51603p-20), in_sgpr(0x1.00dc48dc4d96cp-16));
-    p = __builtin_fma(p, x, in_sgpr(0x1.4308ae274a207p-13));
-    p = __builtin_fma(p, x, in_sgpr(0x1.5d8745a95d2d4p-10));
-    p = __builtin_fma(p, x, in_sgpr(0x1.3b2ab71725c04p-7));
-    p = __builtin_fma(p, x, in_sgpr(0x1.c6b08dd6fb6b1p-5));
-    p = __builtin_fma(p, x, in_sgpr(0x1.ebfbdff824847p-3));
-    p = __builtin_fma(p, x, in_sgpr(0x1.62e42fef84cf7p-1));
-    return __builtin_fma(p, x, 1.0);
+__device__ __forceinline__ double exp2_units(double x) {
+    double p = __builtin_fma(x, in_sgpr(0x1.63cf7dec51603p+16), in_sgpr(0x1.00dc48dc4d96cp+20));
+    p = __builtin_fma(p, x, in_sgpr(0x1.4308ae274a207p+23));
+    p = __builtin_fma(p, x, in_sgpr(0x1.5d8745a95d2d4p+26));
+    p = __builtin_fma(p, x, in_sgpr(0x1.3b2ab71725c04p+29));
+    p = __builtin_fma(p, x, in_sgpr(0x1.c6b08dd6fb6b1p+31));
+    p = __builtin_fma(p, x, in_sgpr(0x1.ebfbdff824847p+33));
+    p = __builtin_fma(p, x, in_sgpr(0x1.62e42fef84cf7p+35));
+    return __builtin_fma(p, x, in_sgpr(0x1p36));
 }
 
 // From |j| = 2^40 on, the neighbours of the largest value lie 2^16 powers of two below it: it has
@@ -174,17 +174,25 @@ __device__ __forceinline__ bool is_far(double j) { return !(__builtin_fabs(j) < 
 struct Scale { double c, j; };
 __device__ __forceinline__ Scale scale_of(double c, double j) { return is_far(j) ? Scale{0.0, 0.0} : Scale{c, j}; }
 
-// Bin and mass of a value at or above its part's `least` (of others, anything) with the part's
-// scale.  Whole numbers come from the low word of a sum with 1.5 * 2^52: o = rint(l c) - j there,
-// with one rounding of the exact product, so o + j and its eighths are the same in every part.
-__device__ __forceinline__ int bin_mass(float v, const Scale& k, uint64_t& mass) {
-    const double l = double(fminf(v, 0x1.fffffep127f)), m = kWhole - k.j;
+// With the part's scale, 2^52 + the mass of a value l at or above its part's `least` (of others,
+// anything), o = rint(l c) - j and x = l c - rint(l c).  Whole numbers come from the low word of a sum
+// with 1.5 * 2^52, with one rounding of the exact product, so o + j and its eighths are the same in
+// every part.
+__device__ __forceinline__ double mass_sum(float v, const Scale& k, int& o, double& x) {
+    const double l = double(v), m = kWhole - k.j;
     const double q = __builtin_fma(l, k.c, m);
-    const double x = __builtin_fma(l, k.c, m - q);                            // l c - rint(l c)
-    const int o = int(uint32_t(__double_as_longlong(q)));                     // <= 0
-    const int f = int(uint32_t(__double_as_longlong(__builtin_fma(x, double(kSub), kWhole))));
-    const double e = __longlong_as_double(__double_as_longlong(exp2_poly(x)) + (int64_t(o + 36) << 52));
-    const uint64_t w = uint64_t(__double_as_longlong(e + 0x1p52));
+    x = __builtin_fma(l, k.c, m - q);
+    o = int(uint32_t(__double_as_longlong(q)));        // <= 0
+    const uint64_t e = uint64_t(__double_as_longlong(exp2_units(x)));
+    const uint32_t hi = uint32_t(e >> 32) + (uint32_t(o) << 20);
+    return __longlong_as_double((int64_t(hi) << 32) | uint32_t(e)) + 0x1p52;
+}
+// Bin and mass of the same.
+__device__ __forceinline__ int bin_mass(float v, const Scale& k, uint64_t& mass) {
+    int o;
+    double x;
+    const uint64_t w = uint64_t(__double_as_longlong(mass_sum(fminf(v, 0x1.fffffep127f), k, o, x)));
+    const int f = int(uint32_t(__double_as_longlong(__builtin_fma(x, double(kSub), in_sgpr(kWhole)))));
     uint32_t lo = uint32_t(w), hi = uint32_t(w >> 32) & 0xfffffu;
     asm volatile("" : "+v"(lo), "+v"(hi));             // (computed for every lane: no branch per value)
     mass = (uint64_t(hi) << 32) | lo;
@@ -325,14 +333,28 @@ __device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting
     const Scale k = scale_of(s.c, j);
     float least = below_bin(0, part_mx, s.inv, j);
     if (!s.cut) {
-        uint64_t sum = 0;
+        // (whole numbers in fp64 as well: below 2^50)
+        uint64_t sum;
+        if (is_far(j)) {
+            int count = 0;
 #pragma unroll
-        for (int u = 0; u < PIECES; ++u)
+            for (int u = 0; u < PIECES; ++u)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                uint64_t m;
-                if (bin_mass(v[u][e], k, m) >= 0 && v[u][e] >= least) sum += m;
-            }
+                for (int e = 0; e < 8; ++e) count += v[u][e] >= least;
+            sum = uint64_t(count) * kPartOne;
+        } else {
+            double masses = 0.0;
+#pragma unroll
+            for (int u = 0; u < PIECES; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    int o;
+                    double x;
+                    const double m = mass_sum(v[u][e], k, o, x) - 0x1p52;
+                    masses += v[u][e] >= least ? m : 0.0;        // (false for NaN)
+                }
+            sum = uint64_t(masses);
+        }
         sum = wave_sum_u64(sum);
         if (lane == 0) sh.mass[wv] = sum;
         __syncthreads();
