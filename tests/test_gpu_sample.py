@@ -18,7 +18,7 @@ from oracle import sampling as S
 pytestmark = pytest.mark.gpu
 
 MARGIN = 2.0 ** -21
-PART, LIST_LDS, LIST_MAX = 8192, 4096, 32768
+PART, LIST_LDS, LIST_MAX = 8192, 8192, 16384
 
 
 def _np(t):
@@ -281,4 +281,80 @@ def test_uniform_ends(device):
         assert token[m] == S.kept(rows[m], 1.0, k)[0][0]
     for m, k in ((2, 3), (3, 1)):
         assert token[m] == S.kept(rows[m], 1.0, k)[0][-1]
+    assert flags == 0
+
+
+@pytest.mark.parametrize('N', [PART + 1, LIST_LDS + LIST_LDS // 2, LIST_MAX, LIST_MAX + 1])
+@pytest.mark.parametrize('levels', [1, 2, 40])
+def test_border_lists_of_every_length(device, N, levels):
+    """All values in one bin: border lists in shared memory, past it, and rows
+    that have none.  The levels differ by 2^-10 in t, less than a bin's eighth;
+    every kept mass is above 2^-14.2 of the sum, so each interval is wide enough."""
+    import torch
+    rng = np.random.default_rng(N + levels)
+    step = 2.0 ** -10 * np.log(2.0)
+    logits = torch.from_numpy((rng.integers(0, levels, (5, N)) * -step).astype(np.float32)).to(device)
+    rows = _np(logits)
+    ks = [0, 1 + N // 3, N - 1, 0, N // 2]
+    ps = [np.float32(S.top_p_for(row, 1.0, k, n)[0]) for row, k, n in
+          zip(rows, ks, (N // 5, N // 4, N - 7, N // 2 + 1, 3))]
+    us, cols = zip(*[_place(rng, row, 1.0, k, float(p), 0.0) for row, k, p in zip(rows, ks, ps)])
+    _check(logits, [1.0] * 5, ks, ps, [0.0] * 5, us, cols)
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp32'])
+@pytest.mark.parametrize('N', [600, 10000, 40000])
+@pytest.mark.parametrize('sign', [1, -1])
+def test_sorted_rows(device, dtype, N, sign):
+    """The largest values side by side at one end, and top-k about its bounds."""
+    import torch
+    rng = np.random.default_rng(N + sign)
+    ks = [1, 2, 63, 64, 65, 255, 256, 257, 300, 500]
+    base = np.sort(rng.standard_normal((len(ks), N)) * 2, axis=1)[:, ::sign]
+    logits = torch.from_numpy(base.astype(np.float32)).to(_dtype(dtype)).to(device)
+    rows = _np(logits)
+    us, cols = zip(*[_place(rng, row, 1.0, k, 1.0, 0.0) for row, k in zip(rows, ks)])
+    _check(logits, [1.0] * len(ks), ks, [1.0] * len(ks), [0.0] * len(ks), us, cols)
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp32'])
+@pytest.mark.parametrize('M', [1, 2, 3])
+@pytest.mark.parametrize('which', ['', 'k', 'p', 'kpq'])
+def test_longest_rows(device, dtype, M, which):
+    """2^20 columns.  Off by half a unit of 2^-36 of at most twice the largest
+    mass each, n masses are off by 2^-16 of the largest together: 2^-22 of
+    a sum of 64 of it or more, within MARGIN."""
+    rng = np.random.default_rng(M * 31 + len(which))
+    N = 1 << 20
+    logits = _logits(rng, M, N, _dtype(dtype), device, lead=1)
+    settings = []
+    for row in _np(logits):
+        T, k, p, q = _settings(rng, row, which)
+        T = max(T, 1.0)
+        if 'p' in which:                               # (of the T that is used)
+            p = float(np.float32(S.top_p_for(row, T, k, 2 + int(rng.integers(0, 20)))[0]))
+        if not k:
+            assert S.masses(row, S.order(row), T).sum() >= 64
+        u, col = _place(rng, row, T, k, p, q)
+        settings.append((T, k, p, q, u, col))
+    Ts, ks, ps, qs, us, cols = zip(*settings)
+    _check(logits, Ts, ks, ps, qs, us, cols, workspace_fill=0xff)
+
+
+@pytest.mark.parametrize('M,N', [(530, 9000), (70, 130000)])
+def test_rows_past_a_chunk(device, M, N):
+    """More rows than one pass takes: as if each part of them were alone."""
+    import torch
+    from ornith_g256 import native
+    rng = np.random.default_rng(M)
+    assert native.logits_sample_bytes(M, N) == native.logits_sample_bytes(2 * M, N)
+    logits = _logits(rng, M, N, torch.bfloat16, device)
+    us = rng.random(M).astype(np.float32)
+    T, k = rng.choice([0.0, 0.5, 1.0], M), rng.choice([0, 1, 50, 2000], M)
+    p, q = rng.choice([1.0, 0.9, 0.3], M), rng.choice([0.0, 0.1], M)
+    token, logprob, flags = _run(logits, us, T, k, p, q)
+    for r in range(0, M, 60):
+        s = slice(r, r + 60)
+        t1, l1, f1 = _run(logits[s], us[s], T[s], k[s], p[s], q[s])
+        assert (t1 == token[s]).all() and (l1 == logprob[s]).all() and f1 == 0, r
     assert flags == 0
