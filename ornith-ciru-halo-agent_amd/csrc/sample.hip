@@ -1379,8 +1379,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_rest_kernel(SampleArgs a, 
 
 // Rows of one part: all of it by one block, the logits in LDS after the histogram.
 template <int TYPE>
-__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
-    const int row = blockIdx.x, tid = threadIdx.x;
+__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a, int row0) {
+    const int row = row0 + int(blockIdx.x), tid = threadIdx.x;
     __shared__ RowShared sh;
     __shared__ union {
         struct { union { PartShared<kRowThreads> part; SmallList small; Descent descent; }; float v[kPart]; };
@@ -1521,13 +1521,14 @@ template <int TYPE> hipError_t sample_rows(const SampleArgs& a, int row0, int ro
 }
 
 template <int TYPE> hipError_t sample_all(const SampleArgs& a, int M, hipStream_t s) {
-    if (a.parts == 1) {
-        timed_launch("sample_row", sample_row_kernel<TYPE>, dim3(M), dim3(kRowThreads), 0, s, a);
-        return hipGetLastError();
-    }
-    const int chunk = sample_chunk(a.N);
-    for (int r = 0; r < M; r += chunk) {
-        const hipError_t st = sample_rows<TYPE>(a, r, std::min(M - r, chunk), s);
+    const int chunk = a.parts == 1 ? 1 << 20 : sample_chunk(a.N);      // (a grid has less than 2^32 threads)
+    for (int64_t r = 0; r < M; r += chunk) {
+        const int row0 = int(r), rows = int(std::min<int64_t>(M - r, chunk));
+        hipError_t st;
+        if (a.parts == 1) {
+            timed_launch("sample_row", sample_row_kernel<TYPE>, dim3(rows), dim3(kRowThreads), 0, s, a, row0);
+            st = hipGetLastError();
+        } else st = sample_rows<TYPE>(a, row0, rows, s);
         if (st != hipSuccess) return st;
     }
     return hipSuccess;

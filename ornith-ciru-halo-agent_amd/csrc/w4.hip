@@ -52,8 +52,8 @@ template <int TYPE> __device__ __forceinline__ u32x4 w4_unpack(uint32_t w) {
 
 // ---- packing --------------------------------------------------------------------
 __global__ __launch_bounds__(256) void w4_pack_codes_kernel(const uint32_t* __restrict__ in, uint32_t* __restrict__ out,
-                                                            int N, int K, size_t words) {
-    const size_t i = size_t(blockIdx.x) * 256 + threadIdx.x;
+                                                            int N, int K, size_t first, size_t words) {
+    const size_t i = first + size_t(blockIdx.x) * 256 + threadIdx.x;
     if (i >= words) return;
     const int j = int(i & 3), lane = int(i >> 2) & 63, blocks = (K + kW4Block - 1) / kW4Block;
     const size_t tb = i >> 8;
@@ -488,10 +488,13 @@ extern "C" hipError_t ornith_w4_pack(const void* codes, const void* scales, int 
                               {packed_meta, m * 4, 4, true, false},
                               {flags, 4, 4, true, false}};
     if (!check_buffers(buffers)) return hipErrorInvalidValue;
-    timed_launch("w4_pack_codes", w4_pack_codes_kernel, dim3(unsigned((c + 255) / 256)), dim3(256), 0, stream,
-                 static_cast<const uint32_t*>(codes), static_cast<uint32_t*>(packed_codes), N, K, c);
-    const hipError_t st = hipGetLastError();
-    if (st != hipSuccess) return st;
+    constexpr size_t kAtOnce = size_t(1) << 31;        // (a grid has less than 2^32 threads)
+    for (size_t first = 0; first < c; first += kAtOnce) {
+        timed_launch("w4_pack_codes", w4_pack_codes_kernel, dim3(unsigned((std::min(c - first, kAtOnce) + 255) / 256)), dim3(256),
+                     0, stream, static_cast<const uint32_t*>(codes), static_cast<uint32_t*>(packed_codes), N, K, first, c);
+        const hipError_t st = hipGetLastError();
+        if (st != hipSuccess) return st;
+    }
     timed_launch("w4_pack_meta", w4_pack_meta_kernel, dim3(unsigned((m + 255) / 256)), dim3(256), 0, stream,
                  static_cast<const uint16_t*>(scales), scale_type, static_cast<const uint8_t*>(zeros),
                  static_cast<uint32_t*>(packed_meta), N, groups,
@@ -516,11 +519,11 @@ extern "C" hipError_t ornith_w4_launch(const void* x, int x_type, int64_t ldx, c
     if (!check_buffers(buffers)) return hipErrorInvalidValue;
     // rows ride on the grid's y axis (65535 blocks of 16 rows at least)
     constexpr int kMost = 65535 * 16;
-    for (int r = 0; r < M; r += kMost) {
+    for (int64_t r = 0; r < M; r += kMost) {
         const W4Args a{static_cast<const uint16_t*>(x) + size_t(r) * size_t(ldx), ldx,
                        static_cast<const uint32_t*>(codes), static_cast<const uint32_t*>(meta),
                        static_cast<uint8_t*>(out) + size_t(r) * size_t(ldo) * size, out_type, ldo,
-                       static_cast<uint32_t*>(flags), M - r < kMost ? M - r : kMost, N, K, w4_log2g(G)};
+                       static_cast<uint32_t*>(flags), int(std::min<int64_t>(M - r, kMost)), N, K, w4_log2g(G)};
         hipError_t st;
         if (!K) {
             timed_launch("w4_zero", w4_zero_kernel, dim3((N + 255) / 256, std::min(a.M, 1024)), dim3(256), 0, stream, a);

@@ -293,3 +293,45 @@ def test_bank_and_output_past_32_bits(device):
         assert (out[:, :100].double().cpu().numpy() == first[:, None]).all()
         del buf, out
     assert int(flags.item()) == 0
+
+
+def test_rows_past_one_grid(device):
+    """More rows than a grid of 1024 threads a row can hold."""
+    import torch
+    from ornith_g256 import native
+    rng = np.random.default_rng(8)
+    n, some, M = 8, 1024, (1 << 22) + 1024
+    near = torch.from_numpy(rng.standard_normal((some, n)).astype(np.float32)).to(torch.bfloat16).to(device)
+    uniform, top_p = torch.rand(some, device=device), torch.full((some,), 0.8, device=device)
+    got = []
+    for times in (1, M // some):
+        token = torch.full((times * some,), -7, dtype=torch.int64, device=device)
+        flags = torch.zeros(1, dtype=torch.int32, device=device)
+        native.logits_sample(near.repeat(times, 1), uniform.repeat(times), torch.empty(0, dtype=torch.uint8, device=device),
+                             token, flags, top_p=top_p.repeat(times))
+        assert int(flags) == 0
+        got.append(token)
+    assert torch.equal(got[1].view(-1, some), got[0].expand(M // some, some))
+
+
+def test_pack_past_one_grid(device):
+    """A bank of more 32-bit words than a grid has threads; its first and last columns are known."""
+    import torch
+    from ornith_g256 import native, storage
+    rng = np.random.default_rng(9)
+    n, k, group = 1 << 20, 32776, 256
+    codes = torch.zeros((n, k // 8), dtype=torch.int32, device=device)
+    words = rng.integers(0, 2 ** 32, (24, k // 8), dtype=np.uint32)
+    codes[:24] = torch.from_numpy(words.view(np.int32)).to(device)
+    codes[-24:] = codes[:24]
+    groups = (k + group - 1) // group
+    banks = storage.pack_w4(codes, torch.full((n, groups), 0.0625, dtype=torch.bfloat16, device=device), None, group)
+    del codes
+    x = torch.from_numpy(rng.integers(-2, 3, (1, k)).astype(np.float32)).to(torch.bfloat16).to(device)
+    flags = torch.zeros(1, dtype=torch.int32, device=device)
+    out = torch.empty((1, n), dtype=torch.float32, device=device)
+    native.w4_out(x, *banks, out, flags, n, k, group)
+    want = x.double().cpu().numpy() @ W.weights(words, np.full((24, groups), 0.0625), None, group).T
+    got = out.double().cpu().numpy()
+    assert (got[:, :24] == want).all() and (got[:, -24:] == want).all()
+    assert (got[:, 24:-24] == -8 * 0.0625 * x.double().sum().item()).all()
