@@ -14,7 +14,17 @@
 //   finish  one block per row: the threshold inside its bin, the kept mass per
 //           part, and the walk through the one part that holds the token (of the
 //           256: threshold and token from the list alone).
-// Rows of one part do all of it in one block and one launch (sample_row).
+// Rows of one part do all of it in one block and one launch (sample_row).  Calls of few parts do the
+// last three steps in one launch (sample_rest), whose last block to list its entries ends the row.
+//
+// What bounds it.  The floor is one pass over the logits (64 rows of 248320 bf16: 31.8 MB, 6.6 us at the
+// rate of a large copy).  `parts` takes 17.2 us there: 10.9 to load and find the maxima, the rest fp64
+// for the masses (eleven instructions a value, 7 to 8 clocks each a wave); top-p's histogram costs 7 us
+// of LDS additions more.  Everything behind it works on bins and lists and is a chain of launches and
+// round trips: a whole row is drawn in 6.9 us, borders take 7 to 8, the list 8 to 9, its end 5 (few
+// candidates) to 19 (2800 entries a row).  Calls in a graph over six inputs in turn: 1 row of top-k and
+// top-p 17.0 us, 8 rows of 151936 fp32 with top-p 25.8, 64 rows of mixed settings 47, 64 uncut 24.7, 256
+// rows of 4096 columns 17.4.
 //
 // Masses.  With c = log2(e) / T and t = l c in fp64, e = 2^(t - j) for the
 // whole number j = ceil(max t) of its part: a degree-8 polynomial in t - rint(t)
@@ -44,11 +54,19 @@ constexpr int kMassBits = 50;
 constexpr uint64_t kMassMask = (uint64_t(1) << kMassBits) - 1;
 constexpr uint64_t kPartOne = uint64_t(1) << 36;     // mass 1 in part units
 constexpr int kRowShift = 6;                         // part units -> row units at j == J
-constexpr int kListMax = 16384, kListLds = 8192;     // border entries kept per row, and in LDS
-constexpr int kSmall = 256;                          // rows decided by a list of all their candidates
-constexpr int kMaximaK = 256;                        // top_k up to which a part drops what cannot be among it
-constexpr int kQueue = 512;                          // a wave's surviving values, compacted up to here
-constexpr int kFewParts = 256;                       // parts of a call up to which two launches do it
+// Sizes that choose a way, with both ways measured (us; 64 rows of 248320 bf16 where nothing else is said):
+constexpr int kListMax = 16384;                      // border entries kept per row (more: the row is read again)
+constexpr int kListLds = 8192;                       // and in LDS (top-p, 2800 a row: finish 18.9, from memory 24.6)
+constexpr int kSmall = 256;                          // rows decided by a list of all their candidates (top-k 20 to 50:
+                                                     // finish 4.8, by borders 13.2; 256 rows of 4096: 11.6 / 20.2)
+constexpr int kMaximaK = 256;                        // top_k up to which a part drops what cannot be among it (top-k
+                                                     // 20 to 50: parts 13.3, without 25.0)
+constexpr int kQueue = 512;                          // a wave's surviving values, compacted up to here (the same:
+                                                     // parts 13.3, without 16.7)
+// Parts of a call up to which two launches do it: a block per part and CU, each with the row's plan (two /
+// four launches: top-k of 1 row 16.9 / 21.1, 8 rows 18.0 / 22.7, 16 rows 30.5 / 24.0; fp32 of 151936,
+// top-p, 8 rows 26.0 / 33.8, 16 rows 34.3 / 37.7, 32 rows 48.2 / 43.1).
+constexpr int kFewParts = 256;
 constexpr int kRowThreads = 1024, kRowWaves = kRowThreads / 64, kPer = kPart / kRowThreads;
 constexpr uint32_t kMinusInf = 0x007fffffu;          // ordered(-inf)
 constexpr uint32_t kKeyEnd = 0xffffffffu;            // above every key
@@ -422,6 +440,11 @@ __device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting
     return PartMeta{j, 0, key, 0, least};
 }
 
+// A block per part, the values in registers, loaded once.  256 threads (four pieces each) where parts are
+// many: 64 rows of 248320 bf16 17.2 us, where 512 and 1024 threads were slower (in an earlier form of the
+// masses 22 / 24 / 30 us: more waves meet at each barrier).  1024 where every part has a CU of its own and the
+// chain of one thread counts: 8 rows of 151936 fp32 5.6 us, with 256 threads 8.0.  Tried and slower: blocks
+// that stay and load a part ahead (27 us against 22), 64 VGPRs a thread forced by launch bounds (spills).
 template <int TYPE, int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_parts_kernel(SampleArgs a, int row0) {
     const int part = blockIdx.x, slot = blockIdx.y, row = row0 + slot, tid = threadIdx.x;
@@ -1170,6 +1193,8 @@ __device__ __forceinline__ void gather_part(const SampleArgs& a, int slot, const
             }
 }
 
+// Reads the logits of the parts that reach a range a second time (mostly from L2 and the memory-side
+// cache: 5.4 MB of 31.8 missed), 8 to 9 us; one addition to the row's count a block.
 template <int TYPE, int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_gather_kernel(SampleArgs a, int row0) {
     const int part = blockIdx.x, slot = blockIdx.y, row = row0 + slot;
@@ -1326,6 +1351,8 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, int slot, int ro
     draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], threshold, v, col0, sh, un.draw);
 }
 
+// Bound by its chain of LDS passes and barriers: 5 us where 256 candidates decide, 14 to 19 where borders
+// are found in lists.
 template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a, int row0) {
     const int slot = blockIdx.x, row = row0 + slot, tid = threadIdx.x;
@@ -1348,7 +1375,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
 }
 
 // Select, gather and finish of few rows in one launch: every block of a row makes its plan, lists its
-// part's entries, and the last one to have done so ends the row.
+// part's entries, and the last one to have done so ends the row.  Entries, their count and the arrivals
+// pass through relaxed accesses of device scope, ordered by a wait for the wave's own stores: a fence of
+// every thread wrote back and dropped the caches, 20 to 90 us.  12.8 us for a row of top-k (7 of them
+// plan and list), 16 to 21 with top-p's list of some thousand entries.
 template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_rest_kernel(SampleArgs a, int row0) {
     const int part = blockIdx.x, slot = blockIdx.y, row = row0 + slot, tid = threadIdx.x;
@@ -1377,7 +1407,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_rest_kernel(SampleArgs a, 
     finish_row<TYPE, true>(a, slot, row, s, sh.plan.mode == kModeWalk ? 0 : int(min(listed, uint32_t(a.list_max))), ahead0, sh, un);
 }
 
-// Rows of one part: all of it by one block, the logits in LDS after the histogram.
+// Rows of one part: all of it by one block, the logits in LDS after the histogram.  One block a CU (78 KB
+// of LDS, 1024 threads), so bound by the chain of its steps: 256 rows of 4096 bf16 17.2 us with mixed
+// settings, 11.4 with top-k of 20 to 50.
 template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a, int row0) {
     const int row = row0 + int(blockIdx.x), tid = threadIdx.x;

@@ -132,7 +132,9 @@ __host__ __device__ inline int w4_blocks(int K) { return (K + kW4Block - 1) / kW
 // parts of a pair meet in LDS, in wave order.  PER: groups in 128 k (1 for groups of 128 and 256).
 // x lies in pieces of 8 k: piece (k / 8) * 16 MT + row; behind it its sums over groups (of 256: over their
 // halves, as the products are added per 128 k), [group, 16 MT].
-// W waves of a block, D units' codes of a wave in flight.
+// W waves of a block, D units' codes of a wave in flight: 12 and 3 for two tiles of rows (151936 x 2048, 32
+// rows, fp32 results, us: 43.2; 16 waves and 2 units 45.1, 8 and 3 44.3, 8 and 4 45.3, 8 and 6 45.1); 8
+// and 4 for more, whose sums and parked parts take 64 registers a tile pair.
 constexpr size_t kW4XBytes = 128 * 1024;               // x of a block, at most
 constexpr size_t w4_x_bytes(int MT, int K) { return size_t(16 * MT) * ((K + kW4Block - 1) / kW4Block) * (2 * kW4Block); }
 
@@ -325,7 +327,9 @@ __global__ __launch_bounds__(64 * W) void w4_run_kernel(W4Args a) {
 }
 
 // A block per NT tiles and 16 rows, whose waves take 128-k blocks in turn, x straight from memory, and
-// meet in LDS in wave order.
+// meet in LDS in wave order.  The waves split K because few columns leave few blocks: at 6144 x 2048 a
+// wave's whole work is two 128-k blocks, and a call (4.5 us, 6.7 MB) is the launch, one round trip for
+// codes and x, eight matrix steps and one exchange.
 template <int TYPE, int PER, int NT, int W>
 __global__ __launch_bounds__(64 * W) void w4_tile_kernel(W4Args a) {
     typedef uint32_t meta_t __attribute__((ext_vector_type(PER)));
