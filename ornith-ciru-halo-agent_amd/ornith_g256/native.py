@@ -573,22 +573,22 @@ def logits_argmax(logits, out):
                                             ptr(out), stream(logits)), 'logits argmax')
 
 
-def call_on(device, entry, operation, *args):
-    """A launch entry on `device` (made current if it is not) and torch's current stream there.  The stream's
-    handle comes without a Stream object, which costs 2 us a call."""
-    if device.index == torch.cuda.current_device():
-        check(entry(*args, torch._C._cuda_getCurrentRawStream(device.index)), operation)
+def call_on(index, entry, operation, *args):
+    """A launch entry on GPU `index` (made current if it is not) and torch's current stream there.  The
+    stream's handle comes without a Stream object, which costs 2 us a call."""
+    if index == torch.cuda.current_device():
+        check(entry(*args, torch._C._cuda_getCurrentRawStream(index)), operation)
     else:
-        with torch.cuda.device(device):
-            check(entry(*args, torch._C._cuda_getCurrentRawStream(device.index)), operation)
+        with torch.cuda.device(index):
+            check(entry(*args, torch._C._cuda_getCurrentRawStream(index)), operation)
 
 
-def _row_ptr(t, name, dtype, shape, device):
+def _row_ptr(t, name, dtype, shape, like):
     """Address of an optional per-row tensor, checked."""
     if t is None:
         return None
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f'{name} must be a contiguous {dtype} {list(shape)} tensor on {device}, '
+    if t.dtype != dtype or t.shape != shape or t.get_device() != like.get_device() or not t.is_contiguous():
+        raise ValueError(f'{name} must be a contiguous {dtype} {list(shape)} tensor on {like.device}, '
                          f'got {tuple(t.shape)} {t.dtype} on {t.device}')
     return t.data_ptr()
 
@@ -615,7 +615,7 @@ def logits_sample(logits, uniform, workspace, out, flags, temperature=None, top_
     kind = LOGITS_TYPES.get(logits.dtype)
     if kind is None or logits.ndim != 2:
         raise ValueError('logits must be bf16, fp16 or fp32 [M, N] with unit column stride')
-    (rows, n), (ld, step), dev = logits.shape, logits.stride(), logits.device
+    (rows, n), (ld, step), gpu = logits.shape, logits.stride(), logits.get_device()
     if step != 1 and n > 1:
         raise ValueError('logits must be bf16, fp16 or fp32 [M, N] with unit column stride')
     if rows <= 1:
@@ -623,7 +623,7 @@ def logits_sample(logits, uniform, workspace, out, flags, temperature=None, top_
     elif ld < n:
         raise ValueError(f'logits rows overlap: row stride {ld} of {n} columns')
     row = (rows,)
-    args = [_row_ptr(t, name, dtype, row, dev) for t, name, dtype in
+    args = [_row_ptr(t, name, dtype, row, logits) for t, name, dtype in
             ((uniform, 'uniform', torch.float32), (temperature, 'temperature', torch.float32),
              (top_k, 'top_k', torch.int32), (top_p, 'top_p', torch.float32), (min_p, 'min_p', torch.float32),
              (out, 'out', torch.int64), (logprob, 'logprob', torch.float32))]
@@ -631,9 +631,9 @@ def logits_sample(logits, uniform, workspace, out, flags, temperature=None, top_
         raise ValueError('uniform and out are required')
     if flags.dtype != torch.int32 or flags.numel() != 1 or workspace.element_size() != 1 or not workspace.is_contiguous():
         raise ValueError('flags must be one int32 word, workspace contiguous bytes')
-    if dev.type != 'cuda' or flags.device != dev or workspace.device != dev:
+    if gpu < 0 or flags.get_device() != gpu or workspace.get_device() != gpu:
         raise ValueError('logits, settings, outputs, flags and workspace must be on one GPU')
-    call_on(dev, lib().ornith_logits_sample_launch, 'logits sample',
+    call_on(gpu, lib().ornith_logits_sample_launch, 'logits sample',
             logits.data_ptr(), kind, rows, n, ld, *args[:5], workspace.data_ptr() or None, workspace.numel(), *args[5:],
             flags.data_ptr())
 
@@ -661,7 +661,7 @@ def w4_out(x, codes, metadata, out, flags, n, k, group):
     x_type, out_type = W4_TYPES.get(x.dtype, 2), W4_TYPES.get(out.dtype)
     if x_type > 1 or x.ndim != 2 or x.shape[1] != k:
         raise ValueError(f'input must be a bf16 or fp16 [rows, {k}] tensor, got {tuple(x.shape)} {x.dtype}')
-    rows, dev = x.shape[0], x.device
+    rows, gpu = x.shape[0], x.get_device()
     if out_type is None or out.shape != (rows, n):
         raise ValueError(f'output must be a bf16, fp16 or fp32 [{rows}, {n}] tensor, got {tuple(out.shape)} {out.dtype}')
     (ldx, sx), (ldo, so) = x.stride(), out.stride()
@@ -683,9 +683,10 @@ def w4_out(x, codes, metadata, out, flags, n, k, group):
                          f'G{group}, got {tuple(codes.shape)} and {tuple(metadata.shape)}')
     if flags.dtype != torch.int32 or flags.numel() != 1:
         raise ValueError('flags must be one int32 word')
-    if dev.type != 'cuda' or codes.device != dev or metadata.device != dev or out.device != dev or flags.device != dev:
+    if (gpu < 0 or codes.get_device() != gpu or metadata.get_device() != gpu or out.get_device() != gpu
+            or flags.get_device() != gpu):
         raise ValueError('input, banks, output and flags must be on one GPU')
-    call_on(dev, lib().ornith_w4_launch, 'w4 linear', x_ptr, x_type, ldx, codes.data_ptr(), metadata.data_ptr(),
+    call_on(gpu, lib().ornith_w4_launch, 'w4 linear', x_ptr, x_type, ldx, codes.data_ptr(), metadata.data_ptr(),
             out.data_ptr(), out_type, ldo, flags.data_ptr(), rows, n, k, group)
 
 

@@ -155,7 +155,7 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     zeros = None if zeros is None else zeros.contiguous()
     packed = [torch.empty(s, dtype=torch.int32, device=codes.device) for s in native.w4_layout(n, k, group)]
     flags = torch.zeros(1, dtype=torch.int32, device=codes.device)
-    native.call_on(codes.device, native.lib().ornith_w4_pack, 'w4 pack', native.ptr(codes), native.ptr(scales),
+    native.call_on(codes.get_device(), native.lib().ornith_w4_pack, 'w4 pack', native.ptr(codes), native.ptr(scales),
                    native.W4_TYPES[scales.dtype], native.ptr(zeros), native.ptr(packed[0]), native.ptr(packed[1]),
                    native.ptr(flags), n, k, group)
     bad = int(flags.item())
