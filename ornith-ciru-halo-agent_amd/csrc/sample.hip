@@ -21,9 +21,9 @@
 // rate of a large copy).  `parts` takes 17.2 us there: 10.9 to load and find the maxima, the rest fp64
 // for the masses (eleven instructions a value, 7 to 8 clocks each a wave); top-p's histogram costs 7 us
 // of LDS additions more.  Everything behind it works on bins and lists and is a chain of launches and
-// round trips: a whole row is drawn in 6.9 us, borders take 7 to 8, the list 8 to 9, its end 5 (few
+// round trips: a whole row is drawn in 6.9 us, borders take 6 to 7, the list 8 to 9, its end 5 (few
 // candidates) to 19 (2800 entries a row).  Calls in a graph over six inputs in turn: 1 row of top-k and
-// top-p 17.0 us, 8 rows of 151936 fp32 with top-p 25.8, 64 rows of mixed settings 47, 64 uncut 24.7, 256
+// top-p 15.7 us, 8 rows of 151936 fp32 with top-p 25.5, 64 rows of mixed settings 46, 64 uncut 24.9, 256
 // rows of 4096 columns 17.4.
 //
 // Masses.  With c = log2(e) / T and t = l c in fp64, e = 2^(t - j) for the
@@ -216,12 +216,18 @@ __device__ __forceinline__ int bin_mass(float v, const Scale& k, uint64_t& mass)
     mass = (uint64_t(hi) << 32) | lo;
     return o * kSub + f + kTopBin;
 }
+__device__ __forceinline__ int bin_alone(float v, const Scale& k) {
+    const double l = double(fminf(v, 0x1.fffffep127f)), m = kWhole - k.j;
+    const double q = __builtin_fma(l, k.c, m);
+    const double x = __builtin_fma(l, k.c, m - q);
+    const int f = int(uint32_t(__double_as_longlong(__builtin_fma(x, double(kSub), kWhole))));
+    return int(uint32_t(__double_as_longlong(q))) * kSub + f + kTopBin;
+}
 // The bin, for the row or part with the largest value mx, of any value up to a little above it (NaN
 // and -inf among them); -1: below the bins.
 __device__ __forceinline__ int bin_of(float v, float mx, double c, double j) {
     if (is_far(j)) return v >= mx ? kTopBin : -1;
-    uint64_t unused;
-    const int bin = bin_mass(v, Scale{c, j}, unused);
+    const int bin = bin_alone(v, Scale{c, j});
     return double(v) * c > j - 64.0 ? max(bin, -1) : -1;
 }
 // A value a little below the lower edge of `bin`; never -inf.
@@ -385,8 +391,7 @@ __device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting
     // those below the bin that holds the k-th largest of the threads' maxima (k values of this
     // part alone lie in or above it).
     if (s.k > 0 && s.k <= kMaximaK && THREADS >= kMaximaK) {
-        uint64_t unused;
-        const int b = bin_mass(mx, k, unused);
+        const int b = bin_alone(mx, k);
         if (b >= 0 && mx >= least) atomicAdd(&sh.count[b], 1u);
         __syncthreads();
         constexpr int per = (kTopBin + 64) / 64;
@@ -485,12 +490,10 @@ struct RowShared {
 
 // What the parts of a row with the given J add to it: scale, shift, least.  (Where J is far, every
 // part that adds anything has that j.)
-__device__ __forceinline__ PartMeta load_part(const SampleArgs& a, int slot, int p, double c, double J, RowShared& sh) {
-    const PartMeta m = a.meta[size_t(slot) * a.parts + p];
+__device__ __forceinline__ void set_part(int p, const PartMeta& m, double c, int shift, RowShared& sh) {
     sh.scale[p] = scale_of(c, m.j);
-    sh.shift[p] = m.key ? part_shift(J, m.j) : 64;
+    sh.shift[p] = shift;
     sh.least[p] = m.least;
-    return m;
 }
 // Sums of the waves before this one, and of all, from every wave's own (in LDS, after a barrier).
 __device__ __forceinline__ uint64_t waves_before(const uint64_t (&w)[kRowWaves], uint64_t& all) {
@@ -775,9 +778,8 @@ __device__ __forceinline__ void draw_column(const SampleArgs& a, int row, const 
 // (four threads an entry), then one wave walks both orders, four entries a lane.
 struct SmallList {
     uint64_t comp[kSmall], mass[kSmall], by_value[kSmall], by_column[kSmall];
-    uint8_t at[kSmall];                               // the entry of a column rank
     float val[kSmall];
-    uint32_t rank[kSmall];
+    uint32_t at[kSmall];                              // of a column rank: value rank << 8 | entry
 };
 __device__ __forceinline__ void finish_small(const SampleArgs& a, int row, const Setting& s, const Plan& plan, int n,
                                              uint64_t threshold, SmallList& sl) {
@@ -799,29 +801,30 @@ __device__ __forceinline__ void finish_small(const SampleArgs& a, int row, const
         by_column += uint32_t(dpp_i<kDppXor1>(int(by_column)));
         by_column += uint32_t(dpp_i<kDppXor2>(int(by_column)));
         if (e < n && (tid & 3) == 0) {
-            sl.by_value[by_value] = sl.mass[e];
-            sl.rank[e] = by_value;
-            sl.at[by_column] = uint8_t(e);
+            const uint64_t mass = sl.mass[e];
+            sl.by_value[by_value] = mass;
+            sl.by_column[by_column] = mass;
+            sl.at[by_column] = by_value << 8 | uint32_t(e);
         }
     }
     __syncthreads();
     if (tid >= 64) return;
     constexpr int per = kSmall / 64;
-    static_assert(kSmall == 256, "four entries a lane, a byte an entry");
+    static_assert(kSmall == 256, "four entries a lane, eight bits an entry");
     uint64_t m[per], sum = 0;
     auto walk = [&](auto&& mass_of) {                 // m[i]: sums up to entry per * tid + i
         sum = 0;
 #pragma unroll
         for (int i = 0; i < per; ++i) {
             const int r = per * tid + i;
-            sum += r < n ? mass_of(r) : 0;
+            sum += r < n ? mass_of(r, i) : 0;
             m[i] = sum;
         }
         const uint64_t before = wave_prefix_u64(sum) - sum;
 #pragma unroll
         for (int i = 0; i < per; ++i) m[i] += before;
     };
-    walk([&](int r) { return sl.by_value[r]; });
+    walk([&](int r, int) { return sl.by_value[r]; });
     // how many the cuts keep
     int keep = n;
     uint64_t of = plan.total;
@@ -846,19 +849,20 @@ __device__ __forceinline__ void finish_small(const SampleArgs& a, int row, const
             above += __popcll(__builtin_amdgcn_ballot_w64(per * tid + i < n && sl.comp[per * tid + i] >= threshold));
         keep = min(keep, above);
     }
-    walk([&](int r) {
-        const int x = sl.at[r];
-        return sl.rank[x] < uint32_t(keep) ? sl.mass[x] : 0;
-    });
+    uint64_t col_mass[per];
+    uint32_t col_at[per];
+#pragma unroll
+    for (int i = 0; i < per; ++i) {
+        col_at[i] = sl.at[per * tid + i];
+        col_mass[i] = per * tid + i < n && col_at[i] >> 8 < uint32_t(keep) ? sl.by_column[per * tid + i] : 0;
+    }
+    walk([&](int, int i) { return col_mass[i]; });
     const uint64_t total = readlane_u64(m[per - 1], 63), target = __umul64hi(fraction(s.u), total);
 #pragma unroll
     for (int i = 0; i < per; ++i) {
-        const int r = per * tid + i;
-        if (r < n) {
-            const int x = sl.at[r];
-            const uint64_t mass = sl.rank[x] < uint32_t(keep) ? sl.mass[x] : 0;
-            if (m[i] > target && m[i] - mass <= target)
-                give(a, row, comp_col(sl.comp[x]), log_share(sl.val[x], s, plan.J, mass, total));
+        if (per * tid + i < n && m[i] > target && m[i] - col_mass[i] <= target) {
+            const int x = int(col_at[i] & 255u);
+            give(a, row, comp_col(sl.comp[x]), log_share(sl.val[x], s, plan.J, col_mass[i], total));
         }
     }
 }
@@ -1043,18 +1047,25 @@ __device__ __forceinline__ bool plan_row(const SampleArgs& a, int slot, int row,
                                          PlanShared& ps, DrawShared& ds) {
     const int tid = threadIdx.x, lane = tid & 63;
     const PartMeta* meta = a.meta + size_t(slot) * a.parts;
-    // the row's largest value and its first part (every wave for itself)
-    uint32_t key[kPartsMax / 64], top = 0;
+    // the parts, a lane each (every wave for itself), and the row's largest value
+    PartMeta part[kPartsMax / 64];
+    uint32_t top = 0;
 #pragma unroll
     for (int h = 0; h < kPartsMax / 64; ++h) {
-        key[h] = h * 64 + lane < a.parts ? meta[h * 64 + lane].key : 0;
-        top = max(top, wave_max_u(key[h]));
+        const int p = h * 64 + lane;
+        part[h] = meta[min(p, a.parts - 1)];
+    }
+#pragma unroll
+    for (int h = 0; h < kPartsMax / 64; ++h) {        // (all of it loaded here, not where it is used)
+        asm volatile("" : "+v"(part[h].j), "+v"(part[h].mass), "+v"(part[h].key), "+v"(part[h].arg), "+v"(part[h].least));
+        if (h * 64 + lane >= a.parts) part[h].key = 0;
+        top = max(top, wave_max_u(part[h].key));
     }
     if (!s.valid || top == 0 || s.T == 0.f) {
         int first = 0;
 #pragma unroll
         for (int h = kPartsMax / 64 - 1; h >= 0; --h) {
-            const uint64_t at = __builtin_amdgcn_ballot_w64(key[h] == top);
+            const uint64_t at = __builtin_amdgcn_ballot_w64(part[h].key == top);
             if (at) first = h * 64 + __builtin_ctzll(at);
         }
         if (lead && tid == 0) {
@@ -1067,29 +1078,37 @@ __device__ __forceinline__ bool plan_row(const SampleArgs& a, int slot, int row,
     if (!s.cut && !lead) return false;
     const float mx = unordered(top);
     const double J = __builtin_ceil(double(mx) * s.c);
-    if (tid < a.parts) {
-        const PartMeta m = load_part(a, slot, tid, s.c, J, sh);
-        sh.part_mass[tid] = row_mass(m.mass, sh.shift[tid]);
+    int shift[kPartsMax / 64];
+#pragma unroll
+    for (int h = 0; h < kPartsMax / 64; ++h) {
+        const int p = h * 64 + lane;
+        shift[h] = part[h].key ? part_shift(J, part[h].j) : 64;
+        if (tid < 64 && p < a.parts) {
+            set_part(p, part[h], s.c, shift[h], sh);
+            sh.part_mass[p] = row_mass(part[h].mass, shift[h]);
+        }
     }
-    __syncthreads();
     if (!s.cut) {
+        __syncthreads();
         draw_part(a.parts, s, sh);
-        const int part = sh.part;
-        if (part < 0) {                               // (logits that changed under the call)
+        const int in = sh.part;
+        if (in < 0) {                                 // (logits that changed under the call)
             if (tid == 0) give(a, row, -1, __builtin_nanf(""));
             return false;
         }
         Piece<TYPE> v;
-        const int col0 = part * kPart + tid * kPer;
+        const int col0 = in * kPart + tid * kPer;
         v.load(row_of<TYPE>(a, row), col0, a.N);
-        draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], 0, v, col0, sh, ds);
+        draw_column<TYPE>(a, row, s, J, sh.scale[in], sh.least[in], sh.shift[in], 0, v, col0, sh, ds);
         return false;
     }
     // the parts' bins: three groups of threads, a third of the parts each
-    const int g = tid / (kTopBin + 24), i = tid % (kTopBin + 24), bin = kTopBin - i;
+    constexpr int kGroup = kTopBin + 24;
+    static_assert(kGroup % 64 == 0, "a wave lies in one group");
+    const int g = __builtin_amdgcn_readfirstlane(tid / kGroup), i = tid - g * kGroup, bin = kTopBin - i;
     uint64_t mass = 0;
     uint32_t count = 0;
-    if (g < 3 && bin >= 0) {
+    if (g < 3) {
         const uint64_t* hist = a.hist + size_t(slot) * a.parts * kBins;
         constexpr int U = 11;                         // (33 parts' loads in flight at once)
         for (int p0 = g; p0 < a.parts; p0 += 3 * U) {
@@ -1097,18 +1116,19 @@ __device__ __forceinline__ bool plan_row(const SampleArgs& a, int slot, int row,
             int sf[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int p = p0 + 3 * u;
-                sf[u] = p < a.parts ? sh.shift[p] : 64;
-                const int at = bin + kSub * sf[u];
-                w[u] = at <= kTopBin ? hist[size_t(p) * kBins + at] : 0;
+                // (no branch may part the loads; bins past kTopBin are zeros, parts past the last add nothing)
+                const int p = min(p0 + 3 * u, a.parts - 1);
+                sf[u] = p0 + 3 * u < a.parts ? __builtin_amdgcn_readlane(p < 64 ? shift[0] : shift[1], p & 63) : 64;
+                w[u] = hist[p * kBins + min(max(bin, 0) + kSub * sf[u], kBins - 1)];
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                count += uint32_t(w[u] >> kMassBits);
-                mass += row_mass(w[u] & kMassMask, sf[u]);
+            for (int u = 0; u < U; ++u) {             // (row_mass of the mass, whose bits the first shift leaves)
+                const uint64_t x = sf[u] < 64 ? w[u] : 0;
+                count += uint32_t(x >> kMassBits);
+                mass += (x << (64 - kMassBits)) >> min(64 - kMassBits - kRowShift + sf[u], 63);
             }
         }
-        if (g) {
+        if (g && bin >= 0) {
             ps.mass[g - 1][i] = mass;
             ps.count[g - 1][i] = count;
         }
@@ -1165,11 +1185,19 @@ __device__ __forceinline__ void gather_part(const SampleArgs& a, int slot, const
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     uint2* list = a.list + size_t(slot) * a.list_max;
     uint32_t in = 0;
+    if (plan.mode == kModeSmall) {                    // the first range alone, which has no upper end
+        const float from = fmaxf(least, unordered(plan.lo[0]));
 #pragma unroll
-    for (int u = 0; u < PIECES; ++u)
+        for (int u = 0; u < PIECES; ++u)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)                   // (v >= least is false for NaN)
-            in |= uint32_t(v[u][e] >= least && in_ranges(plan, ordered(v[u][e]))) << (8 * u + e);
+            for (int e = 0; e < 8; ++e) in |= uint32_t(v[u][e] >= from) << (8 * u + e);
+    } else {
+#pragma unroll
+        for (int u = 0; u < PIECES; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)               // (v >= least is false for NaN)
+                in |= uint32_t(v[u][e] >= least && in_ranges(plan, ordered(v[u][e]))) << (8 * u + e);
+    }
     const int own = __popc(in), run = wave_prefix_sum(own);
     if (lane == 63) gs.n[wv] = run;
     __syncthreads();
@@ -1367,7 +1395,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     const uint32_t listed = st->count;
     const Setting s = setting(a, row);
     if (mode == kDone) return;
-    if (tid < a.parts) load_part(a, slot, tid, s.c, J, sh);
+    if (tid < a.parts) {
+        const PartMeta m = a.meta[size_t(slot) * a.parts + tid];
+        set_part(tid, m, s.c, m.key ? part_shift(J, m.j) : 64, sh);
+    }
     if (tid == 0) sh.plan = st->plan;
     if (tid < kBins) sh.cm[tid] = cum;
     __syncthreads();
@@ -1377,7 +1408,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
 // Select, gather and finish of few rows in one launch: every block of a row makes its plan, lists its
 // part's entries, and the last one to have done so ends the row.  Entries, their count and the arrivals
 // pass through relaxed accesses of device scope, ordered by a wait for the wave's own stores: a fence of
-// every thread wrote back and dropped the caches, 20 to 90 us.  12.8 us for a row of top-k (7 of them
+// every thread wrote back and dropped the caches, 20 to 90 us.  11.5 us for a row of top-k (6 of them
 // plan and list), 16 to 21 with top-p's list of some thousand entries.
 template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_rest_kernel(SampleArgs a, int row0) {
