@@ -358,3 +358,47 @@ def test_rows_past_a_chunk(device, M, N):
         t1, l1, f1 = _run(logits[s], us[s], T[s], k[s], p[s], q[s])
         assert (t1 == token[s]).all() and (l1 == logprob[s]).all() and f1 == 0, r
     assert flags == 0
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
+def test_every_launch_plan_agrees(device, dtype):
+    """Rows of every kind with every cut: few parts at a time (two launches), all
+    at once (four), and in one block, give the same bits."""
+    import torch
+    rng = np.random.default_rng(15)
+    N = 40000
+    top = float(torch.finfo(_dtype(dtype)).max)
+    kinds = rng.standard_normal((12, N)).astype(np.float32) * 2
+    kinds[1] = 0.0
+    kinds[2] = -np.inf
+    kinds[3] = -np.inf
+    kinds[3, 33333] = -4.0
+    kinds[4] = -top
+    kinds[4, 77] = 2.0
+    kinds[5, 5::7] = np.nan
+    kinds[6, [3, 9000, 39999]] = np.inf
+    kinds[7] = np.linspace(-20, 20, N)
+    kinds[8] = top
+    kinds[8, ::2] = -top
+    kinds[9, 8192:16384] = -np.inf
+    kinds[10, rng.random(N) > 0.02] = -np.inf
+    kinds[11] = rng.integers(0, 2, N)
+    cuts = [(0, 1.0, 0.0, 1.0), (1, 1.0, 0.0, 1.0), (50, 0.9, 0.0, 0.7), (0, 0.95, 0.0, 1.0), (0, 1.0, 0.05, 0.8),
+            (300, 1.0, 0.0, 1.5), (20000, 0.5, 1e-6, 1.0), (39999, 0.999, 0.0, 100.0), (40, 0.9, 0.1, 0.0),
+            (5, 0.9, 0.0, -1.0)]
+    logits = torch.from_numpy(kinds).to(_dtype(dtype)).to(device).repeat(len(cuts), 1)
+    us = rng.random(12 * len(cuts)).astype(np.float32)
+    k, p, q, T = (np.repeat([c[i] for c in cuts], 12) for i in range(4))
+    token, logprob, flags = _run(logits, us, T, k, p, q)
+    assert len(us) * 5 > 256 and flags == 7
+    for r in range(0, len(us), 12):
+        s = slice(r, r + 12)
+        t1, l1, _ = _run(logits[s], us[s], T[s], k[s], p[s], q[s])
+        assert (t1 == token[s]).all() and np.array_equal(l1, logprob[s], equal_nan=True), (cuts[r // 12], t1, token[s])
+    # rows of one part: their end is masked, and then it is not there
+    masked = logits.clone()
+    masked[:, PART:] = -float('inf')
+    token, logprob, _ = _run(masked, us, T, k, p, q)
+    t1, l1, _ = _run(masked[:, :PART].contiguous(), us, T, k, p, q)
+    same = (k < PART) | (p < 1)                        # (with a top-k past all that is there, that is all)
+    assert (t1 == token)[same].all() and np.array_equal(l1[same], logprob[same], equal_nan=True)

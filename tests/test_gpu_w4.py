@@ -114,6 +114,42 @@ def test_w4_rows(device, dtype, out_type, M, N, K):
     _check(c, got, out_type)
 
 
+# More than 16 rows of more than 3072 tiles of 16 x 16: x in shared memory, two, three and four tiles of
+# rows a block, runs of columns that waves share in the middle of K and at its ends.
+LONG = [(17, 24600, 8), (20, 25003, 2040), (32, 24592, 2048), (33, 16401, 1160), (40, 16400, 136), (48, 16500, 1304),
+        (49, 12301, 1000), (64, 12320, 1024), (63, 12305, 2048), (130, 5500, 520), (200, 3801, 264)]
+
+
+@pytest.mark.parametrize('group', [32, 64, 128, 256])
+@pytest.mark.parametrize('M,N,K', LONG)
+def test_w4_many_columns(device, group, M, N, K):
+    import torch
+    assert -(-N // 16) * -(-M // 16) > 3072
+    rng = np.random.default_rng(M * 31 + N * 7 + K + group)
+    dtype = ('bf16', 'fp16')[(M + group // 32) % 2]
+    c = _case(rng, M, N, K, group, bool(K // 8 % 2), dtype, device, True, ldx=K + 8 * (N % 3))
+    got, flags = _run(c, 'fp32', ldo=N + N % 5)
+    want, _ = _want(c)
+    assert np.abs(want).max() < 2 ** 20 and flags == 0
+    assert (got == want).all(), np.argwhere(got != want)[:5]
+    got, flags = _run(c, dtype)
+    assert (got == torch.from_numpy(want).to(_dtype(dtype)).double().numpy()).all()
+
+
+@pytest.mark.parametrize('out_type', ['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('M,N,K', [(20, 25003, 2040), (33, 16401, 1160), (64, 12320, 1024)])
+def test_w4_many_columns_rows(device, out_type, M, N, K):
+    rng = np.random.default_rng(M + N + K)
+    c = _case(rng, M, N, K, (32, 64, 128, 256)[M % 4], True, 'bf16' if M % 2 else 'fp16', device, False)
+    got, flags = _run(c, out_type)
+    assert flags == 0
+    _check(c, got, out_type)
+    c['x'][3] = float('nan')                           # raised from this kernel as well, and kept to its row
+    some, flags = _run(c, out_type)
+    assert flags == (4 if out_type == 'fp32' else 12)
+    assert np.isnan(some[3]).all() and np.isfinite(np.delete(some, 3, 0)).all()
+
+
 def test_pack_layout(device):
     import torch
     from ornith_g256 import storage
