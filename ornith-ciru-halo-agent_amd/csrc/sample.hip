@@ -167,6 +167,15 @@ template <int TYPE> __device__ __forceinline__ uint32_t comp_key(uint64_t comp) 
     return k & 0x80000000u ? k : k | ((1u << kDrop<TYPE>) - 1);
 }
 __device__ __forceinline__ int comp_col(uint64_t comp) { return int(kColMask - (uint32_t(comp) & kColMask)); }
+// comp >= threshold on values and columns
+struct Cut {
+    float value;
+    int col;
+    __device__ __forceinline__ bool keeps(float v, int c) const { return v > value || (v == value && c <= col); }
+};
+template <int TYPE> __device__ __forceinline__ Cut cut_of(uint64_t threshold) {
+    return threshold ? Cut{unordered(comp_key<TYPE>(threshold)), comp_col(threshold)} : Cut{-__builtin_huge_valf(), 0};
+}
 
 // 2^(36 + x) for |x| <= 1/2, degree 8 (Chebyshev interpolation; relative error 2^-39.7, 2^36 at 0).
 // The coefficients are kept in scalar registers: as literals, each fma is preceded by two moves.
@@ -696,16 +705,16 @@ __device__ __forceinline__ void draw_part(int parts, const Setting& s, RowShared
 // The token inside the part: thread i holds its columns col0 .. col0 + 7, ascending over the block.
 // Unless most of the part is kept, the kept values are set side by side in LDS first: fewer masses a thread.
 struct DrawShared { float val[kPart]; uint16_t col[kPart]; };
-template <int TYPE>
+template <int TYPE, bool CUT>
 __device__ __forceinline__ void draw_column(const SampleArgs& a, int row, const Setting& s, double J, const Scale& k,
                                             float least, int shift, uint64_t threshold, const Piece<TYPE>& v, int col0,
                                             RowShared& sh, DrawShared& ds) {
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const uint64_t rest = sh.rest, total = sh.total;
+    const Cut cut = cut_of<TYPE>(threshold);
     uint32_t keep = 0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e)
-        keep |= uint32_t(v[e] >= least && comp_of<TYPE>(ordered(v[e]), col0 + e) >= threshold) << e;
+    for (int e = 0; e < kPer; ++e) keep |= uint32_t(v[e] >= least && (!CUT || cut.keeps(v[e], col0 + e))) << e;
     const uint32_t own = uint32_t(__popc(keep));
     uint32_t at = uint32_t(wave_prefix_sum(int(own))), kept;
     if (lane == 63) sh.wave_count[wv] = at;
@@ -1015,21 +1024,29 @@ __device__ __forceinline__ uint64_t threshold_of(const Setting& s, const Plan& p
     }
     if (plan.use_p) {
         const uint64_t target = share(s.p, of);
-        __syncthreads();
-        if (tid == 0) sh.bin[0] = 0;
-        __syncthreads();
-        if (tid <= kTopBin) {
-            const uint64_t next = tid == kTopBin ? 0 : cm[tid + 1];
-            if (cm[tid] >= target && next < target) {
-                sh.bin[0] = tid;
-                sh.lo = target - next;
+        int b = plan.bin_hi[1];
+        uint32_t lo = plan.lo[1], hi = plan.hi[1];
+        const uint64_t above = b == kTopBin ? 0 : cm[b + 1];
+        uint64_t need = target > above ? target - above : 1;      // (the first k can sum to a few units less than their bins)
+        if (plan.bin_lo[1] != b) {                    // one of several bins
+            __syncthreads();
+            if (tid == 0) sh.bin[0] = 0;
+            __syncthreads();
+            if (tid <= kTopBin) {
+                const uint64_t next = tid == kTopBin ? 0 : cm[tid + 1];
+                if (cm[tid] >= target && next < target) {
+                    sh.bin[0] = tid;
+                    sh.lo = target - next;
+                }
             }
+            __syncthreads();
+            b = sh.bin[0];
+            need = sh.lo;
+            bin_range(b, s, plan, sh);
+            lo = sh.edge[0];
+            hi = sh.edge[1];
         }
-        __syncthreads();
-        const int b = sh.bin[0];
-        bin_range(b, s, plan, sh);
-        const uint32_t lo = sh.edge[0], hi = sh.edge[1];
-        descend<TYPE>(lo, hi, true, sh.lo, group, [&](auto&& f) { each(lo, hi, f); }, d);
+        descend<TYPE>(lo, hi, true, need, group, [&](auto&& f) { each(lo, hi, f); }, d);
         if (d.found > threshold) {
             threshold = d.found;
             bf = b;
@@ -1099,7 +1116,7 @@ __device__ __forceinline__ bool plan_row(const SampleArgs& a, int slot, int row,
         Piece<TYPE> v;
         const int col0 = in * kPart + tid * kPer;
         v.load(row_of<TYPE>(a, row), col0, a.N);
-        draw_column<TYPE>(a, row, s, J, sh.scale[in], sh.least[in], sh.shift[in], 0, v, col0, sh, ds);
+        draw_column<TYPE, false>(a, row, s, J, sh.scale[in], sh.least[in], sh.shift[in], 0, v, col0, sh, ds);
         return false;
     }
     // the parts' bins: three groups of threads, a third of the parts each
@@ -1185,7 +1202,7 @@ __device__ __forceinline__ void gather_part(const SampleArgs& a, int slot, const
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     uint2* list = a.list + size_t(slot) * a.list_max;
     uint32_t in = 0;
-    if (plan.mode == kModeSmall) {                    // the first range alone, which has no upper end
+    if (HERE && plan.mode == kModeSmall) {            // the first range alone, which has no upper end
         const float from = fmaxf(least, unordered(plan.lo[0]));
 #pragma unroll
         for (int u = 0; u < PIECES; ++u)
@@ -1259,8 +1276,8 @@ __device__ __forceinline__ void sum_parts(const SampleArgs& a, int slot, int bin
         const int shift = sh.shift[p];
         uint64_t m = 0;
 #pragma unroll
-        for (int i = 0; i < kBinSteps; ++i)
-            m += 64 * i + lane > bin + kSub * shift ? row_mass(w[i] & kMassMask, shift) : 0;
+        for (int i = 0; i < kBinSteps; ++i)            // (row_mass, as in plan_row; a part without bins has shift 64)
+            m += 64 * i + lane > bin + kSub * shift ? (w[i] << (64 - kMassBits)) >> min(64 - kMassBits - kRowShift + shift, 63) : 0;
         m = wave_sum_u64(m);
         if (lane == 0) sh.part_mass[p] = m;
     };
@@ -1376,7 +1393,7 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, int slot, int ro
     Piece<TYPE> v;
     const int col0 = part * kPart + tid * kPer;
     v.load(src, col0, a.N);
-    draw_column<TYPE>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], threshold, v, col0, sh, un.draw);
+    draw_column<TYPE, true>(a, row, s, J, sh.scale[part], sh.least[part], sh.shift[part], threshold, v, col0, sh, un.draw);
 }
 
 // Bound by its chain of LDS passes and barriers: 5 us where 256 candidates decide, 14 to 19 where borders
@@ -1514,12 +1531,13 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a, i
         threshold = threshold_of<TYPE>(s, plan, sh.cm, threshold, ~0u, each, un.descent, sh, bf);
     }
     // the kept mass, and the token
+    const Cut cut = cut_of<TYPE>(threshold);
     uint64_t sum = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
         uint64_t x;
         const int bin = bin_mass(v[0][e], k, x);
-        if (bin >= 0 && v[0][e] >= m.least && comp_of<TYPE>(ordered(v[0][e]), col0 + e) >= threshold) sum += x;
+        if (bin >= 0 && v[0][e] >= m.least && cut.keeps(v[0][e], col0 + e)) sum += x;
     }
     sum = wave_sum_u64(sum);
     __syncthreads();
@@ -1533,7 +1551,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a, i
         sh.rest = __umul64hi(fraction(s.u), sh.total);
     }
     __syncthreads();
-    draw_column<TYPE>(a, row, s, J, k, m.least, 0, threshold, v[0], col0, sh, un.draw);
+    draw_column<TYPE, true>(a, row, s, J, k, m.least, 0, threshold, v[0], col0, sh, un.draw);
 }
 
 // rows of an empty vocabulary
