@@ -19,16 +19,16 @@
 //
 // What bounds it.  The floor is one pass over the logits (64 rows of 248320 bf16: 31.8 MB, 6.6 us at the
 // rate of a large copy).  `parts` takes 17.2 us there: 10.9 to load and find the maxima, the rest fp64
-// for the masses (eleven instructions a value, 7 to 8 clocks each a wave); top-p's histogram costs 7 us
+// for the masses (a dozen instructions a value, 7 to 8 clocks each a wave); top-p's histogram costs 7 us
 // of LDS additions more.  Everything behind it works on bins and lists and is a chain of launches and
 // round trips: a whole row is drawn in 6.9 us, borders take 6 to 7, the list 8 to 9, its end 5 (few
 // candidates) to 19 (2800 entries a row).  Calls in a graph over six inputs in turn: 1 row of top-k and
-// top-p 15.7 us, 8 rows of 151936 fp32 with top-p 25.5, 64 rows of mixed settings 46, 64 uncut 24.9, 256
-// rows of 4096 columns 17.4.
+// top-p 15.7 us, 8 rows of 151936 fp32 with top-p 25.1, 64 rows of mixed settings 46, 64 uncut 24.5, 256
+// rows of 4096 columns 17.1.
 //
 // Masses.  With c = log2(e) / T and t = l c in fp64, e = 2^(t - j) for the
-// whole number j = ceil(max t) of its part: a degree-8 polynomial in t - rint(t)
-// (relative error 2^-39.7), rounded to a whole number of units 2^-36.  One
+// whole number j = ceil(max t) of its part: a degree-7 polynomial in t - rint(t)
+// (relative error 2^-33), rounded to a whole number of units 2^-36.  One
 // 64-bit LDS add carries count (14 bits) and mass (50 bits: 8192 entries of at
 // most 2^36).  Whole numbers make the sums independent of the order of the
 // atomics.  A row adds parts in units of 2^-42 of 2^J, J the largest j:
@@ -177,20 +177,20 @@ template <int TYPE> __device__ __forceinline__ Cut cut_of(uint64_t threshold) {
     return threshold ? Cut{unordered(comp_key<TYPE>(threshold)), comp_col(threshold)} : Cut{-__builtin_huge_valf(), 0};
 }
 
-// 2^(36 + x) for |x| <= 1/2, degree 8 (Chebyshev interpolation; relative error 2^-39.7, 2^36 at 0).
+// 2^(36 + x) for |x| <= 1/2, degree 7 (interpolation of (2^x - 1) / x at Chebyshev points; relative error
+// 2^-33, 2^36 at 0; degree 8, 2^-39.7, costs 0.6 us at 64 rows of 248320; degree 6, 2^-27.6, would save 0.5).
 // The coefficients are kept in scalar registers: as literals, each fma is preceded by two moves.
 __device__ __forceinline__ double in_sgpr(double v) {
     asm("" : "+s"(v));
     return v;
 }
 __device__ __forceinline__ double exp2_units(double x) {
-    double p = __builtin_fma(x, in_sgpr(0x1.63cf7dec51603p+16), in_sgpr(0x1.00dc48dc4d96cp+20));
-    p = __builtin_fma(p, x, in_sgpr(0x1.4308ae274a207p+23));
-    p = __builtin_fma(p, x, in_sgpr(0x1.5d8745a95d2d4p+26));
-    p = __builtin_fma(p, x, in_sgpr(0x1.3b2ab71725c04p+29));
-    p = __builtin_fma(p, x, in_sgpr(0x1.c6b08dd6fb6b1p+31));
-    p = __builtin_fma(p, x, in_sgpr(0x1.ebfbdff824847p+33));
-    p = __builtin_fma(p, x, in_sgpr(0x1.62e42fef84cf7p+35));
+    double p = __builtin_fma(x, in_sgpr(0x1.00a5814f2a63cp+20), in_sgpr(0x1.443fffcaa2337p+23));
+    p = __builtin_fma(p, x, in_sgpr(0x1.5d879ead1c114p+26));
+    p = __builtin_fma(p, x, in_sgpr(0x1.3b2a1b7150c21p+29));
+    p = __builtin_fma(p, x, in_sgpr(0x1.c6b08d883db58p+31));
+    p = __builtin_fma(p, x, in_sgpr(0x1.ebfbe045f4d5cp+33));
+    p = __builtin_fma(p, x, in_sgpr(0x1.62e42fefa39f0p+35));
     return __builtin_fma(p, x, in_sgpr(0x1p36));
 }
 

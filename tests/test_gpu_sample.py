@@ -3,9 +3,9 @@
 A uniform number is placed in the middle of the chosen token's interval and a
 top-p in the middle of its prefix's, so both are decided by arithmetic: the
 kernels' masses are off by half a unit of 2^-36 of their part's power of two
-(at most twice the part's largest mass), by 2^-39.7 of themselves (polynomial)
+(at most twice the part's largest mass), by 2^-33 of themselves (polynomial)
 and by |t| 2^-53 (argument), so a running sum of n masses relative to the
-largest is off by at most n 2^-36 + S 2^-39; fp32 u and p are off by 2^-25.
+largest is off by at most n 2^-36 + S 2^-32; fp32 u and p are off by 2^-25.
 Intervals narrower than MARGIN of the kept mass, eight times fp32's step, are
 not chosen, and n 2^-36 stays below that for the n used here.
 logprob: fp32 of ln(e / S): half a step of the result, and the masses' errors
