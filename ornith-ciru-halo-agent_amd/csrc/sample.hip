@@ -366,7 +366,6 @@ __device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting
     const Scale k = scale_of(s.c, j);
     float least = below_bin(0, part_mx, s.inv, j);
     if (!s.cut) {
-        // (whole numbers in fp64 as well: below 2^50)
         uint64_t sum;
         if (is_far(j)) {
             int count = 0;
@@ -376,17 +375,28 @@ __device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting
                 for (int e = 0; e < 8; ++e) count += v[u][e] >= least;
             sum = uint64_t(count) * kPartOne;
         } else {
-            double masses = 0.0;
+            // The bits of 2^52 + mass are those of 2^52, plus the mass.  From `least` down masses are 0, so
+            // values (NaN too) are clamped to it; but where it was cut off at the lowest fp32, others than
+            // those at or above it must not count.
+            constexpr float kMost = 0x1.fffffep127f;
+            auto bits = [&](float l) -> uint64_t {
+                int o;
+                double x;
+                return uint64_t(__double_as_longlong(mass_sum(l, k, o, x)));
+            };
+            const uint64_t none = uint64_t(__double_as_longlong(0x1p52));
+            sum = -none * uint64_t(8 * PIECES);
+            if (least > -kMost) {
 #pragma unroll
-            for (int u = 0; u < PIECES; ++u)
+                for (int u = 0; u < PIECES; ++u)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    int o;
-                    double x;
-                    const double m = mass_sum(v[u][e], k, o, x) - 0x1p52;
-                    masses += v[u][e] >= least ? m : 0.0;        // (false for NaN)
-                }
-            sum = uint64_t(masses);
+                    for (int e = 0; e < 8; ++e) sum += bits(__builtin_amdgcn_fmed3f(v[u][e], least, kMost));
+            } else {
+#pragma unroll
+                for (int u = 0; u < PIECES; ++u)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum += v[u][e] >= least ? bits(v[u][e]) : none;
+            }
         }
         sum = wave_sum_u64(sum);
         if (lane == 0) sh.mass[wv] = sum;
