@@ -18,12 +18,12 @@
 // last three steps in one launch (sample_rest), whose last block to list its entries ends the row.
 //
 // What bounds it.  The floor is one pass over the logits (64 rows of 248320 bf16: 31.8 MB, 6.6 us at the
-// rate of a large copy).  `parts` takes 17.2 us there: 10.9 to load and find the maxima, the rest fp64
-// for the masses (a dozen instructions a value, 7 to 8 clocks each a wave); top-p's histogram costs 7 us
-// of LDS additions more.  Everything behind it works on bins and lists and is a chain of launches and
+// rate of a large copy).  `parts` takes 15.4 us there: 10.9 to load and find the maxima, the rest fp64
+// for the masses (a dozen instructions a value, 7 to 8 clocks each a wave); top-p's histogram costs 9 us
+// of LDS additions and bins more.  Everything behind it works on bins and lists and is a chain of launches and
 // round trips: a whole row is drawn in 6.9 us, borders take 6 to 7, the list 8 to 9, its end 5 (few
 // candidates) to 19 (2800 entries a row).  Calls in a graph over six inputs in turn: 1 row of top-k and
-// top-p 15.7 us, 8 rows of 151936 fp32 with top-p 25.1, 64 rows of mixed settings 46, 64 uncut 24.5, 256
+// top-p 15.7 us, 8 rows of 151936 fp32 with top-p 25.1, 64 rows of mixed settings 46, 64 uncut 23.0, 256
 // rows of 4096 columns 17.1.
 //
 // Masses.  With c = log2(e) / T and t = l c in fp64, e = 2^(t - j) for the
@@ -465,7 +465,7 @@ __device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting
 }
 
 // A block per part, the values in registers, loaded once.  256 threads (four pieces each) where parts are
-// many: 64 rows of 248320 bf16 17.2 us, where 512 and 1024 threads were slower (in an earlier form of the
+// many: 64 rows of 248320 bf16 15.4 us, where 512 and 1024 threads were slower (in an earlier form of the
 // masses 22 / 24 / 30 us: more waves meet at each barrier).  1024 where every part has a CU of its own and the
 // chain of one thread counts: 8 rows of 151936 fp32 5.6 us, with 256 threads 8.0.  Tried and slower: blocks
 // that stay and load a part ahead (27 us against 22), 64 VGPRs a thread forced by launch bounds (spills).
