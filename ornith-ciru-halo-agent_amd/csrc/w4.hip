@@ -452,7 +452,7 @@ template <int TYPE, int NT, int W> hipError_t w4_tiles(const W4Args& a, hipStrea
 template <int TYPE> hipError_t w4_rows(const W4Args& a, hipStream_t s) {
     const int64_t cells = int64_t((a.N + 15) / 16) * ((a.M + 15) / 16);      // tiles of 16 x 16 results
     const int blocks = w4_blocks(a.K);
-    if (a.M > 16 && cells > 3072) {
+    if (a.M > 16 && cells > 3000) {
         if (a.M > 48 && w4_x_bytes(4, a.K) <= kW4XBytes) return w4_run<TYPE, 4, 8, 4>(a, s);
         if (a.M > 32 && w4_x_bytes(3, a.K) <= kW4XBytes) return w4_run<TYPE, 3, 8, 4>(a, s);
         if (w4_x_bytes(2, a.K) <= kW4XBytes) return w4_run<TYPE, 2, 12, 3>(a, s);

@@ -114,7 +114,7 @@ def test_w4_rows(device, dtype, out_type, M, N, K):
     _check(c, got, out_type)
 
 
-# More than 16 rows of more than 3072 tiles of 16 x 16: x in shared memory, two, three and four tiles of
+# More than 16 rows of more than 3000 tiles of 16 x 16: x in shared memory, two, three and four tiles of
 # rows a block, runs of columns that waves share in the middle of K and at its ends.
 LONG = [(17, 24600, 8), (20, 25003, 2040), (32, 24592, 2048), (33, 16401, 1160), (40, 16400, 136), (48, 16500, 1304),
         (49, 12301, 1000), (64, 12320, 1024), (63, 12305, 2048), (130, 5500, 520), (200, 3801, 264)]
@@ -124,7 +124,7 @@ LONG = [(17, 24600, 8), (20, 25003, 2040), (32, 24592, 2048), (33, 16401, 1160),
 @pytest.mark.parametrize('M,N,K', LONG)
 def test_w4_many_columns(device, group, M, N, K):
     import torch
-    assert -(-N // 16) * -(-M // 16) > 3072
+    assert -(-N // 16) * -(-M // 16) > 3000
     rng = np.random.default_rng(M * 31 + N * 7 + K + group)
     dtype = ('bf16', 'fp16')[(M + group // 32) % 2]
     c = _case(rng, M, N, K, group, bool(K // 8 % 2), dtype, device, True, ldx=K + 8 * (N % 3))
