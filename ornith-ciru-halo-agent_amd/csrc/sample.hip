@@ -1660,7 +1660,7 @@ extern "C" hipError_t ornith_logits_sample_launch(const void* logits, int logits
                               {flags, 4, 4, true, false}};
     if (!check_buffers(buffers)) return hipErrorInvalidValue;
     if (!N) {
-        timed_launch("sample_empty", sample_empty_kernel, dim3((M + 63) / 64), dim3(64), 0, stream, M,
+        timed_launch("sample_empty", sample_empty_kernel, dim3((unsigned(M) + 63) / 64), dim3(64), 0, stream, M,
                      static_cast<int64_t*>(token), static_cast<float*>(logprob), static_cast<uint32_t*>(flags));
         return hipGetLastError();
     }
