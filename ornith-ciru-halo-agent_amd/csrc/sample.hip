@@ -201,8 +201,8 @@ __device__ __forceinline__ bool is_far(double j) { return !(__builtin_fabs(j) < 
 struct Scale { double c, j; };
 __device__ __forceinline__ Scale scale_of(double c, double j) { return is_far(j) ? Scale{0.0, 0.0} : Scale{c, j}; }
 
-// With the part's scale, 2^52 + the mass of a value l at or above its part's `least` (of others,
-// anything), o = rint(l c) - j and x = l c - rint(l c).  Whole numbers come from the low word of a sum
+// With the part's scale, 2^52 + the mass of a value l at or above its part's `least` and no more than
+// 1000 powers of two below j (of others, anything), o = rint(l c) - j and x = l c - rint(l c).  Whole numbers come from the low word of a sum
 // with 1.5 * 2^52, with one rounding of the exact product, so o + j and its eighths are the same in
 // every part.
 __device__ __forceinline__ double mass_sum(float v, const Scale& k, int& o, double& x) {
@@ -214,7 +214,7 @@ __device__ __forceinline__ double mass_sum(float v, const Scale& k, int& o, doub
     const uint32_t hi = uint32_t(e >> 32) + (uint32_t(o) << 20);
     return __longlong_as_double((int64_t(hi) << 32) | uint32_t(e)) + 0x1p52;
 }
-// Bin and mass of the same.
+// Bin and mass of the same (bin < 0: no mass, whatever `mass` holds).
 __device__ __forceinline__ int bin_mass(float v, const Scale& k, uint64_t& mass) {
     int o;
     double x;
@@ -376,26 +376,30 @@ __device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting
             sum = uint64_t(count) * kPartOne;
         } else {
             // The bits of 2^52 + mass are those of 2^52, plus the mass.  From `least` down masses are 0, so
-            // values (NaN too) are clamped to it; but where it was cut off at the lowest fp32, others than
-            // those at or above it must not count.
+            // values (NaN too) are clamped to it; but not where it was cut off at the lowest fp32 (values
+            // below must not count), nor where it lies so far down (it keeps 2^-20 of |j| from the bins)
+            // that its octave leaves the exponent field: there the bins decide, as for cut rows.
             constexpr float kMost = 0x1.fffffep127f;
-            auto bits = [&](float l) -> uint64_t {
-                int o;
-                double x;
-                return uint64_t(__double_as_longlong(mass_sum(l, k, o, x)));
-            };
-            const uint64_t none = uint64_t(__double_as_longlong(0x1p52));
-            sum = -none * uint64_t(8 * PIECES);
-            if (least > -kMost) {
+            if (least > -kMost && double(least) * s.c > j - 1000.0) {
+                sum = -uint64_t(__double_as_longlong(0x1p52)) * uint64_t(8 * PIECES);
 #pragma unroll
                 for (int u = 0; u < PIECES; ++u)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sum += bits(__builtin_amdgcn_fmed3f(v[u][e], least, kMost));
+                    for (int e = 0; e < 8; ++e) {
+                        int o;
+                        double x;
+                        sum += uint64_t(__double_as_longlong(mass_sum(__builtin_amdgcn_fmed3f(v[u][e], least, kMost), k, o, x)));
+                    }
             } else {
+                sum = 0;
 #pragma unroll
                 for (int u = 0; u < PIECES; ++u)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sum += v[u][e] >= least ? bits(v[u][e]) : none;
+                    for (int e = 0; e < 8; ++e) {
+                        uint64_t m;
+                        const int bin = bin_mass(v[u][e], k, m);
+                        sum += bin >= 0 && v[u][e] >= least ? m : 0;
+                    }
             }
         }
         sum = wave_sum_u64(sum);
@@ -740,7 +744,10 @@ __device__ __forceinline__ void draw_column(const SampleArgs& a, int row, const 
         if (lane == 63) sh.wave_mass[wv] = run;
         __syncthreads();
         uint64_t all;
-        return run + waves_before(sh.wave_mass, all);
+        const uint64_t before = waves_before(sh.wave_mass, all);
+        // (logits that changed under the call: no column is past u S)
+        if (tid == 0 && row_mass(all, shift) <= rest) give(a, row, -1, __builtin_nanf(""));
+        return run + before;
     };
     const int per = int(kept + kRowThreads - 1) / kRowThreads;
     if (per <= kPer / 2) {
@@ -877,6 +884,7 @@ __device__ __forceinline__ void finish_small(const SampleArgs& a, int row, const
     }
     walk([&](int, int i) { return col_mass[i]; });
     const uint64_t total = readlane_u64(m[per - 1], 63), target = __umul64hi(fraction(s.u), total);
+    if (tid == 0 && !total) give(a, row, -1, __builtin_nanf(""));      // (logits that changed under the call)
 #pragma unroll
     for (int i = 0; i < per; ++i) {
         if (per * tid + i < n && m[i] > target && m[i] - col_mass[i] <= target) {
