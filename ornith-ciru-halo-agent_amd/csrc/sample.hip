@@ -581,17 +581,32 @@ __device__ __forceinline__ void borders(const SampleArgs& a, const Setting& s, f
             }
         } else if (tid == 0) sh.hi = sh.lo = cm[0];
     }
-    // min-p's least value: the estimate mx + T ln q is off by less than a step of fp32 there, so the
-    // 64 values around it hold the border
+    // min-p's least value: mostly among the 64 keys around the estimate mx + T ln q.  Where those two nearly
+    // cancel, the estimate is off by many steps of the small fp32 numbers there: then all 64 keys pass, or
+    // none, and the rest on that side is searched, 64 keys a round (the largest value passes).
     if (use_q && wv == kRowWaves - 1) {
         const uint32_t top = ordered(mx);
+        const double least_t = log2(double(s.q));
         const float at = float(double(mx) + double(s.T) * log(double(s.q)));
         const uint32_t mid = at == at ? ordered(at) : kMinusInf + 1;
-        const uint32_t k0 = max(min(mid, top), kMinusInf + 33) - 32 + lane;
-        const float v = unordered(k0);
-        const bool in = k0 <= top && (v == mx || (double(v) - double(mx)) * s.c >= log2(double(s.q)));
-        const uint64_t b = __builtin_amdgcn_ballot_w64(in);
-        if (lane == 0) sh.qkey = b ? k0 + uint32_t(__builtin_ctzll(b)) : top;
+        auto passing = [&](uint32_t key) {
+            const float v = unordered(key);
+            return __builtin_amdgcn_ballot_w64(key >= top || v == mx || (double(v) - double(mx)) * s.c >= least_t);
+        };
+        uint32_t lo = kMinusInf + 1, hi = top;         // the least that passes lies in [lo, hi]
+        const uint32_t first = max(min(mid, top), kMinusInf + 33) - 32;
+        const uint64_t near = passing(first + lane);
+        const uint32_t from = first + (near ? uint32_t(__builtin_ctzll(near)) : 64u);
+        if (near) hi = min(from, top);
+        if (from > first) lo = min(from, top);
+        while (lo < hi) {
+            const uint32_t step = (hi - lo + 63) / 64;
+            const uint64_t b = passing(min(lo + step * lane, hi));
+            const uint32_t i = b ? uint32_t(__builtin_ctzll(b)) : 64u;
+            if (b) hi = min(lo + step * i, hi);
+            if (i) lo = min(lo + step * (i - 1) + 1, hi);
+        }
+        if (lane == 0) sh.qkey = hi;
     }
     __syncthreads();
     // the bins that top-p's border can lie in
