@@ -127,6 +127,7 @@ class W4LinearMethod:
                                  layer.w4_zeros.data if self.zeros else None, self.group)
         for name in storage.w4_shapes(self.n, self.k, self.group, self.zeros):
             delattr(layer, name)
+        layer._ornith_loader.release()
         for name, bank in zip(('w4_bank', 'w4_metadata'), packed):
             layer.register_buffer(name, bank, persistent=False)
 

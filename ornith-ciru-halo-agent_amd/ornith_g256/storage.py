@@ -106,6 +106,12 @@ class BankLoader:
         self.sealed = True
         return self.loaded
 
+    def release(self):
+        """Forgets the loaded tensors, once another form of them is the bank."""
+        if not self.sealed:
+            raise AdmissionError('banks not sealed')
+        self.loaded = {}
+
 
 def repack_n32(codes16: torch.Tensor, meta16: torch.Tensor, n: int, k: int):
     """N16 banks (on the GPU) -> new N32 tensors [..., N/32, K/256, 32, 32] and
