@@ -43,3 +43,32 @@ def test_packing_drops_the_loaded_fields(monkeypatch, zeros):
     assert not list(layer.parameters()) and {n for n, _ in layer.named_buffers()} == {'w4_bank', 'w4_metadata'}
     with pytest.raises(storage.AdmissionError):           # still sealed
         layer.load_packed('w4_codes', torch.zeros(48, 8, dtype=torch.int32).view(torch.uint32))
+
+
+def _bound(**kw):
+    layer = _Layer(**kw)
+    layer.w4_bank = layer.w4_metadata = None
+    method = layer.quant_method
+    method.runtime, method.slot = type('Runtime', (), dict(slots=(torch.zeros(1, dtype=torch.int32),))), 0
+    return layer
+
+
+@pytest.mark.parametrize('lead,shape,strides', [(0, (3, 64), (64, 1)), (1, (3, 64), (64, 1)), (4, (1, 64), (64, 1)),
+                                                (7, (2, 3, 64), (192, 64, 1)), (0, (3, 64), (68, 1)), (8, (3, 64), (72, 1)),
+                                                (0, (5, 64), (1, 5)), (0, (3, 64), (0, 1)), (3, (0, 64), (64, 1))])
+def test_rows_off_the_grid_are_copied(monkeypatch, lead, shape, strides):
+    """The launch takes rows on the 16-byte grid; a contiguous view may start off
+    it, where contiguous() copies nothing."""
+    calls = []
+    monkeypatch.setattr(methods.native, 'w4_out', lambda x, *a: calls.append(x))
+    layer = _bound()
+    buf = torch.arange(4096, dtype=torch.float32).to(torch.bfloat16)
+    assert buf.data_ptr() % 16 == 0
+    x = buf[lead:].as_strided(shape, strides)
+    out = layer.quant_method.apply(layer, x)
+    (rows,), want = calls, x.reshape(-1, 64)
+    assert out.shape == (*shape[:-1], 48) and torch.equal(rows, want)
+    if want.numel():
+        assert rows.data_ptr() % 16 == 0 and rows.stride(1) == 1 and rows.stride(0) % 8 == 0
+        # rows that are on it are not
+        assert (rows.data_ptr() == x.data_ptr()) == (lead % 8 == 0 and strides[-1] == 1 and strides[-2] % 8 == 0 and strides[-2] >= 64)
