@@ -136,8 +136,8 @@ class W4LinearMethod:
             raise RuntimeError(f'{self.prefix}: needs packed weights, no bias and a bound runtime')
         shape = x.shape[:-1]
         x = x.reshape(-1, self.k)
-        if x.stride(1) != 1 or x.stride(0) < self.k or x.stride(0) % 8 or x.data_ptr() % 16:
-            x = x.clone(memory_format=torch.contiguous_format)
+        if not native.traced():            # (the op does, on real rows)
+            x = native.w4_grid(x)
         out = torch.empty((x.shape[0], self.n), dtype=self.out_dtype or x.dtype, device=x.device)
         native.w4_out(x, layer.w4_bank, layer.w4_metadata, out, self.runtime.slots[self.slot], self.n, self.k, self.group)
         return out.view(*shape, self.n)

@@ -573,10 +573,22 @@ def logits_argmax(logits, out):
                                             ptr(out), stream(logits)), 'logits argmax')
 
 
+# (names bound once: 0.2 us a call)
+_compiling, _modes = torch.compiler.is_compiling, torch._C._len_torch_dispatch_stack
+
+
+def traced():
+    """Whether a compiler or a dispatch mode records this call.  Then the entries
+    that are plain calls (a torch op costs the host several times what they do)
+    go through their torch ops, which have fakes."""
+    return _compiling() or _modes() > 0
+
+
 def call_on(index, entry, operation, *args):
-    """A launch entry on GPU `index` (made current if it is not) and torch's current stream there.  The
-    stream's handle comes without a Stream object, which costs 2 us a call."""
-    if index == torch.cuda.current_device():
+    """A launch entry on GPU `index` (of a tensor, so CUDA is initialised; made current if it is not) and
+    torch's current stream there.  The stream's handle comes without a Stream object, which costs 2 us a
+    call, and the current device without the check for initialisation."""
+    if index == torch._C._cuda_getDevice():
         check(entry(*args, torch._C._cuda_getCurrentRawStream(index)), operation)
     else:
         with torch.cuda.device(index):
@@ -611,7 +623,13 @@ def logits_sample(logits, uniform, workspace, out, flags, temperature=None, top_
     temperature 0 is greedy.  logprob fp32 [M] (optional): the log of the
     probability the token was drawn with.  What each setting keeps, and the
     sticky flags (1 NaN logit, 2 setting out of range, 4 empty row; the last
-    two give token -1): include/ornith_sample.h."""
+    two give token -1): include/ornith_sample.h.  Traced, the op
+    ornith_g256::logits_sample."""
+    call = logits_sample_op if _compiling() or _modes() else _logits_sample
+    call(logits, uniform, workspace, out, flags, temperature, top_k, top_p, min_p, logprob)
+
+
+def _logits_sample(logits, uniform, workspace, out, flags, temperature, top_k, top_p, min_p, logprob):
     kind = LOGITS_TYPES.get(logits.dtype)
     if kind is None or logits.ndim != 2:
         raise ValueError('logits must be bf16, fp16 or fp32 [M, N] with unit column stride')
@@ -638,6 +656,19 @@ def logits_sample(logits, uniform, workspace, out, flags, temperature=None, top_
             flags.data_ptr())
 
 
+@torch.library.custom_op('ornith_g256::logits_sample', mutates_args={'workspace', 'out', 'flags', 'logprob'},
+                         device_types='cuda')
+def logits_sample_op(logits: torch.Tensor, uniform: torch.Tensor, workspace: torch.Tensor, out: torch.Tensor,
+                     flags: torch.Tensor, temperature: torch.Tensor | None, top_k: torch.Tensor | None,
+                     top_p: torch.Tensor | None, min_p: torch.Tensor | None, logprob: torch.Tensor | None) -> None:
+    _logits_sample(logits, uniform, workspace, out, flags, temperature, top_k, top_p, min_p, logprob)
+
+
+@logits_sample_op.register_fake
+def _(logits, uniform, workspace, out, flags, temperature, top_k, top_p, min_p, logprob):
+    return None
+
+
 W4_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -657,7 +688,21 @@ def w4_out(x, codes, metadata, out, flags, n, k, group):
     """Plain 4-bit linear: out [rows, n] (bf16, fp16 or fp32) = x [rows, k]
     (bf16 or fp16, as it is) times the banks of storage.pack_w4.  Any number of
     rows (made for the few of a decode step).  Flags: 4 a non-finite sum, 8 a
-    non-finite 16-bit result."""
+    non-finite 16-bit result.  Traced, the op ornith_g256::w4_out, which copies
+    rows that w4_grid would."""
+    call = w4_op if _compiling() or _modes() else _w4_out
+    call(x, codes, metadata, out, flags, n, k, group)
+
+
+def w4_grid(x):
+    """x [rows, k] as w4_out takes it: unit column stride, rows that do not
+    overlap and start on the 16-byte grid; a copy if it is not that."""
+    if x.stride(1) != 1 or x.stride(0) < x.shape[1] or x.stride(0) % 8 or x.data_ptr() % 16:
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _w4_out(x, codes, metadata, out, flags, n, k, group):
     x_type, out_type = W4_TYPES.get(x.dtype, 2), W4_TYPES.get(out.dtype)
     if x_type > 1 or x.ndim != 2 or x.shape[1] != k:
         raise ValueError(f'input must be a bf16 or fp16 [rows, {k}] tensor, got {tuple(x.shape)} {x.dtype}')
@@ -688,6 +733,17 @@ def w4_out(x, codes, metadata, out, flags, n, k, group):
         raise ValueError('input, banks, output and flags must be on one GPU')
     call_on(gpu, lib().ornith_w4_launch, 'w4 linear', x_ptr, x_type, ldx, codes.data_ptr(), metadata.data_ptr(),
             out.data_ptr(), out_type, ldo, flags.data_ptr(), rows, n, k, group)
+
+
+@torch.library.custom_op('ornith_g256::w4_out', mutates_args={'out', 'flags'}, device_types='cuda')
+def w4_op(x: torch.Tensor, codes: torch.Tensor, metadata: torch.Tensor, out: torch.Tensor, flags: torch.Tensor,
+          n: int, k: int, group: int) -> None:
+    _w4_out(w4_grid(x) if x.ndim == 2 else x, codes, metadata, out, flags, n, k, group)
+
+
+@w4_op.register_fake
+def _(x, codes, metadata, out, flags, n, k, group):
+    return None
 
 
 def dense_head(x, codes, meta, workspace, logits, logits_bf16, argmax, flags, capacity):

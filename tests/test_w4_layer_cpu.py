@@ -72,3 +72,59 @@ def test_rows_off_the_grid_are_copied(monkeypatch, lead, shape, strides):
         assert rows.data_ptr() % 16 == 0 and rows.stride(1) == 1 and rows.stride(0) % 8 == 0
         # rows that are on it are not
         assert (rows.data_ptr() == x.data_ptr()) == (lead % 8 == 0 and strides[-1] == 1 and strides[-2] % 8 == 0 and strides[-2] >= 64)
+
+
+def _compiled(fn, result):
+    """fn under a full-graph compile whose graphs are kept and not run."""
+    graphs = []
+
+    def backend(graph, _):
+        graphs.append(graph)
+        return lambda *args: result
+    torch._dynamo.reset()
+    return torch.compile(fn, fullgraph=True, backend=backend), graphs
+
+
+def _targets(graph):
+    return [str(n.target) for n in graph.graph.nodes if n.op == 'call_function']
+
+
+def test_the_layer_compiles():
+    """As the G256 linears do: one op in the graph, no break."""
+    layer = _bound()
+    shapes = methods.native.w4_layout(48, 64, 128)
+    layer.w4_bank, layer.w4_metadata = (torch.zeros(s, dtype=torch.int32) for s in shapes)
+    run, graphs = _compiled(lambda x: layer.quant_method.apply(layer, x) * 2, (torch.zeros(3, 48),))
+    run(torch.zeros(3, 64, dtype=torch.bfloat16))
+    assert len(graphs) == 1 and 'ornith_g256.w4_out.default' in _targets(graphs[0])
+
+
+@pytest.mark.parametrize('settings', [{}, dict(top_k=torch.ones(3, dtype=torch.int32)),
+                                      dict(temperature=torch.ones(3), top_p=torch.ones(3), min_p=torch.zeros(3))])
+def test_the_heads_sampler_compiles(settings):
+    head = methods.W8HeadMethod('head')
+    layer = torch.nn.Module()
+    layer._ornith_loader = type('Loader', (), dict(sealed=True))
+    layer.head_tilebank_codes = layer.head_scales = torch.zeros(1, dtype=torch.int32)
+    head.runtime = type('Runtime', (), dict(slots=(torch.zeros(1, dtype=torch.int32),), head_geometry=2,
+                                            workspace=torch.zeros(16, dtype=torch.uint8)))
+    head.slot = 0
+    run, graphs = _compiled(lambda x, u: head.sample(layer, x, u, **settings),
+                            (torch.zeros(3, dtype=torch.int64), torch.zeros(3)))
+    run(torch.zeros(3, 2048, dtype=torch.bfloat16), torch.zeros(3))
+    names = _targets(graphs[0])
+    assert len(graphs) == 1
+    assert names.index('ornith_g256.head_out.default') < names.index('ornith_g256.logits_sample.default')
+
+
+def test_dispatch_modes_see_the_ops():
+    """Tracers that are not the compiler: fake tensors through the plain entries."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from ornith_g256 import native
+    with FakeTensorMode():
+        flags = torch.zeros(1, dtype=torch.int32)
+        out = torch.empty(2, 48, dtype=torch.float32)
+        shapes = native.w4_layout(48, 64, 128)
+        native.w4_out(torch.zeros(2, 64, dtype=torch.bfloat16), *(torch.zeros(s, dtype=torch.int32) for s in shapes), out,
+                      flags, 48, 64, 128)
+        native.logits_sample(out, torch.zeros(2), torch.zeros(0, dtype=torch.uint8), torch.zeros(2, dtype=torch.int64), flags)
