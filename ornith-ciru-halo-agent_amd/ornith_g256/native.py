@@ -256,7 +256,7 @@ def configure(settings, capacity, shapes, shared_expert=False):
         # the GEMM's bf16(H128 x), rows padded to 16, then its split-K slice sums
         sizes.append((int(capacity) + 15) // 16 * 16 * k * 2 + DENSE_SLICE_BYTES)
     sizes.append(head_layout(HEAD_MAX_ROWS, HEAD_VOCAB, tile=roles['head']).workspace_bytes)
-    sizes.append(logits_sample_bytes(HEAD_MAX_ROWS, HEAD_VOCAB))
+    sizes.append(logits_sample_bytes(HEAD_MAX_ROWS, HEAD_VOCAB, tile=roles['head']))
     if shared_expert:
         # the fused ninth slot (at most 16 rows, any routed build) and fixed8
         for tile in {roles['routed'], 32}:
@@ -608,10 +608,10 @@ def _row_ptr(t, name, dtype, shape, like):
 LOGITS_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def logits_sample_bytes(capacity, n):
+def logits_sample_bytes(capacity, n, tile=32):
     """Workspace bytes of logits_sample for up to `capacity` rows of n columns."""
     size = _SZ(0)
-    check(lib().ornith_logits_sample_get_layout(capacity, n, C.byref(size)), f'sampling layout for {capacity} x {n}')
+    check(lib(tile).ornith_logits_sample_get_layout(capacity, n, C.byref(size)), f'sampling layout for {capacity} x {n}')
     return size.value
 
 
