@@ -8,8 +8,10 @@
  * with codes c and zero points z in 0..15, groups of G = 32, 64, 128 or 256
  * consecutive k (the last may be short), rows x bf16 or fp16, products and
  * sums in fp32 (each x * c product is exact), one rounding to the output's
- * type.  Rows below 2^120 in magnitude cannot overflow on the way.  A row's
- * result depends on no other row. */
+ * type.  Over 128 k the kernels sum x (16 + c), up to 31 * 128 |x|: rows below
+ * 2^116 in magnitude cannot overflow inside a group; of larger bf16 rows a
+ * finite result may come out as NaN (flag 4).  A row's result depends on no
+ * other row. */
 #ifndef ORNITH_MI355X_W4_H
 #define ORNITH_MI355X_W4_H
 #include <stddef.h>
