@@ -10,8 +10,12 @@
  * sums in fp32 (each x * c product is exact), one rounding to the output's
  * type.  Over 128 k the kernels sum x (16 + c), up to 31 * 128 |x|: rows below
  * 2^116 in magnitude cannot overflow inside a group; of larger bf16 rows a
- * finite result may come out as NaN (flag 4).  A row's result depends on no
- * other row. */
+ * finite result may come out as NaN (flag 4).  The other half, (16 + z) times
+ * the group's sum of x, is subtracted, so the error before the last rounding is
+ * absolute: below (139 + K/128) 2^-23 * 32 sum |s x| (seen: below 2^-25 * 32 sum
+ * |s x|), also of columns whose codes are their zero points, where the result
+ * is not always 0.  A row's result depends on no other row's values; the order of
+ * its sums goes by the numbers of rows and columns. */
 #ifndef ORNITH_MI355X_W4_H
 #define ORNITH_MI355X_W4_H
 #include <stddef.h>
