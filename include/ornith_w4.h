@@ -54,7 +54,8 @@ ORNITH_EXPORT hipError_t ornith_w4_pack(const void* codes_u32, const void* scale
  * fp16; stride ldx >= K).  x and ldx on the 16-byte grid; out aligned to its
  * element; packed codes 16 bytes, meta 4.  Any number of rows; made for the few
  * of a decode step.
- * Flags (sticky): 4 a non-finite sum, 8 a non-finite stored value.  M, N == 0
+ * Flags (sticky): 4 a non-finite sum, 8 a non-finite 16-bit result (fp32 ones
+ * raise 4 alone).  M, N == 0
  * return hipSuccess without touching memory; K == 0 gives zeros. */
 ORNITH_EXPORT hipError_t ornith_w4_launch(const void* x, int x_type, int64_t ldx, const void* packed_codes,
                                           const void* packed_meta, void* out, int out_type, int64_t ldo,
