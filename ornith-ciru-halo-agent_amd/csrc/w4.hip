@@ -451,30 +451,41 @@ template <int TYPE, int NT, int W> hipError_t w4_tiles(const W4Args& a, hipStrea
     else go(w4_tile_kernel<TYPE, 1, NT, W>);
     return hipGetLastError();
 }
-// Which kernel (us a call, bf16, group 128, calls in a graph over banks of 600 MB in turn or 24, K = 2048
-// but where another is given):
+// Which kernel, by the tiles of 16 x 16 results (us a call, bf16 results, calls in a graph over banks of
+// 600 MB in turn or 24; K = 2048 and groups of 128 where nothing else is said):
 //  - Tiles of a block.  One keeps more blocks than CUs where tiles are few; more read x, which comes from
-//    L2 for every block, less often.  1 / 2 / 4 tiles: 6144 columns, 1 row 4.3 / 4.5 / 5.6, 8 rows 5.1 /
-//    4.9 / 5.9, 16 rows 6.9 / 5.2 / 6.3, 64 rows 14.8 / 10.1 / 9.4; 24576 columns, 1 row 9.6 / 8.3 / 8.8,
-//    8 rows 10.4 / 8.3 / 9.5, 16 rows 14.9 / 10.6 / 10.5; 151936 columns, 1 row 42.8 / 32.3 / 32.5,
-//    8 rows 52.0 / 37.9 / 34.6.  2048 columns, K = 4096, 32 rows 6.7 / 7.0 / 9.3, 64 rows 10.7 / 7.1 / 9.2.
-//  - 16 waves where a wave of 8 would take three 128-k blocks or more in turn, or tiles are few: 8 / 16
-//    waves, 1 row, 2048 columns, K = 4096 5.1 / 4.2, K = 8192 8.6 / 6.4; 1024 columns 3.5 / 3.2; but 12288
-//    columns 6.4 / 6.7 and 16 rows of K = 8192 10.3 / 10.7.
-//  - x in LDS for more than 16 rows of many columns (4 tiles / in LDS): 24576 columns, 32 rows 14.2 / 14.2,
-//    64 rows 25.2 / 17.9; 12288 columns of groups of 32, 64 rows 15.9 / 16.5; 151936 columns, 32 rows
-//    70.6 / 41.9, 64 rows 137 / 68.5 (two passes over the weights: 32 rows are what LDS holds).
+//    L2 for every block, less often.  1 / 2 / 4 tiles: 6144 columns, 1 row 4.6 / 4.6 / 5.9, 8 rows 5.4 / 4.9 /
+//    6.2, 16 rows 7.1 / 5.3 / 6.4, 64 rows 14.9 / 10.3 / 9.6; 12288 columns, 16 rows 8.8 / 7.8 / 6.7; 24576
+//    columns, 1 row 10.1 / 8.6 / 9.6, 8 rows 11.2 / 9.3 / 9.9; 151936 columns, 1 row 48.2 / 40.0 / 33.4, 8 rows
+//    59.2 / 43.5 / 35.8.  Two from 384 on where a wave's blocks are many, for few rows too: 6144 columns, 1 row,
+//    K = 2944 5.8 / 5.6 / -, K = 4096 7.0 / 6.4 / 8.7, K = 8192 11.2 / 10.0 / -.
+//  - Four tiles of groups of 32 and 64 (with their scales 134 to 138 registers: one block a CU) only while each
+//    block has a CU: 2 / 4 tiles, groups of 32, 16 rows of 16384 columns 8.7 / 8.5, 18432 10.9 / 13.8, 32 rows of 8192
+//    8.5 / 7.8, 12288 11.3 / 13.6; 151936 columns, 1 row 44.2 / 58.7; of 64 41.8 / 51.9.
+//  - 16 waves where a wave of 8 would take two 128-k blocks or more in turn and each block has a CU: 8 / 16
+//    waves, 1 row, 1024 columns 3.5 / 3.2, 4096 3.9 / 3.7, K = 4096 5.6 / 4.7, 4608 of K = 4096 6.6 / 7.4; 2048
+//    columns of K = 8192 8.5 / 6.6, 8 rows 8.9 / 7.8, 16 rows 10.5 / 10.9; K = 512 2.6 / 2.7.
+//  - x in LDS for more than 16 rows of many columns.  4 tiles / in LDS: 32 rows, 22528 columns 14.2 / 14.4, 24000
+//    14.8 / 14.6, 24576 14.8 / 14.8, 28672 17.6 / 15.8, of groups of 32 27.0 / 20.1, 24576 of K = 1024 9.9 / 10.0;
+//    151936 73.5 / 42.2, 64 rows 144 / 73.5 (two passes over the weights: 32 rows are what LDS holds).  With three
+//    or four tiles of rows (K up to 1280 and 1024) later: K = 1024, 64 rows, 12288 columns 9.2 / 12.1, 16384 11.8 /
+//    12.5, 18432 13.7 / 13.6, 32768 20.7 / 15.6; 48 rows of 16384 9.5 / 10.7, 24576 14.1 / 12.2; but not of groups
+//    of 32 and 64 (2 tiles / in LDS: groups of 32, 64 rows, 12288 columns 13.9 / 14.7, 16384 17.2 / 14.9, 48 rows
+//    of 16384 13.8 / 12.3).
 template <int TYPE> hipError_t w4_rows(const W4Args& a, hipStream_t s) {
     const int64_t cells = int64_t((a.N + 15) / 16) * ((a.M + 15) / 16);      // tiles of 16 x 16 results
     const int blocks = w4_blocks(a.K);
-    if (a.M > 16 && cells > 3000) {
-        if (a.M > 48 && w4_x_bytes(4, a.K) <= kW4XBytes) return w4_run<TYPE, 4, 8, 4>(a, s);
-        if (a.M > 32 && w4_x_bytes(3, a.K) <= kW4XBytes) return w4_run<TYPE, 3, 8, 4>(a, s);
-        if (w4_x_bytes(2, a.K) <= kW4XBytes) return w4_run<TYPE, 2, 12, 3>(a, s);
+    const bool small_groups = a.log2g < 7;
+    auto fits = [&](int MT) { return a.M > 16 * (MT - 1) && w4_x_bytes(MT, a.K) <= kW4XBytes; };
+    const int MT = fits(4) ? 4 : fits(3) ? 3 : fits(2) ? 2 : 0;
+    if (MT && cells > (MT == 2 || small_groups ? 3000 : 4096)) {
+        if (MT == 4) return w4_run<TYPE, 4, 8, 4>(a, s);
+        if (MT == 3) return w4_run<TYPE, 3, 8, 4>(a, s);
+        return w4_run<TYPE, 2, 12, 3>(a, s);
     }
-    if (cells >= (a.M <= 8 ? 4096 : 768)) return w4_tiles<TYPE, 4, 8>(a, s);
-    if (cells >= (a.M <= 4 ? 1536 : 384)) return w4_tiles<TYPE, 2, 8>(a, s);
-    if (a.M <= 8 && (blocks >= 24 || (blocks > 8 && cells <= 128))) return w4_tiles<TYPE, 1, 16>(a, s);
+    if (cells >= (a.M <= 8 ? 4096 : 768) && (!small_groups || cells <= 1024)) return w4_tiles<TYPE, 4, 8>(a, s);
+    if (cells >= (a.M <= 4 && blocks <= 16 ? 1536 : 384)) return w4_tiles<TYPE, 2, 8>(a, s);
+    if (a.M <= 8 && blocks > 8 && cells <= 256) return w4_tiles<TYPE, 1, 16>(a, s);
     return w4_tiles<TYPE, 1, 8>(a, s);
 }
 
