@@ -135,7 +135,9 @@ __host__ __device__ inline int w4_blocks(int K) { return (K + kW4Block - 1) / kW
 // halves, as the products are added per 128 k), [group, 16 MT].
 // W waves of a block, D units' codes of a wave in flight: 12 and 3 for two tiles of rows (151936 x 2048, 32
 // rows, fp32 results, us: 43.2; 16 waves and 2 units 45.1, 8 and 3 44.3, 8 and 4 45.3, 8 and 6 45.1); 8
-// and 4 for more, whose sums and parked parts take 64 registers a tile pair.
+// and 4 for more, whose sums and parked parts take 64 registers a tile pair.  One unit less for groups of 32,
+// whose scales take four times the registers (32 rows: 151936 x 2048 51.6, spilling 4 registers with 3 units
+// 53.1; 24576 x 2048 16.4 / 18.0; 64 rows of 32768 x 1024 18.3 / 19.5).
 constexpr size_t kW4XBytes = 128 * 1024;               // x of a block, at most
 constexpr size_t w4_x_bytes(int MT, int K) { return size_t(16 * MT) * ((K + kW4Block - 1) / kW4Block) * (2 * kW4Block); }
 
@@ -438,7 +440,7 @@ template <int TYPE, int MT, int W, int D> hipError_t w4_run(const W4Args& a, hip
     const int pairs = (a.N + 31) / 32, rows = (a.M + 16 * MT - 1) / (16 * MT);
     const dim3 grid(std::min(pairs, std::max(device_cu_count() / rows, 1)), rows);
     auto go = [&](auto kernel) { timed_launch("w4_run", kernel, grid, dim3(64 * W), uint32_t(lds), s, a); };
-    if (a.log2g == 5) go(w4_run_kernel<TYPE, MT, 4, W, D>);
+    if (a.log2g == 5) go(w4_run_kernel<TYPE, MT, 4, W, D - 1>);
     else if (a.log2g == 6) go(w4_run_kernel<TYPE, MT, 2, W, D>);
     else go(w4_run_kernel<TYPE, MT, 1, W, D>);
     return hipGetLastError();
@@ -466,12 +468,12 @@ template <int TYPE, int NT, int W> hipError_t w4_tiles(const W4Args& a, hipStrea
 //    waves, 1 row, 1024 columns 3.5 / 3.2, 4096 3.9 / 3.7, K = 4096 5.6 / 4.7, 4608 of K = 4096 6.6 / 7.4; 2048
 //    columns of K = 8192 8.5 / 6.6, 8 rows 8.9 / 7.8, 16 rows 10.5 / 10.9; K = 512 2.6 / 2.7.
 //  - x in LDS for more than 16 rows of many columns.  4 tiles / in LDS: 32 rows, 22528 columns 14.2 / 14.4, 24000
-//    14.8 / 14.6, 24576 14.8 / 14.8, 28672 17.6 / 15.8, of groups of 32 27.0 / 20.1, 24576 of K = 1024 9.9 / 10.0;
+//    14.8 / 14.6, 24576 14.8 / 14.8, 28672 17.6 / 15.8, of groups of 32 27.0 / 18.3, 24576 of K = 1024 9.9 / 10.0;
 //    151936 73.5 / 42.2, 64 rows 144 / 73.5 (two passes over the weights: 32 rows are what LDS holds).  With three
 //    or four tiles of rows (K up to 1280 and 1024) later: K = 1024, 64 rows, 12288 columns 9.2 / 12.1, 16384 11.8 /
 //    12.5, 18432 13.7 / 13.6, 32768 20.7 / 15.6; 48 rows of 16384 9.5 / 10.7, 24576 14.1 / 12.2; but not of groups
-//    of 32 and 64 (2 tiles / in LDS: groups of 32, 64 rows, 12288 columns 13.9 / 14.7, 16384 17.2 / 14.9, 48 rows
-//    of 16384 13.8 / 12.3).
+//    of 32 and 64 (2 tiles / in LDS: groups of 32, 64 rows, 12288 columns 13.9 / 14.2, 16384 17.2 / 14.5, 48 rows
+//    of 16384 13.8 / 12.1).
 template <int TYPE> hipError_t w4_rows(const W4Args& a, hipStream_t s) {
     const int64_t cells = int64_t((a.N + 15) / 16) * ((a.M + 15) / 16);      // tiles of 16 x 16 results
     const int blocks = w4_blocks(a.K);
