@@ -12,7 +12,8 @@
  *     those with e_i >= q;
  *   - token = the first column, in ascending order, up to which the kept mass
  *     exceeds u times the kept mass S;  logprob = ln(e_token / S).
- * T == 0 is greedy (the first maximum, logprob 0; k, p, q and u do not matter).
+ * T == 0 is greedy (the first maximum, logprob 0; k, p, q and u do not matter,
+ * in range or not).
  * Masses are whole numbers: units of 2^-36 of the power of two above the
  * largest of their 8192-column part, so results depend on no order of
  * additions and on no other row.  A token whose mass is below 2^-37 of its
