@@ -28,3 +28,10 @@ def test_many_columns(device, group, M, N, K):
                                    (17, 8192, 2056), (64, 2048, 4104)])
 def test_tiles(device, group, M, N, K):
     G.test_w4_whole_numbers(device, ('bf16', 'fp16')[(N // 16 + group // 32) % 2], group, M, N, K)
+
+
+# the rows of a prompt: many passes over the columns, and more of them than a grid's other axis has blocks for
+@pytest.mark.parametrize('group', [32, 128])
+@pytest.mark.parametrize('M,N,K', [(700, 1000, 520), (2100, 130, 264), (513, 2050, 2056), (16500, 60, 264), (9000, 17, 1544)])
+def test_prompt_rows(device, group, M, N, K):
+    G.test_w4_whole_numbers(device, 'bf16', group, M, N, K)
