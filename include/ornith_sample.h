@@ -14,9 +14,9 @@
  *     exceeds u times the kept mass S;  logprob = ln(e_token / S).
  * T == 0 is greedy (the first maximum, logprob 0; k, p, q and u do not matter,
  * in range or not).
- * Masses are whole numbers: units of 2^-36 of the power of two above the
- * largest of their 8192-column part, so results depend on no order of
- * additions and on no other row.  A token whose mass is below 2^-37 of its
+ * Masses are computed to 2^-33 of themselves and rounded to whole numbers of
+ * units of 2^-36 of the power of two above the largest of their 8192-column
+ * part, so results depend on no order of additions and on no other row.  A token whose mass is below 2^-37 of its
  * part's largest is never drawn.
  *
  * Per-row settings are device memory, [M] each, a NULL pointer meaning off
@@ -48,7 +48,8 @@ ORNITH_EXPORT hipError_t ornith_logits_sample_get_layout(int Mcap, int N, size_t
 /* logits of logits_type [M, N], row stride ld >= N elements, aligned to their
  * element; uniform, temperature, top_p, min_p fp32 [M]; top_k int32 [M];
  * token int64 [M]; logprob fp32 [M] (nullable); flags uint32 [1].  Workspace
- * 256-byte aligned, private to the call until it has finished.  M == 0 returns
+ * 256-byte aligned memory of the stream's device (its blocks meet there through
+ * device atomics), private to the call until it has finished.  M == 0 returns
  * hipSuccess without touching memory; N == 0 gives every row token -1. */
 ORNITH_EXPORT hipError_t ornith_logits_sample_launch(
     const void* logits, int logits_type, int M, int N, int64_t ld, const void* uniform_f32,

@@ -17,14 +17,14 @@
 // Rows of one part do all of it in one block and one launch (sample_row).  Calls of few parts do the
 // last three steps in one launch (sample_rest), whose last block to list its entries ends the row.
 //
-// What bounds it.  The floor is one pass over the logits (64 rows of 248320 bf16: 31.8 MB, 6.6 us at the
-// rate of a large copy).  `parts` takes 15.4 us there: 10.9 to load and find the maxima, the rest fp64
+// What bounds it.  The floor is one pass over the logits (64 rows of 248320 bf16: 31.8 MB, 6.0 us at the
+// 5.3 TB/s of a large copy).  `parts` takes 16.7 us there: 10.9 to load and find the maxima, the rest fp64
 // for the masses (a dozen instructions a value, 7 to 8 clocks each a wave); top-p's histogram costs 9 us
 // of LDS additions and bins more.  Everything behind it works on bins and lists and is a chain of launches and
-// round trips: a whole row is drawn in 6.9 us, borders take 6 to 7, the list 8 to 9, its end 5 (few
+// round trips: a whole row is drawn in 7.0 us, borders take 6 to 7, the list 8 to 9, its end 5 (few
 // candidates) to 19 (2800 entries a row).  Calls in a graph over six inputs in turn: 1 row of top-k and
-// top-p 15.7 us, 8 rows of 151936 fp32 with top-p 25.1, 64 rows of mixed settings 46, 64 uncut 23.0, 256
-// rows of 4096 columns 17.1.
+// top-p 15.7 us, 8 rows of 151936 fp32 with top-p 25.3, 64 rows of mixed settings 46, 64 uncut 22 to 23.5,
+// 256 rows of 4096 columns 17.2.
 //
 // Masses.  With c = log2(e) / T and t = l c in fp64, e = 2^(t - j) for the
 // whole number j = ceil(max t) of its part: a degree-7 polynomial in t - rint(t)
@@ -470,7 +470,7 @@ __device__ __forceinline__ PartMeta part_pass(const SampleArgs& a, const Setting
 }
 
 // A block per part, the values in registers, loaded once.  256 threads (four pieces each) where parts are
-// many: 64 rows of 248320 bf16 15.4 us, where 512 and 1024 threads were slower (in an earlier form of the
+// many: 64 rows of 248320 bf16 16.7 us, where 512 and 1024 threads were slower (in an earlier form of the
 // masses 22 / 24 / 30 us: more waves meet at each barrier).  1024 where every part has a CU of its own and the
 // chain of one thread counts: 8 rows of 151936 fp32 5.6 us, with 256 threads 8.0.  Tried and slower: blocks
 // that stay and load a part ahead (27 us against 22), 64 VGPRs a thread forced by launch bounds (spills).
@@ -1489,9 +1489,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_rest_kernel(SampleArgs a, 
     finish_row<TYPE, true>(a, slot, row, s, sh.plan.mode == kModeWalk ? 0 : int(min(listed, uint32_t(a.list_max))), ahead0, sh, un);
 }
 
-// Rows of one part: all of it by one block, the logits in LDS after the histogram.  One block a CU (78 KB
-// of LDS, 1024 threads), so bound by the chain of its steps: 256 rows of 4096 bf16 17.2 us with mixed
-// settings, 11.4 with top-k of 20 to 50.
+// Rows of one part: all of it by one block, the logits in LDS after the histogram.  One block a CU (its
+// registers, 76 to 80 where two blocks of 1024 threads would need 64; LDS, 78 KB, would hold two), so bound
+// by the chain of its steps: 256 rows of 4096 bf16 17.2 us with mixed settings, 11.4 with top-k of 20 to 50.
 template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a, int row0) {
     const int row = row0 + int(blockIdx.x), tid = threadIdx.x;

@@ -12,10 +12,10 @@
 // waves in ascending order.
 //
 // Bound by the codes' stream where it is long (151936 x 2048, 32 rows, fp32
-// results: 41.7 us, 180 MB, 4.3 TB/s; the steady part streams 7 TB/s, the rest
-// is x to LDS, 5 us, and the last wave's end), and by launch and the round trips
-// of one wave where it is short (6144 x 2048, 1 row: 4.3 us against 1.2 at
-// 5.5 TB/s).  Codes lie so that a lane's 16 bytes are its column's share of four
+// results: 41.7 us, 181 MB, 4.3 TB/s of the 5.3 that a large copy reaches; of
+// the rest x to LDS takes 5 us, and the last wave's end), and by launch and the
+// round trips of one wave where it is short (6144 x 2048, 1 row: 4.5 us against
+// 1.2 at that rate).  Codes lie so that a lane's 16 bytes are its column's share of four
 // matrix steps: 1 KB contiguous a wave and load.
 #include <algorithm>
 #include <type_traits>
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(64 * W) void w4_tile_kernel(W4Args a) {
             if (k + 8 * q < a.K) next_xa[j] = *reinterpret_cast<const u32x4*>(x + k);
         }
     };
-    // one block ahead (151936 x 2048, 1 row 34.0 -> 31.6 us; short ones as before; 2 to 4 ahead 50)
+    // one block ahead (151936 x 2048, 1 row: 2.4 us less; short ones as before; 2 to 4 ahead 16 more)
     if (wv < blocks) load(wv);
     for (int kb = wv; kb < blocks; kb += W) {
         u32x4 cw[NT], xa[4];
@@ -467,7 +467,8 @@ template <int TYPE, int NT, int W> hipError_t w4_tiles(const W4Args& a, hipStrea
 //  - 16 waves where a wave of 8 would take two 128-k blocks or more in turn and each block has a CU: 8 / 16
 //    waves, 1 row, 1024 columns 3.5 / 3.2, 4096 3.9 / 3.7, K = 4096 5.6 / 4.7, 4608 of K = 4096 6.6 / 7.4; 2048
 //    columns of K = 8192 8.5 / 6.6, 8 rows 8.9 / 7.8, 16 rows 10.5 / 10.9; K = 512 2.6 / 2.7.
-//  - x in LDS for more than 16 rows of many columns.  4 tiles / in LDS: 32 rows, 22528 columns 14.2 / 14.4, 24000
+//  - x in LDS, which holds that of 32 rows up to K = 2048 (beyond, the tiles read all codes once per 16 rows:
+//    24576 columns of K = 4096, 32 rows 24.6, 64 rows 46.8), for more than 16 rows of many columns.  4 tiles / in LDS: 32 rows, 22528 columns 14.2 / 14.4, 24000
 //    14.8 / 14.6, 24576 14.8 / 14.8, 28672 17.6 / 15.8, of groups of 32 27.0 / 18.3, 24576 of K = 1024 9.9 / 10.0;
 //    151936 73.5 / 42.2, 64 rows 144 / 73.5 (two passes over the weights: 32 rows are what LDS holds).  With three
 //    or four tiles of rows (K up to 1280 and 1024) later: K = 1024, 64 rows, 12288 columns 9.2 / 12.1, 16384 11.8 /
