@@ -61,3 +61,24 @@ def test_compiled_layer(device):
     assert off.data_ptr() % 16 != 0
     want = layer.quant_method.apply(layer, off.clone())
     assert torch.equal(layer.quant_method.apply(layer, off), want) and torch.equal(compiled(off), torch.relu(want))
+
+
+def test_compiled_without_optional_results(device):
+    """No logprob and no settings: nothing optional among what the op writes."""
+    import torch
+    from ornith_g256 import native
+    rng = np.random.default_rng(3)
+    logits = torch.from_numpy(rng.standard_normal((3, 9000)).astype(np.float32)).to(device)
+    uniform = torch.rand(3, device=device)
+    flags = torch.zeros(1, dtype=torch.int32, device=device)
+    workspace = torch.empty(native.logits_sample_bytes(3, 9000), dtype=torch.uint8, device=device)
+
+    def run(logits, uniform, workspace, flags):
+        token = torch.empty(logits.shape[0], dtype=torch.int64, device=logits.device)
+        native.logits_sample(logits * 2, uniform, workspace, token, flags)
+        return token + 1
+    torch._dynamo.reset()
+    for backend in ('eager', 'aot_eager'):
+        compiled = torch.compile(run, fullgraph=True, backend=backend)
+        assert torch.equal(compiled(logits, uniform, workspace, flags), run(logits, uniform, workspace, flags))
+    assert int(flags) == 0
