@@ -10,6 +10,7 @@ projections and experts, as a serving program calls it.
 
 The plain forms are the definitions in elementary torch operations.
 """
+import functools
 import math
 import sys
 from pathlib import Path
@@ -102,7 +103,9 @@ def _gen(seed, part):
     return gen
 
 
+@functools.cache
 def _library():
+    """The package, found once, as a program imports it."""
     path = str(ROOT / 'ornith-ciru-halo-agent_amd')
     if path not in sys.path:
         sys.path.insert(0, path)
