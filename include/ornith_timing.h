@@ -32,6 +32,7 @@
  *                    sample_gather, sample_finish; sample_empty (no columns)
  *   plain 4-bit      w4_tile, w4_run (more than 16 rows of many columns),
  *                    w4_zero (no inputs), w4_pack_codes, w4_pack_meta
+ *   routing          route_experts
  *   shared expert    fixed8_act, fixed8_gate
  *   other            repack_codes, repack_meta, silu_selfcheck */
 #ifndef ORNITH_TIMING_H

@@ -115,6 +115,8 @@ _PROTOTYPES = {
     'ornith_w4_get_layout': ([_INT] * 3 + [C.POINTER(_SZ)] * 2, _INT),
     'ornith_w4_pack': ([_VP] * 2 + [_INT] + [_VP] * 4 + [_INT] * 3 + [_VP], _INT),
     'ornith_w4_launch': ([_VP, _INT, _I64] + [_VP] * 3 + [_INT, _I64, _VP] + [_INT] * 4 + [_VP], _INT),
+    # routing to experts (include/ornith_route.h)
+    'ornith_route_experts_launch': ([_VP] + [_INT] * 3 + [_I64, _VP] + [_INT] * 6 + [C.c_float] + [_VP] * 4, _INT),
     # measurement (include/ornith_timing.h)
     'ornith_mi355x_timing_arm': ([C.c_char_p, _INT], _INT),
     'ornith_mi355x_timing_read': ([C.c_char_p, C.POINTER(_INT), C.POINTER(C.c_double)], _INT),
@@ -743,6 +745,71 @@ def w4_op(x: torch.Tensor, codes: torch.Tensor, metadata: torch.Tensor, out: tor
 
 @w4_op.register_fake
 def _(x, codes, metadata, out, flags, n, k, group):
+    return None
+
+
+SCORES = {'softmax': 0, 'sigmoid': 1}
+
+
+def route_experts(logits, weights, ids, flags, score='softmax', bias=None, groups=1, kept_groups=1, group_top=1,
+                  renormalize=True, scale=1.0):
+    """Experts of each row of a gate's bf16, fp16 or fp32 logits [M, E]: the k
+    ids int32 [M, k] and weights fp32 [M, k], best first.  Scores are a
+    'softmax' or 'sigmoid' of the logits; bias (fp32 [E]) is added to them for
+    the pick alone; of `groups` groups of consecutive experts the `kept_groups`
+    stay whose `group_top` (1 or 2) best sum to the most; weights are the
+    scores, renormalised to a sum of 1 or not, times `scale`.  Ties, masked
+    logits and the sticky flags (1 a NaN, 4 a row with fewer than k experts,
+    which ends with ids -1): include/ornith_route.h.  Traced, the op
+    ornith_g256::route_experts."""
+    call = route_op if _compiling() or _modes() else _route_experts
+    call(logits, weights, ids, flags, score, bias, groups, kept_groups, group_top, renormalize, scale)
+
+
+def _route_experts(logits, weights, ids, flags, score, bias, groups, kept_groups, group_top, renormalize, scale):
+    kind, by = LOGITS_TYPES.get(logits.dtype), SCORES.get(score)
+    if kind is None or logits.ndim != 2:
+        raise ValueError('logits must be bf16, fp16 or fp32 [M, E] with unit column stride')
+    if by is None:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    (rows, n), (ld, step), gpu = logits.shape, logits.stride(), logits.get_device()
+    if step != 1 and n > 1:
+        raise ValueError('logits must be bf16, fp16 or fp32 [M, E] with unit column stride')
+    if rows <= 1:
+        ld = n
+    elif ld < n:
+        raise ValueError(f'logits rows overlap: row stride {ld} of {n} columns')
+    if weights.ndim != 2:
+        raise ValueError('weights must be fp32 [M, k]')
+    k = weights.shape[1]
+    picks = (rows, k)
+    args = [_row_ptr(t, name, dtype, shape, logits) for t, name, dtype, shape in
+            ((bias, 'bias', torch.float32, (n,)), (weights, 'weights', torch.float32, picks),
+             (ids, 'ids', torch.int32, picks))]
+    if not (1 <= n <= 1024 and 1 <= groups <= 64 and n % groups == 0 and 1 <= kept_groups <= groups
+            and group_top in (1, 2) and 1 <= k <= min(32, kept_groups * (n // groups))):
+        raise ValueError(f'cannot pick {k} of {n} experts in {kept_groups} of {groups} groups by their {group_top} best: '
+                         f'at most 1024 experts, 64 groups that divide them, 32 picks of those in the kept groups, 1 or 2 best')
+    if flags.dtype != torch.int32 or flags.numel() != 1:
+        raise ValueError('flags must be one int32 word')
+    if gpu < 0 or flags.get_device() != gpu:
+        raise ValueError('logits, outputs and flags must be on one GPU')
+    scale = float(scale)
+    if not abs(scale) <= 3.4028234e38:
+        raise ValueError(f'scale must be a finite fp32 number, got {scale}')
+    call_on(gpu, lib().ornith_route_experts_launch, 'expert routing', logits.data_ptr(), kind, rows, n, ld, args[0], by,
+            groups, kept_groups, group_top, k, bool(renormalize), scale, args[1], args[2], flags.data_ptr())
+
+
+@torch.library.custom_op('ornith_g256::route_experts', mutates_args={'weights', 'ids', 'flags'}, device_types='cuda')
+def route_op(logits: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, flags: torch.Tensor, score: str,
+             bias: torch.Tensor | None, groups: int, kept_groups: int, group_top: int, renormalize: bool,
+             scale: float) -> None:
+    _route_experts(logits, weights, ids, flags, score, bias, groups, kept_groups, group_top, renormalize, scale)
+
+
+@route_op.register_fake
+def _(logits, weights, ids, flags, score, bias, groups, kept_groups, group_top, renormalize, scale):
     return None
 
 
