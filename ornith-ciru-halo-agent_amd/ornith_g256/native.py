@@ -27,6 +27,8 @@ from __future__ import annotations
 
 import contextvars
 import ctypes as C
+import functools
+import itertools
 from contextlib import contextmanager
 from dataclasses import dataclass, field
 from pathlib import Path
@@ -117,6 +119,10 @@ _PROTOTYPES = {
     'ornith_w4_launch': ([_VP, _INT, _I64] + [_VP] * 3 + [_INT, _I64, _VP] + [_INT] * 4 + [_VP], _INT),
     # routing to experts (include/ornith_route.h)
     'ornith_route_experts_launch': ([_VP] + [_INT] * 3 + [_I64, _VP] + [_INT] * 6 + [C.c_float] + [_VP] * 4, _INT),
+    # adapters (include/ornith_adapter.h)
+    'ornith_adapter_get_layout': ([_INT] * 3 + [C.POINTER(_SZ)], _INT),
+    'ornith_adapter_launch': ([_VP, _INT, _I64] + [_VP, _I64] * 2 + [_VP] * 3 + [_I64, _VP, _INT, _I64, _VP, _SZ, _VP]
+                              + [_INT] * 5 + [_VP, _INT, _VP], _INT),
     # measurement (include/ornith_timing.h)
     'ornith_mi355x_timing_arm': ([C.c_char_p, _INT], _INT),
     'ornith_mi355x_timing_read': ([C.c_char_p, C.POINTER(_INT), C.POINTER(C.c_double)], _INT),
@@ -810,6 +816,112 @@ def route_op(logits: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, fla
 
 @route_op.register_fake
 def _(logits, weights, ids, flags, score, bias, groups, kept_groups, group_top, renormalize, scale):
+    return None
+
+
+def adapter_bytes(capacity, a_rows):
+    """Workspace bytes of adapter_out for up to `capacity` rows and adapters of
+    `a_rows` rows of A (the rank times the slices)."""
+    if a_rows < 8 or a_rows % 8:
+        raise ValueError(f'adapters have a multiple of 8 rows of A, got {a_rows}')
+    size, slices = _SZ(0), -(-a_rows // 512)
+    while a_rows % (8 * slices):
+        slices += 1
+    check(lib().ornith_adapter_get_layout(capacity, slices, a_rows // slices, C.byref(size)),
+          f'adapter layout for {capacity} rows, {a_rows} rows of A')
+    return size.value
+
+
+@functools.lru_cache(maxsize=1024)
+def _slice_ends(slices, n):
+    """Ends of slices of the given widths, as the launch reads them."""
+    ends = tuple(itertools.accumulate(slices))
+    if not 1 <= len(ends) <= 8 or min(slices) < 0 or ends[-1] != n:
+        raise ValueError(f'slices must be 1 to 8 widths that sum to {n} columns, got {slices}')
+    return (_INT * len(ends))(*ends)
+
+
+def adapter_out(x, a, b, scales, ids, base, out, workspace, flags, slices=None):
+    """What each row's own low-rank adapter adds to a shared projection:
+    out[t] = base[t] + scales[i] * B[i] (A[i] x[t]) with i = ids[t] (int32 [rows],
+    below 0: no adapter, out[t] = base[t]).  x [rows, K], a [slots, S * rank, K]
+    and b [slots, N, rank] bf16 or fp16; scales fp32 [slots]; base and out
+    [rows, N] bf16, fp16 or fp32, base None (or out itself) to add in place.
+    slices: the widths of a merged projection's S parts, each of which has its
+    own `rank` rows of a (one part if None).  Flags: 4 a non-finite result, 8 a
+    non-finite 16-bit result, 16 an id past the slots (include/ornith_adapter.h).
+    Traced, the op ornith_g256::adapter_out, which copies rows that w4_grid
+    would."""
+    if base is out:
+        base = None
+    if _compiling() or _modes():
+        adapter_op(x, a, b, scales, ids, base, out, workspace, flags, None if slices is None else list(slices))
+    else:
+        _adapter_out(x, a, b, scales, ids, base, out, workspace, flags, slices)
+
+
+def _adapter_out(x, a, b, scales, ids, base, out, workspace, flags, slices):
+    dtype, out_type = x.dtype, W4_TYPES.get(out.dtype)
+    x_type = W4_TYPES.get(dtype, 2)
+    if x_type > 1 or x.ndim != 2:
+        raise ValueError(f'input must be a bf16 or fp16 [rows, K] tensor, got {tuple(x.shape)} {dtype}')
+    if a.ndim != 3 or b.ndim != 3 or a.dtype != dtype or b.dtype != dtype:
+        raise ValueError(f'adapters must be {dtype} [slots, S * rank, K] and [slots, N, rank] tensors, got '
+                         f'{tuple(a.shape)} {a.dtype} and {tuple(b.shape)} {b.dtype}')
+    (rows, k), (slots, a_rows, ak), (b_slots, n, rank), gpu = x.shape, a.shape, b.shape, x.get_device()
+    ends = _slice_ends((n,) if slices is None else tuple(slices), n)
+    parts = len(ends)
+    if ak != k or b_slots != slots or a_rows != parts * rank or k % 8 or rank % 8 or not 8 <= rank <= 512 or slots > 4096:
+        raise ValueError(f'adapters {tuple(a.shape)} and {tuple(b.shape)} do not fit inputs of {k} and {parts} slices: '
+                         'K and the rank are multiples of 8, the rank at most 512, slots at most 4096')
+    (ldx, sx), (a_slot, a_row, a_col), (b_slot, b_row, b_col) = x.stride(), a.stride(), b.stride()
+    if slots <= 1 or not k or not n:
+        a_slot, b_slot = a_rows * k, n * rank
+    if ((a_col != 1 or a_row != k) and a_rows * k and slots) or ((b_col != 1 or b_row != rank) and n and slots):
+        raise ValueError('each slot of the adapters must be contiguous')
+    if out_type is None or out.shape != (rows, n):
+        raise ValueError(f'output must be a bf16, fp16 or fp32 [{rows}, {n}] tensor, got {tuple(out.shape)} {out.dtype}')
+    ldo, so = out.stride()
+    if base is None:
+        base, ldb, sb = out, ldo, so
+    elif base.shape != out.shape or base.dtype != out.dtype or base.get_device() != gpu:
+        raise ValueError(f'base must be a {out.dtype} {list(out.shape)} tensor on {x.device}, got {tuple(base.shape)} '
+                         f'{base.dtype} on {base.device}')
+    else:
+        ldb, sb = base.stride()
+    if rows <= 1 or not k:
+        ldx = k
+    if rows <= 1 or not n:
+        ldb = ldo = n
+    if (sx != 1 and k > 1) or ((so != 1 or sb != 1) and n > 1) or ldx < k or ldo < n or ldb < n:
+        raise ValueError('input, base and output rows must have unit column stride and not overlap')
+    x_ptr, a_ptr, b_ptr = x.data_ptr(), a.data_ptr(), b.data_ptr()
+    if ldx % 8 or a_slot % 8 or b_slot % 8 or (x_ptr | a_ptr | b_ptr) % 16:
+        raise ValueError('input rows and adapters must start on the 16-byte grid')
+    row = (rows,)
+    ids_ptr = _row_ptr(ids, 'ids', torch.int32, row, x)
+    scales_ptr = _row_ptr(scales, 'scales', torch.float32, (slots,), x)
+    if ids_ptr is None or scales_ptr is None:
+        raise ValueError('ids and scales are required')
+    if flags.dtype != torch.int32 or flags.numel() != 1 or workspace.element_size() != 1 or not workspace.is_contiguous():
+        raise ValueError('flags must be one int32 word, workspace contiguous bytes')
+    if (gpu < 0 or a.get_device() != gpu or b.get_device() != gpu or out.get_device() != gpu or flags.get_device() != gpu
+            or workspace.get_device() != gpu):
+        raise ValueError('input, adapters, ids, base, output, flags and workspace must be on one GPU')
+    call_on(gpu, lib().ornith_adapter_launch, 'adapters', x_ptr, x_type, ldx, a_ptr, a_slot, b_ptr, b_slot, scales_ptr,
+            ids_ptr, base.data_ptr(), ldb, out.data_ptr(), out_type, ldo, workspace.data_ptr(), workspace.numel(),
+            flags.data_ptr(), rows, n, k, rank, parts, ends, slots)
+
+
+@torch.library.custom_op('ornith_g256::adapter_out', mutates_args={'out', 'workspace', 'flags'}, device_types='cuda')
+def adapter_op(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, ids: torch.Tensor,
+               base: torch.Tensor | None, out: torch.Tensor, workspace: torch.Tensor, flags: torch.Tensor,
+               slices: list[int] | None) -> None:
+    _adapter_out(w4_grid(x) if x.ndim == 2 else x, a, b, scales, ids, base, out, workspace, flags, slices)
+
+
+@adapter_op.register_fake
+def _(x, a, b, scales, ids, base, out, workspace, flags, slices):
     return None
 
 
