@@ -60,14 +60,43 @@ struct AdArgs {
 };
 
 // ---- rows by slot ---------------------------------------------------------------
-// One block: counts per slot in LDS, their running sums, then each row to a place of its slot.  Which
-// place it gets is open (atomics), and no result depends on it: rows of a tile do not meet.
-constexpr int kPlanThreads = 1024;
+// Up to 64 rows: no plan.  Block t of a launch looks at all ids (a lane each), and if row t is the first,
+// 17th, .. of its slot it takes that row and the next 15 of the slot; other blocks end.
+// More: one block counts rows per slot in LDS, sums, and sends each row to a place of its slot.  Which place
+// it gets is open (atomics), and no result depends on it: rows of a tile do not meet.
+constexpr int kFewRows = 64, kPlanThreads = 1024, kPlanBatch = 8;
 
-__device__ __forceinline__ int ad_key(const AdArgs& a, int t) {     // 0: no adapter
-    const int id = a.ids[t];
-    return id >= 0 && id < a.slots ? id + 1 : 0;
+__device__ __forceinline__ int ad_key(int id, int slots) { return id >= 0 && id < slots ? id + 1 : 0; }      // 0: no adapter
+
+// Lane li's row of the tile (past the last row: that one again), and the tile.
+template <int MT, bool FEW> __device__ __forceinline__ bool ad_tile(const AdArgs& a, int& slot, int& rows, int (&t)[MT]) {
+    const int lane = threadIdx.x & 63, li = lane & 15;
+    if constexpr (FEW) {
+        static_assert(MT == 1);
+        const int id = lane < a.M ? a.ids[lane] : -1;
+        if (blockIdx.x == 0 && blockIdx.y == 0) flag_or(a.flags, id >= a.slots ? kAdBadId : 0u);
+        const int key = ad_key(id, a.slots), mine = __builtin_amdgcn_readlane(key, int(blockIdx.x));
+        const uint64_t same = __ballot(key == mine && lane < a.M);
+        const int before = __popcll(same & ((uint64_t(1) << blockIdx.x) - 1));
+        slot = mine - 1;
+        rows = min(__popcll(same) - before, 16);
+        if (before & 15) return false;
+        const int rank = int(__builtin_amdgcn_mbcnt_hi(uint32_t(same >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(same), 0u))) - before;
+        const bool in = (same >> lane & 1) && rank >= 0 && rank < 16;
+        const int sent = __builtin_amdgcn_ds_permute(4 * (in ? rank : 63), lane);
+        t[0] = __builtin_amdgcn_ds_bpermute(4 * min(li, rows - 1), sent);
+    } else {
+        const int n = *a.ntiles;
+        const AdTile tile = a.tiles[blockIdx.x];       // (a tile's place, if not a tile)
+        if (int(blockIdx.x) >= n) return false;
+        slot = tile.slot;
+        rows = tile.rows;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) t[m] = a.order[tile.first + min(16 * m + li, rows - 1)];
+    }
+    return true;
 }
+
 __device__ __forceinline__ int block_prefix(int v, int* s_wave, int& total) {      // inclusive, over kPlanThreads
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int in = wave_prefix_sum(v);
@@ -75,87 +104,151 @@ __device__ __forceinline__ int block_prefix(int v, int* s_wave, int& total) {   
     __syncthreads();
     int before = 0;
     total = 0;
+#pragma unroll
     for (int w = 0; w < kPlanThreads / 64; ++w) {
-        if (w < wv) before += s_wave[w];
-        total += s_wave[w];
+        const int x = s_wave[w];
+        before += w < wv ? x : 0;
+        total += x;
     }
     __syncthreads();
     return in + before;
 }
+// A place of counter[key] for each lane with a key >= 0.  Rows of a request are neighbours: the first two keys
+// that a wave holds take one addition each.
+__device__ __forceinline__ int ad_take(int* counter, int key) {
+    int place = 0;
+    bool left = key >= 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint64_t todo = __ballot(left);
+        if (!todo) return place;
+        const int first = __ffsll((long long)todo) - 1, lead = __builtin_amdgcn_readlane(key, first);
+        const uint64_t same = __ballot(left && key == lead);
+        int at = 0;
+        if (int(threadIdx.x & 63) == first) at = atomicAdd(&counter[lead], __popcll(same));
+        at = __builtin_amdgcn_readlane(at, first);
+        if (left && key == lead) {
+            place = at + int(__builtin_amdgcn_mbcnt_hi(uint32_t(same >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(same), 0u)));
+            left = false;
+        }
+    }
+    if (left) place = atomicAdd(&counter[key], 1);
+    return place;
+}
 
 __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(AdArgs a, int tile_rows) {
-    __shared__ int s_count[kAdMaxSlots + 1], s_at[kAdMaxSlots + 1], s_wave[kPlanThreads / 64];
+    __shared__ int s_at[kAdMaxSlots + 1], s_first[kAdMaxSlots + 2], s_tile[kAdMaxSlots + 2], s_wave[kPlanThreads / 64];
     const int tid = threadIdx.x, keys = a.slots + 1;
-    for (int i = tid; i < keys; i += kPlanThreads) s_count[i] = 0;
+    for (int i = tid; i < keys; i += kPlanThreads) s_at[i] = 0;
     __syncthreads();
     uint32_t flags = 0;
-    for (int t = tid; t < a.M; t += kPlanThreads) {
-        flags |= a.ids[t] >= a.slots ? kAdBadId : 0u;
-        atomicAdd(&s_count[ad_key(a, t)], 1);
-    }
+    auto each = [&](auto&& f) {                        // f(row, key) of a batch of rows, whose ids are loaded at once
+        for (int t0 = 0; t0 < a.M; t0 += kPlanThreads * kPlanBatch) {
+            int id[kPlanBatch];
+#pragma unroll
+            for (int j = 0; j < kPlanBatch; ++j) id[j] = a.ids[min(t0 + j * kPlanThreads + tid, a.M - 1)];
+#pragma unroll
+            for (int j = 0; j < kPlanBatch; ++j) {
+                const int t = t0 + j * kPlanThreads + tid;
+                if (t0 + j * kPlanThreads >= a.M) break;
+                flags |= id[j] >= a.slots ? kAdBadId : 0u;
+                f(t, t < a.M ? ad_key(id[j], a.slots) : -1);
+            }
+        }
+    };
+    each([&](int, int key) { ad_take(s_at, key); });
     flag_or(a.flags, flags);
     __syncthreads();
     int rows = 0, tiles = 0;
     for (int i0 = 0; i0 < keys; i0 += kPlanThreads) {
-        const int i = i0 + tid, n = i < keys ? s_count[i] : 0;
+        const int i = i0 + tid, n = i < keys ? s_at[i] : 0;
         const int nt = i == 0 && a.in_place ? 0 : (n + tile_rows - 1) / tile_rows;
         int all, all_tiles;
         const int first = rows + block_prefix(n, s_wave, all) - n;
         const int tile0 = tiles + block_prefix(nt, s_wave, all_tiles) - nt;
-        if (i < keys) s_at[i] = first;
-        for (int j = 0; j < nt; ++j)
-            a.tiles[tile0 + j] = AdTile{i - 1, first + j * tile_rows, min(n - j * tile_rows, tile_rows)};
+        if (i < keys) {
+            s_at[i] = first;
+            s_first[i] = first;
+            s_tile[i] = tile0;
+        }
         rows += all;
         tiles += all_tiles;
     }
-    if (tid == 0) *a.ntiles = tiles;
+    if (tid == 0) {
+        *a.ntiles = tiles;
+        s_first[keys] = rows;
+    }
     __syncthreads();
-    for (int t = tid; t < a.M; t += kPlanThreads) a.order[atomicAdd(&s_at[ad_key(a, t)], 1)] = t;
+    for (int j = tid; j < tiles; j += kPlanThreads) {  // the last slot that begins at or before tile j
+        int lo = 0, hi = keys;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            (s_tile[mid] <= j ? lo : hi) = mid;
+        }
+        const int first = s_first[lo] + (j - s_tile[lo]) * tile_rows;
+        a.tiles[j] = AdTile{lo - 1, first, min(s_first[lo + 1] - first, tile_rows)};
+    }
+    each([&](int t, int key) {
+        const int place = ad_take(s_at, key);
+        if (key >= 0) a.order[place] = t;
+    });
 }
 
 // ---- shrink ---------------------------------------------------------------------
-constexpr int kShrinkWaves = 8;
-
-template <int TYPE, int MT, int RT>
-__global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(AdArgs a) {
-    constexpr int W = kShrinkWaves;
+// A wave takes 64 k of every 64 W; D such pieces are loaded before the first product.
+template <int TYPE, int MT, int RT, int W, int D, bool FEW>
+__global__ __launch_bounds__(64 * W) void adapter_shrink_kernel(AdArgs a) {
     __shared__ f32x4 s_acc[W][MT * RT][64];
-    if (int(blockIdx.x) >= *a.ntiles) return;
-    const AdTile tile = a.tiles[blockIdx.x];
-    if (tile.slot < 0) return;
+    int slot, rows, t[MT];
+    if (!ad_tile<MT, FEW>(a, slot, rows, t) || slot < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
     const int r0 = int(blockIdx.y) * 16 * RT;
     const uint16_t *x[MT], *w[RT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {                     // (past the last row: that one again)
-        const int t = a.order[tile.first + min(16 * m + li, tile.rows - 1)];
-        x[m] = a.x + size_t(t) * size_t(a.ldx) + 8 * q;
-    }
+    for (int m = 0; m < MT; ++m) x[m] = a.x + size_t(t[m]) * size_t(a.ldx);
 #pragma unroll
     for (int r = 0; r < RT; ++r)
-        w[r] = a.a + size_t(tile.slot) * size_t(a.a_slot) + size_t(min(r0 + 16 * r + li, a.SR - 1)) * size_t(a.K) + 8 * q;
+        w[r] = a.a + size_t(slot) * size_t(a.a_slot) + size_t(min(r0 + 16 * r + li, a.SR - 1)) * size_t(a.K);
     f32x4 acc[MT][RT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 64 * wv; k0 < a.K; k0 += 64 * W) {
-        u32x4 xv[2][MT], wf[2][RT];
+    for (int k0 = 64 * wv; k0 < a.K; k0 += 64 * W * D) {
+        u32x4 xv[D][2][MT], wf[D][2][RT];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int k = k0 + 32 * h;
-            const bool in = k + 8 * q < a.K;
+        for (int d = 0; d < D; ++d) {
+            if (d && k0 + 64 * W * d >= a.K) break;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) xv[h][m] = in ? *reinterpret_cast<const u32x4*>(x[m] + k) : u32x4{0, 0, 0, 0};
+            for (int h = 0; h < 2; ++h) {              // (past K: its last piece, cleared below)
+                const int k = min(k0 + 64 * W * d + 32 * h + 8 * q, a.K - 8);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) wf[h][r] = in ? *reinterpret_cast<const u32x4*>(w[r] + k) : u32x4{0, 0, 0, 0};
+                for (int m = 0; m < MT; ++m) xv[d][h][m] = *reinterpret_cast<const u32x4*>(x[m] + k);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) wf[d][h][r] = *reinterpret_cast<const u32x4*>(w[r] + k);
+            }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int d = 0; d < D; ++d) {
+            const int kd = k0 + 64 * W * d;
+            if (d && kd >= a.K) break;
+            if (kd + 64 > a.K) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+                for (int h = 0; h < 2; ++h)
+                    if (kd + 32 * h + 8 * q >= a.K) {
 #pragma unroll
-                for (int r = 0; r < RT; ++r) acc[m][r] = ad_mfma<TYPE>(xv[h][m], wf[h][r], acc[m][r]);
+                        for (int m = 0; m < MT; ++m) xv[d][h][m] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) wf[d][h][r] = u32x4{0, 0, 0, 0};
+                    }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) acc[m][r] = ad_mfma<TYPE>(xv[d][h][m], wf[d][h][r], acc[m][r]);
+        }
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -171,32 +264,28 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(AdArg
             for (int i = 0; i < 4; ++i) v[i] += p[i];
         }
         const int m = f / RT, r = r0 + 16 * (f % RT) + li;
-        if (r < a.SR) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 16 * m + 4 * q + i;
-                if (row < tile.rows) a.v[size_t(tile.first + row) * a.SR + r] = v[i];
-            }
+        for (int i = 0; i < 4; ++i) {
+            int of = t[0];
+#pragma unroll
+            for (int mm = 1; mm < MT; ++mm) of = m == mm ? t[mm] : of;
+            of = __builtin_amdgcn_ds_bpermute(4 * (4 * q + i), of);
+            if (r < a.SR && 16 * m + 4 * q + i < rows) a.v[size_t(of) * a.SR + r] = v[i];
         }
     }
 }
 
 // ---- expand ---------------------------------------------------------------------
-template <int OUT> __device__ __forceinline__ float ad_get(const void* p, size_t at) {
-    if constexpr (OUT == ORNITH_ADAPTER_F32) return static_cast<const float*>(p)[at];
-    else if constexpr (OUT == ORNITH_ADAPTER_BF16) return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[at]);
-    else return f16_bits_to_f32(static_cast<const uint16_t*>(p)[at]);
+template <int OUT> struct AdOut { typedef uint16_t type; static constexpr int size = 2; };
+template <> struct AdOut<ORNITH_ADAPTER_F32> { typedef uint32_t type; static constexpr int size = 4; };
+template <int OUT> __device__ __forceinline__ float ad_float(uint32_t bits) {
+    if constexpr (OUT == ORNITH_ADAPTER_F32) return __uint_as_float(bits);
+    else if constexpr (OUT == ORNITH_ADAPTER_BF16) return bf16_bits_to_f32(bits);
+    else return f16_bits_to_f32(bits);
 }
-template <int OUT> __device__ __forceinline__ void ad_put(void* p, size_t at, float v) {
-    if constexpr (OUT == ORNITH_ADAPTER_F32) static_cast<float*>(p)[at] = v;
-    else if constexpr (OUT == ORNITH_ADAPTER_BF16) static_cast<__bf16*>(p)[at] = static_cast<__bf16>(v);
-    else static_cast<_Float16*>(p)[at] = static_cast<_Float16>(v);
-}
-template <int TYPE> __device__ __forceinline__ float ad_round(float v) {
-    return TYPE == ORNITH_ADAPTER_BF16 ? float(static_cast<__bf16>(v)) : float(static_cast<_Float16>(v));
-}
-template <int TYPE> __device__ __forceinline__ uint16_t ad_bits(float v) {
-    if constexpr (TYPE == ORNITH_ADAPTER_BF16) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
+template <int OUT> __device__ __forceinline__ uint32_t ad_bits(float v) {
+    if constexpr (OUT == ORNITH_ADAPTER_F32) return __float_as_uint(v);
+    else if constexpr (OUT == ORNITH_ADAPTER_BF16) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
     else return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
 }
 // Power of two that brings a row's largest |v| to [2^14, 2^15) of fp16, as fp32 (1 for 0 and non-finite rows).
@@ -205,49 +294,93 @@ __device__ __forceinline__ float ad_scale16(uint32_t most) {
     if (e == 0 || e == 255) return 1.f;
     return __uint_as_float(uint32_t(min(max(127 + 127 + 14 - e, 1), 254)) << 23);
 }
+// Column, of a wave's 64, of row m = 4 q + i of the instruction's tile j: a lane's results of a tile (fp32) or
+// of two (16-bit) are 16 neighbouring bytes, those of its row's four lanes 64.
+template <int OUT> __device__ __forceinline__ int ad_column(int j, int m) {
+    if constexpr (OUT == ORNITH_ADAPTER_F32) return 16 * j + m;
+    else return 32 * (j >> 1) + 8 * (m >> 2) + 4 * (j & 1) + (m & 3);
+}
 
-constexpr int kExpandWaves = 4, kExpandGroups = 4;      // of 64 columns, a block
+constexpr int kExpandWaves = 4;                        // a block: 64 columns a wave
 
-template <int TYPE, int OUT, int MT>
+template <int TYPE, int OUT, int MT, bool FEW>
 __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArgs a) {
     extern __shared__ __attribute__((aligned(16))) u32x4 s_v[];        // [MT][steps][64]
     __shared__ uint32_t s_most[16 * MT];
-    if (int(blockIdx.x) >= *a.ntiles) return;
-    const AdTile tile = a.tiles[blockIdx.x];
+    __shared__ int s_t[16 * MT];
+    typedef typename AdOut<OUT>::type word;
+    constexpr int size = AdOut<OUT>::size, kPer = 16 / size, kVec = 4 * size / 4;    // values of 16 bytes, such pieces a lane
+    int slot, rows, t[MT];
+    if (!ad_tile<MT, FEW>(a, slot, rows, t) || (slot < 0 && a.in_place)) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
     int p = 0;
     while (int(blockIdx.y) >= a.blocks[p]) ++p;
-    const int begin = p ? a.ends[p - 1] : 0, end = a.ends[p];
-    const int group0 = (int(blockIdx.y) - (p ? a.blocks[p - 1] : 0)) * kExpandGroups;
+    const int end = a.ends[p];
+    const int n0 = (p ? a.ends[p - 1] : 0) + ((int(blockIdx.y) - (p ? a.blocks[p - 1] : 0)) * kExpandWaves + wv) * 64;
+    const word *base[MT];
+    word* out[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        base[m] = static_cast<const word*>(a.base) + size_t(t[m]) * size_t(a.ldb) + n0;
+        out[m] = static_cast<word*>(a.out) + size_t(t[m]) * size_t(a.ldo) + n0;
+    }
+    // whole groups on the 16-byte grid move in pieces of 16 bytes (wave-uniform)
+    const bool whole = n0 + 64 <= end && ((reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out) |
+                                           size_t(a.ldb) * size | size_t(a.ldo) * size | size_t(n0) * size) & 15) == 0;
+    u32x4 have[MT][kVec];
+    if (whole) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int c = 0; c < kVec; ++c) have[m][c] = *reinterpret_cast<const u32x4*>(base[m] + (4 * c + q) * kPer);
+    }
+    if (slot < 0) {
+        if (whole) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int c = 0; c < kVec; ++c)
+                    if (16 * m + li < rows) *reinterpret_cast<u32x4*>(out[m] + (4 * c + q) * kPer) = have[m][c];
+        } else {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+                for (int i = q; i < 64; i += 4)
+                    if (16 * m + li < rows && n0 + i < end) out[m][i] = base[m][i];
+        }
+        return;
+    }
     const int chunks = a.R / 8, steps = (2 * chunks + 3) / 4;
-    if (tile.slot >= 0) {
+    {
         // v of the tile's rows and this slice: hi then lo along r, in pieces of 8, as the instruction's operands
-        const int rows = 16 * MT, pieces = rows * chunks;
+        if (tid < 16) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) s_t[16 * m + tid] = t[m];
+        }
+        if (TYPE == ORNITH_ADAPTER_F16 && tid < 16 * MT) s_most[tid] = 0;
+        __syncthreads();
+        auto piece_of = [&](int row, int c) { return a.v + size_t(s_t[row]) * a.SR + p * a.R + 8 * c; };
         if constexpr (TYPE == ORNITH_ADAPTER_F16) {
-            if (tid < rows) s_most[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < pieces; i += 64 * kExpandWaves) {
-                const int row = i / chunks;
-                if (row >= tile.rows) continue;
-                const float* v = a.v + size_t(tile.first + row) * a.SR + p * a.R + (i % chunks) * 8;
+            for (int i = tid; i < 16 * MT * chunks; i += 64 * kExpandWaves) {
+                const float* v = piece_of(i / chunks, i % chunks);
                 uint32_t most = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
-                atomicMax(&s_most[row], most);
+                atomicMax(&s_most[i / chunks], most);
             }
             __syncthreads();
         }
         for (int i = tid; i < 16 * MT * steps * 4; i += 64 * kExpandWaves) {
             const int row = i / (steps * 4), c = i % (steps * 4);
             u32x4 piece = {0, 0, 0, 0};
-            if (row < tile.rows && c < 2 * chunks) {
-                const float* v = a.v + size_t(tile.first + row) * a.SR + p * a.R + (c % chunks) * 8;
+            if (c < 2 * chunks) {
+                const float* v = piece_of(row, c < chunks ? c : c - chunks);
                 const float by = TYPE == ORNITH_ADAPTER_F16 ? ad_scale16(s_most[row]) : 1.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float f = v[e] * by, hi = ad_round<TYPE>(f);
-                    const float lo = f - hi;           // (inf: no NaN beside it)
-                    const uint32_t bits = c < chunks ? ad_bits<TYPE>(f) : __builtin_isinf(hi) ? 0u : ad_bits<TYPE>(lo);
+                    const float f = v[e] * by;
+                    uint32_t bits = ad_bits<TYPE>(f);
+                    const float hi = ad_float<TYPE>(bits);
+                    if (c >= chunks) bits = __builtin_isinf(hi) ? 0u : ad_bits<TYPE>(f - hi);     // (inf: no NaN beside it)
                     piece[e >> 1] |= bits << (16 * (e & 1));
                 }
             }
@@ -255,67 +388,69 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
         }
         __syncthreads();
     }
-    constexpr int size = OUT == ORNITH_ADAPTER_F32 ? 4 : 2;
-    int t[MT];
+    if (n0 >= end) return;
     float by[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        t[m] = a.order[tile.first + min(16 * m + li, tile.rows - 1)];
-        by[m] = 0.f;
-        if (tile.slot >= 0) {
-            by[m] = a.scales[tile.slot];
-            if constexpr (TYPE == ORNITH_ADAPTER_F16) by[m] = by[m] / ad_scale16(s_most[16 * m + li]);
-        }
+        by[m] = a.scales[slot];
+        if constexpr (TYPE == ORNITH_ADAPTER_F16) by[m] = by[m] / ad_scale16(s_most[16 * m + li]);
     }
-    float most = 0.f, zero = 0.f;
-    for (int gi = wv; gi < kExpandGroups; gi += kExpandWaves) {
-        const int n0 = begin + (group0 + gi) * 64;
-        if (n0 >= end) break;
-        const int n = n0 + 16 * q;                     // this lane's columns n .. n + 15
-        if (tile.slot < 0) {
+    f32x4 acc[MT][4];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-                if (16 * m + li < tile.rows)
-                    for (int i = 0; i < 16; ++i)
-                        if (n + i < end) {
-                            const size_t to = size_t(t[m]) * size_t(a.ldo) + n + i, from = size_t(t[m]) * size_t(a.ldb) + n + i;
-                            if constexpr (size == 4) static_cast<uint32_t*>(a.out)[to] = static_cast<const uint32_t*>(a.base)[from];
-                            else static_cast<uint16_t*>(a.out)[to] = static_cast<const uint16_t*>(a.base)[from];
-                        }
-            continue;
-        }
-        f32x4 acc[MT][4];
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint16_t* b[4];
 #pragma unroll
-            for (int jj = 0; jj < 4; ++jj) acc[m][jj] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const uint16_t* b = a.b + size_t(tile.slot) * size_t(a.b_slot);
-        for (int s = 0; s < steps; ++s) {
-            const int c = 4 * s + q;
-            u32x4 bv[4];
+    for (int j = 0; j < 4; ++j)                        // (past the slice: its last column)
+        b[j] = a.b + size_t(slot) * size_t(a.b_slot) + size_t(min(n0 + ad_column<OUT>(j, li), end - 1)) * a.R;
+    for (int s = 0; s < steps; ++s) {
+        const int c = 4 * s + q, at = 8 * (c < chunks ? c : min(c - chunks, chunks - 1));
+        u32x4 bv[4];
 #pragma unroll
-            for (int jj = 0; jj < 4; ++jj) {
-                const int col = min(n0 + 16 * (li >> 2) + 4 * jj + (li & 3), end - 1);
-                bv[jj] = c < 2 * chunks ? *reinterpret_cast<const u32x4*>(b + size_t(col) * a.R + (c % chunks) * 8) : u32x4{0, 0, 0, 0};
-            }
+        for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const u32x4*>(b[j] + at);
+        if (c >= 2 * chunks) {                         // (no 0 times inf)
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const u32x4 vv = s_v[(m * steps + s) * 64 + lane];
-#pragma unroll
-                for (int jj = 0; jj < 4; ++jj) acc[m][jj] = ad_mfma<TYPE>(bv[jj], vv, acc[m][jj]);
-            }
+            for (int j = 0; j < 4; ++j) bv[j] = u32x4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            if (16 * m + li >= tile.rows) continue;
+            const u32x4 vv = s_v[(m * steps + s) * 64 + lane];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if (n + i >= end) continue;
-                const float r = ad_get<OUT>(a.base, size_t(t[m]) * size_t(a.ldb) + n + i) + by[m] * acc[m][i >> 2][i & 3];
-                most = fmaxf(most, __builtin_fabsf(r));
-                zero = __builtin_fmaf(r, 0.f, zero);
-                ad_put<OUT>(a.out, size_t(t[m]) * size_t(a.ldo) + n + i, r);
+            for (int j = 0; j < 4; ++j) acc[m][j] = ad_mfma<TYPE>(bv[j], vv, acc[m][j]);
+        }
+    }
+    float most = 0.f, zero = 0.f;
+    auto sum = [&](uint32_t bits, int m, int j, int i) {
+        const float r = ad_float<OUT>(bits) + by[m] * acc[m][j][i];
+        most = fmaxf(most, __builtin_fabsf(r));
+        zero = __builtin_fmaf(r, 0.f, zero);
+        return ad_bits<OUT>(r);
+    };
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        if (16 * m + li >= rows) continue;
+        if (whole) {
+#pragma unroll
+            for (int c = 0; c < kVec; ++c) {
+                u32x4 r;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t h = have[m][c][e];
+                    if constexpr (size == 4) r[e] = sum(h, m, c, e);
+                    else r[e] = sum(h & 0xffffu, m, 2 * c + (e >> 1), 2 * (e & 1)) |
+                                sum(h >> 16, m, 2 * c + (e >> 1), 2 * (e & 1) + 1) << 16;
+                }
+                *reinterpret_cast<u32x4*>(out[m] + (4 * c + q) * kPer) = r;
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int n = ad_column<OUT>(j, 4 * q + i);
+                    if (n0 + n < end) out[m][n] = word(sum(base[m][n], m, j, i));
+                }
         }
     }
     // 16-bit results round to infinity from half a step above the type's largest value
@@ -337,22 +472,34 @@ bool ad_layout(int64_t M, int S, int R, AdLayout& l) {
     return true;
 }
 
-template <int TYPE, int MT> hipError_t ad_run(const AdArgs& a, int out_type, int tiles, hipStream_t s) {
+template <int TYPE, int MT, bool FEW> hipError_t ad_run(const AdArgs& a, int out_type, int tiles, hipStream_t s) {
     const int rt = (a.SR + 15) / 16;
-    auto shrink = [&](auto kernel, int RT) {
-        timed_launch("adapter_shrink", kernel, dim3(tiles, (rt + RT - 1) / RT), dim3(64 * kShrinkWaves), 0, s, a);
+    auto shrink = [&](auto kernel, int RT, int W) {
+        timed_launch("adapter_shrink", kernel, dim3(tiles, (rt + RT - 1) / RT), dim3(64 * W), 0, s, a);
     };
-    shrink(adapter_shrink_kernel<TYPE, MT, 1>, 1);
+    if (MT == 1 || rt == 1) shrink(adapter_shrink_kernel<TYPE, MT, 1, 8, MT == 1 ? 4 : 2, FEW>, 1, 8);
+    else shrink(adapter_shrink_kernel<TYPE, MT, 2, 8, 1, FEW>, 2, 8);
     hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
     const int steps = (a.R / 4 + 3) / 4;
     auto expand = [&](auto kernel) {
         timed_launch("adapter_expand", kernel, dim3(tiles, a.blocks[a.S - 1]), dim3(64 * kExpandWaves), uint32_t(MT * steps * 1024), s, a);
     };
-    if (out_type == ORNITH_ADAPTER_F32) expand(adapter_expand_kernel<TYPE, ORNITH_ADAPTER_F32, MT>);
-    else if (out_type == ORNITH_ADAPTER_BF16) expand(adapter_expand_kernel<TYPE, ORNITH_ADAPTER_BF16, MT>);
-    else expand(adapter_expand_kernel<TYPE, ORNITH_ADAPTER_F16, MT>);
+    if (out_type == ORNITH_ADAPTER_F32) expand(adapter_expand_kernel<TYPE, ORNITH_ADAPTER_F32, MT, FEW>);
+    else if (out_type == ORNITH_ADAPTER_BF16) expand(adapter_expand_kernel<TYPE, ORNITH_ADAPTER_BF16, MT, FEW>);
+    else expand(adapter_expand_kernel<TYPE, ORNITH_ADAPTER_F16, MT, FEW>);
     return hipGetLastError();
+}
+
+template <int TYPE> hipError_t ad_rows(const AdArgs& a, int out_type, hipStream_t s) {
+    if (a.M <= kFewRows) return ad_run<TYPE, 1, true>(a, out_type, a.M, s);
+    // tiles of 64 rows where they are many and v of them fits LDS
+    const int tile_rows = a.M >= 1024 && a.R <= 128 ? 64 : 16;
+    const int tiles = std::min(a.M, (a.M + tile_rows - 1) / tile_rows + a.slots + 1);
+    timed_launch("adapter_plan", adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, tile_rows);
+    const hipError_t st = hipGetLastError();
+    if (st != hipSuccess) return st;
+    return tile_rows == 64 ? ad_run<TYPE, 4, false>(a, out_type, tiles, s) : ad_run<TYPE, 1, false>(a, out_type, tiles, s);
 }
 
 }  // namespace
@@ -427,7 +574,7 @@ extern "C" hipError_t ornith_adapter_launch(const void* x, int x_type, int64_t l
     for (int p = 0; p < S; ++p) {
         args.ends[p] = slice_ends[p];
         const int width = slice_ends[p] - (p ? slice_ends[p - 1] : 0);
-        blocks += (width + 64 * kExpandGroups - 1) / (64 * kExpandGroups);
+        blocks += (width + 64 * kExpandWaves - 1) / (64 * kExpandWaves);
         args.blocks[p] = blocks;
     }
     for (int64_t r = 0; r < M; r += kAdRows) {
@@ -436,12 +583,8 @@ extern "C" hipError_t ornith_adapter_launch(const void* x, int x_type, int64_t l
         args.ids = static_cast<const int32_t*>(ids) + r;
         args.base = static_cast<const uint8_t*>(base) + size_t(r) * size_t(ldb) * size;
         args.out = static_cast<uint8_t*>(out) + size_t(r) * size_t(ldo) * size;
-        const int tile_rows = 16, tiles = std::min(args.M, (args.M + tile_rows - 1) / tile_rows + slots + 1);
-        timed_launch("adapter_plan", adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, args, tile_rows);
-        hipError_t st = hipGetLastError();
-        if (st != hipSuccess) return st;
-        st = x_type == ORNITH_ADAPTER_BF16 ? ad_run<ORNITH_ADAPTER_BF16, 1>(args, out_type, tiles, stream)
-                                           : ad_run<ORNITH_ADAPTER_F16, 1>(args, out_type, tiles, stream);
+        const hipError_t st = x_type == ORNITH_ADAPTER_BF16 ? ad_rows<ORNITH_ADAPTER_BF16>(args, out_type, stream)
+                                                            : ad_rows<ORNITH_ADAPTER_F16>(args, out_type, stream);
         if (st != hipSuccess) return st;
     }
     return hipSuccess;
