@@ -33,7 +33,8 @@
  *   plain 4-bit      w4_tile, w4_run (more than 16 rows of many columns),
  *                    w4_zero (no inputs), w4_pack_codes, w4_pack_meta
  *   routing          route_experts
- *   adapters         adapter_plan, adapter_shrink, adapter_expand
+ *   adapters         adapter_both (few rows), or adapter_plan (above 256 rows),
+ *                    adapter_shrink, adapter_expand
  *   shared expert    fixed8_act, fixed8_gate
  *   other            repack_codes, repack_meta, silu_selfcheck */
 #ifndef ORNITH_TIMING_H

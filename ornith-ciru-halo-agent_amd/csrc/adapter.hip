@@ -60,31 +60,50 @@ struct AdArgs {
 };
 
 // ---- rows by slot ---------------------------------------------------------------
-// Up to 64 rows: no plan.  Block t of a launch looks at all ids (a lane each), and if row t is the first,
-// 17th, .. of its slot it takes that row and the next 15 of the slot; other blocks end.
+// Up to 256 rows: no plan.  Block t of a launch looks at all ids, and if row t is the first, 17th, .. of its
+// slot it takes that row and the next 15 of the slot; other blocks end.
 // More: one block counts rows per slot in LDS, sums, and sends each row to a place of its slot.  Which place
 // it gets is open (atomics), and no result depends on it: rows of a tile do not meet.
-constexpr int kFewRows = 64, kPlanThreads = 1024, kPlanBatch = 8;
+constexpr int kFewRows = 256, kPlanThreads = 1024, kPlanBatch = 8;
 
 __device__ __forceinline__ int ad_key(int id, int slots) { return id >= 0 && id < slots ? id + 1 : 0; }      // 0: no adapter
 
-// Lane li's row of the tile (past the last row: that one again), and the tile.
-template <int MT, bool FEW> __device__ __forceinline__ bool ad_tile(const AdArgs& a, int& slot, int& rows, int (&t)[MT]) {
+// Lane li's row of the tile (past the last row: that one again), and the tile.  FEW: ids a lane looks at (0: a plan).
+template <int MT, int FEW> __device__ __forceinline__ bool ad_tile(const AdArgs& a, int& slot, int& rows, int (&t)[MT]) {
     const int lane = threadIdx.x & 63, li = lane & 15;
-    if constexpr (FEW) {
+    if constexpr (FEW > 0) {
         static_assert(MT == 1);
-        const int id = lane < a.M ? a.ids[lane] : -1;
-        if (blockIdx.x == 0 && blockIdx.y == 0) flag_or(a.flags, id >= a.slots ? kAdBadId : 0u);
-        const int key = ad_key(id, a.slots), mine = __builtin_amdgcn_readlane(key, int(blockIdx.x));
-        const uint64_t same = __ballot(key == mine && lane < a.M);
-        const int before = __popcll(same & ((uint64_t(1) << blockIdx.x) - 1));
+        int key[FEW], mine = 0, before = 0, all = 0;
+        uint64_t same[FEW];
+        uint32_t bad = 0;
+#pragma unroll
+        for (int j = 0; j < FEW; ++j) key[j] = 64 * j + lane < a.M ? a.ids[64 * j + lane] : -1;
+#pragma unroll
+        for (int j = 0; j < FEW; ++j) {
+            bad |= key[j] >= a.slots ? kAdBadId : 0u;
+            key[j] = ad_key(key[j], a.slots);
+            if (int(blockIdx.x >> 6) == j) mine = __builtin_amdgcn_readlane(key[j], int(blockIdx.x & 63));
+        }
+        if (blockIdx.x == 0 && blockIdx.y == 0) flag_or(a.flags, bad);
+#pragma unroll
+        for (int j = 0; j < FEW; ++j) {
+            same[j] = __ballot(key[j] == mine && 64 * j + lane < a.M);
+            const int below = min(max(int(blockIdx.x) - 64 * j, 0), 64);       // lanes of rows before this block's
+            before += __popcll(below < 64 ? same[j] & ((uint64_t(1) << below) - 1) : same[j]);
+            all += __popcll(same[j]);
+        }
         slot = mine - 1;
-        rows = min(__popcll(same) - before, 16);
+        rows = min(all - before, 16);
         if (before & 15) return false;
-        const int rank = int(__builtin_amdgcn_mbcnt_hi(uint32_t(same >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(same), 0u))) - before;
-        const bool in = (same >> lane & 1) && rank >= 0 && rank < 16;
-        const int sent = __builtin_amdgcn_ds_permute(4 * (in ? rank : 63), lane);
-        t[0] = __builtin_amdgcn_ds_bpermute(4 * min(li, rows - 1), sent);
+        int sent = 0, rank = -before;
+#pragma unroll
+        for (int j = 0; j < FEW; ++j) {
+            const int r = rank + int(__builtin_amdgcn_mbcnt_hi(uint32_t(same[j] >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(same[j]), 0u)));
+            const bool in = (same[j] >> lane & 1) && r >= 0 && r < 16;
+            sent |= __builtin_amdgcn_ds_permute(4 * (in ? r : 63), in ? 64 * j + lane + 1 : 0);
+            rank += __popcll(same[j]);
+        }
+        t[0] = __builtin_amdgcn_ds_bpermute(4 * min(li, rows - 1), sent) - 1;
     } else {
         const int n = *a.ntiles;
         const AdTile tile = a.tiles[blockIdx.x];       // (a tile's place, if not a tile)
@@ -196,7 +215,7 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(AdArgs a, in
 
 // ---- shrink ---------------------------------------------------------------------
 // A wave takes 64 k of every 64 W; D such pieces are loaded before the first product.
-template <int TYPE, int MT, int RT, int W, int D, bool FEW>
+template <int TYPE, int MT, int RT, int W, int D, int FEW>
 __global__ __launch_bounds__(64 * W) void adapter_shrink_kernel(AdArgs a) {
     __shared__ f32x4 s_acc[W][MT * RT][64];
     int slot, rows, t[MT];
@@ -301,9 +320,82 @@ template <int OUT> __device__ __forceinline__ int ad_column(int j, int m) {
     else return 32 * (j >> 1) + 8 * (m >> 2) + 4 * (j & 1) + (m & 3);
 }
 
+// The two 16-bit numbers whose sum v is (inf: no NaN beside it).
+template <int TYPE> __device__ __forceinline__ void ad_halves(float v, uint32_t& hi, uint32_t& lo) {
+    hi = ad_bits<TYPE>(v);
+    const float h = ad_float<TYPE>(hi);
+    lo = __builtin_isinf(h) ? 0u : ad_bits<TYPE>(v - h);
+}
+// Whether a wave's 64 columns lie whole on the 16-byte grid, and move in pieces of 16 bytes (wave-uniform).
+template <int SIZE> __device__ __forceinline__ bool ad_whole(const AdArgs& a, int n0, int end) {
+    return n0 + 64 <= end && ((reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out) |
+                               size_t(a.ldb) * SIZE | size_t(a.ldo) * SIZE | size_t(n0) * SIZE) & 15) == 0;
+}
+// base to out, as it is.
+template <int OUT, int MT, int V, class T>
+__device__ __forceinline__ void ad_copy(const u32x4 (&have)[MT][V], const T* const (&base)[MT], T* const (&out)[MT], int rows, int n0,
+                                        int end, bool whole) {
+    constexpr int kPer = 16 / AdOut<OUT>::size;
+    const int lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        if (16 * m + li >= rows) continue;
+        if (whole) {
+#pragma unroll
+            for (int c = 0; c < V; ++c) *reinterpret_cast<u32x4*>(out[m] + (4 * c + q) * kPer) = have[m][c];
+        } else {
+            for (int i = q; i < 64 && n0 + i < end; i += 4) out[m][i] = base[m][i];
+        }
+    }
+}
+// base + by * acc, rounded, and what it raises.
+template <int OUT, int MT, int V, class T>
+__device__ __forceinline__ void ad_finish(const AdArgs& a, const f32x4 (&acc)[MT][4], const float (&by)[MT], const u32x4 (&have)[MT][V],
+                                          const T* const (&base)[MT], T* const (&out)[MT], int rows, int n0, int end, bool whole) {
+    constexpr int size = AdOut<OUT>::size, kPer = 16 / size;
+    const int lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
+    float most = 0.f, zero = 0.f;
+    auto sum = [&](uint32_t bits, int m, int j, int i) {
+        const float r = ad_float<OUT>(bits) + by[m] * acc[m][j][i];
+        most = fmaxf(most, __builtin_fabsf(r));
+        zero = __builtin_fmaf(r, 0.f, zero);
+        return ad_bits<OUT>(r);
+    };
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        if (16 * m + li >= rows) continue;
+        if (whole) {
+#pragma unroll
+            for (int c = 0; c < V; ++c) {
+                u32x4 r;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t h = have[m][c][e];
+                    if constexpr (size == 4) r[e] = sum(h, m, c, e);
+                    else r[e] = sum(h & 0xffffu, m, 2 * c + (e >> 1), 2 * (e & 1)) |
+                                sum(h >> 16, m, 2 * c + (e >> 1), 2 * (e & 1) + 1) << 16;
+                }
+                *reinterpret_cast<u32x4*>(out[m] + (4 * c + q) * kPer) = r;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int n = ad_column<OUT>(j, 4 * q + i);
+                    if (n0 + n < end) out[m][n] = T(sum(base[m][n], m, j, i));
+                }
+        }
+    }
+    // 16-bit results round to infinity from half a step above the type's largest value
+    const bool bad = zero != zero;
+    constexpr float limit = OUT == ORNITH_ADAPTER_BF16 ? 0x1.ffp127f : 65520.f;
+    flag_or(a.flags, (bad ? kAdNonfinite : 0u) | (OUT != ORNITH_ADAPTER_F32 && (bad || most >= limit) ? kAdNonfinite16 : 0u));
+}
+
 constexpr int kExpandWaves = 4;                        // a block: 64 columns a wave
 
-template <int TYPE, int OUT, int MT, bool FEW>
+template <int TYPE, int OUT, int MT, int FEW>
 __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArgs a) {
     extern __shared__ __attribute__((aligned(16))) u32x4 s_v[];        // [MT][steps][64]
     __shared__ uint32_t s_most[16 * MT];
@@ -324,9 +416,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
         base[m] = static_cast<const word*>(a.base) + size_t(t[m]) * size_t(a.ldb) + n0;
         out[m] = static_cast<word*>(a.out) + size_t(t[m]) * size_t(a.ldo) + n0;
     }
-    // whole groups on the 16-byte grid move in pieces of 16 bytes (wave-uniform)
-    const bool whole = n0 + 64 <= end && ((reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out) |
-                                           size_t(a.ldb) * size | size_t(a.ldo) * size | size_t(n0) * size) & 15) == 0;
+    const bool whole = ad_whole<size>(a, n0, end);
     u32x4 have[MT][kVec];
     if (whole) {
 #pragma unroll
@@ -335,18 +425,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
             for (int c = 0; c < kVec; ++c) have[m][c] = *reinterpret_cast<const u32x4*>(base[m] + (4 * c + q) * kPer);
     }
     if (slot < 0) {
-        if (whole) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int c = 0; c < kVec; ++c)
-                    if (16 * m + li < rows) *reinterpret_cast<u32x4*>(out[m] + (4 * c + q) * kPer) = have[m][c];
-        } else {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-                for (int i = q; i < 64; i += 4)
-                    if (16 * m + li < rows && n0 + i < end) out[m][i] = base[m][i];
-        }
+        ad_copy<OUT, MT>(have, base, out, rows, n0, end, whole);
         return;
     }
     const int chunks = a.R / 8, steps = (2 * chunks + 3) / 4;
@@ -377,11 +456,9 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
                 const float by = TYPE == ORNITH_ADAPTER_F16 ? ad_scale16(s_most[row]) : 1.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float f = v[e] * by;
-                    uint32_t bits = ad_bits<TYPE>(f);
-                    const float hi = ad_float<TYPE>(bits);
-                    if (c >= chunks) bits = __builtin_isinf(hi) ? 0u : ad_bits<TYPE>(f - hi);     // (inf: no NaN beside it)
-                    piece[e >> 1] |= bits << (16 * (e & 1));
+                    uint32_t hi, lo;
+                    ad_halves<TYPE>(v[e] * by, hi, lo);
+                    piece[e >> 1] |= (c < chunks ? hi : lo) << (16 * (e & 1));
                 }
             }
             s_v[((row >> 4) * steps + (c >> 2)) * 64 + (c & 3) * 16 + (row & 15)] = piece;
@@ -420,43 +497,147 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
             for (int j = 0; j < 4; ++j) acc[m][j] = ad_mfma<TYPE>(bv[j], vv, acc[m][j]);
         }
     }
-    float most = 0.f, zero = 0.f;
-    auto sum = [&](uint32_t bits, int m, int j, int i) {
-        const float r = ad_float<OUT>(bits) + by[m] * acc[m][j][i];
-        most = fmaxf(most, __builtin_fabsf(r));
-        zero = __builtin_fmaf(r, 0.f, zero);
-        return ad_bits<OUT>(r);
-    };
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        if (16 * m + li >= rows) continue;
+    ad_finish<OUT, MT>(a, acc, by, have, base, out, rows, n0, end, whole);
+}
+
+// ---- both in one ----------------------------------------------------------------
+// Few rows of a small rank: a block forms v of its tile for itself (its waves share k) and then 64 columns a
+// wave.  Every block of columns reads x and A again, from L2, and spares the second launch; what the second
+// product reads is on its way meanwhile.
+constexpr int kBothWaves = 8;
+
+template <int TYPE, int OUT, int RT, int FEW>
+__global__ __launch_bounds__(64 * kBothWaves) void adapter_both_kernel(AdArgs a) {
+    constexpr int W = kBothWaves, D = RT == 4 ? 2 : 4;
+    typedef typename AdOut<OUT>::type word;
+    constexpr int size = AdOut<OUT>::size, kPer = 16 / size, kVec = 4 * size / 4;
+    __shared__ f32x4 s_acc[W][RT][64];
+    __shared__ u32x4 s_v[RT][64];
+    __shared__ uint32_t s_most[16];
+    int slot, rows, t[1];
+    if (!ad_tile<1, FEW>(a, slot, rows, t) || (slot < 0 && a.in_place)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
+    int p = 0;
+    while (int(blockIdx.y) >= a.blocks[p]) ++p;
+    const int end = a.ends[p];
+    const int n0 = (p ? a.ends[p - 1] : 0) + ((int(blockIdx.y) - (p ? a.blocks[p - 1] : 0)) * W + wv) * 64;
+    const word* base[1] = {static_cast<const word*>(a.base) + size_t(t[0]) * size_t(a.ldb) + n0};
+    word* out[1] = {static_cast<word*>(a.out) + size_t(t[0]) * size_t(a.ldo) + n0};
+    const bool whole = ad_whole<size>(a, n0, end);
+    u32x4 have[1][kVec];
+    auto load_base = [&] {
         if (whole) {
 #pragma unroll
-            for (int c = 0; c < kVec; ++c) {
-                u32x4 r;
+            for (int c = 0; c < kVec; ++c) have[0][c] = *reinterpret_cast<const u32x4*>(base[0] + (4 * c + q) * kPer);
+        }
+    };
+    if (slot < 0) {
+        load_base();
+        ad_copy<OUT, 1>(have, base, out, rows, n0, end, whole);
+        return;
+    }
+    const int chunks = a.R / 8;
+    const uint16_t *x = a.x + size_t(t[0]) * size_t(a.ldx), *w[RT];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t h = have[m][c][e];
-                    if constexpr (size == 4) r[e] = sum(h, m, c, e);
-                    else r[e] = sum(h & 0xffffu, m, 2 * c + (e >> 1), 2 * (e & 1)) |
-                                sum(h >> 16, m, 2 * c + (e >> 1), 2 * (e & 1) + 1) << 16;
-                }
-                *reinterpret_cast<u32x4*>(out[m] + (4 * c + q) * kPer) = r;
+    for (int r = 0; r < RT; ++r)
+        w[r] = a.a + size_t(slot) * size_t(a.a_slot) + size_t(p * a.R + min(16 * r + li, a.R - 1)) * size_t(a.K);
+    const uint16_t* b[4];
+    u32x4 bv[RT][4];
+    const float scale = a.scales[slot];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        b[j] = a.b + size_t(slot) * size_t(a.b_slot) + size_t(min(n0 + ad_column<OUT>(j, li), end - 1)) * a.R;
+    f32x4 acc[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 64 * wv; k0 < a.K; k0 += 64 * W * D) {
+        u32x4 xv[D][2], wf[D][2][RT];
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (d && k0 + 64 * W * d >= a.K) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {              // (past K: its last piece, cleared below)
+                const int k = min(k0 + 64 * W * d + 32 * h + 8 * q, a.K - 8);
+                xv[d][h] = *reinterpret_cast<const u32x4*>(x + k);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) wf[d][h][r] = *reinterpret_cast<const u32x4*>(w[r] + k);
             }
-        } else {
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int d = 0; d < D; ++d) {
+            const int kd = k0 + 64 * W * d;
+            if (d && kd >= a.K) break;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int n = ad_column<OUT>(j, 4 * q + i);
-                    if (n0 + n < end) out[m][n] = word(sum(base[m][n], m, j, i));
+            for (int h = 0; h < 2; ++h) {
+                if (kd + 64 > a.K && kd + 32 * h + 8 * q >= a.K) {
+                    xv[d][h] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) wf[d][h][r] = u32x4{0, 0, 0, 0};
                 }
+#pragma unroll
+                for (int r = 0; r < RT; ++r) acc[r] = ad_mfma<TYPE>(xv[d][h], wf[d][h][r], acc[r]);
+            }
         }
     }
-    // 16-bit results round to infinity from half a step above the type's largest value
-    const bool bad = zero != zero;
-    constexpr float limit = OUT == ORNITH_ADAPTER_BF16 ? 0x1.ffp127f : 65520.f;
-    flag_or(a.flags, (bad ? kAdNonfinite : 0u) | (OUT != ORNITH_ADAPTER_F32 && (bad || most >= limit) ? kAdNonfinite16 : 0u));
+    load_base();
+#pragma unroll
+    for (int s = 0; s < RT; ++s) {
+        const int c = 4 * s + q, at = 8 * min(c < chunks ? c : c - chunks, chunks - 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bv[s][j] = *reinterpret_cast<const u32x4*>(b[j] + at);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) s_acc[wv][r][lane] = acc[r];
+    if (wv < RT) s_v[wv][lane] = u32x4{0, 0, 0, 0};
+    if (TYPE == ORNITH_ADAPTER_F16 && tid < 16) s_most[tid] = 0;
+    __syncthreads();
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    const int r = 16 * wv + li;                        // wave r's 16 of the rank
+    if (wv < RT) {
+        v = s_acc[0][wv][lane];
+#pragma unroll
+        for (int u = 1; u < W; ++u) {
+            const f32x4 part = s_acc[u][wv][lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += part[i];
+        }
+        if (TYPE == ORNITH_ADAPTER_F16 && r < a.R) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) atomicMax(&s_most[4 * q + i], __float_as_uint(v[i]) & 0x7fffffffu);
+        }
+    }
+    if (TYPE == ORNITH_ADAPTER_F16) __syncthreads();
+    if (wv < RT && r < a.R) {
+        uint16_t* s16 = reinterpret_cast<uint16_t*>(&s_v[0][0]);
+        auto put = [&](int c, int row, uint32_t bits) { s16[((c >> 2) * 64 + (c & 3) * 16 + row) * 8 + (r & 7)] = uint16_t(bits); };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 4 * q + i;
+            uint32_t hi, lo;
+            ad_halves<TYPE>(v[i] * (TYPE == ORNITH_ADAPTER_F16 ? ad_scale16(s_most[row]) : 1.f), hi, lo);
+            put(r >> 3, row, hi);
+            put((r >> 3) + chunks, row, lo);
+        }
+    }
+    __syncthreads();
+    if (n0 >= end) return;
+    float by[1] = {scale};
+    if constexpr (TYPE == ORNITH_ADAPTER_F16) by[0] = by[0] / ad_scale16(s_most[li]);
+    f32x4 sum[1][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < RT; ++s) {
+        if (4 * s >= 2 * chunks) break;
+        const u32x4 vv = s_v[s][lane];
+        if (4 * s + q >= 2 * chunks) {                 // (no 0 times inf)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bv[s][j] = u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[0][j] = ad_mfma<TYPE>(bv[s][j], vv, sum[0][j]);
+    }
+    ad_finish<OUT, 1>(a, sum, by, have, base, out, rows, n0, end, whole);
 }
 
 struct AdLayout { size_t v, order, tiles, count, bytes; };
@@ -472,34 +653,66 @@ bool ad_layout(int64_t M, int S, int R, AdLayout& l) {
     return true;
 }
 
-template <int TYPE, int MT, bool FEW> hipError_t ad_run(const AdArgs& a, int out_type, int tiles, hipStream_t s) {
+// Column blocks of 64 W columns, slice by slice.
+int ad_blocks(AdArgs& a, int W) {
+    int blocks = 0;
+    for (int p = 0; p < a.S; ++p) {
+        blocks += (a.ends[p] - (p ? a.ends[p - 1] : 0) + 64 * W - 1) / (64 * W);
+        a.blocks[p] = blocks;
+    }
+    return blocks;
+}
+// f with the output's type as a constant.
+template <class F> void ad_by_type(int out_type, F&& f) {
+    if (out_type == ORNITH_ADAPTER_F32) f(std::integral_constant<int, ORNITH_ADAPTER_F32>{});
+    else if (out_type == ORNITH_ADAPTER_BF16) f(std::integral_constant<int, ORNITH_ADAPTER_BF16>{});
+    else f(std::integral_constant<int, ORNITH_ADAPTER_F16>{});
+}
+
+template <int TYPE, int FEW> hipError_t ad_both(AdArgs& a, int out_type, hipStream_t s) {
+    const dim3 grid(a.M, ad_blocks(a, kBothWaves));
+    auto go = [&](auto kernel) { timed_launch("adapter_both", kernel, grid, dim3(64 * kBothWaves), 0, s, a); };
+    ad_by_type(out_type, [&](auto out) {
+        constexpr int OUT = decltype(out)::value;
+        if (a.R <= 16) go(adapter_both_kernel<TYPE, OUT, 1, FEW>);
+        else if (a.R <= 32) go(adapter_both_kernel<TYPE, OUT, 2, FEW>);
+        else go(adapter_both_kernel<TYPE, OUT, 4, FEW>);
+    });
+    return hipGetLastError();
+}
+
+template <int TYPE, int MT, int FEW> hipError_t ad_two(AdArgs& a, int out_type, int tiles, hipStream_t s) {
     const int rt = (a.SR + 15) / 16;
     auto shrink = [&](auto kernel, int RT, int W) {
         timed_launch("adapter_shrink", kernel, dim3(tiles, (rt + RT - 1) / RT), dim3(64 * W), 0, s, a);
     };
-    if (MT == 1 || rt == 1) shrink(adapter_shrink_kernel<TYPE, MT, 1, 8, MT == 1 ? 4 : 2, FEW>, 1, 8);
+    if constexpr (MT == 1) shrink(adapter_shrink_kernel<TYPE, MT, 1, 8, 4, FEW>, 1, 8);
+    else if (rt == 1) shrink(adapter_shrink_kernel<TYPE, MT, 1, 8, 2, FEW>, 1, 8);
     else shrink(adapter_shrink_kernel<TYPE, MT, 2, 8, 1, FEW>, 2, 8);
-    hipError_t st = hipGetLastError();
+    const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
+    const dim3 grid(tiles, ad_blocks(a, kExpandWaves));
     const int steps = (a.R / 4 + 3) / 4;
-    auto expand = [&](auto kernel) {
-        timed_launch("adapter_expand", kernel, dim3(tiles, a.blocks[a.S - 1]), dim3(64 * kExpandWaves), uint32_t(MT * steps * 1024), s, a);
-    };
-    if (out_type == ORNITH_ADAPTER_F32) expand(adapter_expand_kernel<TYPE, ORNITH_ADAPTER_F32, MT, FEW>);
-    else if (out_type == ORNITH_ADAPTER_BF16) expand(adapter_expand_kernel<TYPE, ORNITH_ADAPTER_BF16, MT, FEW>);
-    else expand(adapter_expand_kernel<TYPE, ORNITH_ADAPTER_F16, MT, FEW>);
+    ad_by_type(out_type, [&](auto out) {
+        timed_launch("adapter_expand", adapter_expand_kernel<TYPE, decltype(out)::value, MT, FEW>, grid, dim3(64 * kExpandWaves),
+                     uint32_t(MT * steps * 1024), s, a);
+    });
     return hipGetLastError();
 }
 
-template <int TYPE> hipError_t ad_rows(const AdArgs& a, int out_type, hipStream_t s) {
-    if (a.M <= kFewRows) return ad_run<TYPE, 1, true>(a, out_type, a.M, s);
+template <int TYPE> hipError_t ad_rows(AdArgs& a, int out_type, hipStream_t s) {
+    if (a.M <= kFewRows) {
+        const bool both = a.R <= 64;
+        if (a.M <= 64) return both ? ad_both<TYPE, 1>(a, out_type, s) : ad_two<TYPE, 1, 1>(a, out_type, a.M, s);
+        return both ? ad_both<TYPE, 4>(a, out_type, s) : ad_two<TYPE, 1, 4>(a, out_type, a.M, s);
+    }
     // tiles of 64 rows where they are many and v of them fits LDS
     const int tile_rows = a.M >= 1024 && a.R <= 128 ? 64 : 16;
     const int tiles = std::min(a.M, (a.M + tile_rows - 1) / tile_rows + a.slots + 1);
     timed_launch("adapter_plan", adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, tile_rows);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
-    return tile_rows == 64 ? ad_run<TYPE, 4, false>(a, out_type, tiles, s) : ad_run<TYPE, 1, false>(a, out_type, tiles, s);
+    return tile_rows == 64 ? ad_two<TYPE, 4, 0>(a, out_type, tiles, s) : ad_two<TYPE, 1, 0>(a, out_type, tiles, s);
 }
 
 }  // namespace
@@ -570,13 +783,7 @@ extern "C" hipError_t ornith_adapter_launch(const void* x, int x_type, int64_t l
     args.S = S;
     args.slots = slots;
     args.in_place = in_place;
-    int blocks = 0;
-    for (int p = 0; p < S; ++p) {
-        args.ends[p] = slice_ends[p];
-        const int width = slice_ends[p] - (p ? slice_ends[p - 1] : 0);
-        blocks += (width + 64 * kExpandWaves - 1) / (64 * kExpandWaves);
-        args.blocks[p] = blocks;
-    }
+    for (int p = 0; p < S; ++p) args.ends[p] = slice_ends[p];
     for (int64_t r = 0; r < M; r += kAdRows) {
         args.M = int(std::min<int64_t>(M - r, kAdRows));
         args.x = static_cast<const uint16_t*>(x) + size_t(r) * size_t(ldx);
