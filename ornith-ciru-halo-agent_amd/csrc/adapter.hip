@@ -49,11 +49,12 @@ struct AdArgs {
     const void* base; int64_t ldb;
     void* out; int64_t ldo;
     uint32_t* flags;
-    float* v;                                          // [M, SR]
+    float* v;                                          // [splits, M, SR]
     int32_t* order;                                    // [M]
     AdTile* tiles;
     int32_t* ntiles;
     int M, N, K, R, SR, slots, S;
+    int sub, splits;                                   // shrink: parts of a tile, and of K
     bool in_place;
     int ends[kAdMaxSlices];                            // of the slices, in columns
     int blocks[kAdMaxSlices];                          // of the expand's column blocks, running
@@ -69,7 +70,7 @@ constexpr int kFewRows = 256, kPlanThreads = 1024, kPlanBatch = 8;
 __device__ __forceinline__ int ad_key(int id, int slots) { return id >= 0 && id < slots ? id + 1 : 0; }      // 0: no adapter
 
 // Lane li's row of the tile (past the last row: that one again), and the tile.  FEW: ids a lane looks at (0: a plan).
-template <int MT, int FEW> __device__ __forceinline__ bool ad_tile(const AdArgs& a, int& slot, int& rows, int (&t)[MT]) {
+template <int MT, int FEW> __device__ __forceinline__ bool ad_tile(const AdArgs& a, int unit, int sub, bool first, int& slot, int& rows, int (&t)[MT]) {
     const int lane = threadIdx.x & 63, li = lane & 15;
     if constexpr (FEW > 0) {
         static_assert(MT == 1);
@@ -82,13 +83,13 @@ template <int MT, int FEW> __device__ __forceinline__ bool ad_tile(const AdArgs&
         for (int j = 0; j < FEW; ++j) {
             bad |= key[j] >= a.slots ? kAdBadId : 0u;
             key[j] = ad_key(key[j], a.slots);
-            if (int(blockIdx.x >> 6) == j) mine = __builtin_amdgcn_readlane(key[j], int(blockIdx.x & 63));
+            if (unit >> 6 == j) mine = __builtin_amdgcn_readlane(key[j], unit & 63);
         }
-        if (blockIdx.x == 0 && blockIdx.y == 0) flag_or(a.flags, bad);
+        if (first) flag_or(a.flags, bad);
 #pragma unroll
         for (int j = 0; j < FEW; ++j) {
             same[j] = __ballot(key[j] == mine && 64 * j + lane < a.M);
-            const int below = min(max(int(blockIdx.x) - 64 * j, 0), 64);       // lanes of rows before this block's
+            const int below = min(max(unit - 64 * j, 0), 64);                  // lanes of rows before this one
             before += __popcll(below < 64 ? same[j] & ((uint64_t(1) << below) - 1) : same[j]);
             all += __popcll(same[j]);
         }
@@ -106,12 +107,13 @@ template <int MT, int FEW> __device__ __forceinline__ bool ad_tile(const AdArgs&
         t[0] = __builtin_amdgcn_ds_bpermute(4 * min(li, rows - 1), sent) - 1;
     } else {
         const int n = *a.ntiles;
-        const AdTile tile = a.tiles[blockIdx.x];       // (a tile's place, if not a tile)
-        if (int(blockIdx.x) >= n) return false;
+        const AdTile tile = a.tiles[unit / sub];     // (a tile's place, if not a tile)
+        const int at = unit % sub * (16 * MT);       // (a tile in several parts)
+        if (unit / sub >= n || at >= tile.rows) return false;
         slot = tile.slot;
-        rows = tile.rows;
+        rows = tile.rows - at;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) t[m] = a.order[tile.first + min(16 * m + li, rows - 1)];
+        for (int m = 0; m < MT; ++m) t[m] = a.order[tile.first + at + min(16 * m + li, rows - 1)];
     }
     return true;
 }
@@ -214,71 +216,115 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(AdArgs a, in
 }
 
 // ---- shrink ---------------------------------------------------------------------
-// A wave takes 64 k of every 64 W; D such pieces are loaded before the first product.
-template <int TYPE, int MT, int RT, int W, int D, int FEW>
-__global__ __launch_bounds__(64 * W) void adapter_shrink_kernel(AdArgs a) {
-    __shared__ f32x4 s_acc[W][MT * RT][64];
-    int slot, rows, t[MT];
-    if (!ad_tile<MT, FEW>(a, slot, rows, t) || slot < 0) return;
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
-    const int r0 = int(blockIdx.y) * 16 * RT;
-    const uint16_t *x[MT], *w[RT];
+// acc[m][r] += x A over k in [kbegin, kend), a wave's share of it: 64 k of every 64 W, D such pieces loaded
+// before the first product.  The instruction wants neighbouring lanes in different rows, and such loads (64
+// lines' halves at a time) were what few rows waited for: one block's 16 x 2048 of A took 2.4 us, of the 3.3 of
+// a call without them, against 0.9 with eight lanes on the 128 bytes of a row.  So those, and through LDS to the
+// operands' order: piece c (16 bytes) of row r at 8 r + (c ^ r % 8), free of bank conflicts both ways; a wave's
+// own LDS, which needs no barrier.
+template <int TYPE, int MT, int RT, int W, int D>
+__device__ __forceinline__ void ad_accumulate(const AdArgs& a, const int (&t)[MT], int rows, const uint16_t* w, int wrows,
+                                              u32x4* stage, int kbegin, int kend, f32x4 (&acc)[MT][RT]) {
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), li = lane & 15, q = lane >> 4;
+    const int lrow = lane >> 3, piece = lane & 7;
+    const uint16_t* x[MT][2];
+    uint32_t of[RT][2];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) x[m] = a.x + size_t(t[m]) * size_t(a.ldx);
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
-        w[r] = a.a + size_t(slot) * size_t(a.a_slot) + size_t(min(r0 + 16 * r + li, a.SR - 1)) * size_t(a.K);
-    f32x4 acc[MT][RT];
+        for (int m = 0; m < MT; ++m)
+            x[m][h] = a.x + size_t(__builtin_amdgcn_ds_bpermute(4 * (8 * h + lrow), t[m])) * size_t(a.ldx);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 64 * wv; k0 < a.K; k0 += 64 * W * D) {
+        for (int r = 0; r < RT; ++r) of[r][h] = uint32_t(min(16 * r + 8 * h + lrow, wrows - 1)) * uint32_t(a.K);
+    }
+    u32x4* const put = stage + 8 * lrow + (piece ^ lrow);              // (row 8 h + lrow: 64 h further)
+    const u32x4* const get[2] = {stage + 8 * li + (q ^ (li & 7)), stage + 8 * li + ((4 + q) ^ (li & 7))};
+    for (int k0 = kbegin + 64 * wv; k0 < kend; k0 += 64 * W * D) {
         u32x4 xv[D][2][MT], wf[D][2][RT];
 #pragma unroll
         for (int d = 0; d < D; ++d) {
-            if (d && k0 + 64 * W * d >= a.K) break;
+            if (d && k0 + 64 * W * d >= kend) break;
+            const int k = min(k0 + 64 * W * d + 8 * piece, a.K - 8);   // (past K: its last piece, cleared below)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {              // (past K: its last piece, cleared below)
-                const int k = min(k0 + 64 * W * d + 32 * h + 8 * q, a.K - 8);
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m) xv[d][h][m] = *reinterpret_cast<const u32x4*>(x[m] + k);
+                for (int r = 0; r < RT; ++r) wf[d][h][r] = *reinterpret_cast<const u32x4*>(w + (of[r][h] + uint32_t(k)));
 #pragma unroll
-                for (int r = 0; r < RT; ++r) wf[d][h][r] = *reinterpret_cast<const u32x4*>(w[r] + k);
+                for (int m = 0; m < MT; ++m)
+                    if (16 * m + 8 * h < rows) xv[d][h][m] = *reinterpret_cast<const u32x4*>(x[m][h] + k);
             }
         }
 #pragma unroll
         for (int d = 0; d < D; ++d) {
             const int kd = k0 + 64 * W * d;
-            if (d && kd >= a.K) break;
-            if (kd + 64 > a.K) {
+            if (d && kd >= kend) break;
+            if (kd + 64 > a.K && kd + 8 * piece >= a.K) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (kd + 32 * h + 8 * q >= a.K) {
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) xv[d][h][m] = u32x4{0, 0, 0, 0};
+                    for (int r = 0; r < RT; ++r) wf[d][h][r] = u32x4{0, 0, 0, 0};
 #pragma unroll
-                        for (int r = 0; r < RT; ++r) wf[d][h][r] = u32x4{0, 0, 0, 0};
-                    }
+                    for (int m = 0; m < MT; ++m) xv[d][h][m] = u32x4{0, 0, 0, 0};
+                }
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) put[128 * r + 64 * h] = wf[d][h][r];
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    if (16 * m + 8 * h < rows) put[128 * (RT + m) + 64 * h] = xv[d][h][m];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                u32x4 av[MT], bv[RT];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) av[m] = get[h][128 * (RT + m)];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) bv[r] = get[h][128 * r];
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) acc[m][r] = ad_mfma<TYPE>(xv[d][h][m], wf[d][h][r], acc[m][r]);
+                    for (int r = 0; r < RT; ++r) acc[m][r] = ad_mfma<TYPE>(av[m], bv[r], acc[m][r]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
     }
+}
+
+constexpr int kShrinkWaves = 8;
+
+template <int TYPE, int MT, int RT, int D, int FEW>
+__global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(AdArgs a) {
+    constexpr int W = kShrinkWaves;
+    __shared__ u32x4 s_stage[W][(MT + RT) * 128];      // (then the waves' sums)
+    static_assert((MT + RT) * 128 >= MT * RT * 64);
+    int slot, rows, t[MT];
+    if (!ad_tile<MT, FEW>(a, blockIdx.x, a.sub, blockIdx.x + blockIdx.y + blockIdx.z == 0, slot, rows, t) || slot < 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
+    const int part = ((a.K + 63) / 64 + a.splits - 1) / a.splits * 64, kbegin = int(blockIdx.z) * part, kend = min(kbegin + part, a.K);
+    const int r0 = int(blockIdx.y) * 16 * RT;
+    f32x4 acc[MT][RT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int r = 0; r < RT; ++r) s_acc[wv][m * RT + r][lane] = acc[m][r];
+        for (int r = 0; r < RT; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    ad_accumulate<TYPE, MT, RT, W, D>(a, t, rows, a.a + size_t(slot) * size_t(a.a_slot) + size_t(r0) * size_t(a.K), a.SR - r0,
+                                      s_stage[wv], kbegin, kend, acc);
+    f32x4* mine = reinterpret_cast<f32x4*>(s_stage[wv]) + lane;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) mine[64 * (m * RT + r)] = acc[m][r];
     __syncthreads();
     for (int f = wv; f < MT * RT; f += W) {
-        f32x4 v = s_acc[0][f][lane];
+        f32x4 v = reinterpret_cast<const f32x4*>(s_stage[0])[64 * f + lane];
 #pragma unroll
         for (int u = 1; u < W; ++u) {
-            const f32x4 p = s_acc[u][f][lane];
+            const f32x4 p = reinterpret_cast<const f32x4*>(s_stage[u])[64 * f + lane];
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += p[i];
         }
@@ -289,7 +335,7 @@ __global__ __launch_bounds__(64 * W) void adapter_shrink_kernel(AdArgs a) {
 #pragma unroll
             for (int mm = 1; mm < MT; ++mm) of = m == mm ? t[mm] : of;
             of = __builtin_amdgcn_ds_bpermute(4 * (4 * q + i), of);
-            if (r < a.SR && 16 * m + 4 * q + i < rows) a.v[size_t(of) * a.SR + r] = v[i];
+            if (r < a.SR && 16 * m + 4 * q + i < rows) a.v[(size_t(blockIdx.z) * a.M + of) * a.SR + r] = v[i];
         }
     }
 }
@@ -403,7 +449,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
     typedef typename AdOut<OUT>::type word;
     constexpr int size = AdOut<OUT>::size, kPer = 16 / size, kVec = 4 * size / 4;    // values of 16 bytes, such pieces a lane
     int slot, rows, t[MT];
-    if (!ad_tile<MT, FEW>(a, slot, rows, t) || (slot < 0 && a.in_place)) return;
+    if (!ad_tile<MT, FEW>(a, blockIdx.x, 1, false, slot, rows, t) || (slot < 0 && a.in_place)) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
     int p = 0;
     while (int(blockIdx.y) >= a.blocks[p]) ++p;
@@ -437,13 +483,27 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
         }
         if (TYPE == ORNITH_ADAPTER_F16 && tid < 16 * MT) s_most[tid] = 0;
         __syncthreads();
-        auto piece_of = [&](int row, int c) { return a.v + size_t(s_t[row]) * a.SR + p * a.R + 8 * c; };
+        struct Piece { f32x4 v[2]; };
+        auto piece_of = [&](int row, int c) {          // the parts of K in order
+            const float* from = a.v + size_t(s_t[row]) * a.SR + p * a.R + 8 * c;
+            Piece sum{{*reinterpret_cast<const f32x4*>(from), *reinterpret_cast<const f32x4*>(from + 4)}};
+            for (int z = 1; z < a.splits; ++z) {
+                from += size_t(a.M) * a.SR;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x4 part = *reinterpret_cast<const f32x4*>(from + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum.v[h][e] += part[e];
+                }
+            }
+            return sum;
+        };
         if constexpr (TYPE == ORNITH_ADAPTER_F16) {
             for (int i = tid; i < 16 * MT * chunks; i += 64 * kExpandWaves) {
-                const float* v = piece_of(i / chunks, i % chunks);
+                const Piece v = piece_of(i / chunks, i % chunks);
                 uint32_t most = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
+                for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v.v[e >> 2][e & 3]) & 0x7fffffffu);
                 atomicMax(&s_most[i / chunks], most);
             }
             __syncthreads();
@@ -452,12 +512,12 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
             const int row = i / (steps * 4), c = i % (steps * 4);
             u32x4 piece = {0, 0, 0, 0};
             if (c < 2 * chunks) {
-                const float* v = piece_of(row, c < chunks ? c : c - chunks);
+                const Piece v = piece_of(row, c < chunks ? c : c - chunks);
                 const float by = TYPE == ORNITH_ADAPTER_F16 ? ad_scale16(s_most[row]) : 1.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     uint32_t hi, lo;
-                    ad_halves<TYPE>(v[e] * by, hi, lo);
+                    ad_halves<TYPE>(v.v[e >> 2][e & 3] * by, hi, lo);
                     piece[e >> 1] |= (c < chunks ? hi : lo) << (16 * (e & 1));
                 }
             }
@@ -511,16 +571,19 @@ __global__ __launch_bounds__(64 * kBothWaves) void adapter_both_kernel(AdArgs a)
     constexpr int W = kBothWaves, D = RT == 4 ? 2 : 4;
     typedef typename AdOut<OUT>::type word;
     constexpr int size = AdOut<OUT>::size, kPer = 16 / size, kVec = 4 * size / 4;
-    __shared__ f32x4 s_acc[W][RT][64];
+    __shared__ u32x4 s_stage[W][(1 + RT) * 128];       // (then the waves' sums)
     __shared__ u32x4 s_v[RT][64];
     __shared__ uint32_t s_most[16];
     int slot, rows, t[1];
-    if (!ad_tile<1, FEW>(a, slot, rows, t) || (slot < 0 && a.in_place)) return;
+    // blocks go to the 8 XCDs in turn: a row's column blocks on one of them, whose L2 keeps its A
+    const int nblocks = a.blocks[a.S - 1], unit = int(blockIdx.x / 8) / nblocks * 8 + int(blockIdx.x % 8);
+    const int cb = int(blockIdx.x / 8) % nblocks;
+    if (unit >= a.M || !ad_tile<1, FEW>(a, unit, 1, blockIdx.x == 0, slot, rows, t) || (slot < 0 && a.in_place)) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
     int p = 0;
-    while (int(blockIdx.y) >= a.blocks[p]) ++p;
+    while (cb >= a.blocks[p]) ++p;
     const int end = a.ends[p];
-    const int n0 = (p ? a.ends[p - 1] : 0) + ((int(blockIdx.y) - (p ? a.blocks[p - 1] : 0)) * W + wv) * 64;
+    const int n0 = (p ? a.ends[p - 1] : 0) + ((cb - (p ? a.blocks[p - 1] : 0)) * W + wv) * 64;
     const word* base[1] = {static_cast<const word*>(a.base) + size_t(t[0]) * size_t(a.ldb) + n0};
     word* out[1] = {static_cast<word*>(a.out) + size_t(t[0]) * size_t(a.ldo) + n0};
     const bool whole = ad_whole<size>(a, n0, end);
@@ -537,48 +600,17 @@ __global__ __launch_bounds__(64 * kBothWaves) void adapter_both_kernel(AdArgs a)
         return;
     }
     const int chunks = a.R / 8;
-    const uint16_t *x = a.x + size_t(t[0]) * size_t(a.ldx), *w[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-        w[r] = a.a + size_t(slot) * size_t(a.a_slot) + size_t(p * a.R + min(16 * r + li, a.R - 1)) * size_t(a.K);
     const uint16_t* b[4];
     u32x4 bv[RT][4];
     const float scale = a.scales[slot];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         b[j] = a.b + size_t(slot) * size_t(a.b_slot) + size_t(min(n0 + ad_column<OUT>(j, li), end - 1)) * a.R;
-    f32x4 acc[RT];
+    f32x4 acc[1][RT];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 64 * wv; k0 < a.K; k0 += 64 * W * D) {
-        u32x4 xv[D][2], wf[D][2][RT];
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-            if (d && k0 + 64 * W * d >= a.K) break;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {              // (past K: its last piece, cleared below)
-                const int k = min(k0 + 64 * W * d + 32 * h + 8 * q, a.K - 8);
-                xv[d][h] = *reinterpret_cast<const u32x4*>(x + k);
-#pragma unroll
-                for (int r = 0; r < RT; ++r) wf[d][h][r] = *reinterpret_cast<const u32x4*>(w[r] + k);
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-            const int kd = k0 + 64 * W * d;
-            if (d && kd >= a.K) break;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (kd + 64 > a.K && kd + 32 * h + 8 * q >= a.K) {
-                    xv[d][h] = u32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) wf[d][h][r] = u32x4{0, 0, 0, 0};
-                }
-#pragma unroll
-                for (int r = 0; r < RT; ++r) acc[r] = ad_mfma<TYPE>(xv[d][h], wf[d][h][r], acc[r]);
-            }
-        }
-    }
+    for (int r = 0; r < RT; ++r) acc[0][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    ad_accumulate<TYPE, 1, RT, W, D>(a, t, rows, a.a + size_t(slot) * size_t(a.a_slot) + size_t(p * a.R) * size_t(a.K), a.R,
+                                     s_stage[wv], 0, a.K, acc);
     load_base();
 #pragma unroll
     for (int s = 0; s < RT; ++s) {
@@ -587,17 +619,17 @@ __global__ __launch_bounds__(64 * kBothWaves) void adapter_both_kernel(AdArgs a)
         for (int j = 0; j < 4; ++j) bv[s][j] = *reinterpret_cast<const u32x4*>(b[j] + at);
     }
 #pragma unroll
-    for (int r = 0; r < RT; ++r) s_acc[wv][r][lane] = acc[r];
+    for (int r = 0; r < RT; ++r) reinterpret_cast<f32x4*>(s_stage[wv])[64 * r + lane] = acc[0][r];
     if (wv < RT) s_v[wv][lane] = u32x4{0, 0, 0, 0};
     if (TYPE == ORNITH_ADAPTER_F16 && tid < 16) s_most[tid] = 0;
     __syncthreads();
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     const int r = 16 * wv + li;                        // wave r's 16 of the rank
     if (wv < RT) {
-        v = s_acc[0][wv][lane];
+        v = reinterpret_cast<const f32x4*>(s_stage[0])[64 * wv + lane];
 #pragma unroll
         for (int u = 1; u < W; ++u) {
-            const f32x4 part = s_acc[u][wv][lane];
+            const f32x4 part = reinterpret_cast<const f32x4*>(s_stage[u])[64 * wv + lane];
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += part[i];
         }
@@ -642,11 +674,14 @@ __global__ __launch_bounds__(64 * kBothWaves) void adapter_both_kernel(AdArgs a)
 
 struct AdLayout { size_t v, order, tiles, count, bytes; };
 
+// Parts of K that a shrink of M rows may have (each has a v of its own).
+int ad_splits(int64_t M) { return M <= kFewRows ? 4 : 1; }
+
 bool ad_layout(int64_t M, int S, int R, AdLayout& l) {
     if (M < 0 || S < 1 || S > kAdMaxSlices || R < 8 || R > kAdMaxR || R % 8) return false;
     const size_t rows = size_t(std::min<int64_t>(M, kAdRows));
     l.v = 0;
-    l.order = align256(rows * size_t(S) * size_t(R) * 4);
+    l.order = align256(rows * size_t(S) * size_t(R) * 4 * size_t(ad_splits(M)));
     l.tiles = l.order + align256(rows * 4);
     l.count = l.tiles + align256(rows * sizeof(AdTile));
     l.bytes = l.count + 256;
@@ -670,7 +705,7 @@ template <class F> void ad_by_type(int out_type, F&& f) {
 }
 
 template <int TYPE, int FEW> hipError_t ad_both(AdArgs& a, int out_type, hipStream_t s) {
-    const dim3 grid(a.M, ad_blocks(a, kBothWaves));
+    const dim3 grid((a.M + 7) / 8 * 8 * ad_blocks(a, kBothWaves));
     auto go = [&](auto kernel) { timed_launch("adapter_both", kernel, grid, dim3(64 * kBothWaves), 0, s, a); };
     ad_by_type(out_type, [&](auto out) {
         constexpr int OUT = decltype(out)::value;
@@ -683,12 +718,14 @@ template <int TYPE, int FEW> hipError_t ad_both(AdArgs& a, int out_type, hipStre
 
 template <int TYPE, int MT, int FEW> hipError_t ad_two(AdArgs& a, int out_type, int tiles, hipStream_t s) {
     const int rt = (a.SR + 15) / 16;
-    auto shrink = [&](auto kernel, int RT, int W) {
-        timed_launch("adapter_shrink", kernel, dim3(tiles, (rt + RT - 1) / RT), dim3(64 * W), 0, s, a);
+    constexpr int SMT = 1;
+    a.sub = MT / SMT;
+    a.splits = std::min(ad_splits(a.M), (a.K + 511) / 512);
+    a.splits = std::max(a.splits, 1);
+    auto shrink = [&](auto kernel, int RT) {
+        timed_launch("adapter_shrink", kernel, dim3(tiles * a.sub, (rt + RT - 1) / RT, a.splits), dim3(64 * kShrinkWaves), 0, s, a);
     };
-    if constexpr (MT == 1) shrink(adapter_shrink_kernel<TYPE, MT, 1, 8, 4, FEW>, 1, 8);
-    else if (rt == 1) shrink(adapter_shrink_kernel<TYPE, MT, 1, 8, 2, FEW>, 1, 8);
-    else shrink(adapter_shrink_kernel<TYPE, MT, 2, 8, 1, FEW>, 2, 8);
+    shrink(adapter_shrink_kernel<TYPE, SMT, 1, 4, FEW>, 1);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
     const dim3 grid(tiles, ad_blocks(a, kExpandWaves));
