@@ -8,9 +8,8 @@
 //   expand  out[t, n] = base[t, n] + scale sum_r B[n, r] v[t, r]: v, fp32, as the
 //           sum of two 16-bit numbers hi + lo side by side along r, so the
 //           second product loses no more than 2^-17 of it.  The product is
-//           formed transposed (columns as rows of the instruction), with the
-//           columns dealt so that a lane ends with 16 neighbouring ones of one
-//           row: base and out move in 16-byte accesses, 128 bytes a row and wave.
+//           formed transposed (columns as rows of the instruction) and goes
+//           through LDS to lanes that move whole rows' pieces of base and out.
 #include <algorithm>
 #include <type_traits>
 #include "kernels.hpp"
@@ -24,6 +23,7 @@ namespace {
 constexpr int kAdMaxN = 1 << 20, kAdMaxK = 65536, kAdMaxSlices = ORNITH_ADAPTER_MAX_SLICES,
               kAdMaxSlots = ORNITH_ADAPTER_MAX_SLOTS, kAdMaxR = ORNITH_ADAPTER_MAX_RANK;
 constexpr int kAdRows = 1 << 20;                       // rows of one pass
+constexpr int kBothRank = 64;                          // ranks that both products of one launch take
 enum : uint32_t { kAdNonfinite = 4, kAdNonfinite16 = 8, kAdBadId = 16 };
 
 typedef __bf16 ad_bf16x8 __attribute__((ext_vector_type(8)));
@@ -38,7 +38,8 @@ template <int TYPE> __device__ __forceinline__ f32x4 ad_mfma(u32x4 a, u32x4 b, f
                                                       __builtin_bit_cast(ad_f16x8, b), c, 0, 0, 0);
 }
 
-struct AdTile { int slot, first, rows; };              // rows order[first ..]; slot -1: no adapter
+// A planned tile: its slot (-1: no adapter, -2: no tile), its number of rows, and them; 2 + tile_rows words.
+constexpr int kTileHead = 2;
 
 struct AdArgs {
     const uint16_t* x; int64_t ldx;
@@ -50,11 +51,11 @@ struct AdArgs {
     void* out; int64_t ldo;
     uint32_t* flags;
     float* v;                                          // [splits, M, SR]
-    int32_t* order;                                    // [M]
-    AdTile* tiles;
-    int32_t* ntiles;
+    int32_t* tiles;                                    // [units, 2 + tile_rows]
+    int tile_rows;
     int M, N, K, R, SR, slots, S;
     int sub, splits;                                   // shrink: parts of a tile, and of K
+    int units, groups;                                 // tiles at most; both: groups of 64 columns a wave
     bool in_place;
     int ends[kAdMaxSlices];                            // of the slices, in columns
     int blocks[kAdMaxSlices];                          // of the expand's column blocks, running
@@ -106,14 +107,24 @@ template <int MT, int FEW> __device__ __forceinline__ bool ad_tile(const AdArgs&
         }
         t[0] = __builtin_amdgcn_ds_bpermute(4 * min(li, rows - 1), sent) - 1;
     } else {
-        const int n = *a.ntiles;
-        const AdTile tile = a.tiles[unit / sub];     // (a tile's place, if not a tile)
-        const int at = unit % sub * (16 * MT);       // (a tile in several parts)
-        if (unit / sub >= n || at >= tile.rows) return false;
-        slot = tile.slot;
-        rows = tile.rows - at;
+        const int32_t* tile = a.tiles + size_t(unit / sub) * size_t(kTileHead + a.tile_rows);
+        const int at = unit % sub * (16 * MT);         // (a tile in several parts)
+        slot = tile[0];
+        rows = tile[1] - at;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) t[m] = a.order[tile.first + at + min(16 * m + li, rows - 1)];
+        for (int m = 0; m < MT; ++m) t[m] = tile[kTileHead + at + 16 * m + li];    // (past its rows: of no use)
+        if (slot < -1 || rows <= 0) return false;
+#pragma unroll
+        for (int m = MT - 1; m >= 0; --m) {            // (from the last: its source is not yet replaced)
+            const int last = min(rows - 1, 16 * MT - 1), from = 16 * m + li <= last ? 16 * m + li : last;
+            int row = t[0];
+#pragma unroll
+            for (int mm = 0; mm < MT; ++mm) {
+                const int other = __builtin_amdgcn_ds_bpermute(4 * (from & 15), t[mm]);
+                row = from >> 4 == mm ? other : row;
+            }
+            t[m] = row;
+        }
     }
     return true;
 }
@@ -157,62 +168,72 @@ __device__ __forceinline__ int ad_take(int* counter, int key) {
     return place;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(AdArgs a, int tile_rows) {
-    __shared__ int s_at[kAdMaxSlots + 1], s_first[kAdMaxSlots + 2], s_tile[kAdMaxSlots + 2], s_wave[kPlanThreads / 64];
-    const int tid = threadIdx.x, keys = a.slots + 1;
-    for (int i = tid; i < keys; i += kPlanThreads) s_at[i] = 0;
+__global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(AdArgs a) {
+    __shared__ int s_count[kAdMaxSlots + 1], s_tile[kAdMaxSlots + 2], s_wave[kPlanThreads / 64];
+    const int tid = threadIdx.x, keys = a.slots + 1, span = kTileHead + a.tile_rows;
+    for (int i = tid; i < keys; i += kPlanThreads) s_count[i] = 0;
     __syncthreads();
     uint32_t flags = 0;
-    auto each = [&](auto&& f) {                        // f(row, key) of a batch of rows, whose ids are loaded at once
-        for (int t0 = 0; t0 < a.M; t0 += kPlanThreads * kPlanBatch) {
-            int id[kPlanBatch];
+    int id[kPlanBatch], place[kPlanBatch];
+    auto take = [&](int t0) {                          // ids of a batch of rows, loaded at once, and their places
 #pragma unroll
-            for (int j = 0; j < kPlanBatch; ++j) id[j] = a.ids[min(t0 + j * kPlanThreads + tid, a.M - 1)];
+        for (int j = 0; j < kPlanBatch; ++j) id[j] = a.ids[min(t0 + j * kPlanThreads + tid, a.M - 1)];
 #pragma unroll
-            for (int j = 0; j < kPlanBatch; ++j) {
-                const int t = t0 + j * kPlanThreads + tid;
-                if (t0 + j * kPlanThreads >= a.M) break;
-                flags |= id[j] >= a.slots ? kAdBadId : 0u;
-                f(t, t < a.M ? ad_key(id[j], a.slots) : -1);
-            }
+        for (int j = 0; j < kPlanBatch; ++j) {
+            if (t0 + j * kPlanThreads >= a.M) break;
+            flags |= id[j] >= a.slots ? kAdBadId : 0u;
+            id[j] = t0 + j * kPlanThreads + tid < a.M ? ad_key(id[j], a.slots) : -1;
+            place[j] = ad_take(s_count, id[j]);
         }
     };
-    each([&](int, int key) { ad_take(s_at, key); });
+    constexpr int kBatchRows = kPlanThreads * kPlanBatch;
+    for (int t0 = 0; t0 < a.M; t0 += kBatchRows) take(t0);
     flag_or(a.flags, flags);
     __syncthreads();
-    int rows = 0, tiles = 0;
+    int tiles = 0;
     for (int i0 = 0; i0 < keys; i0 += kPlanThreads) {
-        const int i = i0 + tid, n = i < keys ? s_at[i] : 0;
-        const int nt = i == 0 && a.in_place ? 0 : (n + tile_rows - 1) / tile_rows;
-        int all, all_tiles;
-        const int first = rows + block_prefix(n, s_wave, all) - n;
-        const int tile0 = tiles + block_prefix(nt, s_wave, all_tiles) - nt;
-        if (i < keys) {
-            s_at[i] = first;
-            s_first[i] = first;
-            s_tile[i] = tile0;
-        }
-        rows += all;
-        tiles += all_tiles;
-    }
-    if (tid == 0) {
-        *a.ntiles = tiles;
-        s_first[keys] = rows;
+        const int i = i0 + tid, n = i < keys ? s_count[i] : 0;
+        const int nt = i == 0 && a.in_place ? 0 : (n + a.tile_rows - 1) / a.tile_rows;
+        int all;
+        const int first = tiles + block_prefix(nt, s_wave, all) - nt;
+        if (i < keys) s_tile[i] = first;
+        tiles += all;
     }
     __syncthreads();
-    for (int j = tid; j < tiles; j += kPlanThreads) {  // the last slot that begins at or before tile j
-        int lo = 0, hi = keys;
+    for (int j = tid; j < a.units; j += kPlanThreads) {
+        int32_t* tile = a.tiles + size_t(j) * span;
+        if (j >= tiles) {
+            tile[0] = -2;
+            continue;
+        }
+        int lo = 0, hi = keys;                         // the last slot that begins at or before tile j
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             (s_tile[mid] <= j ? lo : hi) = mid;
         }
-        const int first = s_first[lo] + (j - s_tile[lo]) * tile_rows;
-        a.tiles[j] = AdTile{lo - 1, first, min(s_first[lo + 1] - first, tile_rows)};
+        tile[0] = lo - 1;
+        tile[1] = min(s_count[lo] - (j - s_tile[lo]) * a.tile_rows, a.tile_rows);
     }
-    each([&](int t, int key) {
-        const int place = ad_take(s_at, key);
-        if (key >= 0) a.order[place] = t;
-    });
+    auto put = [&](int t0) {
+#pragma unroll
+        for (int j = 0; j < kPlanBatch; ++j) {
+            if (t0 + j * kPlanThreads >= a.M) break;
+            if (id[j] < 0 || (id[j] == 0 && a.in_place)) continue;
+            const int tile = s_tile[id[j]] + place[j] / a.tile_rows;
+            a.tiles[size_t(tile) * span + kTileHead + place[j] % a.tile_rows] = t0 + j * kPlanThreads + tid;
+        }
+    };
+    if (a.M <= kBatchRows) {
+        put(0);
+        return;
+    }
+    __syncthreads();                                   // (more rows than a batch: places again)
+    for (int i = tid; i < keys; i += kPlanThreads) s_count[i] = 0;
+    __syncthreads();
+    for (int t0 = 0; t0 < a.M; t0 += kBatchRows) {
+        take(t0);
+        put(t0);
+    }
 }
 
 // ---- shrink ---------------------------------------------------------------------
@@ -341,8 +362,6 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(AdArg
 }
 
 // ---- expand ---------------------------------------------------------------------
-template <int OUT> struct AdOut { typedef uint16_t type; static constexpr int size = 2; };
-template <> struct AdOut<ORNITH_ADAPTER_F32> { typedef uint32_t type; static constexpr int size = 4; };
 template <int OUT> __device__ __forceinline__ float ad_float(uint32_t bits) {
     if constexpr (OUT == ORNITH_ADAPTER_F32) return __uint_as_float(bits);
     else if constexpr (OUT == ORNITH_ADAPTER_BF16) return bf16_bits_to_f32(bits);
@@ -359,13 +378,6 @@ __device__ __forceinline__ float ad_scale16(uint32_t most) {
     if (e == 0 || e == 255) return 1.f;
     return __uint_as_float(uint32_t(min(max(127 + 127 + 14 - e, 1), 254)) << 23);
 }
-// Column, of a wave's 64, of row m = 4 q + i of the instruction's tile j: a lane's results of a tile (fp32) or
-// of two (16-bit) are 16 neighbouring bytes, those of its row's four lanes 64.
-template <int OUT> __device__ __forceinline__ int ad_column(int j, int m) {
-    if constexpr (OUT == ORNITH_ADAPTER_F32) return 16 * j + m;
-    else return 32 * (j >> 1) + 8 * (m >> 2) + 4 * (j & 1) + (m & 3);
-}
-
 // The two 16-bit numbers whose sum v is (inf: no NaN beside it).
 template <int TYPE> __device__ __forceinline__ void ad_halves(float v, uint32_t& hi, uint32_t& lo) {
     hi = ad_bits<TYPE>(v);
@@ -377,67 +389,116 @@ template <int SIZE> __device__ __forceinline__ bool ad_whole(const AdArgs& a, in
     return n0 + 64 <= end && ((reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out) |
                                size_t(a.ldb) * SIZE | size_t(a.ldo) * SIZE | size_t(n0) * SIZE) & 15) == 0;
 }
-// base to out, as it is.
-template <int OUT, int MT, int V, class T>
-__device__ __forceinline__ void ad_copy(const u32x4 (&have)[MT][V], const T* const (&base)[MT], T* const (&out)[MT], int rows, int n0,
-                                        int end, bool whole) {
-    constexpr int kPer = 16 / AdOut<OUT>::size;
-    const int lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
+// A wave's 16 MT rows x 64 columns of base and out, as they move: eight lanes (fp32: 16) on a row's 16-byte
+// pieces, H accesses for 16 rows.  (Neighbouring lanes in different rows, as the products leave them, halve
+// the rate.)  B: of the buffers, the one that holds base.  ONCE: stores that leave the caches alone.
+template <int OUT, int MT, int BUFS = 1, bool ONCE = false> struct AdCells {
+    typedef std::conditional_t<OUT == ORNITH_ADAPTER_F32, uint32_t, uint16_t> word;
+    static constexpr int size = sizeof(word), per = 16 / size, lanes = 64 / per, rows_at_once = 64 / lanes, H = 16 / rows_at_once;
+    const word* base[MT][H];
+    word* out[MT][H];
+    u32x4 have[BUFS][MT][H];
+
+    // rows as lane li of each 16 holds them
+    __device__ __forceinline__ AdCells(const AdArgs& a, const int (&t)[MT]) {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        if (16 * m + li >= rows) continue;
-        if (whole) {
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int c = 0; c < V; ++c) *reinterpret_cast<u32x4*>(out[m] + (4 * c + q) * kPer) = have[m][c];
-        } else {
-            for (int i = q; i < 64 && n0 + i < end; i += 4) out[m][i] = base[m][i];
-        }
+            for (int h = 0; h < H; ++h) {
+                const size_t row = size_t(__builtin_amdgcn_ds_bpermute(4 * (rows_at_once * h + lane / lanes), t[m]));
+                base[m][h] = static_cast<const word*>(a.base) + row * size_t(a.ldb) + per * (lane % lanes);
+                out[m][h] = static_cast<word*>(a.out) + row * size_t(a.ldo) + per * (lane % lanes);
+            }
     }
-}
-// base + by * acc, rounded, and what it raises.
-template <int OUT, int MT, int V, class T>
-__device__ __forceinline__ void ad_finish(const AdArgs& a, const f32x4 (&acc)[MT][4], const float (&by)[MT], const u32x4 (&have)[MT][V],
-                                          const T* const (&base)[MT], T* const (&out)[MT], int rows, int n0, int end, bool whole) {
-    constexpr int size = AdOut<OUT>::size, kPer = 16 / size;
-    const int lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
-    float most = 0.f, zero = 0.f;
-    auto sum = [&](uint32_t bits, int m, int j, int i) {
-        const float r = ad_float<OUT>(bits) + by[m] * acc[m][j][i];
-        most = fmaxf(most, __builtin_fabsf(r));
-        zero = __builtin_fmaf(r, 0.f, zero);
-        return ad_bits<OUT>(r);
-    };
+    template <int B = 0> __device__ __forceinline__ void load(int n0, int end, bool whole) {
+        if (n0 >= end) return;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        if (16 * m + li >= rows) continue;
-        if (whole) {
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int c = 0; c < V; ++c) {
+            for (int h = 0; h < H; ++h) {
+                if (whole) have[B][m][h] = *reinterpret_cast<const u32x4*>(base[m][h] + n0);
+                else {                                 // (past the end: the last value)
+                    const int left = end - 1 - n0 - per * int((threadIdx.x & 63) % lanes);
+                    u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < per; ++i) v[i * size / 4] |= uint32_t(base[m][h][n0 + min(i, left)]) << (size == 4 ? 0 : 16 * (i & 1));
+                    have[B][m][h] = v;
+                }
+            }
+    }
+    // f(m, h, i, value of base) of this lane's cells, stored
+    template <int B, class F> __device__ __forceinline__ void store(int n0, int end, bool whole, int rows, F&& f) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                if (16 * m + rows_at_once * h + lane / lanes >= rows) continue;
+                const int left = whole ? per : end - n0 - per * (lane % lanes);
+                if (left <= 0) continue;
                 u32x4 r;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t h = have[m][c][e];
-                    if constexpr (size == 4) r[e] = sum(h, m, c, e);
-                    else r[e] = sum(h & 0xffffu, m, 2 * c + (e >> 1), 2 * (e & 1)) |
-                                sum(h >> 16, m, 2 * c + (e >> 1), 2 * (e & 1) + 1) << 16;
+                    const uint32_t w = have[B][m][h][e];
+                    if constexpr (size == 4) r[e] = f(m, h, e, w);
+                    else r[e] = f(m, h, 2 * e, w & 0xffffu) | f(m, h, 2 * e + 1, w >> 16) << 16;
                 }
-                *reinterpret_cast<u32x4*>(out[m] + (4 * c + q) * kPer) = r;
+                u32x4* const to = reinterpret_cast<u32x4*>(out[m][h] + n0);
+                if (whole && ONCE) __builtin_nontemporal_store(r, to);
+                else if (whole) *to = r;
+                else {
+#pragma unroll
+                    for (int i = 0; i < per; ++i)
+                        if (i < left) out[m][h][n0 + i] = word(r[i * size / 4] >> (size == 4 ? 0 : 16 * (i & 1)));
+                }
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int n = ad_column<OUT>(j, 4 * q + i);
-                    if (n0 + n < end) out[m][n] = T(sum(base[m][n], m, j, i));
-                }
-        }
     }
-    // 16-bit results round to infinity from half a step above the type's largest value
-    const bool bad = zero != zero;
-    constexpr float limit = OUT == ORNITH_ADAPTER_BF16 ? 0x1.ffp127f : 65520.f;
-    flag_or(a.flags, (bad ? kAdNonfinite : 0u) | (OUT != ORNITH_ADAPTER_F32 && (bad || most >= limit) ? kAdNonfinite16 : 0u));
-}
+    // base to out, as it is
+    __device__ __forceinline__ void copy(int n0, int end, bool whole, int rows) {
+        store<0>(n0, end, whole, rows, [](int, int, int, uint32_t bits) { return bits; });
+    }
+    // base + acc, rounded, and what it raises; acc[m][j] of lane 16 q + li: row li's columns 16 j + 4 q .. + 3.
+    // Through LDS to the lanes that move them: 16 bytes c of row r at 16 r + (c ^ r), no bank conflicts; stage: the
+    // wave's own, 256 pieces.
+    template <int B = 0> __device__ __forceinline__ void finish(const AdArgs& a, const f32x4 (&acc)[MT][4], const float (&by)[MT], f32x4* stage, int n0,
+                                           int end, bool whole, int rows) {
+        const int lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
+        float most = 0.f, zero = 0.f;
+        f32x4 sum[MT][H][per / 4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f32x4 v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = by[m] * acc[m][j][i];
+                stage[16 * li + ((4 * j + q) ^ li)] = v;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int c = 0; c < per / 4; ++c) {
+                    const int row = rows_at_once * h + lane / lanes;
+                    sum[m][h][c] = stage[16 * row + ((per / 4 * (lane % lanes) + c) ^ row)];
+                }
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        store<B>(n0, end, whole, rows, [&](int m, int h, int i, uint32_t bits) {
+            const float r = ad_float<OUT>(bits) + sum[m][h][i >> 2][i & 3];
+            most = fmaxf(most, __builtin_fabsf(r));
+            zero = __builtin_fmaf(r, 0.f, zero);
+            return ad_bits<OUT>(r);
+        });
+        // 16-bit results round to infinity from half a step above the type's largest value
+        const bool bad = zero != zero;
+        constexpr float limit = OUT == ORNITH_ADAPTER_BF16 ? 0x1.ffp127f : 65520.f;
+        flag_or(a.flags, (bad ? kAdNonfinite : 0u) | (OUT != ORNITH_ADAPTER_F32 && (bad || most >= limit) ? kAdNonfinite16 : 0u));
+    }
+};
 
 constexpr int kExpandWaves = 4;                        // a block: 64 columns a wave
 
@@ -446,8 +507,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
     extern __shared__ __attribute__((aligned(16))) u32x4 s_v[];        // [MT][steps][64]
     __shared__ uint32_t s_most[16 * MT];
     __shared__ int s_t[16 * MT];
-    typedef typename AdOut<OUT>::type word;
-    constexpr int size = AdOut<OUT>::size, kPer = 16 / size, kVec = 4 * size / 4;    // values of 16 bytes, such pieces a lane
+    __shared__ f32x4 s_stage[kExpandWaves][256];
     int slot, rows, t[MT];
     if (!ad_tile<MT, FEW>(a, blockIdx.x, 1, false, slot, rows, t) || (slot < 0 && a.in_place)) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
@@ -455,23 +515,11 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
     while (int(blockIdx.y) >= a.blocks[p]) ++p;
     const int end = a.ends[p];
     const int n0 = (p ? a.ends[p - 1] : 0) + ((int(blockIdx.y) - (p ? a.blocks[p - 1] : 0)) * kExpandWaves + wv) * 64;
-    const word *base[MT];
-    word* out[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        base[m] = static_cast<const word*>(a.base) + size_t(t[m]) * size_t(a.ldb) + n0;
-        out[m] = static_cast<word*>(a.out) + size_t(t[m]) * size_t(a.ldo) + n0;
-    }
-    const bool whole = ad_whole<size>(a, n0, end);
-    u32x4 have[MT][kVec];
-    if (whole) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int c = 0; c < kVec; ++c) have[m][c] = *reinterpret_cast<const u32x4*>(base[m] + (4 * c + q) * kPer);
-    }
+    const bool whole = n0 < end && ad_whole<AdCells<OUT, MT>::size>(a, n0, end);
+    AdCells<OUT, MT, 1, FEW == 0> cells(a, t);
+    cells.load(n0, end, whole);
     if (slot < 0) {
-        ad_copy<OUT, MT>(have, base, out, rows, n0, end, whole);
+        cells.copy(n0, end, whole, rows);
         return;
     }
     const int chunks = a.R / 8, steps = (2 * chunks + 3) / 4;
@@ -540,7 +588,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
     const uint16_t* b[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)                        // (past the slice: its last column)
-        b[j] = a.b + size_t(slot) * size_t(a.b_slot) + size_t(min(n0 + ad_column<OUT>(j, li), end - 1)) * a.R;
+        b[j] = a.b + size_t(slot) * size_t(a.b_slot) + size_t(min(n0 + 16 * j + li, end - 1)) * a.R;
     for (int s = 0; s < steps; ++s) {
         const int c = 4 * s + q, at = 8 * (c < chunks ? c : min(c - chunks, chunks - 1));
         u32x4 bv[4];
@@ -557,142 +605,183 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
             for (int j = 0; j < 4; ++j) acc[m][j] = ad_mfma<TYPE>(bv[j], vv, acc[m][j]);
         }
     }
-    ad_finish<OUT, MT>(a, acc, by, have, base, out, rows, n0, end, whole);
+    cells.finish(a, acc, by, s_stage[wv], n0, end, whole, rows);
 }
 
 // ---- both in one ----------------------------------------------------------------
-// Few rows of a small rank: a block forms v of its tile for itself (its waves share k) and then 64 columns a
-// wave.  Every block of columns reads x and A again, from L2, and spares the second launch; what the second
-// product reads is on its way meanwhile.
-constexpr int kBothWaves = 8;
-
-template <int TYPE, int OUT, int RT, int FEW>
-__global__ __launch_bounds__(64 * kBothWaves) void adapter_both_kernel(AdArgs a) {
-    constexpr int W = kBothWaves, D = RT == 4 ? 2 : 4;
-    typedef typename AdOut<OUT>::type word;
-    constexpr int size = AdOut<OUT>::size, kPer = 16 / size, kVec = 4 * size / 4;
-    __shared__ u32x4 s_stage[W][(1 + RT) * 128];       // (then the waves' sums)
-    __shared__ u32x4 s_v[RT][64];
-    __shared__ uint32_t s_most[16];
-    int slot, rows, t[1];
+// A small rank: a block forms v of its tile for itself (its waves share k) and then its columns, 64 a wave at
+// a time.  Every block of columns reads x and A again, from its XCD's L2, and spares the second launch.
+template <int TYPE, int OUT, int MT, int RT, int W, int FEW>
+__global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
+    constexpr int D = FEW && MT + RT <= 3 ? 4 : 2, BUFS = FEW || RT == 4 ? 1 : 2;
+    typedef AdCells<OUT, MT, BUFS, FEW == 0> Cells;
+    static_assert((MT + RT) * 128 >= std::max(MT * RT * 64, 256));
+    __shared__ u32x4 s_stage[W][(MT + RT) * 128];      // (then the waves' sums)
+    __shared__ u32x4 s_v[MT][RT][64];
+    __shared__ uint32_t s_most[16 * MT];
+    int slot, rows, t[MT];
     // blocks go to the 8 XCDs in turn: a row's column blocks on one of them, whose L2 keeps its A
     const int nblocks = a.blocks[a.S - 1], unit = int(blockIdx.x / 8) / nblocks * 8 + int(blockIdx.x % 8);
     const int cb = int(blockIdx.x / 8) % nblocks;
-    if (unit >= a.M || !ad_tile<1, FEW>(a, unit, 1, blockIdx.x == 0, slot, rows, t) || (slot < 0 && a.in_place)) return;
+    if (unit >= a.units || !ad_tile<MT, FEW>(a, unit, 1, blockIdx.x == 0, slot, rows, t) || (slot < 0 && a.in_place)) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
     int p = 0;
     while (cb >= a.blocks[p]) ++p;
-    const int end = a.ends[p];
-    const int n0 = (p ? a.ends[p - 1] : 0) + ((cb - (p ? a.blocks[p - 1] : 0)) * W + wv) * 64;
-    const word* base[1] = {static_cast<const word*>(a.base) + size_t(t[0]) * size_t(a.ldb) + n0};
-    word* out[1] = {static_cast<word*>(a.out) + size_t(t[0]) * size_t(a.ldo) + n0};
-    const bool whole = ad_whole<size>(a, n0, end);
-    u32x4 have[1][kVec];
-    auto load_base = [&] {
-        if (whole) {
-#pragma unroll
-            for (int c = 0; c < kVec; ++c) have[0][c] = *reinterpret_cast<const u32x4*>(base[0] + (4 * c + q) * kPer);
-        }
-    };
+    const int begin = (p ? a.ends[p - 1] : 0) + (cb - (p ? a.blocks[p - 1] : 0)) * (64 * W * a.groups);
+    const int end = min(a.ends[p], begin + 64 * W * a.groups);
+    Cells cells(a, t);
     if (slot < 0) {
-        load_base();
-        ad_copy<OUT, 1>(have, base, out, rows, n0, end, whole);
+        for (int n0 = begin + 64 * wv; n0 < end; n0 += 64 * W) {
+            const bool whole = ad_whole<Cells::size>(a, n0, end);
+            cells.load(n0, end, whole);
+            cells.copy(n0, end, whole, rows);
+        }
         return;
     }
     const int chunks = a.R / 8;
-    const uint16_t* b[4];
-    u32x4 bv[RT][4];
-    const float scale = a.scales[slot];
+    float by[MT];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        b[j] = a.b + size_t(slot) * size_t(a.b_slot) + size_t(min(n0 + ad_column<OUT>(j, li), end - 1)) * a.R;
-    f32x4 acc[1][RT];
+    for (int m = 0; m < MT; ++m) by[m] = a.scales[slot];
+    {
+        f32x4 acc[MT][RT];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) acc[0][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    ad_accumulate<TYPE, 1, RT, W, D>(a, t, rows, a.a + size_t(slot) * size_t(a.a_slot) + size_t(p * a.R) * size_t(a.K), a.R,
-                                     s_stage[wv], 0, a.K, acc);
-    load_base();
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int s = 0; s < RT; ++s) {
-        const int c = 4 * s + q, at = 8 * min(c < chunks ? c : c - chunks, chunks - 1);
+            for (int r = 0; r < RT; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+        ad_accumulate<TYPE, MT, RT, W, D>(a, t, rows, a.a + size_t(slot) * size_t(a.a_slot) + size_t(p * a.R) * size_t(a.K), a.R,
+                                          s_stage[wv], 0, a.K, acc);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bv[s][j] = *reinterpret_cast<const u32x4*>(b[j] + at);
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) reinterpret_cast<f32x4*>(s_stage[wv])[64 * (m * RT + r) + lane] = acc[m][r];
     }
+    for (int f = wv; f < MT * RT; f += W) s_v[f / RT][f % RT][lane] = u32x4{0, 0, 0, 0};
+    if (TYPE == ORNITH_ADAPTER_F16 && tid < 16 * MT) s_most[tid] = 0;
+    // the first columns on their way meanwhile
+    const uint16_t* const bs = a.b + size_t(slot) * size_t(a.b_slot);
+    u32x4 bv[BUFS][RT][4];
+    auto load_b = [&](auto buf, int n0) {              // (past the slice: its last column)
+        if (n0 >= end) return;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) reinterpret_cast<f32x4*>(s_stage[wv])[64 * r + lane] = acc[0][r];
-    if (wv < RT) s_v[wv][lane] = u32x4{0, 0, 0, 0};
-    if (TYPE == ORNITH_ADAPTER_F16 && tid < 16) s_most[tid] = 0;
+        for (int s = 0; s < RT; ++s) {
+            const int c = 4 * s + q, from = 8 * min(c < chunks ? c : c - chunks, chunks - 1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                bv[decltype(buf)::value][s][j] =
+                    *reinterpret_cast<const u32x4*>(bs + uint32_t(min(n0 + 16 * j + li, end - 1)) * uint32_t(a.R) + from);
+        }
+    };
+    int n0 = begin + 64 * wv;
+    bool whole = n0 < end && ad_whole<Cells::size>(a, n0, end);
+    cells.load(n0, end, whole);
+    load_b(std::integral_constant<int, 0>{}, n0);
     __syncthreads();
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    const int r = 16 * wv + li;                        // wave r's 16 of the rank
-    if (wv < RT) {
-        v = reinterpret_cast<const f32x4*>(s_stage[0])[64 * wv + lane];
+    constexpr int F = (MT * RT + W - 1) / W;           // pieces of 16 rows and 16 of the rank, a wave
+    f32x4 v[F];
+#pragma unroll
+    for (int i0 = 0; i0 < F; ++i0) {
+        const int f = wv + W * i0;
+        if (f >= MT * RT) break;
+        v[i0] = reinterpret_cast<const f32x4*>(s_stage[0])[64 * f + lane];
 #pragma unroll
         for (int u = 1; u < W; ++u) {
-            const f32x4 part = reinterpret_cast<const f32x4*>(s_stage[u])[64 * wv + lane];
+            const f32x4 part = reinterpret_cast<const f32x4*>(s_stage[u])[64 * f + lane];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += part[i];
+            for (int i = 0; i < 4; ++i) v[i0][i] += part[i];
         }
-        if (TYPE == ORNITH_ADAPTER_F16 && r < a.R) {
+        if (TYPE == ORNITH_ADAPTER_F16 && 16 * (f % RT) + li < a.R) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) atomicMax(&s_most[4 * q + i], __float_as_uint(v[i]) & 0x7fffffffu);
+            for (int i = 0; i < 4; ++i) atomicMax(&s_most[16 * (f / RT) + 4 * q + i], __float_as_uint(v[i0][i]) & 0x7fffffffu);
         }
     }
     if (TYPE == ORNITH_ADAPTER_F16) __syncthreads();
-    if (wv < RT && r < a.R) {
-        uint16_t* s16 = reinterpret_cast<uint16_t*>(&s_v[0][0]);
+#pragma unroll
+    for (int i0 = 0; i0 < F; ++i0) {
+        const int f = wv + W * i0, m = f / RT, r = 16 * (f % RT) + li;
+        if (f >= MT * RT || r >= a.R) break;
+        uint16_t* s16 = reinterpret_cast<uint16_t*>(&s_v[m][0][0]);
         auto put = [&](int c, int row, uint32_t bits) { s16[((c >> 2) * 64 + (c & 3) * 16 + row) * 8 + (r & 7)] = uint16_t(bits); };
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = 4 * q + i;
             uint32_t hi, lo;
-            ad_halves<TYPE>(v[i] * (TYPE == ORNITH_ADAPTER_F16 ? ad_scale16(s_most[row]) : 1.f), hi, lo);
+            ad_halves<TYPE>(v[i0][i] * (TYPE == ORNITH_ADAPTER_F16 ? ad_scale16(s_most[16 * m + row]) : 1.f), hi, lo);
             put(r >> 3, row, hi);
             put((r >> 3) + chunks, row, lo);
         }
     }
     __syncthreads();
-    if (n0 >= end) return;
-    float by[1] = {scale};
-    if constexpr (TYPE == ORNITH_ADAPTER_F16) by[0] = by[0] / ad_scale16(s_most[li]);
-    f32x4 sum[1][4];
+    if constexpr (TYPE == ORNITH_ADAPTER_F16) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < RT; ++s) {
-        if (4 * s >= 2 * chunks) break;
-        const u32x4 vv = s_v[s][lane];
-        if (4 * s + q >= 2 * chunks) {                 // (no 0 times inf)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) bv[s][j] = u32x4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum[0][j] = ad_mfma<TYPE>(bv[s][j], vv, sum[0][j]);
+        for (int mm = 0; mm < MT; ++mm) by[mm] = by[mm] / ad_scale16(s_most[16 * mm + li]);
     }
-    ad_finish<OUT, 1>(a, sum, by, have, base, out, rows, n0, end, whole);
+    // 64 columns of buffer C, the next ones' loads before them
+    auto columns = [&](auto buf) {
+        constexpr int C = decltype(buf)::value, N = BUFS == 2 ? 1 - C : C;
+        const int next = n0 + 64 * W;
+        const bool next_whole = next < end && ad_whole<Cells::size>(a, next, end);
+        if constexpr (BUFS == 2) {
+            cells.template load<N>(next, end, next_whole);
+            load_b(std::integral_constant<int, N>{}, next);
+        }
+        f32x4 sum[MT][4];
+#pragma unroll
+        for (int mm = 0; mm < MT; ++mm)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[mm][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < RT; ++s) {
+            if (4 * s >= 2 * chunks) break;
+            if (4 * s + q >= 2 * chunks) {             // (no 0 times inf)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) bv[C][s][j] = u32x4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int mm = 0; mm < MT; ++mm) {
+                const u32x4 vv = s_v[mm][s][lane];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[mm][j] = ad_mfma<TYPE>(bv[C][s][j], vv, sum[mm][j]);
+            }
+        }
+        if constexpr (BUFS == 1) load_b(buf, next);
+        cells.template finish<C>(a, sum, by, reinterpret_cast<f32x4*>(s_stage[wv]), n0, end, whole, rows);
+        if constexpr (BUFS == 1) cells.load(next, end, next_whole);
+        n0 = next;
+        whole = next_whole;
+    };
+    while (n0 < end) {
+        columns(std::integral_constant<int, 0>{});
+        if constexpr (BUFS == 2) {
+            if (n0 >= end) break;
+            columns(std::integral_constant<int, 1>{});
+        }
+    }
 }
 
-struct AdLayout { size_t v, order, tiles, count, bytes; };
+struct AdLayout { size_t v, tiles, bytes; };
 
 // Parts of K that a shrink of M rows may have (each has a v of its own).
 int ad_splits(int64_t M) { return M <= kFewRows ? 4 : 1; }
+
+// Rows of a planned tile, and tiles at most.
+int ad_tile_rows(int M, int R) { return R <= kBothRank ? 16 : M >= 1024 && R <= 128 ? 64 : 16; }
+int ad_tiles(int M, int slots, int tile_rows) { return std::min(M, (M + tile_rows - 1) / tile_rows + slots + 1); }
 
 bool ad_layout(int64_t M, int S, int R, AdLayout& l) {
     if (M < 0 || S < 1 || S > kAdMaxSlices || R < 8 || R > kAdMaxR || R % 8) return false;
     const size_t rows = size_t(std::min<int64_t>(M, kAdRows));
     l.v = 0;
-    l.order = align256(rows * size_t(S) * size_t(R) * 4 * size_t(ad_splits(M)));
-    l.tiles = l.order + align256(rows * 4);
-    l.count = l.tiles + align256(rows * sizeof(AdTile));
-    l.bytes = l.count + 256;
+    l.tiles = align256(rows * size_t(S) * size_t(R) * 4 * size_t(ad_splits(M)));
+    const size_t most = M <= kFewRows ? 0 : size_t(ad_tiles(int(rows), kAdMaxSlots, ad_tile_rows(int(rows), R)));
+    l.bytes = l.tiles + align256(most * size_t(kTileHead + ad_tile_rows(int(rows), R)) * 4) + 256;
     return true;
 }
 
-// Column blocks of 64 W columns, slice by slice.
-int ad_blocks(AdArgs& a, int W) {
+// Blocks of columns, slice by slice.
+int ad_blocks(AdArgs& a, int columns) {
     int blocks = 0;
     for (int p = 0; p < a.S; ++p) {
-        blocks += (a.ends[p] - (p ? a.ends[p - 1] : 0) + 64 * W - 1) / (64 * W);
+        blocks += (a.ends[p] - (p ? a.ends[p - 1] : 0) + columns - 1) / columns;
         a.blocks[p] = blocks;
     }
     return blocks;
@@ -704,31 +793,32 @@ template <class F> void ad_by_type(int out_type, F&& f) {
     else f(std::integral_constant<int, ORNITH_ADAPTER_F16>{});
 }
 
-template <int TYPE, int FEW> hipError_t ad_both(AdArgs& a, int out_type, hipStream_t s) {
-    const dim3 grid((a.M + 7) / 8 * 8 * ad_blocks(a, kBothWaves));
-    auto go = [&](auto kernel) { timed_launch("adapter_both", kernel, grid, dim3(64 * kBothWaves), 0, s, a); };
+template <int TYPE, int MT, int W, int FEW> hipError_t ad_both(AdArgs& a, int out_type, int groups, hipStream_t s) {
+    a.groups = groups;
+    const dim3 grid((a.units + 7) / 8 * 8 * ad_blocks(a, 64 * W * groups));
+    auto go = [&](auto kernel) { timed_launch("adapter_both", kernel, grid, dim3(64 * W), 0, s, a); };
     ad_by_type(out_type, [&](auto out) {
         constexpr int OUT = decltype(out)::value;
-        if (a.R <= 16) go(adapter_both_kernel<TYPE, OUT, 1, FEW>);
-        else if (a.R <= 32) go(adapter_both_kernel<TYPE, OUT, 2, FEW>);
-        else go(adapter_both_kernel<TYPE, OUT, 4, FEW>);
+        if (a.R <= 16) go(adapter_both_kernel<TYPE, OUT, MT, 1, W, FEW>);
+        else if (a.R <= 32) go(adapter_both_kernel<TYPE, OUT, MT, 2, W, FEW>);
+        else go(adapter_both_kernel<TYPE, OUT, MT, 4, W, FEW>);
     });
     return hipGetLastError();
 }
 
-template <int TYPE, int MT, int FEW> hipError_t ad_two(AdArgs& a, int out_type, int tiles, hipStream_t s) {
+template <int TYPE, int MT, int FEW> hipError_t ad_two(AdArgs& a, int out_type, hipStream_t s) {
     const int rt = (a.SR + 15) / 16;
     constexpr int SMT = 1;
     a.sub = MT / SMT;
     a.splits = std::min(ad_splits(a.M), (a.K + 511) / 512);
     a.splits = std::max(a.splits, 1);
     auto shrink = [&](auto kernel, int RT) {
-        timed_launch("adapter_shrink", kernel, dim3(tiles * a.sub, (rt + RT - 1) / RT, a.splits), dim3(64 * kShrinkWaves), 0, s, a);
+        timed_launch("adapter_shrink", kernel, dim3(a.units * a.sub, (rt + RT - 1) / RT, a.splits), dim3(64 * kShrinkWaves), 0, s, a);
     };
     shrink(adapter_shrink_kernel<TYPE, SMT, 1, 4, FEW>, 1);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
-    const dim3 grid(tiles, ad_blocks(a, kExpandWaves));
+    const dim3 grid(a.units, ad_blocks(a, 64 * kExpandWaves));
     const int steps = (a.R / 4 + 3) / 4;
     ad_by_type(out_type, [&](auto out) {
         timed_launch("adapter_expand", adapter_expand_kernel<TYPE, decltype(out)::value, MT, FEW>, grid, dim3(64 * kExpandWaves),
@@ -738,18 +828,17 @@ template <int TYPE, int MT, int FEW> hipError_t ad_two(AdArgs& a, int out_type, 
 }
 
 template <int TYPE> hipError_t ad_rows(AdArgs& a, int out_type, hipStream_t s) {
-    if (a.M <= kFewRows) {
-        const bool both = a.R <= 64;
-        if (a.M <= 64) return both ? ad_both<TYPE, 1>(a, out_type, s) : ad_two<TYPE, 1, 1>(a, out_type, a.M, s);
-        return both ? ad_both<TYPE, 4>(a, out_type, s) : ad_two<TYPE, 1, 4>(a, out_type, a.M, s);
-    }
-    // tiles of 64 rows where they are many and v of them fits LDS
-    const int tile_rows = a.M >= 1024 && a.R <= 128 ? 64 : 16;
-    const int tiles = std::min(a.M, (a.M + tile_rows - 1) / tile_rows + a.slots + 1);
-    timed_launch("adapter_plan", adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, tile_rows);
+    const bool both = a.R <= kBothRank;
+    a.units = a.M;
+    if (a.M <= 64) return both ? ad_both<TYPE, 1, 8, 1>(a, out_type, 1, s) : ad_two<TYPE, 1, 1>(a, out_type, s);
+    if (a.M <= kFewRows) return both ? ad_both<TYPE, 1, 8, 4>(a, out_type, 1, s) : ad_two<TYPE, 1, 4>(a, out_type, s);
+    a.tile_rows = ad_tile_rows(a.M, a.R);
+    a.units = ad_tiles(a.M, a.slots, a.tile_rows);
+    timed_launch("adapter_plan", adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
-    return tile_rows == 64 ? ad_two<TYPE, 4, 0>(a, out_type, tiles, s) : ad_two<TYPE, 1, 0>(a, out_type, tiles, s);
+    if (both) return ad_both<TYPE, 1, 8, 0>(a, out_type, 6, s);
+    return a.tile_rows == 64 ? ad_two<TYPE, 4, 0>(a, out_type, s) : ad_two<TYPE, 1, 0>(a, out_type, s);
 }
 
 }  // namespace
@@ -810,9 +899,7 @@ extern "C" hipError_t ornith_adapter_launch(const void* x, int x_type, int64_t l
     args.ldo = ldo;
     args.flags = static_cast<uint32_t*>(flags);
     args.v = at<float>(workspace, l.v);
-    args.order = at<int32_t>(workspace, l.order);
-    args.tiles = at<AdTile>(workspace, l.tiles);
-    args.ntiles = at<int32_t>(workspace, l.count);
+    args.tiles = at<int32_t>(workspace, l.tiles);
     args.N = N;
     args.K = K;
     args.R = R;
