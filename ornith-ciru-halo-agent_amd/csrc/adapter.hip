@@ -372,6 +372,17 @@ template <int OUT> __device__ __forceinline__ uint32_t ad_bits(float v) {
     else if constexpr (OUT == ORNITH_ADAPTER_BF16) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
     else return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
 }
+// Two rounded values in a word.
+template <int OUT> __device__ __forceinline__ uint32_t ad_pair(float a, float b) {
+    typedef float pair __attribute__((ext_vector_type(2)));
+    if constexpr (OUT == ORNITH_ADAPTER_BF16) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(pair{a, b}, bf16x2));
+    } else {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(pair{a, b}, f16x2));
+    }
+}
 // Power of two that brings a row's largest |v| to [2^14, 2^15) of fp16, as fp32 (1 for 0 and non-finite rows).
 __device__ __forceinline__ float ad_scale16(uint32_t most) {
     const int e = int(most >> 23);
@@ -384,119 +395,151 @@ template <int TYPE> __device__ __forceinline__ void ad_halves(float v, uint32_t&
     const float h = ad_float<TYPE>(hi);
     lo = __builtin_isinf(h) ? 0u : ad_bits<TYPE>(v - h);
 }
-// Whether a wave's 64 columns lie whole on the 16-byte grid, and move in pieces of 16 bytes (wave-uniform).
-template <int SIZE> __device__ __forceinline__ bool ad_whole(const AdArgs& a, int n0, int end) {
-    return n0 + 64 <= end && ((reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out) |
-                               size_t(a.ldb) * SIZE | size_t(a.ldo) * SIZE | size_t(n0) * SIZE) & 15) == 0;
+// Columns from which on 64 are not whole and on the 16-byte grid, of the columns from begin to end (whose
+// groups of 64 start at begin): the last ones, or all.
+template <int SIZE> __device__ __forceinline__ int ad_whole_end(const AdArgs& a, int begin, int end) {
+    return ((reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out) | size_t(a.ldb) * SIZE | size_t(a.ldo) * SIZE |
+             size_t(begin) * SIZE) & 15) == 0 ? end - 63 : begin;
 }
 // A wave's 16 MT rows x 64 columns of base and out, as they move: eight lanes (fp32: 16) on a row's 16-byte
 // pieces, H accesses for 16 rows.  (Neighbouring lanes in different rows, as the products leave them, halve
-// the rate.)  B: of the buffers, the one that holds base.  ONCE: stores that leave the caches alone.
-template <int OUT, int MT, int BUFS = 1, bool ONCE = false> struct AdCells {
+// the rate.)  ONCE: stores that leave the caches alone.
+template <int OUT, int MT, bool ONCE> struct AdCells {
     typedef std::conditional_t<OUT == ORNITH_ADAPTER_F32, uint32_t, uint16_t> word;
     static constexpr int size = sizeof(word), per = 16 / size, lanes = 64 / per, rows_at_once = 64 / lanes, H = 16 / rows_at_once;
-    const word* base[MT][H];
+    const word* base[MT][H];                           // of this wave's next columns
     word* out[MT][H];
-    u32x4 have[BUFS][MT][H];
+    u32x4 have[MT][H];
+    float most = 0.f, zero = 0.f;                      // largest magnitude; 0, NaN once a result was not finite
+    uint32_t mine = 0;                                 // rows of the tile that this lane moves, a bit each
 
     // rows as lane li of each 16 holds them
-    __device__ __forceinline__ AdCells(const AdArgs& a, const int (&t)[MT]) {
+    __device__ __forceinline__ AdCells(const AdArgs& a, const int (&t)[MT], int rows, int n0) {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < H; ++h) {
                 const size_t row = size_t(__builtin_amdgcn_ds_bpermute(4 * (rows_at_once * h + lane / lanes), t[m]));
-                base[m][h] = static_cast<const word*>(a.base) + row * size_t(a.ldb) + per * (lane % lanes);
-                out[m][h] = static_cast<word*>(a.out) + row * size_t(a.ldo) + per * (lane % lanes);
+                base[m][h] = static_cast<const word*>(a.base) + row * size_t(a.ldb) + n0 + per * (lane % lanes);
+                out[m][h] = static_cast<word*>(a.out) + row * size_t(a.ldo) + n0 + per * (lane % lanes);
+                mine |= 16 * m + rows_at_once * h + lane / lanes < rows ? 1u << (m * H + h) : 0u;
             }
     }
-    template <int B = 0> __device__ __forceinline__ void load(int n0, int end, bool whole) {
-        if (n0 >= end) return;
+    __device__ __forceinline__ void step(int columns) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                if (whole) have[B][m][h] = *reinterpret_cast<const u32x4*>(base[m][h] + n0);
-                else {                                 // (past the end: the last value)
-                    const int left = end - 1 - n0 - per * int((threadIdx.x & 63) % lanes);
+                base[m][h] += columns;
+                out[m][h] += columns;
+            }
+    }
+    // base of the wave's 64 columns: whole pieces, or (left: of the 64, inside the slice) value by value, past
+    // the end the last one
+    __device__ __forceinline__ void load(bool whole, int left) {
+        const int last = left - 1 - per * int((threadIdx.x & 63) % lanes);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                if (whole) have[m][h] = *reinterpret_cast<const u32x4*>(base[m][h]);
+                else {
                     u32x4 v = {0, 0, 0, 0};
 #pragma unroll
-                    for (int i = 0; i < per; ++i) v[i * size / 4] |= uint32_t(base[m][h][n0 + min(i, left)]) << (size == 4 ? 0 : 16 * (i & 1));
-                    have[B][m][h] = v;
+                    for (int i = 0; i < per; ++i) v[i * size / 4] |= uint32_t(base[m][h][min(i, last)]) << (size == 4 ? 0 : 16 * (i & 1));
+                    have[m][h] = v;
                 }
             }
     }
-    // f(m, h, i, value of base) of this lane's cells, stored
-    template <int B, class F> __device__ __forceinline__ void store(int n0, int end, bool whole, int rows, F&& f) {
-        const int lane = threadIdx.x & 63;
+    __device__ __forceinline__ bool has(int m, int h) const { return mine >> (m * H + h) & 1; }
+    __device__ __forceinline__ void put(int m, int h, u32x4 r, bool whole, int left) {
+        if (whole) {
+            u32x4* const to = reinterpret_cast<u32x4*>(out[m][h]);
+            if constexpr (ONCE) __builtin_nontemporal_store(r, to);
+            else *to = r;
+            return;
+        }
+        const int mine_left = left - per * int((threadIdx.x & 63) % lanes);
+#pragma unroll
+        for (int i = 0; i < per; ++i)
+            if (i < mine_left) out[m][h][i] = word(r[i * size / 4] >> (size == 4 ? 0 : 16 * (i & 1)));
+    }
+    // base to out, as it is
+    __device__ __forceinline__ void copy(bool whole, int left) {
+        load(whole, left);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                if (16 * m + rows_at_once * h + lane / lanes >= rows) continue;
-                const int left = whole ? per : end - n0 - per * (lane % lanes);
-                if (left <= 0) continue;
-                u32x4 r;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t w = have[B][m][h][e];
-                    if constexpr (size == 4) r[e] = f(m, h, e, w);
-                    else r[e] = f(m, h, 2 * e, w & 0xffffu) | f(m, h, 2 * e + 1, w >> 16) << 16;
-                }
-                u32x4* const to = reinterpret_cast<u32x4*>(out[m][h] + n0);
-                if (whole && ONCE) __builtin_nontemporal_store(r, to);
-                else if (whole) *to = r;
-                else {
-#pragma unroll
-                    for (int i = 0; i < per; ++i)
-                        if (i < left) out[m][h][n0 + i] = word(r[i * size / 4] >> (size == 4 ? 0 : 16 * (i & 1)));
-                }
-            }
+            for (int h = 0; h < H; ++h)
+                if (has(m, h)) put(m, h, have[m][h], whole, left);
     }
-    // base to out, as it is
-    __device__ __forceinline__ void copy(int n0, int end, bool whole, int rows) {
-        store<0>(n0, end, whole, rows, [](int, int, int, uint32_t bits) { return bits; });
-    }
-    // base + acc, rounded, and what it raises; acc[m][j] of lane 16 q + li: row li's columns 16 j + 4 q .. + 3.
-    // Through LDS to the lanes that move them: 16 bytes c of row r at 16 r + (c ^ r), no bank conflicts; stage: the
-    // wave's own, 256 pieces.
-    template <int B = 0> __device__ __forceinline__ void finish(const AdArgs& a, const f32x4 (&acc)[MT][4], const float (&by)[MT], f32x4* stage, int n0,
-                                           int end, bool whole, int rows) {
+    // base + by * acc, rounded; acc[m][j] of lane 16 q + li: row li's columns 16 j + 4 q .. + 3.  Through LDS to
+    // the lanes that move them: 16 bytes c of row r at 16 r + (c ^ r), no bank conflicts; stage: the wave's own,
+    // 256 pieces.
+    template <bool SCALED> __device__ __forceinline__ void add(const f32x4 (&acc)[MT][4], const float (&by)[MT], f32x4* stage, bool whole,
+                                                               int left) {
         const int lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
-        float most = 0.f, zero = 0.f;
-        f32x4 sum[MT][H][per / 4];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                f32x4 v;
+                f32x4 v = acc[m][j];
+                if constexpr (SCALED) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = by[m] * acc[m][j][i];
+                    for (int i = 0; i < 4; ++i) v[i] *= by[m];
+                }
                 stage[16 * li + ((4 * j + q) ^ li)] = v;
             }
             __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int h = 0; h < H; ++h)
+            for (int h = 0; h < H; ++h) {
+                if (!has(m, h)) continue;              // (such rows' sums are of anything)
+                const int row = rows_at_once * h + lane / lanes;
+                float r[per];
 #pragma unroll
                 for (int c = 0; c < per / 4; ++c) {
-                    const int row = rows_at_once * h + lane / lanes;
-                    sum[m][h][c] = stage[16 * row + ((per / 4 * (lane % lanes) + c) ^ row)];
+                    const f32x4 v = stage[16 * row + ((per / 4 * (lane % lanes) + c) ^ row)];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = 4 * c + i;
+                        const uint32_t w = have[m][h][e * size / 4];
+                        r[e] = v[i] + (size == 4 ? __uint_as_float(w) : OUT == ORNITH_ADAPTER_F16 ? f16_bits_to_f32(w >> (16 * (e & 1)) & 0xffffu)
+                                                                    : __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16));
+                    }
                 }
+                u32x4 bits;
+#pragma unroll
+                for (int e = 0; e < per; e += 2) {
+                    if (whole) {
+                        most = fmaxf(fmaxf(most, __builtin_fabsf(r[e])), __builtin_fabsf(r[e + 1]));
+                        zero = __builtin_fmaf(r[e], 0.f, zero);
+                        zero = __builtin_fmaf(r[e + 1], 0.f, zero);
+                    } else {
+#pragma unroll
+                        for (int i = e; i < e + 2; ++i) {
+                            const float in = per * (lane % lanes) + i < left ? r[i] : 0.f;
+                            most = fmaxf(most, __builtin_fabsf(in));
+                            zero = __builtin_fmaf(in, 0.f, zero);
+                        }
+                    }
+                    if constexpr (size == 4) {
+                        bits[e] = __float_as_uint(r[e]);
+                        bits[e + 1] = __float_as_uint(r[e + 1]);
+                    } else bits[e / 2] = ad_pair<OUT>(r[e], r[e + 1]);
+                }
+                put(m, h, bits, whole, left);
+            }
             __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
-        store<B>(n0, end, whole, rows, [&](int m, int h, int i, uint32_t bits) {
-            const float r = ad_float<OUT>(bits) + sum[m][h][i >> 2][i & 3];
-            most = fmaxf(most, __builtin_fabsf(r));
-            zero = __builtin_fmaf(r, 0.f, zero);
-            return ad_bits<OUT>(r);
-        });
-        // 16-bit results round to infinity from half a step above the type's largest value
+    }
+    // 16-bit results round to infinity from half a step above the type's largest value
+    __device__ __forceinline__ uint32_t flags() const {
         const bool bad = zero != zero;
         constexpr float limit = OUT == ORNITH_ADAPTER_BF16 ? 0x1.ffp127f : 65520.f;
-        flag_or(a.flags, (bad ? kAdNonfinite : 0u) | (OUT != ORNITH_ADAPTER_F32 && (bad || most >= limit) ? kAdNonfinite16 : 0u));
+        return (bad ? kAdNonfinite : 0u) | (OUT != ORNITH_ADAPTER_F32 && (bad || most >= limit) ? kAdNonfinite16 : 0u);
     }
 };
 
@@ -504,10 +547,10 @@ constexpr int kExpandWaves = 4;                        // a block: 64 columns a 
 
 template <int TYPE, int OUT, int MT, int FEW>
 __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArgs a) {
-    extern __shared__ __attribute__((aligned(16))) u32x4 s_v[];        // [MT][steps][64]
+    extern __shared__ __attribute__((aligned(16))) u32x4 s_v[];        // [MT][hi, lo][steps][64]
     __shared__ uint32_t s_most[16 * MT];
     __shared__ int s_t[16 * MT];
-    __shared__ f32x4 s_stage[kExpandWaves][256];
+    __shared__ u32x4 s_stage[kExpandWaves][512];       // a wave's B of 64 columns and 64 r, then its results
     int slot, rows, t[MT];
     if (!ad_tile<MT, FEW>(a, blockIdx.x, 1, false, slot, rows, t) || (slot < 0 && a.in_place)) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
@@ -515,16 +558,17 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
     while (int(blockIdx.y) >= a.blocks[p]) ++p;
     const int end = a.ends[p];
     const int n0 = (p ? a.ends[p - 1] : 0) + ((int(blockIdx.y) - (p ? a.blocks[p - 1] : 0)) * kExpandWaves + wv) * 64;
-    const bool whole = n0 < end && ad_whole<AdCells<OUT, MT>::size>(a, n0, end);
-    AdCells<OUT, MT, 1, FEW == 0> cells(a, t);
-    cells.load(n0, end, whole);
+    typedef AdCells<OUT, MT, FEW == 0> Cells;
+    const bool whole = n0 < ad_whole_end<Cells::size>(a, n0, end);
+    Cells cells(a, t, rows, n0);
     if (slot < 0) {
-        cells.copy(n0, end, whole, rows);
+        if (n0 < end) cells.copy(whole, end - n0);
         return;
     }
-    const int chunks = a.R / 8, steps = (2 * chunks + 3) / 4;
+    if (n0 < end) cells.load(whole, end - n0);
+    const int chunks = a.R / 8, steps = (chunks + 3) / 4;
     {
-        // v of the tile's rows and this slice: hi then lo along r, in pieces of 8, as the instruction's operands
+        // scale v of the tile's rows and this slice: hi then lo along r, in pieces of 8, as the instruction's operands
         if (tid < 16) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) s_t[16 * m + tid] = t[m];
@@ -532,6 +576,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
         if (TYPE == ORNITH_ADAPTER_F16 && tid < 16 * MT) s_most[tid] = 0;
         __syncthreads();
         struct Piece { f32x4 v[2]; };
+        const float scale = a.scales[slot];
         auto piece_of = [&](int row, int c) {          // the parts of K in order
             const float* from = a.v + size_t(s_t[row]) * a.SR + p * a.R + 8 * c;
             Piece sum{{*reinterpret_cast<const f32x4*>(from), *reinterpret_cast<const f32x4*>(from + 4)}};
@@ -544,6 +589,8 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
                     for (int e = 0; e < 4; ++e) sum.v[h][e] += part[e];
                 }
             }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum.v[e >> 2][e & 3] *= scale;
             return sum;
         };
         if constexpr (TYPE == ORNITH_ADAPTER_F16) {
@@ -558,18 +605,21 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
         }
         for (int i = tid; i < 16 * MT * steps * 4; i += 64 * kExpandWaves) {
             const int row = i / (steps * 4), c = i % (steps * 4);
-            u32x4 piece = {0, 0, 0, 0};
-            if (c < 2 * chunks) {
-                const Piece v = piece_of(row, c < chunks ? c : c - chunks);
+            u32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+            if (c < chunks) {
+                const Piece v = piece_of(row, c);
                 const float by = TYPE == ORNITH_ADAPTER_F16 ? ad_scale16(s_most[row]) : 1.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    uint32_t hi, lo;
-                    ad_halves<TYPE>(v.v[e >> 2][e & 3] * by, hi, lo);
-                    piece[e >> 1] |= (c < chunks ? hi : lo) << (16 * (e & 1));
+                    uint32_t h, l;
+                    ad_halves<TYPE>(v.v[e >> 2][e & 3] * by, h, l);
+                    hi[e >> 1] |= h << (16 * (e & 1));
+                    lo[e >> 1] |= l << (16 * (e & 1));
                 }
             }
-            s_v[((row >> 4) * steps + (c >> 2)) * 64 + (c & 3) * 16 + (row & 15)] = piece;
+            u32x4* const to = &s_v[((row >> 4) * 2 * steps + (c >> 2)) * 64 + (c & 3) * 16 + (row & 15)];
+            to[0] = hi;
+            to[64 * steps] = lo;
         }
         __syncthreads();
     }
@@ -577,35 +627,53 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
     float by[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        by[m] = a.scales[slot];
-        if constexpr (TYPE == ORNITH_ADAPTER_F16) by[m] = by[m] / ad_scale16(s_most[16 * m + li]);
+        by[m] = 1.f;
+        if constexpr (TYPE == ORNITH_ADAPTER_F16) by[m] = 1.f / ad_scale16(s_most[16 * m + li]);
     }
     f32x4 acc[MT][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const uint16_t* b[4];
+    // 64 r at a time: eight lanes on a column's 128 bytes, through LDS to the operands' order (piece c of column
+    // n at 8 n + (c ^ n % 8)); the next ones on their way meanwhile
+    const uint16_t* const bank = a.b + size_t(slot) * size_t(a.b_slot);
+    uint32_t of[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)                        // (past the slice: its last column)
-        b[j] = a.b + size_t(slot) * size_t(a.b_slot) + size_t(min(n0 + 16 * j + li, end - 1)) * a.R;
-    for (int s = 0; s < steps; ++s) {
-        const int c = 4 * s + q, at = 8 * (c < chunks ? c : min(c - chunks, chunks - 1));
-        u32x4 bv[4];
+    for (int i = 0; i < 8; ++i) of[i] = uint32_t(min(n0 + 8 * i + (lane >> 3), end - 1)) * uint32_t(a.R);  // (past the slice: its last column)
+    u32x4 bv[8];
+    auto load_b = [&](int s) {
+        const int c = min(4 * s + (lane & 7), chunks - 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const u32x4*>(b[j] + at);
-        if (c >= 2 * chunks) {                         // (no 0 times inf)
+        for (int i = 0; i < 8; ++i) bv[i] = *reinterpret_cast<const u32x4*>(bank + (of[i] + uint32_t(8 * c)));
+    };
+    u32x4* const put = s_stage[wv] + 8 * (lane >> 3) + ((lane & 7) ^ (lane >> 3));
+    load_b(0);
+    for (int s = 0; s < steps; s += 2) {
+        const bool none = 4 * s + (lane & 7) >= chunks;          // (no 0 times inf)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bv[j] = u32x4{0, 0, 0, 0};
+        for (int i = 0; i < 8; ++i) put[64 * i] = none ? u32x4{0, 0, 0, 0} : bv[i];
+        if (s + 2 < steps) load_b(s + 2);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (s + h >= steps) break;
+            u32x4 bw[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bw[j] = s_stage[wv][8 * (16 * j + li) + ((4 * h + q) ^ (li & 7))];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const u32x4 *from = &s_v[(m * 2 * steps + s + h) * 64 + lane], hi = from[0], lo = from[64 * steps];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[m][j] = ad_mfma<TYPE>(bw[j], lo, ad_mfma<TYPE>(bw[j], hi, acc[m][j]));
+            }
         }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const u32x4 vv = s_v[(m * steps + s) * 64 + lane];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[m][j] = ad_mfma<TYPE>(bv[j], vv, acc[m][j]);
-        }
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
-    cells.finish(a, acc, by, s_stage[wv], n0, end, whole, rows);
+    cells.template add<TYPE == ORNITH_ADAPTER_F16>(acc, by, reinterpret_cast<f32x4*>(s_stage[wv]), whole, end - n0);
+    flag_or(a.flags, cells.flags());
 }
 
 // ---- both in one ----------------------------------------------------------------
@@ -613,9 +681,9 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
 // a time.  Every block of columns reads x and A again, from its XCD's L2, and spares the second launch.
 template <int TYPE, int OUT, int MT, int RT, int W, int FEW>
 __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
-    constexpr int D = FEW && MT + RT <= 3 ? 4 : 2, BUFS = FEW || RT == 4 ? 1 : 2;
-    typedef AdCells<OUT, MT, BUFS, FEW == 0> Cells;
-    static_assert((MT + RT) * 128 >= std::max(MT * RT * 64, 256));
+    constexpr int D = FEW && MT + RT <= 3 ? 4 : 2;
+    typedef AdCells<OUT, MT, FEW == 0> Cells;
+    static_assert((MT + RT) * 128 >= std::max(MT * RT * 64, std::max(256, 128 * RT)));
     __shared__ u32x4 s_stage[W][(MT + RT) * 128];      // (then the waves' sums)
     __shared__ u32x4 s_v[MT][RT][64];
     __shared__ uint32_t s_most[16 * MT];
@@ -629,19 +697,18 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
     while (cb >= a.blocks[p]) ++p;
     const int begin = (p ? a.ends[p - 1] : 0) + (cb - (p ? a.blocks[p - 1] : 0)) * (64 * W * a.groups);
     const int end = min(a.ends[p], begin + 64 * W * a.groups);
-    Cells cells(a, t);
+    const int whole_end = ad_whole_end<Cells::size>(a, begin, end);
+    int n0 = begin + 64 * wv;
+    Cells cells(a, t, rows, n0);
     if (slot < 0) {
-        for (int n0 = begin + 64 * wv; n0 < end; n0 += 64 * W) {
-            const bool whole = ad_whole<Cells::size>(a, n0, end);
-            cells.load(n0, end, whole);
-            cells.copy(n0, end, whole, rows);
+        for (; n0 < end; n0 += 64 * W) {
+            cells.copy(n0 < whole_end, end - n0);
+            cells.step(64 * W);
         }
         return;
     }
     const int chunks = a.R / 8;
-    float by[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) by[m] = a.scales[slot];
+    const float scale = a.scales[slot];
     {
         f32x4 acc[MT][RT];
 #pragma unroll
@@ -657,24 +724,33 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
     }
     for (int f = wv; f < MT * RT; f += W) s_v[f / RT][f % RT][lane] = u32x4{0, 0, 0, 0};
     if (TYPE == ORNITH_ADAPTER_F16 && tid < 16 * MT) s_most[tid] = 0;
-    // the first columns on their way meanwhile
-    const uint16_t* const bs = a.b + size_t(slot) * size_t(a.b_slot);
-    u32x4 bv[BUFS][RT][4];
-    auto load_b = [&](auto buf, int n0) {              // (past the slice: its last column)
-        if (n0 >= end) return;
+    // B of 64 columns: 128 R neighbouring bytes, loaded as they lie (the first on their way while the waves meet)
+    // and through LDS to the operands' order: piece c of column n at chunks n + (c ^ swap(n)), few bank conflicts.
+    const char* const bank = reinterpret_cast<const char*>(a.b + size_t(slot) * size_t(a.b_slot));
+    const int swap_bits = chunks & (chunks - 1) ? 0 : chunks - 1, swap_shift = chunks == 2 ? 2 : chunks == 4 ? 1 : 0;
+    u32x4 bv[2 * RT];
+    int to_b[2 * RT], from_b[RT];                      // places in LDS: of the pieces loaded, of the steps' operands
 #pragma unroll
-        for (int s = 0; s < RT; ++s) {
-            const int c = 4 * s + q, from = 8 * min(c < chunks ? c : c - chunks, chunks - 1);
+    for (int i = 0; i < 2 * RT; ++i) {
+        const int col = (64 * i + lane) / chunks, c = (64 * i + lane) % chunks;
+        to_b[i] = chunks * col + (c ^ (col >> swap_shift & swap_bits));
+    }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                bv[decltype(buf)::value][s][j] =
-                    *reinterpret_cast<const u32x4*>(bs + uint32_t(min(n0 + 16 * j + li, end - 1)) * uint32_t(a.R) + from);
-        }
+    for (int s = 0; s < RT; ++s) {
+        const int c = (4 * s + q) % chunks;
+        from_b[s] = chunks * li + (c ^ (li >> swap_shift & swap_bits));    // (column 16 j + li: 16 j chunks further)
+    }
+    auto load_b = [&](int last) {                      // (past the last piece: that one again)
+        const char* const from = bank + uint32_t(n0) * uint32_t(2 * a.R);
+#pragma unroll
+        for (int i = 0; i < 2 * RT; ++i)
+            if (i < chunks) bv[i] = *reinterpret_cast<const u32x4*>(from + 16u * uint32_t(min(64 * i + lane, last)));
     };
-    int n0 = begin + 64 * wv;
-    bool whole = n0 < end && ad_whole<Cells::size>(a, n0, end);
-    cells.load(n0, end, whole);
-    load_b(std::integral_constant<int, 0>{}, n0);
+    const int all_b = 64 * chunks - 1;
+    if (n0 < whole_end) {
+        cells.load(true, 64);
+        load_b(all_b);
+    }
     __syncthreads();
     constexpr int F = (MT * RT + W - 1) / W;           // pieces of 16 rows and 16 of the rank, a wave
     f32x4 v[F];
@@ -689,6 +765,8 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i0][i] += part[i];
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i0][i] *= scale;
         if (TYPE == ORNITH_ADAPTER_F16 && 16 * (f % RT) + li < a.R) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) atomicMax(&s_most[16 * (f / RT) + 4 * q + i], __float_as_uint(v[i0][i]) & 0x7fffffffu);
@@ -711,51 +789,58 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
         }
     }
     __syncthreads();
-    if constexpr (TYPE == ORNITH_ADAPTER_F16) {
+    float by[MT];
 #pragma unroll
-        for (int mm = 0; mm < MT; ++mm) by[mm] = by[mm] / ad_scale16(s_most[16 * mm + li]);
-    }
-    // 64 columns of buffer C, the next ones' loads before them
-    auto columns = [&](auto buf) {
-        constexpr int C = decltype(buf)::value, N = BUFS == 2 ? 1 - C : C;
-        const int next = n0 + 64 * W;
-        const bool next_whole = next < end && ad_whole<Cells::size>(a, next, end);
-        if constexpr (BUFS == 2) {
-            cells.template load<N>(next, end, next_whole);
-            load_b(std::integral_constant<int, N>{}, next);
-        }
-        f32x4 sum[MT][4];
+    for (int m = 0; m < MT; ++m) by[m] = TYPE == ORNITH_ADAPTER_F16 ? 1.f / ad_scale16(s_most[16 * m + li]) : 1.f;
+    f32x4 sum[MT][4];
+    f32x4* const stage = reinterpret_cast<f32x4*>(s_stage[wv]);
+    auto product = [&] {
+        u32x4* const stage_b = s_stage[wv];
 #pragma unroll
-        for (int mm = 0; mm < MT; ++mm)
+        for (int i = 0; i < 2 * RT; ++i)
+            if (i < chunks) stage_b[to_b[i]] = bv[i];
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[mm][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < RT; ++s) {
             if (4 * s >= 2 * chunks) break;
-            if (4 * s + q >= 2 * chunks) {             // (no 0 times inf)
+            u32x4 step[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) bv[C][s][j] = u32x4{0, 0, 0, 0};
+            for (int j = 0; j < 4; ++j) {
+                step[j] = stage_b[from_b[s] + 16 * j * chunks];
+                if (4 * s + 4 > 2 * chunks && 4 * s + q >= 2 * chunks) step[j] = u32x4{0, 0, 0, 0};      // (no 0 times inf)
             }
 #pragma unroll
-            for (int mm = 0; mm < MT; ++mm) {
-                const u32x4 vv = s_v[mm][s][lane];
+            for (int m = 0; m < MT; ++m) {
+                const u32x4 vv = s_v[m][s][lane];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sum[mm][j] = ad_mfma<TYPE>(bv[C][s][j], vv, sum[mm][j]);
+                for (int j = 0; j < 4; ++j) sum[m][j] = ad_mfma<TYPE>(step[j], vv, sum[m][j]);
             }
         }
-        if constexpr (BUFS == 1) load_b(buf, next);
-        cells.template finish<C>(a, sum, by, reinterpret_cast<f32x4*>(s_stage[wv]), n0, end, whole, rows);
-        if constexpr (BUFS == 1) cells.load(next, end, next_whole);
-        n0 = next;
-        whole = next_whole;
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     };
-    while (n0 < end) {
-        columns(std::integral_constant<int, 0>{});
-        if constexpr (BUFS == 2) {
-            if (n0 >= end) break;
-            columns(std::integral_constant<int, 1>{});
-        }
+    constexpr bool SCALED = TYPE == ORNITH_ADAPTER_F16;
+    while (n0 < whole_end) {
+        product();
+        n0 += 64 * W;
+        if (n0 < whole_end) load_b(all_b);
+        cells.template add<SCALED>(sum, by, stage, true, 64);
+        cells.step(64 * W);
+        if (n0 < whole_end) cells.load(true, 64);
     }
+    for (; n0 < end; n0 += 64 * W) {
+        cells.load(false, end - n0);
+        load_b(min(all_b, (end - n0) * chunks - 1));
+        product();
+        cells.template add<SCALED>(sum, by, stage, false, end - n0);
+        cells.step(64 * W);
+    }
+    flag_or(a.flags, cells.flags());
 }
 
 struct AdLayout { size_t v, tiles, bytes; };
@@ -764,7 +849,12 @@ struct AdLayout { size_t v, tiles, bytes; };
 int ad_splits(int64_t M) { return M <= kFewRows ? 4 : 1; }
 
 // Rows of a planned tile, and tiles at most.
-int ad_tile_rows(int M, int R) { return R <= kBothRank ? 16 : M >= 1024 && R <= 128 ? 64 : 16; }
+// (us: both products of one launch in tiles of 16 / 32 rows, 6144 columns of K = 2048: rank 16, 8192 rows 66.4 /
+// 69.6; rank 32, 76.3 / 75.5, 1120 rows 18.0 / 18.2; rank 64, 8192 rows 119 / 93.6, 1120 rows of 2048 columns 18.8 / 21.4)
+int ad_tile_rows(int M, int R) {
+    if (R <= kBothRank) return R > 32 && M >= 4096 ? 32 : 16;
+    return M >= 1024 && R <= 128 ? 64 : 16;
+}
 int ad_tiles(int M, int slots, int tile_rows) { return std::min(M, (M + tile_rows - 1) / tile_rows + slots + 1); }
 
 bool ad_layout(int64_t M, int S, int R, AdLayout& l) {
@@ -793,36 +883,51 @@ template <class F> void ad_by_type(int out_type, F&& f) {
     else f(std::integral_constant<int, ORNITH_ADAPTER_F16>{});
 }
 
-template <int TYPE, int MT, int W, int FEW> hipError_t ad_both(AdArgs& a, int out_type, int groups, hipStream_t s) {
-    a.groups = groups;
-    const dim3 grid((a.units + 7) / 8 * 8 * ad_blocks(a, 64 * W * groups));
+// Columns of a block, in 64 a wave: all that a tile has in as many even parts as make about 1024 blocks of 16 rows
+// (two rounds of the chip's CUs with two each) of many tiles, and three groups a block, or two, of fewer, since each
+// block forms v again (us, 1 / 2 / 3 / 6 groups, rank 16: 8192 x 6144 101 / 77 / 68 / 66; 4096 x 6144 57 / 35 / 32 / 34;
+// 512 x 6144 14.3 / 13.6 / 13.4 / 16.8; 1120 x 2048 13.9 / 13.5 / 14.9 / 14.6; 300 x 2048 10.5 / 11.6).
+int ad_groups(const AdArgs& a, int FEW, int W) {
+    if (FEW) return 1;
+    const int all = (a.N + 64 * W - 1) / (64 * W);
+    const int64_t cells = int64_t(all) * ((a.M + 15) / 16);
+    const int64_t groups = std::max<int64_t>((cells + 1023) / 1024, std::min<int64_t>(3, (cells + 159) / 160));
+    const int parts = int((all + groups - 1) / groups);
+    return (all + parts - 1) / parts;
+}
+
+template <int TYPE, int MT, int FEW> hipError_t ad_both(AdArgs& a, int out_type, hipStream_t s) {
+    constexpr int W = 8;
+    a.groups = ad_groups(a, FEW, W);
+    const dim3 grid((a.units + 7) / 8 * 8 * ad_blocks(a, 64 * W * a.groups));
     auto go = [&](auto kernel) { timed_launch("adapter_both", kernel, grid, dim3(64 * W), 0, s, a); };
     ad_by_type(out_type, [&](auto out) {
         constexpr int OUT = decltype(out)::value;
-        if (a.R <= 16) go(adapter_both_kernel<TYPE, OUT, MT, 1, W, FEW>);
-        else if (a.R <= 32) go(adapter_both_kernel<TYPE, OUT, MT, 2, W, FEW>);
-        else go(adapter_both_kernel<TYPE, OUT, MT, 4, W, FEW>);
+        if constexpr (MT == 2) go(adapter_both_kernel<TYPE, OUT, 2, 4, W, FEW>);
+        else if (a.R <= 16) go(adapter_both_kernel<TYPE, OUT, 1, 1, W, FEW>);
+        else if (a.R <= 32) go(adapter_both_kernel<TYPE, OUT, 1, 2, W, FEW>);
+        else go(adapter_both_kernel<TYPE, OUT, 1, 4, W, FEW>);
     });
     return hipGetLastError();
 }
 
 template <int TYPE, int MT, int FEW> hipError_t ad_two(AdArgs& a, int out_type, hipStream_t s) {
     const int rt = (a.SR + 15) / 16;
-    constexpr int SMT = 1;
-    a.sub = MT / SMT;
-    a.splits = std::min(ad_splits(a.M), (a.K + 511) / 512);
-    a.splits = std::max(a.splits, 1);
+    a.sub = MT;                                        // (16 rows a block: more blocks to read x)
+    a.splits = std::max(1, std::min(ad_splits(a.M), (a.K + 511) / 512));
     auto shrink = [&](auto kernel, int RT) {
         timed_launch("adapter_shrink", kernel, dim3(a.units * a.sub, (rt + RT - 1) / RT, a.splits), dim3(64 * kShrinkWaves), 0, s, a);
     };
-    shrink(adapter_shrink_kernel<TYPE, SMT, 1, 4, FEW>, 1);
+    // few rows: 16 of A's a block, more blocks; many: 64, which reads x less often
+    if (FEW || rt < 4) shrink(adapter_shrink_kernel<TYPE, 1, 1, 4, FEW>, 1);
+    else shrink(adapter_shrink_kernel<TYPE, 1, 4, 2, FEW>, 4);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
     const dim3 grid(a.units, ad_blocks(a, 64 * kExpandWaves));
-    const int steps = (a.R / 4 + 3) / 4;
+    const int steps = (a.R / 8 + 3) / 4;
     ad_by_type(out_type, [&](auto out) {
         timed_launch("adapter_expand", adapter_expand_kernel<TYPE, decltype(out)::value, MT, FEW>, grid, dim3(64 * kExpandWaves),
-                     uint32_t(MT * steps * 1024), s, a);
+                     uint32_t(MT * steps * 2048), s, a);
     });
     return hipGetLastError();
 }
@@ -830,14 +935,14 @@ template <int TYPE, int MT, int FEW> hipError_t ad_two(AdArgs& a, int out_type, 
 template <int TYPE> hipError_t ad_rows(AdArgs& a, int out_type, hipStream_t s) {
     const bool both = a.R <= kBothRank;
     a.units = a.M;
-    if (a.M <= 64) return both ? ad_both<TYPE, 1, 8, 1>(a, out_type, 1, s) : ad_two<TYPE, 1, 1>(a, out_type, s);
-    if (a.M <= kFewRows) return both ? ad_both<TYPE, 1, 8, 4>(a, out_type, 1, s) : ad_two<TYPE, 1, 4>(a, out_type, s);
+    if (a.M <= 64) return both ? ad_both<TYPE, 1, 1>(a, out_type, s) : ad_two<TYPE, 1, 1>(a, out_type, s);
+    if (a.M <= kFewRows) return both ? ad_both<TYPE, 1, 4>(a, out_type, s) : ad_two<TYPE, 1, 4>(a, out_type, s);
     a.tile_rows = ad_tile_rows(a.M, a.R);
     a.units = ad_tiles(a.M, a.slots, a.tile_rows);
     timed_launch("adapter_plan", adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
-    if (both) return ad_both<TYPE, 1, 8, 0>(a, out_type, 6, s);
+    if (both) return a.tile_rows == 32 ? ad_both<TYPE, 2, 0>(a, out_type, s) : ad_both<TYPE, 1, 0>(a, out_type, s);
     return a.tile_rows == 64 ? ad_two<TYPE, 4, 0>(a, out_type, s) : ad_two<TYPE, 1, 0>(a, out_type, s);
 }
 
