@@ -778,33 +778,34 @@ def _route_experts(logits, weights, ids, flags, score, bias, groups, kept_groups
         raise ValueError('logits must be bf16, fp16 or fp32 [M, E] with unit column stride')
     if by is None:
         raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
-    (rows, n), (ld, step), gpu = logits.shape, logits.stride(), logits.get_device()
+    (rows, n), (ld, step), gpu, picks = logits.shape, logits.stride(), logits.get_device(), weights.shape
     if step != 1 and n > 1:
         raise ValueError('logits must be bf16, fp16 or fp32 [M, E] with unit column stride')
     if rows <= 1:
         ld = n
     elif ld < n:
         raise ValueError(f'logits rows overlap: row stride {ld} of {n} columns')
-    if weights.ndim != 2:
-        raise ValueError('weights must be fp32 [M, k]')
-    k = weights.shape[1]
-    picks = (rows, k)
-    args = [_row_ptr(t, name, dtype, shape, logits) for t, name, dtype, shape in
-            ((bias, 'bias', torch.float32, (n,)), (weights, 'weights', torch.float32, picks),
-             (ids, 'ids', torch.int32, picks))]
+    if len(picks) != 2 or picks[0] != rows:
+        raise ValueError(f'weights must be fp32 [{rows}, k], got {tuple(picks)}')
+    k = picks[1]
+    bias_ptr = _row_ptr(bias, 'bias', torch.float32, (n,), logits)
+    weights_ptr, ids_ptr = weights.data_ptr(), ids.data_ptr()
+    if (weights.dtype != torch.float32 or ids.dtype != torch.int32 or ids.shape != picks or not weights.is_contiguous()
+            or not ids.is_contiguous()):
+        raise ValueError(f'weights and ids must be contiguous fp32 and int32 {list(picks)} tensors, got {weights.dtype} and '
+                         f'{tuple(ids.shape)} {ids.dtype}')
     if not (1 <= n <= 1024 and 1 <= groups <= 64 and n % groups == 0 and 1 <= kept_groups <= groups
-            and group_top in (1, 2) and 1 <= k <= min(32, kept_groups * (n // groups))):
+            and 1 <= group_top <= 2 and 1 <= k <= 32 and k <= kept_groups * (n // groups)):
         raise ValueError(f'cannot pick {k} of {n} experts in {kept_groups} of {groups} groups by their {group_top} best: '
                          f'at most 1024 experts, 64 groups that divide them, 32 picks of those in the kept groups, 1 or 2 best')
+    if not -3.4028234e38 <= scale <= 3.4028234e38:
+        raise ValueError(f'scale must be a finite fp32 number, got {scale}')
     if flags.dtype != torch.int32 or flags.numel() != 1:
         raise ValueError('flags must be one int32 word')
-    if gpu < 0 or flags.get_device() != gpu:
+    if gpu < 0 or weights.get_device() != gpu or ids.get_device() != gpu or flags.get_device() != gpu:
         raise ValueError('logits, outputs and flags must be on one GPU')
-    scale = float(scale)
-    if not abs(scale) <= 3.4028234e38:
-        raise ValueError(f'scale must be a finite fp32 number, got {scale}')
-    call_on(gpu, lib().ornith_route_experts_launch, 'expert routing', logits.data_ptr(), kind, rows, n, ld, args[0], by,
-            groups, kept_groups, group_top, k, bool(renormalize), scale, args[1], args[2], flags.data_ptr())
+    call_on(gpu, lib().ornith_route_experts_launch, 'expert routing', logits.data_ptr(), kind, rows, n, ld, bias_ptr, by,
+            groups, kept_groups, group_top, k, 1 if renormalize else 0, scale, weights_ptr, ids_ptr, flags.data_ptr())
 
 
 @torch.library.custom_op('ornith_g256::route_experts', mutates_args={'weights', 'ids', 'flags'}, device_types='cuda')
@@ -896,10 +897,9 @@ def _adapter_out(x, a, b, scales, ids, base, out, workspace, flags, slices):
     if (sx != 1 and k > 1) or ((so != 1 or sb != 1) and n > 1) or ldx < k or ldo < n or ldb < n:
         raise ValueError('input, base and output rows must have unit column stride and not overlap')
     x_ptr, a_ptr, b_ptr = x.data_ptr(), a.data_ptr(), b.data_ptr()
-    if ldx % 8 or a_slot % 8 or b_slot % 8 or (x_ptr | a_ptr | b_ptr) % 16:
+    if (ldx | a_slot | b_slot) % 8 or (x_ptr | a_ptr | b_ptr) % 16:
         raise ValueError('input rows and adapters must start on the 16-byte grid')
-    row = (rows,)
-    ids_ptr = _row_ptr(ids, 'ids', torch.int32, row, x)
+    ids_ptr = _row_ptr(ids, 'ids', torch.int32, (rows,), x)
     scales_ptr = _row_ptr(scales, 'scales', torch.float32, (slots,), x)
     if ids_ptr is None or scales_ptr is None:
         raise ValueError('ids and scales are required')
