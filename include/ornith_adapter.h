@@ -9,10 +9,12 @@
  *
  * x, A and B are all bf16 or all fp16; base and out bf16, fp16 or fp32, out perhaps
  * base itself (the same rows), which leaves rows without an adapter untouched.
- * Each product is exact and summed in fp32; v enters the second product as
- * the sum of two 16-bit numbers, off by at most 2^-16 (bf16) or 2^-21 (fp16) of
- * the largest of its row and slice; one rounding to the output's type.  A row
- * depends on no other row.
+ * Each product is exact and summed in fp32; scale v enters the second product
+ * as the sum of 16-bit numbers, off by at most 2^-18 of itself (bf16, 16-bit
+ * results), 2^-26 (bf16, fp32 results) or 2^-23 and 2^-38 of the largest of its
+ * row and slice (fp16); one rounding to the output's type.  A row depends on no
+ * other row's values; the order of its sums goes by the numbers of rows and of
+ * columns.
  *
  * A merged projection (q, k and v, or gate and up) has S slices of consecutive
  * columns, R rows of A each; a plain one has one slice.  Slots with a smaller

@@ -5,9 +5,8 @@
 // matrix cores, each row's sums its own:
 //   shrink  v[t, r] = sum_k x[t, k] A[r, k]: a block per tile and chunk of r,
 //           its waves share k and meet in LDS in wave order;
-//   expand  out[t, n] = base[t, n] + scale sum_r B[n, r] v[t, r]: v, fp32, as the
-//           sum of two 16-bit numbers hi + lo side by side along r, so the
-//           second product loses no more than 2^-17 of it.  The product is
+//   expand  out[t, n] = base[t, n] + scale sum_r B[n, r] v[t, r]: scale v, fp32, as
+//           the sum of two or three 16-bit numbers side by side along r.  The product is
 //           formed transposed (columns as rows of the instruction) and goes
 //           through LDS to lanes that move whole rows' pieces of base and out.
 #include <algorithm>
@@ -389,11 +388,16 @@ __device__ __forceinline__ float ad_scale16(uint32_t most) {
     if (e == 0 || e == 255) return 1.f;
     return __uint_as_float(uint32_t(min(max(127 + 127 + 14 - e, 1), 254)) << 23);
 }
-// The two 16-bit numbers whose sum v is (inf: no NaN beside it).
-template <int TYPE> __device__ __forceinline__ void ad_halves(float v, uint32_t& hi, uint32_t& lo) {
-    hi = ad_bits<TYPE>(v);
-    const float h = ad_float<TYPE>(hi);
-    lo = __builtin_isinf(h) ? 0u : ad_bits<TYPE>(v - h);
+// 16-bit numbers whose sum v is: two (off by 2^-18 of v at most in bf16, 2^-24 in fp16), and three of bf16 for
+// fp32 results (2^-27).
+template <int TYPE, int OUT> constexpr int kAdParts = TYPE == ORNITH_ADAPTER_BF16 && OUT == ORNITH_ADAPTER_F32 ? 3 : 2;
+template <int TYPE, int PARTS> __device__ __forceinline__ void ad_split(float v, uint32_t (&bits)[PARTS]) {
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        bits[p] = ad_bits<TYPE>(v);
+        const float part = ad_float<TYPE>(bits[p]);
+        v = __builtin_isinf(part) ? 0.f : v - part;    // (inf: no NaN beside it)
+    }
 }
 // Columns from which on 64 are not whole and on the 16-byte grid, of the columns from begin to end (whose
 // groups of 64 start at begin): the last ones, or all.
@@ -547,7 +551,8 @@ constexpr int kExpandWaves = 4;                        // a block: 64 columns a 
 
 template <int TYPE, int OUT, int MT, int FEW>
 __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArgs a) {
-    extern __shared__ __attribute__((aligned(16))) u32x4 s_v[];        // [MT][hi, lo][steps][64]
+    extern __shared__ __attribute__((aligned(16))) u32x4 s_v[];        // [MT][parts][steps][64]
+    constexpr int PARTS = kAdParts<TYPE, OUT>;
     __shared__ uint32_t s_most[16 * MT];
     __shared__ int s_t[16 * MT];
     __shared__ u32x4 s_stage[kExpandWaves][512];       // a wave's B of 64 columns and 64 r, then its results
@@ -605,21 +610,21 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
         }
         for (int i = tid; i < 16 * MT * steps * 4; i += 64 * kExpandWaves) {
             const int row = i / (steps * 4), c = i % (steps * 4);
-            u32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+            u32x4 part[PARTS] = {};
             if (c < chunks) {
                 const Piece v = piece_of(row, c);
                 const float by = TYPE == ORNITH_ADAPTER_F16 ? ad_scale16(s_most[row]) : 1.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    uint32_t h, l;
-                    ad_halves<TYPE>(v.v[e >> 2][e & 3] * by, h, l);
-                    hi[e >> 1] |= h << (16 * (e & 1));
-                    lo[e >> 1] |= l << (16 * (e & 1));
+                    uint32_t bits[PARTS];
+                    ad_split<TYPE, PARTS>(v.v[e >> 2][e & 3] * by, bits);
+#pragma unroll
+                    for (int u = 0; u < PARTS; ++u) part[u][e >> 1] |= bits[u] << (16 * (e & 1));
                 }
             }
-            u32x4* const to = &s_v[((row >> 4) * 2 * steps + (c >> 2)) * 64 + (c & 3) * 16 + (row & 15)];
-            to[0] = hi;
-            to[64 * steps] = lo;
+#pragma unroll
+            for (int u = 0; u < PARTS; ++u)
+                s_v[(((row >> 4) * PARTS + u) * steps + (c >> 2)) * 64 + (c & 3) * 16 + (row & 15)] = part[u];
         }
         __syncthreads();
     }
@@ -664,9 +669,12 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
             for (int j = 0; j < 4; ++j) bw[j] = s_stage[wv][8 * (16 * j + li) + ((4 * h + q) ^ (li & 7))];
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const u32x4 *from = &s_v[(m * 2 * steps + s + h) * 64 + lane], hi = from[0], lo = from[64 * steps];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[m][j] = ad_mfma<TYPE>(bw[j], lo, ad_mfma<TYPE>(bw[j], hi, acc[m][j]));
+                for (int u = 0; u < PARTS; ++u) {
+                    const u32x4 vv = s_v[((m * PARTS + u) * steps + s + h) * 64 + lane];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[m][j] = ad_mfma<TYPE>(bw[j], vv, acc[m][j]);
+                }
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
@@ -681,11 +689,11 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
 // a time.  Every block of columns reads x and A again, from its XCD's L2, and spares the second launch.
 template <int TYPE, int OUT, int MT, int RT, int W, int FEW>
 __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
-    constexpr int D = FEW && MT + RT <= 3 ? 4 : 2;
+    constexpr int D = FEW && MT + RT <= 3 ? 4 : 2, PARTS = kAdParts<TYPE, OUT>, STEPS = (PARTS * RT + 1) / 2;
     typedef AdCells<OUT, MT, FEW == 0> Cells;
     static_assert((MT + RT) * 128 >= std::max(MT * RT * 64, std::max(256, 128 * RT)));
     __shared__ u32x4 s_stage[W][(MT + RT) * 128];      // (then the waves' sums)
-    __shared__ u32x4 s_v[MT][RT][64];
+    __shared__ u32x4 s_v[MT][STEPS][64];
     __shared__ uint32_t s_most[16 * MT];
     int slot, rows, t[MT];
     // blocks go to the 8 XCDs in turn: a row's column blocks on one of them, whose L2 keeps its A
@@ -722,21 +730,21 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
 #pragma unroll
             for (int r = 0; r < RT; ++r) reinterpret_cast<f32x4*>(s_stage[wv])[64 * (m * RT + r) + lane] = acc[m][r];
     }
-    for (int f = wv; f < MT * RT; f += W) s_v[f / RT][f % RT][lane] = u32x4{0, 0, 0, 0};
+    for (int f = wv; f < MT * STEPS; f += W) s_v[f / STEPS][f % STEPS][lane] = u32x4{0, 0, 0, 0};
     if (TYPE == ORNITH_ADAPTER_F16 && tid < 16 * MT) s_most[tid] = 0;
     // B of 64 columns: 128 R neighbouring bytes, loaded as they lie (the first on their way while the waves meet)
     // and through LDS to the operands' order: piece c of column n at chunks n + (c ^ swap(n)), few bank conflicts.
     const char* const bank = reinterpret_cast<const char*>(a.b + size_t(slot) * size_t(a.b_slot));
     const int swap_bits = chunks & (chunks - 1) ? 0 : chunks - 1, swap_shift = chunks == 2 ? 2 : chunks == 4 ? 1 : 0;
     u32x4 bv[2 * RT];
-    int to_b[2 * RT], from_b[RT];                      // places in LDS: of the pieces loaded, of the steps' operands
+    int to_b[2 * RT], from_b[STEPS];                     // places in LDS: of the pieces loaded, of the steps' operands
 #pragma unroll
     for (int i = 0; i < 2 * RT; ++i) {
         const int col = (64 * i + lane) / chunks, c = (64 * i + lane) % chunks;
         to_b[i] = chunks * col + (c ^ (col >> swap_shift & swap_bits));
     }
 #pragma unroll
-    for (int s = 0; s < RT; ++s) {
+    for (int s = 0; s < STEPS; ++s) {
         const int c = (4 * s + q) % chunks;
         from_b[s] = chunks * li + (c ^ (li >> swap_shift & swap_bits));    // (column 16 j + li: 16 j chunks further)
     }
@@ -782,10 +790,10 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = 4 * q + i;
-            uint32_t hi, lo;
-            ad_halves<TYPE>(v[i0][i] * (TYPE == ORNITH_ADAPTER_F16 ? ad_scale16(s_most[16 * m + row]) : 1.f), hi, lo);
-            put(r >> 3, row, hi);
-            put((r >> 3) + chunks, row, lo);
+            uint32_t bits[PARTS];
+            ad_split<TYPE, PARTS>(v[i0][i] * (TYPE == ORNITH_ADAPTER_F16 ? ad_scale16(s_most[16 * m + row]) : 1.f), bits);
+#pragma unroll
+            for (int u = 0; u < PARTS; ++u) put((r >> 3) + u * chunks, row, bits[u]);
         }
     }
     __syncthreads();
@@ -806,13 +814,13 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) sum[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < RT; ++s) {
-            if (4 * s >= 2 * chunks) break;
+        for (int s = 0; s < STEPS; ++s) {
+            if (4 * s >= PARTS * chunks) break;
             u32x4 step[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 step[j] = stage_b[from_b[s] + 16 * j * chunks];
-                if (4 * s + 4 > 2 * chunks && 4 * s + q >= 2 * chunks) step[j] = u32x4{0, 0, 0, 0};      // (no 0 times inf)
+                if (4 * s + 4 > PARTS * chunks && 4 * s + q >= PARTS * chunks) step[j] = u32x4{0, 0, 0, 0};      // (no 0 times inf)
             }
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
@@ -926,8 +934,9 @@ template <int TYPE, int MT, int FEW> hipError_t ad_two(AdArgs& a, int out_type, 
     const dim3 grid(a.units, ad_blocks(a, 64 * kExpandWaves));
     const int steps = (a.R / 8 + 3) / 4;
     ad_by_type(out_type, [&](auto out) {
-        timed_launch("adapter_expand", adapter_expand_kernel<TYPE, decltype(out)::value, MT, FEW>, grid, dim3(64 * kExpandWaves),
-                     uint32_t(MT * steps * 2048), s, a);
+        constexpr int OUT = decltype(out)::value;
+        timed_launch("adapter_expand", adapter_expand_kernel<TYPE, OUT, MT, FEW>, grid, dim3(64 * kExpandWaves),
+                     uint32_t(MT * steps * kAdParts<TYPE, OUT> * 1024), s, a);
     });
     return hipGetLastError();
 }
