@@ -37,7 +37,8 @@ extern "C" {
 enum { ORNITH_ADAPTER_BF16 = 0, ORNITH_ADAPTER_F16 = 1, ORNITH_ADAPTER_F32 = 2 };
 enum { ORNITH_ADAPTER_MAX_SLICES = 8, ORNITH_ADAPTER_MAX_SLOTS = 4096, ORNITH_ADAPTER_MAX_RANK = 512 };
 
-/* Workspace for calls of up to Mcap rows with S * R rows of A. */
+/* Workspace for calls of up to Mcap rows with S * R rows of A (however they are
+ * divided). */
 ORNITH_EXPORT hipError_t ornith_adapter_get_layout(int Mcap, int S, int R, size_t* workspace_bytes);
 
 /* x [M, K] of x_type with row stride ldx; A [slots, S R, K] and B [slots, N, R] of

@@ -573,7 +573,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
     if (n0 < end) cells.load(whole, end - n0);
     const int chunks = a.R / 8, steps = (chunks + 3) / 4;
     {
-        // scale v of the tile's rows and this slice: hi then lo along r, in pieces of 8, as the instruction's operands
+        // scale v of the tile's rows and this slice in its parts, in pieces of 8 along r, as the instruction's operands
         if (tid < 16) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) s_t[16 * m + tid] = t[m];
@@ -869,9 +869,13 @@ bool ad_layout(int64_t M, int S, int R, AdLayout& l) {
     if (M < 0 || S < 1 || S > kAdMaxSlices || R < 8 || R > kAdMaxR || R % 8) return false;
     const size_t rows = size_t(std::min<int64_t>(M, kAdRows));
     l.v = 0;
-    l.tiles = align256(rows * size_t(S) * size_t(R) * 4 * size_t(ad_splits(M)));
-    const size_t most = M <= kFewRows ? 0 : size_t(ad_tiles(int(rows), kAdMaxSlots, ad_tile_rows(int(rows), R)));
-    l.bytes = l.tiles + align256(most * size_t(kTileHead + ad_tile_rows(int(rows), R)) * 4) + 256;
+    // (no less than fewer rows need, whose K may be in parts)
+    l.tiles = align256(std::max(rows * size_t(ad_splits(M)), std::min(rows, size_t(kFewRows)) * size_t(ad_splits(kFewRows))) *
+                       size_t(S) * size_t(R) * 4);
+    size_t words = 0;                                  // of a plan's tiles, whichever rows and slots
+    for (int tile_rows : {16, 32, 64})
+        words = std::max(words, size_t(ad_tiles(int(rows), kAdMaxSlots, tile_rows)) * size_t(kTileHead + tile_rows));
+    l.bytes = l.tiles + align256((M <= kFewRows ? 0 : words) * 4) + 256;
     return true;
 }
 

@@ -12,6 +12,12 @@ registration that routes vLLM's layers to them is in vllm_plugin.py.
 * ``W4LinearMethod`` - a linear of plain 4-bit weights with group scales and
   perhaps zero points, on unrotated bf16 or fp16 rows (no reference
   counterpart); the banks are packed once on the GPU.
+* ``LinearAdapters`` - low-rank adapters of many requests beside a linear of
+  either kind (``attach_adapters``; no reference counterpart): the layer adds
+  each row's own, by the runtime's ``adapter_ids``, to its shared results.
+* ``ExpertRouting`` - how a MoE block picks experts from its gate's logits,
+  other contracts than the router kernel's among them (no reference
+  counterpart).
 * ``G256MoEMethod`` - the routed experts: four N16 banks
   (method.py:100-122), optionally repacked to N32 once on the GPU
   (method.py:124-158), and ``apply`` (method.py:165-183).
@@ -47,6 +53,96 @@ def _register(layer, shapes, dtypes=None):
     return loader
 
 
+class LinearAdapters(torch.nn.Module):
+    """`slots` low-rank adapters of one linear [n, k], of rank `rank` at most:
+    a [slots, S * rank, k], b [slots, n, rank] and a scale each.  slices: the
+    widths of a merged projection's S parts, each with rows of a of its own.  An
+    empty slot adds nothing."""
+
+    def __init__(self, n, k, slots, rank, slices=None, dtype=torch.bfloat16, device=None):
+        super().__init__()
+        self.slices = (int(n),) if slices is None else tuple(int(w) for w in slices)
+        if sum(self.slices) != n or not 1 <= len(self.slices) <= 8 or min(self.slices) < 0:
+            raise ValueError(f'slices must be 1 to 8 widths that sum to {n} columns, got {slices}')
+        if rank % 8 or not 8 <= rank <= 512 or k % 8 or not 1 <= slots <= 4096 or dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f'adapters need a rank of 8 to 512 and inputs that are multiples of 8, 1 to 4096 slots and bf16 or '
+                             f'fp16, got rank {rank}, {k} inputs, {slots} slots, {dtype}')
+        self.n, self.k, self.slots, self.rank = int(n), int(k), int(slots), int(rank)
+        for name, shape, kind in (('a', (slots, len(self.slices) * rank, k), dtype), ('b', (slots, n, rank), dtype),
+                                  ('scales', (slots,), torch.float32)):
+            self.register_buffer(name, torch.zeros(shape, dtype=kind, device=device), persistent=False)
+
+    def _slot(self, slot):
+        if not 0 <= slot < self.slots:
+            raise ValueError(f'slot {slot} outside 0..{self.slots - 1}')
+        return int(slot)
+
+    def load(self, slot, a, b, scale=1.0):
+        """Puts an adapter of rank r <= rank into a slot: a [r, k], or one such for
+        each slice (None: that slice has none), and b [n, r].  The slot's rows
+        must not be in flight."""
+        slot = self._slot(slot)
+        parts = [a] if isinstance(a, torch.Tensor) else list(a)
+        r = b.shape[1] if b.ndim == 2 else -1
+        if b.ndim != 2 or b.shape[0] != self.n or not 0 <= r <= self.rank or len(parts) != len(self.slices) or any(
+                p is not None and tuple(p.shape) != (r, self.k) for p in parts):
+            raise ValueError(f'an adapter here is a [r, {self.k}] for each of {len(self.slices)} slices and b [{self.n}, r] '
+                             f'with r at most {self.rank}, got b {tuple(b.shape)}')
+        with torch.no_grad():
+            self.a[slot].zero_()
+            self.b[slot].zero_()
+            for i, p in enumerate(parts):
+                if p is not None:
+                    self.a[slot, i * self.rank:i * self.rank + r] = p
+            self.b[slot, :, :r] = b
+            self.scales[slot] = scale
+
+    def drop(self, slot):
+        """Empties a slot: its rows get the shared results."""
+        slot = self._slot(slot)
+        with torch.no_grad():
+            for t in (self.a, self.b, self.scales):
+                t[slot].zero_()
+
+    def add(self, runtime, x, out, flags):
+        """Adds to out [rows, n] what the rows' adapters make of x, by the
+        runtime's adapter_ids."""
+        if x.shape[0] > runtime.capacity:
+            raise ValueError(f'{x.shape[0]} rows exceed the configured capacity {runtime.capacity}')
+        native.adapter_out(x, self.a, self.b, self.scales, runtime.adapter_ids[:x.shape[0]], None, out, runtime.workspace,
+                           flags, slices=self.slices)
+
+
+def attach_adapters(layer, slots, rank, slices=None, dtype=torch.bfloat16):
+    """Gives a layer of G256LinearMethod or W4LinearMethod adapters (before the
+    Runtime that binds it, which sizes the workspace for them)."""
+    method = getattr(layer, 'quant_method', None)
+    if type(method) not in (G256LinearMethod, W4LinearMethod):
+        raise ValueError('adapters go beside a dense G256 or plain 4-bit linear')
+    if method.runtime is not None:
+        raise RuntimeError(f'{method.prefix}: adapters are attached before binding')
+    device = next((t.device for t in list(layer.parameters()) + list(layer.buffers())), None)
+    layer.adapters = LinearAdapters(method.n, method.k, slots, rank, slices, dtype, device)
+    return layer.adapters
+
+
+class ExpertRouting:
+    """The experts of each row of a gate's logits and their weights
+    (native.route_experts).  bias: fp32 [experts] or None, for the pick alone."""
+
+    def __init__(self, top, score='softmax', groups=1, kept_groups=1, group_top=1, renormalize=True, scale=1.0, bias=None):
+        self.top, self.score, self.groups, self.kept_groups = int(top), score, int(groups), int(kept_groups)
+        self.group_top, self.renormalize, self.scale, self.bias = int(group_top), bool(renormalize), float(scale), bias
+
+    def apply(self, logits, flags):
+        """Weights fp32 and ids int32, both [rows, top], of logits [rows, experts]."""
+        weights = torch.empty((logits.shape[0], self.top), dtype=torch.float32, device=logits.device)
+        ids = torch.empty((logits.shape[0], self.top), dtype=torch.int32, device=logits.device)
+        native.route_experts(logits, weights, ids, flags, self.score, self.bias, self.groups, self.kept_groups,
+                             self.group_top, self.renormalize, self.scale)
+        return weights, ids
+
+
 class G256LinearMethod:
     fields = ('g256_codes', 'g256_metadata')
 
@@ -69,6 +165,8 @@ class G256LinearMethod:
         rt = self.runtime
         native.dense_out(x, layer.g256_codes, layer.g256_metadata, rt.workspace, out, rt.slots[self.slot],
                          rt.capacity, self.n, self.k, rt.dense_geometry, rt.dense_a8_max_rows)
+        if hasattr(layer, 'adapters'):
+            layer.adapters.add(rt, x, out, rt.slots[self.slot])
         return out.view(*shape, self.n)
 
 
@@ -140,14 +238,21 @@ class W4LinearMethod:
             x = native.w4_grid(x)
         out = torch.empty((x.shape[0], self.n), dtype=self.out_dtype or x.dtype, device=x.device)
         native.w4_out(x, layer.w4_bank, layer.w4_metadata, out, self.runtime.slots[self.slot], self.n, self.k, self.group)
+        if hasattr(layer, 'adapters'):
+            layer.adapters.add(self.runtime, x, out, self.runtime.slots[self.slot])
         return out.view(*shape, self.n)
 
 
 class G256MoEMethod:
     experts, hidden, inter, top = 256, 2048, 512, 8
 
-    def __init__(self, prefix):
+    def __init__(self, prefix, routing=None):
+        """routing: an ExpertRouting of 8 of 256 experts for apply_logits (None: the
+        router kernel's contract, softmax and renormalised weights)."""
         self.prefix = prefix
+        self.routing = ExpertRouting(self.top) if routing is None else routing
+        if self.routing.top != self.top:
+            raise ValueError(f'{prefix}: the routed banks take {self.top} experts a row, not {self.routing.top}')
         self.runtime, self.slot = None, None
 
     def create_weights(self, layer):
@@ -215,6 +320,16 @@ class G256MoEMethod:
             native.routed_out(x, topk_weights, topk_ids, *banks, rt.workspace, out, rt.slots[self.slot],
                               rt.capacity)
         return out
+
+
+    def apply_logits(self, layer, x, logits, **kw):
+        """apply with the experts that this block's routing picks from its gate's
+        logits [T, 256]."""
+        if self.runtime is None:
+            raise RuntimeError(f'{self.prefix}: needs a bound runtime')
+        if logits.ndim != 2 or logits.shape[1] != self.experts:
+            raise ValueError(f'{self.prefix}: the gate gives [T, {self.experts}] logits, got {tuple(logits.shape)}')
+        return self.apply(layer, x, *self.routing.apply(logits, self.runtime.slots[self.slot]), **kw)
 
 
 class RouterGateMethod:
@@ -358,6 +473,10 @@ class Runtime:
                 raise RuntimeError('a layer is already bound to a runtime')
         shapes = sorted({(m.quant_method.n, m.quant_method.k) for m in dense})
         size = native.configure(settings, self.capacity, shapes, shared_expert=bool(self.shared))
+        adapters = [m.adapters for _, m in self.layers if hasattr(m, 'adapters')]
+        size = max([size] + [native.adapter_bytes(self.capacity, ad.a.shape[1]) for ad in adapters])
+        # the adapter slot of each row of the current step (below 0: none); read by every layer that has adapters
+        self.adapter_ids = torch.full((self.capacity,), -1, dtype=torch.int32, device=self.device) if adapters else None
         self.repacked_bytes = 0
         for m in routed:
             if self.routed_storage_n32 or self.routed_decode_n32:
@@ -379,6 +498,17 @@ class Runtime:
         self.layer_names = tuple(name for name, _ in self.layers)
         for slot, (_, m) in enumerate(self.layers):
             m.quant_method.runtime, m.quant_method.slot = self, slot
+
+    def set_adapter_ids(self, ids):
+        """The adapter slots of the step's rows (int32 [rows], below 0: none); rows
+        past them have none.  A captured step reads what is here when it is
+        replayed."""
+        if self.adapter_ids is None:
+            raise RuntimeError('no layer of this runtime has adapters')
+        if ids.ndim != 1 or ids.shape[0] > self.capacity or ids.dtype != torch.int32:
+            raise ValueError(f'adapter ids must be int32 [rows] of at most {self.capacity} rows, got {tuple(ids.shape)} {ids.dtype}')
+        self.adapter_ids[:ids.shape[0]].copy_(ids, non_blocking=True)
+        self.adapter_ids[ids.shape[0]:].fill_(-1)
 
     def reset_error_flags(self):
         if torch.cuda.is_current_stream_capturing():

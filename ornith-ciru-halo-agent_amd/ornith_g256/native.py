@@ -821,13 +821,12 @@ def _(logits, weights, ids, flags, score, bias, groups, kept_groups, group_top, 
 
 
 def adapter_bytes(capacity, a_rows):
-    """Workspace bytes of adapter_out for up to `capacity` rows and adapters of
-    `a_rows` rows of A (the rank times the slices)."""
-    if a_rows < 8 or a_rows % 8:
-        raise ValueError(f'adapters have a multiple of 8 rows of A, got {a_rows}')
-    size, slices = _SZ(0), -(-a_rows // 512)
-    while a_rows % (8 * slices):
-        slices += 1
+    """Workspace bytes of adapter_out for up to `capacity` rows and adapters with
+    `a_rows` rows of A (the rank times the slices, which may be any)."""
+    size = _SZ(0)
+    slices = next((s for s in range(1, 9) if 0 < a_rows <= 512 * s and a_rows % (8 * s) == 0), None)
+    if slices is None:
+        raise ValueError(f'adapters have 1 to 8 slices of 8 to 512 rows of A, a multiple of 8 each, got {a_rows} in all')
     check(lib().ornith_adapter_get_layout(capacity, slices, a_rows // slices, C.byref(size)),
           f'adapter layout for {capacity} rows, {a_rows} rows of A')
     return size.value

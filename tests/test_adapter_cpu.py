@@ -56,6 +56,16 @@ def test_layout(lib):
         rows = min(m, 1 << 20)
         assert size.value >= rows * (s * r * 4 + 4)
         assert native.adapter_bytes(m, s * r) == size.value
+    # what a capacity has room for, every smaller batch has, however its rows of A are divided
+    for rows_of_a, ways in ((64, ((1, 64), (8, 8), (2, 32))), (512, ((1, 512), (8, 64), (2, 256))), (192, ((3, 64), (1, 192)))):
+        last = 0
+        for m in (0, 1, 63, 64, 65, 255, 256, 257, 1000, 1023, 1024, 4095, 4096, 8192, 1 << 20, (1 << 20) + 1):
+            sizes = set()
+            for s, r in ways:
+                assert lib.ornith_adapter_get_layout(m, s, r, C.byref(size)) == 0
+                sizes.add(size.value)
+            assert len(sizes) == 1 and size.value >= last
+            last = size.value
     for bad in ((-1, 1, 8), (1, 0, 8), (1, 9, 8), (1, 1, 4), (1, 1, 12), (1, 1, 520)):
         assert lib.ornith_adapter_get_layout(*bad, C.byref(size)) == INVALID
     assert lib.ornith_adapter_get_layout(1, 1, 8, None) == INVALID
