@@ -861,30 +861,32 @@ def adapter_out(x, a, b, scales, ids, base, out, workspace, flags, slices=None):
 
 
 def _adapter_out(x, a, b, scales, ids, base, out, workspace, flags, slices):
-    dtype, out_type = x.dtype, W4_TYPES.get(out.dtype)
+    dtype, out_type, x_shape, a_shape, b_shape = x.dtype, W4_TYPES.get(out.dtype), x.shape, a.shape, b.shape
     x_type = W4_TYPES.get(dtype, 2)
-    if x_type > 1 or x.ndim != 2:
-        raise ValueError(f'input must be a bf16 or fp16 [rows, K] tensor, got {tuple(x.shape)} {dtype}')
-    if a.ndim != 3 or b.ndim != 3 or a.dtype != dtype or b.dtype != dtype:
+    if x_type > 1 or len(x_shape) != 2:
+        raise ValueError(f'input must be a bf16 or fp16 [rows, K] tensor, got {tuple(x_shape)} {dtype}')
+    if len(a_shape) != 3 or len(b_shape) != 3 or a.dtype != dtype or b.dtype != dtype:
         raise ValueError(f'adapters must be {dtype} [slots, S * rank, K] and [slots, N, rank] tensors, got '
-                         f'{tuple(a.shape)} {a.dtype} and {tuple(b.shape)} {b.dtype}')
-    (rows, k), (slots, a_rows, ak), (b_slots, n, rank), gpu = x.shape, a.shape, b.shape, x.get_device()
-    ends = _slice_ends((n,) if slices is None else tuple(slices), n)
+                         f'{tuple(a_shape)} {a.dtype} and {tuple(b_shape)} {b.dtype}')
+    (rows, k), (slots, n, rank), gpu = x_shape, b_shape, x.get_device()
+    ends = _slice_ends(tuple(slices) if slices else (n,), n)
     parts = len(ends)
-    if ak != k or b_slots != slots or a_rows != parts * rank or k % 8 or rank % 8 or not 8 <= rank <= 512 or slots > 4096:
-        raise ValueError(f'adapters {tuple(a.shape)} and {tuple(b.shape)} do not fit inputs of {k} and {parts} slices: '
+    if a_shape != (slots, parts * rank, k) or k % 8 or rank % 8 or not 8 <= rank <= 512 or slots > 4096:
+        raise ValueError(f'adapters {tuple(a_shape)} and {tuple(b_shape)} do not fit inputs of {k} and {parts} slices: '
                          'K and the rank are multiples of 8, the rank at most 512, slots at most 4096')
-    (ldx, sx), (a_slot, a_row, a_col), (b_slot, b_row, b_col) = x.stride(), a.stride(), b.stride()
-    if slots <= 1 or not k or not n:
-        a_slot, b_slot = a_rows * k, n * rank
-    if ((a_col != 1 or a_row != k) and a_rows * k and slots) or ((b_col != 1 or b_row != rank) and n and slots):
+    a_slot, b_slot = parts * rank * k, n * rank
+    if not (a.is_contiguous() and b.is_contiguous()) and slots > 1 and k and n:
+        (a_slot, a_row, a_col), (b_slot, b_row, b_col) = a.stride(), b.stride()
+        if a_col != 1 or a_row != k or b_col != 1 or b_row != rank or (a_slot | b_slot) % 8:
+            raise ValueError('each slot of the adapters must be contiguous, and start on the 16-byte grid')
+    elif slots == 1 and not (a[0].is_contiguous() and b[0].is_contiguous()):
         raise ValueError('each slot of the adapters must be contiguous')
     if out_type is None or out.shape != (rows, n):
         raise ValueError(f'output must be a bf16, fp16 or fp32 [{rows}, {n}] tensor, got {tuple(out.shape)} {out.dtype}')
-    ldo, so = out.stride()
+    (ldx, sx), (ldo, so) = x.stride(), out.stride()
     if base is None:
         base, ldb, sb = out, ldo, so
-    elif base.shape != out.shape or base.dtype != out.dtype or base.get_device() != gpu:
+    elif base.shape != (rows, n) or base.dtype != out.dtype or base.get_device() != gpu:
         raise ValueError(f'base must be a {out.dtype} {list(out.shape)} tensor on {x.device}, got {tuple(base.shape)} '
                          f'{base.dtype} on {base.device}')
     else:
@@ -896,20 +898,22 @@ def _adapter_out(x, a, b, scales, ids, base, out, workspace, flags, slices):
     if (sx != 1 and k > 1) or ((so != 1 or sb != 1) and n > 1) or ldx < k or ldo < n or ldb < n:
         raise ValueError('input, base and output rows must have unit column stride and not overlap')
     x_ptr, a_ptr, b_ptr = x.data_ptr(), a.data_ptr(), b.data_ptr()
-    if (ldx | a_slot | b_slot) % 8 or (x_ptr | a_ptr | b_ptr) % 16:
+    if ldx % 8 or (x_ptr | a_ptr | b_ptr) % 16:
         raise ValueError('input rows and adapters must start on the 16-byte grid')
-    ids_ptr = _row_ptr(ids, 'ids', torch.int32, (rows,), x)
-    scales_ptr = _row_ptr(scales, 'scales', torch.float32, (slots,), x)
-    if ids_ptr is None or scales_ptr is None:
+    if ids is None or scales is None:
         raise ValueError('ids and scales are required')
+    if ids.dtype != torch.int32 or ids.shape != (rows,) or scales.dtype != torch.float32 or scales.shape != (slots,) or not (
+            ids.is_contiguous() and scales.is_contiguous()):
+        raise ValueError(f'ids must be a contiguous int32 [{rows}] and scales a contiguous fp32 [{slots}] tensor, got '
+                         f'{tuple(ids.shape)} {ids.dtype} and {tuple(scales.shape)} {scales.dtype}')
     if flags.dtype != torch.int32 or flags.numel() != 1 or workspace.element_size() != 1 or not workspace.is_contiguous():
         raise ValueError('flags must be one int32 word, workspace contiguous bytes')
-    if (gpu < 0 or a.get_device() != gpu or b.get_device() != gpu or out.get_device() != gpu or flags.get_device() != gpu
-            or workspace.get_device() != gpu):
+    if gpu < 0 or not (gpu == a.get_device() == b.get_device() == out.get_device() == ids.get_device() == scales.get_device()
+                       == flags.get_device() == workspace.get_device()):
         raise ValueError('input, adapters, ids, base, output, flags and workspace must be on one GPU')
-    call_on(gpu, lib().ornith_adapter_launch, 'adapters', x_ptr, x_type, ldx, a_ptr, a_slot, b_ptr, b_slot, scales_ptr,
-            ids_ptr, base.data_ptr(), ldb, out.data_ptr(), out_type, ldo, workspace.data_ptr(), workspace.numel(),
-            flags.data_ptr(), rows, n, k, rank, parts, ends, slots)
+    call_on(gpu, lib().ornith_adapter_launch, 'adapters', x_ptr, x_type, ldx, a_ptr, a_slot, b_ptr, b_slot,
+            scales.data_ptr(), ids.data_ptr(), base.data_ptr(), ldb, out.data_ptr(), out_type, ldo, workspace.data_ptr(),
+            workspace.numel(), flags.data_ptr(), rows, n, k, rank, parts, ends, slots)
 
 
 @torch.library.custom_op('ornith_g256::adapter_out', mutates_args={'out', 'workspace', 'flags'}, device_types='cuda')
