@@ -69,8 +69,11 @@ constexpr int kFewRows = 256, kPlanThreads = 1024, kPlanBatch = 8;
 
 __device__ __forceinline__ int ad_key(int id, int slots) { return id >= 0 && id < slots ? id + 1 : 0; }      // 0: no adapter
 
-// Lane li's row of the tile (past the last row: that one again), and the tile.  FEW: ids a lane looks at (0: a plan).
-template <int MT, int FEW> __device__ __forceinline__ bool ad_tile(const AdArgs& a, int unit, int sub, bool first, int& slot, int& rows, int (&t)[MT]) {
+// Lane li's row of tile unit / sub's part unit % sub (past the last row: that one again), its slot and how many
+// rows from there on; false where there is nothing to do.  FEW: ids a lane looks at (0: a plan).  first: the
+// launch's block that raises flags.
+template <int MT, int FEW>
+__device__ __forceinline__ bool ad_tile(const AdArgs& a, int unit, int sub, bool first, int& slot, int& rows, int (&t)[MT]) {
     const int lane = threadIdx.x & 63, li = lane & 15;
     if constexpr (FEW > 0) {
         static_assert(MT == 1);
@@ -692,7 +695,7 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
     constexpr int D = FEW && MT + RT <= 3 ? 4 : 2, PARTS = kAdParts<TYPE, OUT>, STEPS = (PARTS * RT + 1) / 2;
     typedef AdCells<OUT, MT, FEW == 0> Cells;
     static_assert((MT + RT) * 128 >= std::max(MT * RT * 64, std::max(256, 128 * RT)));
-    __shared__ u32x4 s_stage[W][(MT + RT) * 128];      // (then the waves' sums)
+    __shared__ u32x4 s_stage[W][(MT + RT) * 128];      // (then the waves' sums, B, and results)
     __shared__ u32x4 s_v[MT][STEPS][64];
     __shared__ uint32_t s_most[16 * MT];
     int slot, rows, t[MT];
@@ -737,7 +740,7 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
     const char* const bank = reinterpret_cast<const char*>(a.b + size_t(slot) * size_t(a.b_slot));
     const int swap_bits = chunks & (chunks - 1) ? 0 : chunks - 1, swap_shift = chunks == 2 ? 2 : chunks == 4 ? 1 : 0;
     u32x4 bv[2 * RT];
-    int to_b[2 * RT], from_b[STEPS];                     // places in LDS: of the pieces loaded, of the steps' operands
+    int to_b[2 * RT], from_b[STEPS];                   // places in LDS: of the pieces loaded, of the steps' operands
 #pragma unroll
     for (int i = 0; i < 2 * RT; ++i) {
         const int col = (64 * i + lane) / chunks, c = (64 * i + lane) % chunks;

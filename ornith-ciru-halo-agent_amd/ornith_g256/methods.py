@@ -507,7 +507,7 @@ class Runtime:
             raise RuntimeError('no layer of this runtime has adapters')
         if ids.ndim != 1 or ids.shape[0] > self.capacity or ids.dtype != torch.int32:
             raise ValueError(f'adapter ids must be int32 [rows] of at most {self.capacity} rows, got {tuple(ids.shape)} {ids.dtype}')
-        self.adapter_ids[:ids.shape[0]].copy_(ids, non_blocking=True)
+        self.adapter_ids[:ids.shape[0]].copy_(ids)
         self.adapter_ids[ids.shape[0]:].fill_(-1)
 
     def reset_error_flags(self):

@@ -875,12 +875,13 @@ def _adapter_out(x, a, b, scales, ids, base, out, workspace, flags, slices):
         raise ValueError(f'adapters {tuple(a_shape)} and {tuple(b_shape)} do not fit inputs of {k} and {parts} slices: '
                          'K and the rank are multiples of 8, the rank at most 512, slots at most 4096')
     a_slot, b_slot = parts * rank * k, n * rank
-    if not (a.is_contiguous() and b.is_contiguous()) and slots > 1 and k and n:
-        (a_slot, a_row, a_col), (b_slot, b_row, b_col) = a.stride(), b.stride()
-        if a_col != 1 or a_row != k or b_col != 1 or b_row != rank or (a_slot | b_slot) % 8:
-            raise ValueError('each slot of the adapters must be contiguous, and start on the 16-byte grid')
-    elif slots == 1 and not (a[0].is_contiguous() and b[0].is_contiguous()):
-        raise ValueError('each slot of the adapters must be contiguous')
+    if not (a.is_contiguous() and b.is_contiguous()):
+        (a_far, a_row, a_col), (b_far, b_row, b_col) = a.stride(), b.stride()
+        if (a_col, a_row) != (1, k) or (b_col, b_row) != (1, rank) or (slots > 1 and (a_far % 8 or b_far % 8 or a_far < a_slot
+                                                                                     or b_far < b_slot)):
+            raise ValueError('each slot of the adapters must be contiguous, start on the 16-byte grid and not overlap the next')
+        if slots > 1:
+            a_slot, b_slot = a_far, b_far
     if out_type is None or out.shape != (rows, n):
         raise ValueError(f'output must be a bf16, fp16 or fp32 [{rows}, {n}] tensor, got {tuple(out.shape)} {out.dtype}')
     (ldx, sx), (ldo, so) = x.stride(), out.stride()
