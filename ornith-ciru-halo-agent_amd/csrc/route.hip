@@ -4,10 +4,15 @@
 // experts a lane.  Values to pick by are fp64 numbers with the expert's id in
 // their lowest ten bits, so no two are equal and a maximum over lanes is a
 // pick; what those bits displace is below 2^-42 of the value.  An fp32 logit
-// leaves 29 bits clear, so picks without a bias are exact.  Each lane sorts its
-// own once; a pick is then the largest of the lanes' first, which its lane
-// drops.  Scores in fp64 (which the vector unit multiplies at the rate of
+// leaves 29 bits clear, so picks without a bias are exact.  On a whole wave the
+// picks come from a threshold and a count (route_pick); on fewer lanes each sorts
+// its own once, and a pick is the largest of the lanes' first, which its lane drops.  Scores in fp64 (which the vector unit multiplies at the rate of
 // fp32): without a bias only those of the picks.
+//
+// Bound by vector issue where rows are many (8192 rows of 256 in 8 groups, sigmoid
+// and bias: 12.4 us in a graph, 770 instructions a row, 8.4 MB that a copy's rate
+// would read in 1.7; without bias and groups 7.9), by launch and one chain where they
+// are few (1 row 3.3 us: logits, threshold, count, the picks' logits again).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
