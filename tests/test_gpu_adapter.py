@@ -123,7 +123,10 @@ SHAPES = [(1, 1, 8, 8, 1, 1), (1, 100, 64, 8, 3, 1), (1, 6144, 2048, 16, 4, 1), 
           (40, 77, 2120, 32, 40, 8), (64, 1024, 2048, 64, 16, 2), (65, 513, 1000, 16, 7, 1), (77, 5003, 136, 24, 6, 1),
           (130, 200, 4096, 8, 3, 3), (256, 320, 1024, 16, 200, 1), (300, 2048, 512, 128, 4, 1), (1121, 192, 264, 16, 3, 1),
           (2100, 100, 64, 8, 2, 2), (5000, 70, 72, 16, 17, 1), (9, 300, 32768, 8, 2, 1), (33, 90, 128, 512, 3, 1),
-          (7, 40, 64, 256, 2, 3), (4, 70000, 64, 8, 2, 1)]
+          (7, 40, 64, 256, 2, 3), (4, 70000, 64, 8, 2, 1),
+          # tiles of 32 rows, and of 64 above rank 64
+          (4100, 90, 136, 64, 3, 2), (4099, 200, 72, 40, 5, 1), (4200, 64, 1096, 56, 2, 1), (1100, 130, 264, 128, 3, 1),
+          (1500, 70, 72, 72, 5, 2), (2000, 300, 64, 120, 40, 1)]
 
 
 @pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
