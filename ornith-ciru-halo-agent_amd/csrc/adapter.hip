@@ -403,17 +403,15 @@ template <int TYPE, int PARTS> __device__ __forceinline__ void ad_split(float v,
         v = __builtin_isinf(part) ? 0.f : v - part;    // (inf: no NaN beside it)
     }
 }
-// Columns from which on 64 are not whole and on the 16-byte grid, of the columns from begin to end (whose
-// groups of 64 start at begin): the last ones, or all.
-template <int SIZE> __device__ __forceinline__ int ad_whole_end(const AdArgs& a, int begin, int end) {
-    return ((reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out) | size_t(a.ldb) * SIZE | size_t(a.ldo) * SIZE |
-             size_t(begin) * SIZE) & 15) == 0 ? end - 63 : begin;
-}
+// 16 bytes on their values' grid: global accesses need no more, so rows of any stride move in these.
+typedef u32x4 ad_piece2 __attribute__((aligned(2)));
+typedef u32x4 ad_piece4 __attribute__((aligned(4)));
 // A wave's 16 MT rows x 64 columns of base and out, as they move: eight lanes (fp32: 16) on a row's 16-byte
 // pieces, H accesses for 16 rows.  (Neighbouring lanes in different rows, as the products leave them, halve
 // the rate.)  ONCE: stores that leave the caches alone.
 template <int OUT, int MT, bool ONCE> struct AdCells {
     typedef std::conditional_t<OUT == ORNITH_ADAPTER_F32, uint32_t, uint16_t> word;
+    typedef std::conditional_t<OUT == ORNITH_ADAPTER_F32, ad_piece4, ad_piece2> piece_t;
     static constexpr int size = sizeof(word), per = 16 / size, lanes = 64 / per, rows_at_once = 64 / lanes, H = 16 / rows_at_once;
     const word* base[MT][H];                           // of this wave's next columns
     word* out[MT][H];
@@ -451,7 +449,7 @@ template <int OUT, int MT, bool ONCE> struct AdCells {
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                if (whole) have[m][h] = *reinterpret_cast<const u32x4*>(base[m][h]);
+                if (whole) have[m][h] = *reinterpret_cast<const piece_t*>(base[m][h]);
                 else {
                     u32x4 v = {0, 0, 0, 0};
 #pragma unroll
@@ -463,7 +461,7 @@ template <int OUT, int MT, bool ONCE> struct AdCells {
     __device__ __forceinline__ bool has(int m, int h) const { return mine >> (m * H + h) & 1; }
     __device__ __forceinline__ void put(int m, int h, u32x4 r, bool whole, int left) {
         if (whole) {
-            u32x4* const to = reinterpret_cast<u32x4*>(out[m][h]);
+            piece_t* const to = reinterpret_cast<piece_t*>(out[m][h]);
             if constexpr (ONCE) __builtin_nontemporal_store(r, to);
             else *to = r;
             return;
@@ -568,7 +566,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
     const int end = a.ends[p];
     const int n0 = (p ? a.ends[p - 1] : 0) + ((int(blockIdx.y) - (p ? a.blocks[p - 1] : 0)) * kExpandWaves + wv) * 64;
     typedef AdCells<OUT, MT, FEW == 0> Cells;
-    const bool whole = n0 < ad_whole_end<Cells::size>(a, n0, end);
+    const bool whole = n0 + 64 <= end;
     Cells cells(a, t, rows, n0);
     if (slot < 0) {
         if (n0 < end) cells.copy(whole, end - n0);
@@ -713,7 +711,7 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
     while (cb >= a.blocks[p]) ++p;
     const int begin = (p ? a.ends[p - 1] : 0) + (cb - (p ? a.blocks[p - 1] : 0)) * (64 * W * a.groups);
     const int end = min(a.ends[p], begin + 64 * W * a.groups);
-    const int whole_end = ad_whole_end<Cells::size>(a, begin, end);
+    const int whole_end = end - 63;                    // 64 columns from before it are inside
     int n0 = begin + 64 * wv;
     Cells cells(a, t, rows, n0);
     if (slot < 0) {
