@@ -71,7 +71,7 @@ constexpr int kFewRows = 256, kPlanThreads = 1024, kPlanBatch = 8;
 __device__ __forceinline__ int ad_key(int id, int slots) { return id >= 0 && id < slots ? id + 1 : 0; }      // 0: no adapter
 
 // Lane li's row of tile unit / sub's part unit % sub (past the last row: that one again), its slot and how many
-// rows from there on; false where there is nothing to do.  FEW: ids a lane looks at (0: a plan).  first: the
+// rows from there on; false where there is nothing to do.  FEW: ids a lane looks at (0 and below: a plan).  first: the
 // launch's block that raises flags.
 template <int MT, int FEW>
 __device__ __forceinline__ bool ad_tile(const AdArgs& a, int unit, int sub, bool first, int& slot, int& rows, int (&t)[MT]) {
@@ -408,7 +408,8 @@ typedef u32x4 ad_piece2 __attribute__((aligned(2)));
 typedef u32x4 ad_piece4 __attribute__((aligned(4)));
 // A wave's 16 MT rows x 64 columns of base and out, as they move: eight lanes (fp32: 16) on a row's 16-byte
 // pieces, H accesses for 16 rows.  (Neighbouring lanes in different rows, as the products leave them, halve
-// the rate.)  ONCE: stores that leave the caches alone.
+// the rate.)  ONCE: stores that leave the caches alone,
+// of many rows on the 16-byte grid (8192 rows 69.3 / 66.5 us, 4096 rows 42.4 / 31.9; off it 79.4 / 96.6).
 template <int OUT, int MT, bool ONCE> struct AdCells {
     typedef std::conditional_t<OUT == ORNITH_ADAPTER_F32, uint32_t, uint16_t> word;
     typedef std::conditional_t<OUT == ORNITH_ADAPTER_F32, ad_piece4, ad_piece2> piece_t;
@@ -693,9 +694,10 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
 // for one chain: id, x and A, the waves' exchange, B, the store.  Many stream base and out: 8192 rows 57 us for 239
 // MB, 4.2 TB/s of the 5.1 that a copy reaches; the rest goes into the exchange of results through LDS and the
 // time before a block's first columns.
+// FEW -1: a plan, and rows off the 16-byte grid.
 template <int TYPE, int OUT, int MT, int RT, int W, int FEW>
 __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
-    constexpr int D = FEW && MT + RT <= 3 ? 4 : 2, PARTS = kAdParts<TYPE, OUT>, STEPS = (PARTS * RT + 1) / 2;
+    constexpr int D = FEW > 0 && MT + RT <= 3 ? 4 : 2, PARTS = kAdParts<TYPE, OUT>, STEPS = (PARTS * RT + 1) / 2;
     typedef AdCells<OUT, MT, FEW == 0> Cells;
     static_assert((MT + RT) * 128 >= std::max(MT * RT * 64, std::max(256, 128 * RT)));
     __shared__ u32x4 s_stage[W][(MT + RT) * 128];      // (then the waves' sums, B, and results)
@@ -906,7 +908,7 @@ template <class F> void ad_by_type(int out_type, F&& f) {
 // block forms v again (us, 1 / 2 / 3 / 6 groups, rank 16: 8192 x 6144 101 / 77 / 68 / 66; 4096 x 6144 57 / 35 / 32 / 34;
 // 512 x 6144 14.3 / 13.6 / 13.4 / 16.8; 1120 x 2048 13.9 / 13.5 / 14.9 / 14.6; 300 x 2048 10.5 / 11.6).
 int ad_groups(const AdArgs& a, int FEW, int W) {
-    if (FEW) return 1;
+    if (FEW > 0) return 1;
     const int all = (a.N + 64 * W - 1) / (64 * W);
     const int64_t cells = int64_t(all) * ((a.M + 15) / 16);
     const int64_t groups = std::max<int64_t>((cells + 1023) / 1024, std::min<int64_t>(3, (cells + 159) / 160));
@@ -961,7 +963,11 @@ template <int TYPE> hipError_t ad_rows(AdArgs& a, int out_type, hipStream_t s) {
     timed_launch("adapter_plan", adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
-    if (both) return a.tile_rows == 32 ? ad_both<TYPE, 2, 0>(a, out_type, s) : ad_both<TYPE, 1, 0>(a, out_type, s);
+    if (both) {
+        const bool grid = ((reinterpret_cast<uintptr_t>(a.out) | size_t(a.ldo) * (out_type == ORNITH_ADAPTER_F32 ? 4 : 2)) & 15) == 0;
+        if (a.tile_rows == 32) return grid ? ad_both<TYPE, 2, 0>(a, out_type, s) : ad_both<TYPE, 2, -1>(a, out_type, s);
+        return grid ? ad_both<TYPE, 1, 0>(a, out_type, s) : ad_both<TYPE, 1, -1>(a, out_type, s);
+    }
     return a.tile_rows == 64 ? ad_two<TYPE, 4, 0>(a, out_type, s) : ad_two<TYPE, 1, 0>(a, out_type, s);
 }
 
