@@ -242,8 +242,8 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(AdArgs a) {
 // ---- shrink ---------------------------------------------------------------------
 // acc[m][r] += x A over k in [kbegin, kend), a wave's share of it: 64 k of every 64 W, D such pieces loaded
 // before the first product.  The instruction wants neighbouring lanes in different rows, and such loads (64
-// lines' halves at a time) were what few rows waited for: one block's 16 x 2048 of A took 2.4 us, of the 3.3 of
-// a call without them, against 0.9 with eight lanes on the 128 bytes of a row.  So those, and through LDS to the
+// lines' halves at a time) were what few rows waited for: one block's 16 x 2048 of A added 2.4 us to the 3.3 of a
+// call without it, against 0.9 with eight lanes on the 128 bytes of a row.  So those, and through LDS to the
 // operands' order: piece c (16 bytes) of row r at 8 r + (c ^ r % 8), free of bank conflicts both ways; a wave's
 // own LDS, which needs no barrier.
 template <int TYPE, int MT, int RT, int W, int D>
