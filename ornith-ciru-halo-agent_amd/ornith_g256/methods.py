@@ -389,6 +389,8 @@ class SharedExpert:
             m = getattr(lin, 'quant_method', None)
             if type(m) is not G256LinearMethod or (m.n, m.k) != nk:
                 raise ValueError(f'{prefix}: shared expert projections must be G256 linears {nk}')
+            if hasattr(lin, 'adapters'):
+                raise ValueError(f'{prefix}: the fused slot and fixed8 read the banks alone: no adapters on a shared expert')
         g = mlp.expert_gate.weight
         if g.dtype != torch.bfloat16 or tuple(g.shape) != (1, native.HIDDEN):
             raise ValueError(f'{prefix}: expert_gate must be a bf16 [1, 2048] row')

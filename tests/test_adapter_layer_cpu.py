@@ -107,3 +107,16 @@ def test_routing_of_a_block(monkeypatch):
     with pytest.raises(ValueError):
         methods.G256MoEMethod('moe', methods.ExpertRouting(6))
     assert methods.G256MoEMethod('moe').routing.score == 'softmax'
+
+
+@pytest.mark.parametrize('name', ['gate_up_proj', 'down_proj'])
+def test_no_adapters_on_a_shared_expert(name):
+    """Its fused slot and fixed8 would not see them."""
+    mlp = torch.nn.Module()
+    for proj, n, k in (('gate_up_proj', 1024, 2048), ('down_proj', 2048, 512)):
+        setattr(mlp, proj, _Layer(methods.G256LinearMethod(proj, n, k)))
+    mlp.expert_gate = torch.nn.Linear(2048, 1, bias=False, dtype=BF)
+    methods.SharedExpert('shared', mlp)
+    methods.attach_adapters(getattr(mlp, name), 2, 8)
+    with pytest.raises(ValueError, match='no adapters'):
+        methods.SharedExpert('shared', mlp)
