@@ -483,10 +483,13 @@ template <int OUT, int MT, bool ONCE> struct AdCells {
     }
     // base + by * acc, rounded; acc[m][j] of lane 16 q + li: row li's columns 16 j + 4 q .. + 3.  Through LDS to
     // the lanes that move them: 16 bytes c of row r at 16 r + (c ^ r), no bank conflicts; stage: the wave's own,
-    // 256 pieces.
-    template <bool SCALED> __device__ __forceinline__ void add(const f32x4 (&acc)[MT][4], const float (&by)[MT], f32x4* stage, bool whole,
-                                                               int left) {
+    // 256 pieces.  A piece with a result that is not finite stays unwritten, and then is base + sum(m, row, column)
+    // (the parts of v make NaN of inf in B, where a part is 0 or of the other sign, and inf of a v above their
+    // type's largest value).
+    template <bool SCALED, class F> __device__ __forceinline__ void add(const f32x4 (&acc)[MT][4], const float (&by)[MT], f32x4* stage,
+                                                                        bool whole, int left, F&& sum) {
         const int lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
+        uint32_t todo = 0;                             // such pieces, as in mine
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -512,23 +515,23 @@ template <int OUT, int MT, bool ONCE> struct AdCells {
                     for (int i = 0; i < 4; ++i) {
                         const int e = 4 * c + i;
                         const uint32_t w = have[m][h][e * size / 4];
-                        r[e] = v[i] + (size == 4 ? __uint_as_float(w) : OUT == ORNITH_ADAPTER_F16 ? f16_bits_to_f32(w >> (16 * (e & 1)) & 0xffffu)
-                                                                    : __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16));
+                        r[e] = v[i] + ad_float<OUT>(size == 4 ? w : e & 1 ? w >> 16 : w & 0xffffu);
                     }
                 }
                 u32x4 bits;
+                float largest = most, none = 0.f;      // none: NaN beside a result that is not finite
 #pragma unroll
                 for (int e = 0; e < per; e += 2) {
                     if (whole) {
-                        most = fmaxf(fmaxf(most, __builtin_fabsf(r[e])), __builtin_fabsf(r[e + 1]));
-                        zero = __builtin_fmaf(r[e], 0.f, zero);
-                        zero = __builtin_fmaf(r[e + 1], 0.f, zero);
+                        largest = fmaxf(fmaxf(largest, __builtin_fabsf(r[e])), __builtin_fabsf(r[e + 1]));
+                        none = __builtin_fmaf(r[e], 0.f, none);
+                        none = __builtin_fmaf(r[e + 1], 0.f, none);
                     } else {
 #pragma unroll
                         for (int i = e; i < e + 2; ++i) {
                             const float in = per * (lane % lanes) + i < left ? r[i] : 0.f;
-                            most = fmaxf(most, __builtin_fabsf(in));
-                            zero = __builtin_fmaf(in, 0.f, zero);
+                            largest = fmaxf(largest, __builtin_fabsf(in));
+                            none = __builtin_fmaf(in, 0.f, none);
                         }
                     }
                     if constexpr (size == 4) {
@@ -536,10 +539,32 @@ template <int OUT, int MT, bool ONCE> struct AdCells {
                         bits[e + 1] = __float_as_uint(r[e + 1]);
                     } else bits[e / 2] = ad_pair<OUT>(r[e], r[e + 1]);
                 }
-                put(m, h, bits, whole, left);
+                if (none == none) {
+                    most = largest;
+                    put(m, h, bits, whole, left);
+                } else todo |= 1u << (m * H + h);
             }
             __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
             __builtin_amdgcn_wave_barrier();
+        }
+        for (; __builtin_expect(todo != 0, 0); todo &= todo - 1) {
+            const int at = __ffs(int(todo)) - 1;
+            const word* from = base[0][0];
+            word* to = out[0][0];
+#pragma unroll
+            for (int i = 1; i < MT * H; ++i) {
+                from = at == i ? base[i / H][i % H] : from;
+                to = at == i ? out[i / H][i % H] : to;
+            }
+#pragma unroll 1
+            for (int e = 0; e < per; ++e) {
+                const int column = per * (lane % lanes) + e;
+                if (column >= left) break;
+                const float r = sum(at / H, rows_at_once * (at % H) + lane / lanes, column) + ad_float<OUT>(from[e]);
+                most = fmaxf(most, __builtin_fabsf(r));
+                zero = __builtin_fmaf(r, 0.f, zero);
+                to[e] = word(ad_bits<OUT>(r));
+            }
         }
     }
     // 16-bit results round to infinity from half a step above the type's largest value
@@ -549,6 +574,14 @@ template <int OUT, int MT, bool ONCE> struct AdCells {
         return (bad ? kAdNonfinite : 0u) | (OUT != ORNITH_ADAPTER_F32 && (bad || most >= limit) ? kAdNonfinite16 : 0u);
     }
 };
+
+// scale sum_r B[r] v(r) of one row and column, in fp64: for results that the parts of v may have driven out of range.
+template <int TYPE, class F> __device__ __forceinline__ float ad_sum(const uint16_t* b, int R, float scale, F&& v) {
+    double sum = 0.0;
+#pragma unroll 1
+    for (int r = 0; r < R; ++r) sum += double(ad_float<TYPE>(b[r])) * double(v(r));
+    return float(sum * double(scale));
+}
 
 constexpr int kExpandWaves = 4;                        // a block: 64 columns a wave
 
@@ -683,7 +716,15 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
-    cells.template add<TYPE == ORNITH_ADAPTER_F16>(acc, by, reinterpret_cast<f32x4*>(s_stage[wv]), whole, end - n0);
+    auto form = [&](int m, int row, int column) {
+        const float* from = a.v + size_t(s_t[16 * m + row]) * a.SR + p * a.R;
+        return ad_sum<TYPE>(bank + size_t(n0 + column) * size_t(a.R), a.R, a.scales[slot], [&](int r) {
+            float v = from[r];                         // (the parts of K in order)
+            for (int z = 1; z < a.splits; ++z) v += from[size_t(z) * size_t(a.M) * a.SR + r];
+            return v;
+        });
+    };
+    cells.template add<TYPE == ORNITH_ADAPTER_F16>(acc, by, reinterpret_cast<f32x4*>(s_stage[wv]), whole, end - n0, form);
     flag_or(a.flags, cells.flags());
 }
 
@@ -703,6 +744,7 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
     __shared__ u32x4 s_stage[W][(MT + RT) * 128];      // (then the waves' sums, B, and results)
     __shared__ u32x4 s_v[MT][STEPS][64];
     __shared__ uint32_t s_most[16 * MT];
+    __shared__ f32x4 s_sum[MT * RT][64];               // v: row 4 q + i of piece m RT + r / 16 in [16 q + r % 16][i]
     int slot, rows, t[MT];
     // blocks go to the 8 XCDs in turn: a row's column blocks on one of them, whose L2 keeps its A
     const int nblocks = a.blocks[a.S - 1], unit = int(blockIdx.x / 8) / nblocks * 8 + int(blockIdx.x % 8);
@@ -723,6 +765,7 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
         }
         return;
     }
+    slot = __builtin_amdgcn_readfirstlane(slot);
     const int chunks = a.R / 8;
     const float scale = a.scales[slot];
     {
@@ -781,6 +824,7 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i0][i] += part[i];
         }
+        s_sum[f][lane] = v[i0];
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i0][i] *= scale;
         if (TYPE == ORNITH_ADAPTER_F16 && 16 * (f % RT) + li < a.R) {
@@ -841,11 +885,17 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
         __builtin_amdgcn_wave_barrier();
     };
     constexpr bool SCALED = TYPE == ORNITH_ADAPTER_F16;
+    int at = n0;                                       // the columns of the present sums
+    auto form = [&](int m, int row, int column) {
+        return ad_sum<TYPE>(reinterpret_cast<const uint16_t*>(bank) + size_t(at + column) * size_t(a.R), a.R, a.scales[slot],
+                            [&](int r) { return s_sum[m * RT + r / 16][16 * (row >> 2) + r % 16][row & 3]; });
+    };
     while (n0 < whole_end) {
         product();
+        at = n0;
         n0 += 64 * W;
         if (n0 < whole_end) load_b(all_b);
-        cells.template add<SCALED>(sum, by, stage, true, 64);
+        cells.template add<SCALED>(sum, by, stage, true, 64, form);
         cells.step(64 * W);
         if (n0 < whole_end) cells.load(true, 64);
     }
@@ -853,7 +903,8 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
         cells.load(false, end - n0);
         load_b(min(all_b, (end - n0) * chunks - 1));
         product();
-        cells.template add<SCALED>(sum, by, stage, false, end - n0);
+        at = n0;
+        cells.template add<SCALED>(sum, by, stage, false, end - n0, form);
         cells.step(64 * W);
     }
     flag_or(a.flags, cells.flags());
