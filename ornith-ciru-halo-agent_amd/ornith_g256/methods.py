@@ -57,10 +57,12 @@ class LinearAdapters(torch.nn.Module):
     """`slots` low-rank adapters of one linear [n, k], of rank `rank` at most:
     a [slots, S * rank, k], b [slots, n, rank] and a scale each.  slices: the
     widths of a merged projection's S parts, each with rows of a of its own.  An
-    empty slot adds nothing."""
+    empty slot adds nothing.  step_rows: whether the layer is called on the rows
+    of the step, whose slots the runtime holds; else each call names its own."""
 
-    def __init__(self, n, k, slots, rank, slices=None, dtype=torch.bfloat16, device=None):
+    def __init__(self, n, k, slots, rank, slices=None, dtype=torch.bfloat16, device=None, step_rows=True):
         super().__init__()
+        self.step_rows = bool(step_rows)
         self.slices = (int(n),) if slices is None else tuple(int(w) for w in slices)
         if sum(self.slices) != n or not 1 <= len(self.slices) <= 8 or min(self.slices) < 0:
             raise ValueError(f'slices must be 1 to 8 widths that sum to {n} columns, got {slices}')
@@ -104,25 +106,44 @@ class LinearAdapters(torch.nn.Module):
             for t in (self.a, self.b, self.scales):
                 t[slot].zero_()
 
-    def add(self, runtime, x, out, flags):
-        """Adds to out [rows, n] what the rows' adapters make of x, by the
-        runtime's adapter_ids."""
-        if x.shape[0] > runtime.capacity:
-            raise ValueError(f'{x.shape[0]} rows exceed the configured capacity {runtime.capacity}')
-        native.adapter_out(x, self.a, self.b, self.scales, runtime.adapter_ids[:x.shape[0]], None, out, runtime.workspace,
-                           flags, slices=self.slices)
+    def add(self, runtime, x, out, flags, ids=None):
+        """Adds to out [rows, n] what the rows' adapters make of x, by ids (int32
+        [rows]) or the runtime's adapter_ids."""
+        rows = x.shape[0]
+        if rows > runtime.capacity:
+            raise ValueError(f'{rows} rows exceed the configured capacity {runtime.capacity}')
+        if ids is None:
+            if not self.step_rows:
+                raise ValueError("a layer whose rows are not the step's needs their adapter_ids")
+            # (a traced call would be traced again for each number of rows)
+            if not native.traced() and 0 < rows < runtime.adapter_rows:
+                raise ValueError(f'{rows} rows of a step of {runtime.adapter_rows}: which of them is for adapter_ids to say')
+            ids = runtime.adapter_ids[:rows]
+        native.adapter_out(x, self.a, self.b, self.scales, ids, None, out, runtime.workspace, flags, slices=self.slices)
 
 
-def attach_adapters(layer, slots, rank, slices=None, dtype=torch.bfloat16):
+def _add_adapters(layer, runtime, x, out, flags, ids):
+    if hasattr(layer, 'adapters'):
+        layer.adapters.add(runtime, x, out, flags, ids)
+    elif ids is not None:
+        raise ValueError('adapter_ids for a layer without adapters')
+
+
+def attach_adapters(layer, slots, rank, slices=None, dtype=torch.bfloat16, step_rows=None):
     """Gives a layer of G256LinearMethod or W4LinearMethod adapters (before the
-    Runtime that binds it, which sizes the workspace for them)."""
+    Runtime that binds it, which sizes the workspace for them).  step_rows: False
+    for a layer that is called on other rows than the step's, such as a head on
+    the gathered last rows of prompts: each of its calls then names its rows' slots
+    (``adapter_ids``).  None: False for a W4LinearMethod with an out_dtype, a head's."""
     method = getattr(layer, 'quant_method', None)
     if type(method) not in (G256LinearMethod, W4LinearMethod):
         raise ValueError('adapters go beside a dense G256 or plain 4-bit linear')
     if method.runtime is not None:
         raise RuntimeError(f'{method.prefix}: adapters are attached before binding')
     device = next((t.device for t in list(layer.parameters()) + list(layer.buffers())), None)
-    layer.adapters = LinearAdapters(method.n, method.k, slots, rank, slices, dtype, device)
+    if step_rows is None:
+        step_rows = getattr(method, 'out_dtype', None) is None
+    layer.adapters = LinearAdapters(method.n, method.k, slots, rank, slices, dtype, device, step_rows)
     return layer.adapters
 
 
@@ -156,7 +177,9 @@ class G256LinearMethod:
     def process_weights_after_loading(self, layer):
         layer._ornith_loader.seal()
 
-    def apply(self, layer, x, bias=None):
+    def apply(self, layer, x, bias=None, adapter_ids=None):
+        """adapter_ids: the adapter slots of x's rows (int32 [rows]) where they are not
+        the step's."""
         if self.runtime is None or not layer._ornith_loader.sealed or bias is not None:
             raise RuntimeError(f'{self.prefix}: needs sealed weights, no bias and a bound runtime')
         shape = x.shape[:-1]
@@ -165,8 +188,7 @@ class G256LinearMethod:
         rt = self.runtime
         native.dense_out(x, layer.g256_codes, layer.g256_metadata, rt.workspace, out, rt.slots[self.slot],
                          rt.capacity, self.n, self.k, rt.dense_geometry, rt.dense_a8_max_rows)
-        if hasattr(layer, 'adapters'):
-            layer.adapters.add(rt, x, out, rt.slots[self.slot])
+        _add_adapters(layer, rt, x, out, rt.slots[self.slot], adapter_ids)
         return out.view(*shape, self.n)
 
 
@@ -229,7 +251,8 @@ class W4LinearMethod:
         for name, bank in zip(('w4_bank', 'w4_metadata'), packed):
             layer.register_buffer(name, bank, persistent=False)
 
-    def apply(self, layer, x, bias=None):
+    def apply(self, layer, x, bias=None, adapter_ids=None):
+        """adapter_ids: as G256LinearMethod's."""
         if self.runtime is None or not hasattr(layer, 'w4_bank') or bias is not None:
             raise RuntimeError(f'{self.prefix}: needs packed weights, no bias and a bound runtime')
         shape = x.shape[:-1]
@@ -238,8 +261,7 @@ class W4LinearMethod:
             x = native.w4_grid(x)
         out = torch.empty((x.shape[0], self.n), dtype=self.out_dtype or x.dtype, device=x.device)
         native.w4_out(x, layer.w4_bank, layer.w4_metadata, out, self.runtime.slots[self.slot], self.n, self.k, self.group)
-        if hasattr(layer, 'adapters'):
-            layer.adapters.add(self.runtime, x, out, self.runtime.slots[self.slot])
+        _add_adapters(layer, self.runtime, x, out, self.runtime.slots[self.slot], adapter_ids)
         return out.view(*shape, self.n)
 
 
@@ -479,6 +501,7 @@ class Runtime:
         size = max([size] + [native.adapter_bytes(self.capacity, ad.a.shape[1]) for ad in adapters])
         # the adapter slot of each row of the current step (below 0: none); read by every layer that has adapters
         self.adapter_ids = torch.full((self.capacity,), -1, dtype=torch.int32, device=self.device) if adapters else None
+        self.adapter_rows = 0                          # rows of the current step, as set_adapter_ids was given them
         self.repacked_bytes = 0
         for m in routed:
             if self.routed_storage_n32 or self.routed_decode_n32:
@@ -503,7 +526,8 @@ class Runtime:
 
     def set_adapter_ids(self, ids):
         """The adapter slots of the step's rows (int32 [rows], below 0: none); rows
-        past them have none.  A captured step reads what is here when it is
+        past them have none, and a layer called on fewer rows is given theirs
+        (``adapter_ids``).  A captured step reads what is here when it is
         replayed."""
         if self.adapter_ids is None:
             raise RuntimeError('no layer of this runtime has adapters')
@@ -511,6 +535,7 @@ class Runtime:
             raise ValueError(f'adapter ids must be int32 [rows] of at most {self.capacity} rows, got {tuple(ids.shape)} {ids.dtype}')
         self.adapter_ids[:ids.shape[0]].copy_(ids)
         self.adapter_ids[ids.shape[0]:].fill_(-1)
+        self.adapter_rows = ids.shape[0]
 
     def reset_error_flags(self):
         if torch.cuda.is_current_stream_capturing():
