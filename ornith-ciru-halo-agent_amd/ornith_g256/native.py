@@ -869,7 +869,7 @@ def _adapter_out(x, a, b, scales, ids, base, out, workspace, flags, slices):
         raise ValueError(f'adapters must be {dtype} [slots, S * rank, K] and [slots, N, rank] tensors, got '
                          f'{tuple(a_shape)} {a.dtype} and {tuple(b_shape)} {b.dtype}')
     (rows, k), (slots, n, rank), gpu = x_shape, b_shape, x.get_device()
-    ends = _slice_ends(tuple(slices) if slices else (n,), n)
+    ends = _slice_ends((n,) if slices is None else tuple(slices), n)
     parts = len(ends)
     if a_shape != (slots, parts * rank, k) or k % 8 or rank % 8 or not 8 <= rank <= 512 or slots > 4096:
         raise ValueError(f'adapters {tuple(a_shape)} and {tuple(b_shape)} do not fit inputs of {k} and {parts} slices: '
