@@ -798,7 +798,7 @@ def _route_experts(logits, weights, ids, flags, score, bias, groups, kept_groups
             and 1 <= group_top <= 2 and 1 <= k <= 32 and k <= kept_groups * (n // groups)):
         raise ValueError(f'cannot pick {k} of {n} experts in {kept_groups} of {groups} groups by their {group_top} best: '
                          f'at most 1024 experts, 64 groups that divide them, 32 picks of those in the kept groups, 1 or 2 best')
-    if not -3.4028234e38 <= scale <= 3.4028234e38:
+    if not -3.4028234663852886e38 <= scale <= 3.4028234663852886e38:
         raise ValueError(f'scale must be a finite fp32 number, got {scale}')
     if flags.dtype != torch.int32 or flags.numel() != 1:
         raise ValueError('flags must be one int32 word')
