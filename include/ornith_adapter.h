@@ -10,12 +10,12 @@
  * x, A and B are all bf16 or all fp16; base and out bf16, fp16 or fp32, out perhaps
  * base itself (the same rows), which leaves rows without an adapter untouched.
  * Each product is exact and summed in fp32; scale v enters the second product
- * as the sum of 16-bit numbers, off by at most 2^-18 of itself (bf16, 16-bit
- * results), 2^-26 (bf16, fp32 results) or 2^-23 and 2^-38 of the largest of its
- * row and slice (fp16); one rounding to the output's type.  Where a result so
- * formed is not finite, it and those that share 16 bytes of its row are formed again
- * from v itself, in fp64: an infinity or NaN of A, B, x or base gives what it gives in
- * the formula, in its own rows and columns alone.  A row depends on no
+ * as the sum of 16-bit numbers, off by at most 2^-17 of itself (bf16, 16-bit
+ * results), by nothing from 2^-103 up (bf16, fp32 results), or by 2^-23 and 2^-38 of
+ * the largest of its row and slice (fp16); one rounding to the output's type.  Where a
+ * result so formed is not finite, it and those that share 16 bytes of its row are
+ * formed again from v itself, in fp64: an infinity or NaN of A, B, x or base gives what
+ * it gives in the formula, in its own rows and columns alone.  A row depends on no
  * other row's values; the order of its sums goes by the numbers of rows and of
  * columns.
  *

@@ -392,8 +392,8 @@ __device__ __forceinline__ float ad_scale16(uint32_t most) {
     if (e == 0 || e == 255) return 1.f;
     return __uint_as_float(uint32_t(min(max(127 + 127 + 14 - e, 1), 254)) << 23);
 }
-// 16-bit numbers whose sum v is: two (off by 2^-18 of v at most in bf16, 2^-24 in fp16), and three of bf16 for
-// fp32 results (2^-27).
+// 16-bit numbers whose sum v is: two (off by 2^-17 of v at most in bf16, 2^-23 in fp16), and three of bf16, which
+// hold its 24 bits, for fp32 results.
 template <int TYPE, int OUT> constexpr int kAdParts = TYPE == ORNITH_ADAPTER_BF16 && OUT == ORNITH_ADAPTER_F32 ? 3 : 2;
 template <int TYPE, int PARTS> __device__ __forceinline__ void ad_split(float v, uint32_t (&bits)[PARTS]) {
 #pragma unroll

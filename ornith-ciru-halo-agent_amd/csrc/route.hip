@@ -109,7 +109,7 @@ template <int TYPE> __device__ __forceinline__ float route_logit(const void* row
     else if constexpr (TYPE == 1) return f16_bits_to_f32(static_cast<const uint16_t*>(row)[e]);
     else return bf16_bits_to_f32(static_cast<const uint16_t*>(row)[e]);
 }
-// exp(x) of x <= 700 (below -800: 0): x = n ln 2 + r, |r| <= ln 2 / 2, the exponential series to r^11 (2^-47 off at
+// exp(x) of x <= 700 (below -800: 0): x = n ln 2 + r, |r| <= ln 2 / 2, the exponential series to r^11 (2^-46 off at
 // most), 2^n.
 __device__ __forceinline__ double exp_d(double x) {
     x = max_d(x, -800.0);
