@@ -53,7 +53,7 @@ struct AdArgs {
     int32_t* tiles;                                    // [units, 2 + tile_rows]
     int tile_rows;
     int M, N, K, R, SR, slots, S;
-    int sub, splits;                                   // shrink: parts of a tile, and of K
+    int splits;                                        // shrink: parts of K
     int units, groups;                                 // tiles at most; both: groups of 64 columns a wave
     bool in_place;
     int ends[kAdMaxSlices];                            // of the slices, in columns
@@ -70,11 +70,11 @@ constexpr int kFewRows = 256, kPlanThreads = 1024, kPlanBatch = 8;
 
 __device__ __forceinline__ int ad_key(int id, int slots) { return id >= 0 && id < slots ? id + 1 : 0; }      // 0: no adapter
 
-// Lane li's row of tile unit / sub's part unit % sub (past the last row: that one again), its slot and how many
-// rows from there on; false where there is nothing to do.  FEW: ids a lane looks at (0 and below: a plan).  first: the
+// Lane li's row of tile `unit` (past the last row: that one again), its slot and how many rows; false where there is
+// nothing to do.  FEW: ids a lane looks at (0 and below: a plan).  first: the
 // launch's block that raises flags.
 template <int MT, int FEW>
-__device__ __forceinline__ bool ad_tile(const AdArgs& a, int unit, int sub, bool first, int& slot, int& rows, int (&t)[MT]) {
+__device__ __forceinline__ bool ad_tile(const AdArgs& a, int unit, bool first, int& slot, int& rows, int (&t)[MT]) {
     const int lane = threadIdx.x & 63, li = lane & 15;
     if constexpr (FEW > 0) {
         static_assert(MT == 1);
@@ -110,13 +110,12 @@ __device__ __forceinline__ bool ad_tile(const AdArgs& a, int unit, int sub, bool
         }
         t[0] = __builtin_amdgcn_ds_bpermute(4 * min(li, rows - 1), sent) - 1;
     } else {
-        const int32_t* tile = a.tiles + size_t(unit / sub) * size_t(kTileHead + a.tile_rows);
-        const int at = unit % sub * (16 * MT);         // (a tile in several parts)
+        const int32_t* tile = a.tiles + size_t(unit) * size_t(kTileHead + a.tile_rows);
         slot = tile[0];
-        rows = tile[1] - at;
+        rows = tile[1];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) t[m] = tile[kTileHead + at + 16 * m + li];    // (past its rows: of no use)
-        if (slot < -1 || rows <= 0) return false;
+        for (int m = 0; m < MT; ++m) t[m] = tile[kTileHead + 16 * m + li];    // (past its rows: of no use)
+        if (slot < -1) return false;
 #pragma unroll
         for (int m = MT - 1; m >= 0; --m) {            // (from the last: its source is not yet replaced)
             const int last = min(rows - 1, 16 * MT - 1), from = 16 * m + li <= last ? 16 * m + li : last;
@@ -321,30 +320,25 @@ __device__ __forceinline__ void ad_accumulate(const AdArgs& a, const int (&t)[MT
 
 constexpr int kShrinkWaves = 8;
 
-template <int TYPE, int MT, int RT, int D, int FEW>
+template <int TYPE, int RT, int D, int FEW>
 __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(AdArgs a) {
     constexpr int W = kShrinkWaves;
-    __shared__ u32x4 s_stage[W][(MT + RT) * 128];      // (then the waves' sums)
-    static_assert((MT + RT) * 128 >= MT * RT * 64);
-    int slot, rows, t[MT];
-    if (!ad_tile<MT, FEW>(a, blockIdx.x, a.sub, blockIdx.x + blockIdx.y + blockIdx.z == 0, slot, rows, t) || slot < 0) return;
+    __shared__ u32x4 s_stage[W][(1 + RT) * 128];       // (then the waves' sums)
+    int slot, rows, t[1];
+    if (!ad_tile<1, FEW>(a, blockIdx.x, blockIdx.x + blockIdx.y + blockIdx.z == 0, slot, rows, t) || slot < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
     const int part = ((a.K + 63) / 64 + a.splits - 1) / a.splits * 64, kbegin = int(blockIdx.z) * part, kend = min(kbegin + part, a.K);
     const int r0 = int(blockIdx.y) * 16 * RT;
-    f32x4 acc[MT][RT];
+    f32x4 acc[1][RT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    ad_accumulate<TYPE, MT, RT, W, D>(a, t, rows, a.a + size_t(slot) * size_t(a.a_slot) + size_t(r0) * size_t(a.K), a.SR - r0,
+    for (int r = 0; r < RT; ++r) acc[0][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    ad_accumulate<TYPE, 1, RT, W, D>(a, t, rows, a.a + size_t(slot) * size_t(a.a_slot) + size_t(r0) * size_t(a.K), a.SR - r0,
                                       s_stage[wv], kbegin, kend, acc);
     f32x4* mine = reinterpret_cast<f32x4*>(s_stage[wv]) + lane;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) mine[64 * (m * RT + r)] = acc[m][r];
+    for (int r = 0; r < RT; ++r) mine[64 * r] = acc[0][r];
     __syncthreads();
-    for (int f = wv; f < MT * RT; f += W) {
+    for (int f = wv; f < RT; f += W) {
         f32x4 v = reinterpret_cast<const f32x4*>(s_stage[0])[64 * f + lane];
 #pragma unroll
         for (int u = 1; u < W; ++u) {
@@ -352,14 +346,11 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(AdArg
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += p[i];
         }
-        const int m = f / RT, r = r0 + 16 * (f % RT) + li;
+        const int r = r0 + 16 * f + li;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            int of = t[0];
-#pragma unroll
-            for (int mm = 1; mm < MT; ++mm) of = m == mm ? t[mm] : of;
-            of = __builtin_amdgcn_ds_bpermute(4 * (4 * q + i), of);
-            if (r < a.SR && 16 * m + 4 * q + i < rows) a.v[(size_t(blockIdx.z) * a.M + of) * a.SR + r] = v[i];
+            const int of = __builtin_amdgcn_ds_bpermute(4 * (4 * q + i), t[0]);
+            if (r < a.SR && 4 * q + i < rows) a.v[(size_t(blockIdx.z) * a.M + of) * a.SR + r] = v[i];
         }
     }
 }
@@ -585,21 +576,21 @@ template <int TYPE, class F> __device__ __forceinline__ float ad_sum(const uint1
 
 constexpr int kExpandWaves = 4;                        // a block: 64 columns a wave
 
-template <int TYPE, int OUT, int MT, int FEW>
+template <int TYPE, int OUT, int FEW>
 __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArgs a) {
-    extern __shared__ __attribute__((aligned(16))) u32x4 s_v[];        // [MT][parts][steps][64]
+    extern __shared__ __attribute__((aligned(16))) u32x4 s_v[];        // [parts][steps][64]
     constexpr int PARTS = kAdParts<TYPE, OUT>;
-    __shared__ uint32_t s_most[16 * MT];
-    __shared__ int s_t[16 * MT];
+    __shared__ uint32_t s_most[16];
+    __shared__ int s_t[16];
     __shared__ u32x4 s_stage[kExpandWaves][512];       // a wave's B of 64 columns and 64 r, then its results
-    int slot, rows, t[MT];
-    if (!ad_tile<MT, FEW>(a, blockIdx.x, 1, false, slot, rows, t) || (slot < 0 && a.in_place)) return;
+    int slot, rows, t[1];
+    if (!ad_tile<1, FEW>(a, blockIdx.x, false, slot, rows, t) || (slot < 0 && a.in_place)) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
     int p = 0;
     while (int(blockIdx.y) >= a.blocks[p]) ++p;
     const int end = a.ends[p];
     const int n0 = (p ? a.ends[p - 1] : 0) + ((int(blockIdx.y) - (p ? a.blocks[p - 1] : 0)) * kExpandWaves + wv) * 64;
-    typedef AdCells<OUT, MT, FEW == 0> Cells;
+    typedef AdCells<OUT, 1, FEW == 0> Cells;
     const bool whole = n0 + 64 <= end;
     Cells cells(a, t, rows, n0);
     if (slot < 0) {
@@ -610,11 +601,8 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
     const int chunks = a.R / 8, steps = (chunks + 3) / 4;
     {
         // scale v of the tile's rows and this slice in its parts, in pieces of 8 along r, as the instruction's operands
-        if (tid < 16) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m) s_t[16 * m + tid] = t[m];
-        }
-        if (TYPE == ORNITH_ADAPTER_F16 && tid < 16 * MT) s_most[tid] = 0;
+        if (tid < 16) s_t[tid] = t[0];
+        if (TYPE == ORNITH_ADAPTER_F16 && tid < 16) s_most[tid] = 0;
         __syncthreads();
         struct Piece { f32x4 v[2]; };
         const float scale = a.scales[slot];
@@ -635,7 +623,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
             return sum;
         };
         if constexpr (TYPE == ORNITH_ADAPTER_F16) {
-            for (int i = tid; i < 16 * MT * chunks; i += 64 * kExpandWaves) {
+            for (int i = tid; i < 16 * chunks; i += 64 * kExpandWaves) {
                 const Piece v = piece_of(i / chunks, i % chunks);
                 uint32_t most = 0;
 #pragma unroll
@@ -644,7 +632,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
             }
             __syncthreads();
         }
-        for (int i = tid; i < 16 * MT * steps * 4; i += 64 * kExpandWaves) {
+        for (int i = tid; i < 16 * steps * 4; i += 64 * kExpandWaves) {
             const int row = i / (steps * 4), c = i % (steps * 4);
             u32x4 part[PARTS] = {};
             if (c < chunks) {
@@ -660,22 +648,16 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
             }
 #pragma unroll
             for (int u = 0; u < PARTS; ++u)
-                s_v[(((row >> 4) * PARTS + u) * steps + (c >> 2)) * 64 + (c & 3) * 16 + (row & 15)] = part[u];
+                s_v[(u * steps + (c >> 2)) * 64 + (c & 3) * 16 + row] = part[u];
         }
         __syncthreads();
     }
     if (n0 >= end) return;
-    float by[MT];
+    float by[1] = {1.f};
+    if constexpr (TYPE == ORNITH_ADAPTER_F16) by[0] = 1.f / ad_scale16(s_most[li]);
+    f32x4 acc[1][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        by[m] = 1.f;
-        if constexpr (TYPE == ORNITH_ADAPTER_F16) by[m] = 1.f / ad_scale16(s_most[16 * m + li]);
-    }
-    f32x4 acc[MT][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 4; ++j) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     // 64 r at a time: eight lanes on a column's 128 bytes, through LDS to the operands' order (piece c of column
     // n at 8 n + (c ^ n % 8)); the next ones on their way meanwhile
     const uint16_t* const bank = a.b + size_t(slot) * size_t(a.b_slot);
@@ -704,20 +686,17 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
 #pragma unroll
             for (int j = 0; j < 4; ++j) bw[j] = s_stage[wv][8 * (16 * j + li) + ((4 * h + q) ^ (li & 7))];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
+            for (int u = 0; u < PARTS; ++u) {
+                const u32x4 vv = s_v[(u * steps + s + h) * 64 + lane];
 #pragma unroll
-                for (int u = 0; u < PARTS; ++u) {
-                    const u32x4 vv = s_v[((m * PARTS + u) * steps + s + h) * 64 + lane];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[m][j] = ad_mfma<TYPE>(bw[j], vv, acc[m][j]);
-                }
+                for (int j = 0; j < 4; ++j) acc[0][j] = ad_mfma<TYPE>(bw[j], vv, acc[0][j]);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
-    auto form = [&](int m, int row, int column) {
-        const float* from = a.v + size_t(s_t[16 * m + row]) * a.SR + p * a.R;
+    auto form = [&](int, int row, int column) {
+        const float* from = a.v + size_t(s_t[row]) * a.SR + p * a.R;
         return ad_sum<TYPE>(bank + size_t(n0 + column) * size_t(a.R), a.R, a.scales[slot], [&](int r) {
             float v = from[r];                         // (the parts of K in order)
             for (int z = 1; z < a.splits; ++z) v += from[size_t(z) * size_t(a.M) * a.SR + r];
@@ -749,7 +728,7 @@ __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
     // blocks go to the 8 XCDs in turn: a row's column blocks on one of them, whose L2 keeps its A
     const int nblocks = a.blocks[a.S - 1], unit = int(blockIdx.x / 8) / nblocks * 8 + int(blockIdx.x % 8);
     const int cb = int(blockIdx.x / 8) % nblocks;
-    if (unit >= a.units || !ad_tile<MT, FEW>(a, unit, 1, blockIdx.x == 0, slot, rows, t) || (slot < 0 && a.in_place)) return;
+    if (unit >= a.units || !ad_tile<MT, FEW>(a, unit, blockIdx.x == 0, slot, rows, t) || (slot < 0 && a.in_place)) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, q = lane >> 4;
     int p = 0;
     while (cb >= a.blocks[p]) ++p;
@@ -917,11 +896,10 @@ int ad_splits(int64_t M) { return M <= kFewRows ? 4 : 1; }
 
 // Rows of a planned tile, and tiles at most.
 // (us: both products of one launch in tiles of 16 / 32 rows, 6144 columns of K = 2048: rank 16, 8192 rows 66.4 /
-// 69.6; rank 32, 76.3 / 75.5, 1120 rows 18.0 / 18.2; rank 64, 8192 rows 119 / 93.6, 1120 rows of 2048 columns 18.8 / 21.4)
-int ad_tile_rows(int M, int R) {
-    if (R <= kBothRank) return R > 32 && M >= 4096 ? 32 : 16;
-    return M >= 1024 && R <= 128 ? 64 : 16;
-}
+// 69.6; rank 32, 76.3 / 75.5, 1120 rows 18.0 / 18.2; rank 64, 8192 rows 119 / 93.6, 1120 rows of 2048 columns 18.8 / 21.4.
+// In two launches 64 rows, which read B less often, took 10 to 80 % longer than 16 from 512 to 8192 rows, ranks 72 to 256, 1024
+// to 12288 columns and 2 to 300 requests: 8192 x 6144 of rank 128 182 / 144, 1024 rows 43 / 27.)
+int ad_tile_rows(int M, int R) { return R > 32 && R <= kBothRank && M >= 4096 ? 32 : 16; }
 int ad_tiles(int M, int slots, int tile_rows) { return std::min(M, (M + tile_rows - 1) / tile_rows + slots + 1); }
 
 bool ad_layout(int64_t M, int S, int R, AdLayout& l) {
@@ -932,7 +910,7 @@ bool ad_layout(int64_t M, int S, int R, AdLayout& l) {
     l.tiles = align256(std::max(rows * size_t(ad_splits(M)), std::min(rows, size_t(kFewRows)) * size_t(ad_splits(kFewRows))) *
                        size_t(S) * size_t(R) * 4);
     size_t words = 0;                                  // of a plan's tiles, whichever rows and slots
-    for (int tile_rows : {16, 32, 64})
+    for (int tile_rows : {16, 32})
         words = std::max(words, size_t(ad_tiles(int(rows), kAdMaxSlots, tile_rows)) * size_t(kTileHead + tile_rows));
     l.bytes = l.tiles + align256((M <= kFewRows ? 0 : words) * 4) + 256;
     return true;
@@ -982,24 +960,23 @@ template <int TYPE, int MT, int FEW> hipError_t ad_both(AdArgs& a, int out_type,
     return hipGetLastError();
 }
 
-template <int TYPE, int MT, int FEW> hipError_t ad_two(AdArgs& a, int out_type, hipStream_t s) {
+template <int TYPE, int FEW> hipError_t ad_two(AdArgs& a, int out_type, hipStream_t s) {
     const int rt = (a.SR + 15) / 16;
-    a.sub = MT;                                        // (16 rows a block: more blocks to read x)
     a.splits = std::max(1, std::min(ad_splits(a.M), (a.K + 511) / 512));
     auto shrink = [&](auto kernel, int RT) {
-        timed_launch("adapter_shrink", kernel, dim3(a.units * a.sub, (rt + RT - 1) / RT, a.splits), dim3(64 * kShrinkWaves), 0, s, a);
+        timed_launch("adapter_shrink", kernel, dim3(a.units, (rt + RT - 1) / RT, a.splits), dim3(64 * kShrinkWaves), 0, s, a);
     };
     // few rows: 16 of A's a block, more blocks; many: 64, which reads x less often
-    if (FEW || rt < 4) shrink(adapter_shrink_kernel<TYPE, 1, 1, 4, FEW>, 1);
-    else shrink(adapter_shrink_kernel<TYPE, 1, 4, 2, FEW>, 4);
+    if (FEW || rt < 4) shrink(adapter_shrink_kernel<TYPE, 1, 4, FEW>, 1);
+    else shrink(adapter_shrink_kernel<TYPE, 4, 2, FEW>, 4);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
     const dim3 grid(a.units, ad_blocks(a, 64 * kExpandWaves));
     const int steps = (a.R / 8 + 3) / 4;
     ad_by_type(out_type, [&](auto out) {
         constexpr int OUT = decltype(out)::value;
-        timed_launch("adapter_expand", adapter_expand_kernel<TYPE, OUT, MT, FEW>, grid, dim3(64 * kExpandWaves),
-                     uint32_t(MT * steps * kAdParts<TYPE, OUT> * 1024), s, a);
+        timed_launch("adapter_expand", adapter_expand_kernel<TYPE, OUT, FEW>, grid, dim3(64 * kExpandWaves),
+                     uint32_t(steps * kAdParts<TYPE, OUT> * 1024), s, a);
     });
     return hipGetLastError();
 }
@@ -1007,8 +984,8 @@ template <int TYPE, int MT, int FEW> hipError_t ad_two(AdArgs& a, int out_type, 
 template <int TYPE> hipError_t ad_rows(AdArgs& a, int out_type, hipStream_t s) {
     const bool both = a.R <= kBothRank;
     a.units = a.M;
-    if (a.M <= 64) return both ? ad_both<TYPE, 1, 1>(a, out_type, s) : ad_two<TYPE, 1, 1>(a, out_type, s);
-    if (a.M <= kFewRows) return both ? ad_both<TYPE, 1, 4>(a, out_type, s) : ad_two<TYPE, 1, 4>(a, out_type, s);
+    if (a.M <= 64) return both ? ad_both<TYPE, 1, 1>(a, out_type, s) : ad_two<TYPE, 1>(a, out_type, s);
+    if (a.M <= kFewRows) return both ? ad_both<TYPE, 1, 4>(a, out_type, s) : ad_two<TYPE, 4>(a, out_type, s);
     a.tile_rows = ad_tile_rows(a.M, a.R);
     a.units = ad_tiles(a.M, a.slots, a.tile_rows);
     timed_launch("adapter_plan", adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
@@ -1019,7 +996,7 @@ template <int TYPE> hipError_t ad_rows(AdArgs& a, int out_type, hipStream_t s) {
         if (a.tile_rows == 32) return grid ? ad_both<TYPE, 2, 0>(a, out_type, s) : ad_both<TYPE, 2, -1>(a, out_type, s);
         return grid ? ad_both<TYPE, 1, 0>(a, out_type, s) : ad_both<TYPE, 1, -1>(a, out_type, s);
     }
-    return a.tile_rows == 64 ? ad_two<TYPE, 4, 0>(a, out_type, s) : ad_two<TYPE, 1, 0>(a, out_type, s);
+    return ad_two<TYPE, 0>(a, out_type, s);
 }
 
 }  // namespace
