@@ -33,7 +33,7 @@
  *   plain 4-bit      w4_tile, w4_run (more than 16 rows of many columns),
  *                    w4_zero (no inputs), w4_pack_codes, w4_pack_meta
  *   routing          route_experts
- *   adapters         adapter_plan (above 256 rows); adapter_both (ranks up to 64),
+ *   adapters         adapter_plan (many rows); adapter_both (ranks up to 64),
  *                    or adapter_shrink and adapter_expand (above)
  *   shared expert    fixed8_act, fixed8_gate
  *   other            repack_codes, repack_meta, silu_selfcheck */

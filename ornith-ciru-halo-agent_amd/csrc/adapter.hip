@@ -61,12 +61,13 @@ struct AdArgs {
 };
 
 // ---- rows by slot ---------------------------------------------------------------
-// Up to 256 rows: no plan.  Block t of a launch looks at all ids, and if row t is the first, 17th, .. of its
-// slot it takes that row and the next 15 of the slot; other blocks end.
+// Few rows (ad_few): no plan.  Block t of a launch looks at all ids, and if row t is the first, 17th, .. of its
+// slot it takes that row and the next 15 of the slot; other blocks end.  (Up to 64 rows one id a lane, 64 rows of 6144
+// columns, rank 16, 7.5 us; with four a lane 8.2.)
 // More: one block counts rows per slot in LDS, sums, and sends each row to a place of its slot.  Which place
 // it gets is open (atomics), and no result depends on it: rows of a tile do not meet.  (A launch, the ids'
 // round trip and two passes over LDS: 4.2 us at 1120 rows, 7.8 at 8192.)
-constexpr int kFewRows = 256, kPlanThreads = 1024, kPlanBatch = 8;
+constexpr int kWaveRows = 64, kFewRows = 256, kPlanThreads = 1024, kPlanBatch = 8;
 
 __device__ __forceinline__ int ad_key(int id, int slots) { return id >= 0 && id < slots ? id + 1 : 0; }      // 0: no adapter
 
@@ -894,6 +895,20 @@ struct AdLayout { size_t v, tiles, bytes; };
 // Parts of K that a shrink of M rows may have (each has a v of its own).
 int ad_splits(int64_t M) { return M <= kFewRows ? 4 : 1; }
 
+// Whether a call goes without a plan.  It then takes one launch less (3 us of the host's time too, which a call of 8.5
+// waits for), but the tiles of a long run of one request lie 16 rows apart, on one XCD, and each 512 columns form v again.
+// Up to 256 rows while full tiles and 512s of columns make up to 160 blocks, above rank 16 80; in two launches up to 64
+// rows.  (us of eager calls, without / with a plan, rows of as many requests and of three, K = 2048, 16 slots: rank 16, 6144
+// columns, 128 rows 8.6 / 11.6 and 12.1 / 11.4, 192 rows 10.3 / 11.6 and 16.1 / 11.4, 256 rows 13.5 / 12.1 and 21.4 / 11.5;
+// 12288 columns, 128 rows 14.1 / 11.9 and 19.5 / 11.7; rank 32, 4096 columns, 160 rows 11.5 / 11.6 and 18.0 / 11.6, 6144
+// columns, 128 rows 13.5 / 11.9 and 18.3 / 11.6; rank 64, 4096 columns, 160 rows 12.4 / 13.9 and 20.1 / 13.9, 6144 columns,
+// 128 rows 18.1 / 14.3 and 24.7 / 13.8; rank 128, 1024 columns, 72 rows 16.2 / 15.1 and 15.8 / 14.5, 6144 columns, 128 rows
+// 32.3 / 18.6 and 40.3 / 15.9.)
+bool ad_few(int64_t M, int N, int R) {
+    if (M <= kWaveRows) return true;
+    return R <= kBothRank && M <= kFewRows && (M + 15) / 16 * ((N + 511) / 512) <= (R <= 16 ? 160 : 80);
+}
+
 // Rows of a planned tile, and tiles at most.
 // (us: both products of one launch in tiles of 16 / 32 rows, 6144 columns of K = 2048: rank 16, 8192 rows 66.4 /
 // 69.6; rank 32, 76.3 / 75.5, 1120 rows 18.0 / 18.2; rank 64, 8192 rows 119 / 93.6, 1120 rows of 2048 columns 18.8 / 21.4.
@@ -912,7 +927,7 @@ bool ad_layout(int64_t M, int S, int R, AdLayout& l) {
     size_t words = 0;                                  // of a plan's tiles, whichever rows and slots
     for (int tile_rows : {16, 32})
         words = std::max(words, size_t(ad_tiles(int(rows), kAdMaxSlots, tile_rows)) * size_t(kTileHead + tile_rows));
-    l.bytes = l.tiles + align256((M <= kFewRows ? 0 : words) * 4) + 256;
+    l.bytes = l.tiles + align256((M <= kWaveRows ? 0 : words) * 4) + 256;
     return true;
 }
 
@@ -983,9 +998,11 @@ template <int TYPE, int FEW> hipError_t ad_two(AdArgs& a, int out_type, hipStrea
 
 template <int TYPE> hipError_t ad_rows(AdArgs& a, int out_type, hipStream_t s) {
     const bool both = a.R <= kBothRank;
-    a.units = a.M;
-    if (a.M <= 64) return both ? ad_both<TYPE, 1, 1>(a, out_type, s) : ad_two<TYPE, 1>(a, out_type, s);
-    if (a.M <= kFewRows) return both ? ad_both<TYPE, 1, 4>(a, out_type, s) : ad_two<TYPE, 4>(a, out_type, s);
+    if (ad_few(a.M, a.N, a.R)) {
+        a.units = a.M;
+        if (!both) return ad_two<TYPE, 1>(a, out_type, s);
+        return a.M <= kWaveRows ? ad_both<TYPE, 1, 1>(a, out_type, s) : ad_both<TYPE, 1, 4>(a, out_type, s);
+    }
     a.tile_rows = ad_tile_rows(a.M, a.R);
     a.units = ad_tiles(a.M, a.slots, a.tile_rows);
     timed_launch("adapter_plan", adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
