@@ -710,8 +710,11 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
 
 // ---- both in one ----------------------------------------------------------------
 // A small rank: a block forms v of its tile for itself (its waves share k) and then its columns, 64 a wave at
-// a time.  Every block of columns reads x and A again, from its XCD's L2, and spares the second launch (2048 to
-// 6144, rank 16, 1 row 5.4 us against 7.2 in two, 32 rows 6.9 / 7.5; rank 64 of 8192 rows 94 / 142).  Few rows wait
+// a time.  Every block of columns reads x and A again, from its XCD's L2, and spares the second launch (us, one / two,
+// 2048 to 6144: rank 16, 1 row 5.5 / 7.6, 32 rows 7.1 / 8.7, 1120 rows 16.3 / 30.9; rank 32, 1 row 6.6 / 7.9, 32 rows
+// 11.0 / 9.1, 1120 rows 20.7 / 32.2; rank 64, 8192 rows 90 / 142, 1120 rows 30.4 / 36.7, 1 row 9.0 / 8.0, 32 rows 15.5 /
+// 11.1, of 2048 columns 9.3 / 8.0, 64 rows of two times 512 columns 9.9 / 10.7.  In a graph two are faster for up to 64
+// rows of rank 33 and up, but for few columns; an eager call waits for the host, which a second launch costs 3).  Few rows wait
 // for one chain: id, x and A, the waves' exchange, B, the store.  Many stream base and out: 8192 rows 57 us for 239
 // MB, 4.2 TB/s of the 5.1 that a copy reaches; the rest goes into the exchange of results through LDS and the
 // time before a block's first columns.
@@ -981,9 +984,15 @@ template <int TYPE, int FEW> hipError_t ad_two(AdArgs& a, int out_type, hipStrea
     auto shrink = [&](auto kernel, int RT) {
         timed_launch("adapter_shrink", kernel, dim3(a.units, (rt + RT - 1) / RT, a.splits), dim3(64 * kShrinkWaves), 0, s, a);
     };
-    // few rows: 16 of A's a block, more blocks; many: 64, which reads x less often
-    if (FEW || rt < 4) shrink(adapter_shrink_kernel<TYPE, 1, 4, FEW>, 1);
-    else shrink(adapter_shrink_kernel<TYPE, 4, 2, FEW>, 4);
+    // Rows of A a block: 64 reads x less often, 16 makes more blocks, for up to 160 rows of x times 16s of A (us, both
+    // launches, 16 / 64, as many requests as rows, K = 2048, 6144 columns: rank 128, 16 rows 12.2 / 12.6, 32 rows 15.3 / 14.0;
+    // rank 256, 8 rows 13.7 / 13.9, 16 rows 16.8 / 15.8; rank 512, 4 rows 17.4 / 17.6, 8 rows 19.4 / 18.6; one row 8.7 / 9.3).
+    bool narrow = false;
+    if constexpr (FEW > 0) {
+        narrow = a.M * rt <= 160;
+        if (narrow) shrink(adapter_shrink_kernel<TYPE, 1, 4, FEW>, 1);
+    }
+    if (!narrow) shrink(adapter_shrink_kernel<TYPE, 4, 2, FEW>, 4);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
     const dim3 grid(a.units, ad_blocks(a, 64 * kExpandWaves));
