@@ -72,8 +72,8 @@ constexpr int kWaveRows = 64, kFewRows = 256, kPlanThreads = 1024, kPlanBatch = 
 __device__ __forceinline__ int ad_key(int id, int slots) { return id >= 0 && id < slots ? id + 1 : 0; }      // 0: no adapter
 
 // Lane li's row of tile `unit` (past the last row: that one again), its slot and how many rows; false where there is
-// nothing to do.  FEW: ids a lane looks at (0 and below: a plan).  first: the
-// launch's block that raises flags.
+// nothing to do.  FEW: ids a lane looks at (0: a plan; -1: a plan, and results off the 16-byte grid).  first: the launch's
+// block that raises flags.
 template <int MT, int FEW>
 __device__ __forceinline__ bool ad_tile(const AdArgs& a, int unit, bool first, int& slot, int& rows, int (&t)[MT]) {
     const int lane = threadIdx.x & 63, li = lane & 15;
@@ -401,7 +401,8 @@ typedef u32x4 ad_piece4 __attribute__((aligned(4)));
 // A wave's 16 MT rows x 64 columns of base and out, as they move: eight lanes (fp32: 16) on a row's 16-byte
 // pieces, H accesses for 16 rows.  (Neighbouring lanes in different rows, as the products leave them, halve
 // the rate.)  ONCE: stores that leave the caches alone,
-// of many rows on the 16-byte grid (8192 rows 69.3 / 66.5 us, 4096 rows 42.4 / 31.9; off it 79.4 / 96.6).
+// of many rows on the 16-byte grid (us without / with: 8192 rows 69.3 / 66.5, 4096 rows 42.4 / 31.9, off it 79.4 / 96.6;
+// in two launches, rank 128, 8192 rows 146.8 / 144.9, 1120 rows 31.3 / 29.8, off it 150.4 / 155.7 and 33.1 / 32.4).
 template <int OUT, int MT, bool ONCE> struct AdCells {
     typedef std::conditional_t<OUT == ORNITH_ADAPTER_F32, uint32_t, uint16_t> word;
     typedef std::conditional_t<OUT == ORNITH_ADAPTER_F32, ad_piece4, ad_piece2> piece_t;
@@ -718,7 +719,6 @@ __global__ __launch_bounds__(64 * kExpandWaves) void adapter_expand_kernel(AdArg
 // for one chain: id, x and A, the waves' exchange, B, the store.  Many stream base and out: 8192 rows 57 us for 239
 // MB, 4.2 TB/s of the 5.1 that a copy reaches; the rest goes into the exchange of results through LDS and the
 // time before a block's first columns.
-// FEW -1: a plan, and rows off the 16-byte grid.
 template <int TYPE, int OUT, int MT, int RT, int W, int FEW>
 __global__ __launch_bounds__(64 * W) void adapter_both_kernel(AdArgs a) {
     constexpr int D = FEW > 0 && MT + RT <= 3 ? 4 : 2, PARTS = kAdParts<TYPE, OUT>, STEPS = (PARTS * RT + 1) / 2;
@@ -992,7 +992,7 @@ template <int TYPE, int FEW> hipError_t ad_two(AdArgs& a, int out_type, hipStrea
         narrow = a.M * rt <= 160;
         if (narrow) shrink(adapter_shrink_kernel<TYPE, 1, 4, FEW>, 1);
     }
-    if (!narrow) shrink(adapter_shrink_kernel<TYPE, 4, 2, FEW>, 4);
+    if (!narrow) shrink(adapter_shrink_kernel<TYPE, 4, 2, std::max(FEW, 0)>, 4);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
     const dim3 grid(a.units, ad_blocks(a, 64 * kExpandWaves));
@@ -1017,12 +1017,12 @@ template <int TYPE> hipError_t ad_rows(AdArgs& a, int out_type, hipStream_t s) {
     timed_launch("adapter_plan", adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     const hipError_t st = hipGetLastError();
     if (st != hipSuccess) return st;
+    const bool grid = ((reinterpret_cast<uintptr_t>(a.out) | size_t(a.ldo) * (out_type == ORNITH_ADAPTER_F32 ? 4 : 2)) & 15) == 0;
     if (both) {
-        const bool grid = ((reinterpret_cast<uintptr_t>(a.out) | size_t(a.ldo) * (out_type == ORNITH_ADAPTER_F32 ? 4 : 2)) & 15) == 0;
         if (a.tile_rows == 32) return grid ? ad_both<TYPE, 2, 0>(a, out_type, s) : ad_both<TYPE, 2, -1>(a, out_type, s);
         return grid ? ad_both<TYPE, 1, 0>(a, out_type, s) : ad_both<TYPE, 1, -1>(a, out_type, s);
     }
-    return ad_two<TYPE, 0>(a, out_type, s);
+    return grid ? ad_two<TYPE, 0>(a, out_type, s) : ad_two<TYPE, -1>(a, out_type, s);
 }
 
 }  // namespace
