@@ -569,10 +569,12 @@ template <int OUT, int MT, bool ONCE> struct AdCells {
 };
 
 // scale sum_r B[r] v(r) of one row and column, in fp64: for results that the parts of v may have driven out of range.
+// A sum that is NaN stays one, so a row of NaN costs its batch little (8192 x 6144, rank 16 59 -> 68 us, 32 rows of rank 512
+// 40 -> 54; to the end of every sum 144 and 2084).
 template <int TYPE, class F> __device__ __forceinline__ float ad_sum(const uint16_t* b, int R, float scale, F&& v) {
     double sum = 0.0;
 #pragma unroll 1
-    for (int r = 0; r < R; ++r) sum += double(ad_float<TYPE>(b[r])) * double(v(r));
+    for (int r = 0; r < R && sum == sum; ++r) sum += double(ad_float<TYPE>(b[r])) * double(v(r));
     return float(sum * double(scale));
 }
 
